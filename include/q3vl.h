@@ -563,6 +563,63 @@ int q3_qk_norm_rope_backward(const void* grad_q, const void* grad_k, const void*
                              const int64_t* section, float eps, const int64_t* strides, int dtype, void* workspace,
                              int64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- four-bit weights and caches (MXFP4)
+ * No counterpart in the reference (bf16 and fp32 only); for serving with weights and KV caches at a quarter of
+ * their bf16 bytes. A row is cut into blocks of 32 consecutive values; a value is a 4-bit float (E2M1: sign, then
+ * 0, 0.5, 1, 1.5, 2, 3, 4, 6), a block has one power-of-two scale held as its exponent (E8M0: byte s stands for
+ * 2^(s - 127), 255 for NaN). Byte j of a row of codes holds value 2j in its low and value 2j + 1 in its high half.
+ * Quantisation: s = max(0, 125 + floor(log2 t)), t the block's largest magnitude (0 for a block of zeros); values
+ * over the scale round to the nearest code, ties to the even one, 6 from there on (sign kept, also of zeros); a
+ * block with an infinity or a NaN gets s = 255 and codes 0 and reads as NaN. A code times its scale is exact in
+ * bf16.
+ *
+ * q3_mxfp4_quantize: x (rows, cols) with row stride ldx -> codes (rows, cols / 2) and scales (rows, cols / 32),
+ * packed. cols a multiple of 32 (else Q3_ERR_SHAPE); x 16-byte aligned, ldx whole 16-byte pieces.
+ * q3_mxfp4_dequantize: (n0, n1) planes of `run` consecutive values (a multiple of 32) to y (n0, n1, run), packed,
+ * of type dtype; strides = [codes n0, n1, scales n0, n1] in bytes. n0 * n1 <= 65535. */
+int q3_mxfp4_quantize(const void* x, void* codes, void* scales, int64_t rows, int64_t cols, int64_t ldx, int dtype,
+                      void* stream);
+int q3_mxfp4_dequantize(const void* codes, const void* scales, void* y, int64_t n0, int64_t n1, int64_t run,
+                        const int64_t* strides, int dtype, void* stream);
+
+/* y = x w^T (+ bias) (+ residual), one rounding: q3_matmul with w (N, K) in MXFP4, code rows ldw and scale rows lds
+ * bytes apart. bf16; K a multiple of 32; x and the code rows 16-byte aligned. Up to 32 rows stream the weights;
+ * more rows need packed weights (ldw = K / 2, lds = K / 32). */
+int64_t q3_matmul_mxfp4_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, const void* bias, const void* residual,
+                    void* y, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t lds, int64_t ldr,
+                    int64_t ldc, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Four-bit KV cache: codes (B, Hkv, cap, D / 2) and scales (B, Hkv, cap, D / 32) of keys and values, the rows of a
+ * head packed, any batch and head strides (codes 16-byte aligned).
+ * q3_kv_append_mxfp4: rows k, v (B, S, Hkv, D) quantised into cache rows kv_lens[b] + s; rows at or past cap (or
+ * before 0) are not written. kv_lens is not advanced. D a multiple of 32 up to 256. strides = [k b, s, h, v b, s, h]
+ * in elements, then [b, h] of k_codes, k_scales, v_codes, v_scales in bytes. */
+int q3_kv_append_mxfp4(const void* k, const void* v, void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                       const int* kv_lens, int64_t B, int64_t S, int64_t Hkv, int64_t D, int64_t cap,
+                       const int64_t* strides, int dtype, void* stream);
+
+/* q3_decode_attention over a four-bit cache: sequence b attends to rows [0, kv_lens[b] + advance) (advance = 1: the
+ * step, whose row is already written; kv_lens[b] is then incremented in place), at most cap. q, o (B, Hq, D);
+ * strides = [qb, qh, 0, ob, oh, 0] in elements, then [b, h] of k_codes, k_scales, v_codes, v_scales in bytes. An
+ * empty sequence gives zeros; a NaN reaches only the queries that see its row. bf16, D = 64 or 128, B <= 1024 (else
+ * Q3_ERR_UNSUPPORTED). */
+int64_t q3_decode_attention_mxfp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
+int q3_decode_attention_mxfp4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                              const void* v_scales, int* kv_lens, int advance, void* o, int64_t B, int64_t Hq,
+                              int64_t Hkv, int64_t D, int64_t cap, const int64_t* strides, float scale, int dtype,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* q3_flash_attention_cache over a four-bit cache: query i of sequence b attends to rows [0, kv_lens[b] + i], whose
+ * last Sq are already written; kv_lens[b] += Sq afterwards with `advance`. max_len >= every kv_lens[b] + Sq bounds
+ * the rows (and the workspace). strides = [qb, qh, qs, ob, oh, os], then as q3_decode_attention_mxfp4. */
+int64_t q3_flash_attention_cache_mxfp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
+                                                       int64_t max_len);
+int q3_flash_attention_cache_mxfp4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                                   const void* v_scales, int* kv_lens, void* o, int64_t B, int64_t Hq, int64_t Hkv,
+                                   int64_t Sq, int64_t D, int64_t max_len, const int64_t* strides, float scale,
+                                   int advance, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

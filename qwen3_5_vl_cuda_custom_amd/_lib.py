@@ -114,6 +114,17 @@ _SIGS: dict[str, tuple] = {
     "q3_flash_attention_backward_mfma_workspace_bytes": (c_int64, [_I, _I, _I, _I, _I, _I, c_int]),
     "q3_flash_attention_backward": (c_int, [_V, _V, _V, _V, _f32p, _V, _V, _V, _V, _I, _I, _I, _I, _I, _I, c_float,
                                             c_int, c_int, _V, _I, _V]),
+    "q3_mxfp4_quantize": (c_int, [_V, _V, _V, _I, _I, _I, c_int, _V]),
+    "q3_mxfp4_dequantize": (c_int, [_V, _V, _V, _I, _I, _I, _i64p, c_int, _V]),
+    "q3_matmul_mxfp4_workspace_bytes": (c_int64, [_I, _I, _I]),
+    "q3_matmul_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, _I, _I, _I, c_int, _V, _I, _V]),
+    "q3_kv_append_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, _i64p, c_int, _V]),
+    "q3_decode_attention_mxfp4_workspace_bytes": (c_int64, [_I, _I, _I, _I]),
+    "q3_decode_attention_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, c_int, _V, _I, _I, _I, _I, _I, _i64p, c_float, c_int,
+                                          _V, _I, _V]),
+    "q3_flash_attention_cache_mxfp4_workspace_bytes": (c_int64, [_I, _I, _I, _I, _I, _I]),
+    "q3_flash_attention_cache_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, _I, _i64p, c_float,
+                                               c_int, c_int, _V, _I, _V]),
 }
 
 EXPORTED = tuple(_SIGS)

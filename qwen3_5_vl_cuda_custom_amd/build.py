@@ -37,7 +37,7 @@ HIPFLAGS = [
 # AGPRs (its kernels' whole state fits the 256 registers of 2 waves per SIMD;
 # with AGPRs the softmax copied every score tile out of them).
 EXTRA_FLAGS: dict[str, list[str]] = {src: ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-                                     for src in ("attention.hip", "attention_bwd.hip")}
+                                     for src in ("attention.hip", "attention_bwd.hip", "mxfp4_attention.hip")}
 
 
 def _hipcc() -> str:

@@ -1,0 +1,420 @@
+"""MXFP4 operators on the GPU against their definition in float64 (oracle/mxfp4.py).
+
+Quantisation and its inverse are exact, so they must agree to the bit. The products round once to bf16 (relative
+2^-8 at most) after an fp32 sum of K terms (each addition 2^-24 of the magnitudes summed so far; twice that is
+allowed). Attention adds the rounding of its weights to bf16 (2^-8 of each) and the fp32 error of a score s, which
+its weight sees as a relative error: the dot product's D 2^-24 sum |q k|, and 2^-22 (1 + |s|) for the scaling and
+the exponential.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import mxfp4 as M
+from qwen3_5_vl_cuda_custom_amd import _lib
+from qwen3_5_vl_cuda_custom_amd import kernels as K
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+HALF = 2.0 ** -8  # half a step of bf16, relative
+
+
+def rnd(*shape, seed=0, dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=g).to(dtype)
+
+
+def same_bits(a, b):
+    a, b = a.cpu(), b.cpu()
+    return a.dtype == b.dtype and torch.equal(torch.nan_to_num(a.double(), nan=12345.0),
+                                              torch.nan_to_num(b.double(), nan=12345.0))
+
+
+def special_rows(dtype):
+    """Blocks at which quantisation can go wrong: zeros, one value, ties, saturation, the smallest and largest."""
+    t = torch.zeros(12, 32, dtype=torch.float64)
+    t[1, 5] = -3.5
+    t[2] = torch.linspace(-7.9, 7.9, 32)
+    t[3, :16] = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5.0,
+                              4.0])
+    t[4] = t[3] * 2.0 ** -120
+    t[5] = t[3] * 2.0 ** 100
+    t[6] = torch.arange(32) * 2.0 ** -131  # below the smallest scale's reach: subnormal inputs
+    t[7, 0], t[7, 1:] = 3.0e38, 1e-3
+    t[8, 3] = math.inf
+    t[9, 31] = math.nan
+    t[10, 0], t[10, 1] = -0.0, -1e-30
+    t[10, 2] = 1.0
+    t[11] = 2.0 ** -126 * torch.linspace(-1, 1, 32)
+    return t.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(1, 32), (3, 96), (257, 128), (64, 4096), (5, 1152 * 2)])
+def test_quantize_and_back_match_the_definition(rows, cols, dtype):
+    x = rnd(rows, cols, seed=rows, dtype=dtype) * torch.exp2(torch.randint(-20, 20, (rows, 1))).to(dtype)
+    codes, scales = K.mxfp4_quantize(x.to(DEV))
+    want_c, want_s = M.quantize(x)
+    assert torch.equal(scales.cpu(), want_s) and torch.equal(codes.cpu(), want_c)
+    for out in (torch.bfloat16, torch.float32):
+        back = K.mxfp4_dequantize(codes, scales, out)
+        assert back.dtype == out and same_bits(back.double(), M.values(want_c, want_s))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantize_special_blocks(dtype):
+    x = special_rows(dtype)
+    codes, scales = K.mxfp4_quantize(x.to(DEV))
+    want_c, want_s = M.quantize(x)
+    assert torch.equal(scales.cpu(), want_s) and torch.equal(codes.cpu(), want_c)
+    back = K.mxfp4_dequantize(codes, scales).cpu()
+    assert torch.isnan(back[8:10]).all() and torch.isfinite(back[:8]).all()
+
+
+def test_quantize_strided_and_empty_inputs():
+    x = rnd(6, 7, 256, seed=3).to(DEV)
+    for view in (x[:, :, 64:128], x[::2], x.transpose(0, 1), x[:, 1:, 8:200:2][..., :96], x[:0], x[..., :0]):
+        codes, scales = K.mxfp4_quantize(view)
+        assert codes.shape == (*view.shape[:-1], view.shape[-1] // 2)
+        if view.numel():
+            want_c, want_s = M.quantize(view.cpu())
+            assert torch.equal(codes.cpu(), want_c) and torch.equal(scales.cpu(), want_s)
+
+
+def test_dequantize_every_code_and_scale():
+    codes = torch.arange(256, dtype=torch.uint8).view(1, 16, 16).expand(256, 16, 16).contiguous()
+    scales = torch.arange(256, dtype=torch.uint8).view(256, 1, 1).expand(256, 16, 1).contiguous()
+    for out in (torch.bfloat16, torch.float32):  # scales 253 and 254 reach past the types' range: infinities
+        want = M.values(codes, scales).to(out)
+        assert bool((same_bits(K.mxfp4_dequantize(codes.to(DEV), scales.to(DEV), out), want)))
+        assert torch.equal(want.double()[:253], M.values(codes, scales)[:253])
+
+
+def test_dequantize_reads_cache_slices_in_place():
+    codes = torch.randint(0, 256, (3, 4, 50, 64), dtype=torch.uint8)
+    scales = torch.randint(100, 140, (3, 4, 50, 4), dtype=torch.uint8)
+    c, s = codes.to(DEV), scales.to(DEV)
+    for sl in ((slice(None), slice(None), slice(7, 30)), (slice(1, 3), slice(2, 3), slice(0, 1)),
+               (slice(None), slice(None), slice(0, 50, 7)), (slice(0, 0),), (2, slice(1, 3), slice(5, 9))):
+        assert same_bits(K.mxfp4_dequantize(c[sl], s[sl]).double(), M.values(codes[sl], scales[sl]))
+
+
+# ------------------------------------------------------------------ products
+def check_matmul(y, x, codes, scales, b=None, r=None):
+    w, x = M.values(codes, scales), x.double()
+    ref, mag = x @ w.T, x.abs() @ w.abs().T
+    for t in (b, r):
+        if t is not None:
+            ref, mag = ref + t.double(), mag + t.double().abs()
+    err = (x.shape[-1] + 2) * 2.0 ** -23 * mag
+    tol = HALF * (ref.abs() + err) + err
+    d = (y.double().cpu() - ref).abs()
+    assert y.dtype == torch.bfloat16 and bool((d <= tol).all()), float((d / tol).max())
+
+
+def weight(n, k, seed):
+    return M.quantize(rnd(n, k, seed=seed, dtype=torch.float32) * 0.05)
+
+
+@pytest.mark.parametrize("m", [1, 2, 4, 5, 16, 17, 32, 33, 64, 65, 130, 300])
+@pytest.mark.parametrize("n,k", [(1, 32), (17, 96), (130, 160), (256, 4096), (1000, 1056), (64, 8224)])
+def test_matmul_matches_float64(m, n, k):
+    codes, scales = weight(n, k, seed=n)
+    x = rnd(m, k, seed=m)
+    y = K.matmul_mxfp4(x.to(DEV), codes.to(DEV), scales.to(DEV))
+    check_matmul(y, x, codes, scales)
+
+
+@pytest.mark.parametrize("m", [1, 3, 20, 70])
+def test_matmul_bias_residual_out_and_strides(m):
+    n, k = 136, 320
+    codes, scales = weight(n, k, seed=9)
+    wide = rnd(m, k + 64, seed=1)
+    x, b, r = wide[:, 32:32 + k], rnd(n, seed=2), rnd(m, n, seed=3)
+    buf = torch.full((m, 3 * n), 7.0, dtype=torch.bfloat16, device=DEV)
+    y = K.matmul_mxfp4(wide.to(DEV)[:, 32:32 + k], codes.to(DEV), scales.to(DEV), b.to(DEV), r.to(DEV),
+                       out=buf[:, n:2 * n])
+    assert y.data_ptr() == buf[:, n:].data_ptr()
+    check_matmul(buf[:, n:2 * n], x, codes, scales, b, r)
+    assert bool((buf[:, :n] == 7).all()) and bool((buf[:, 2 * n:] == 7).all())
+    x3 = rnd(2, m, k, seed=4)
+    y3 = K.matmul_mxfp4(x3.to(DEV), codes.to(DEV), scales.to(DEV), None, None)
+    assert y3.shape == (2, m, n)
+    check_matmul(y3.reshape(-1, n), x3.reshape(-1, k), codes, scales)
+    assert K.matmul_mxfp4(x3.to(DEV)[:0], codes.to(DEV), scales.to(DEV)).shape == (0, m, n)
+
+
+@pytest.mark.parametrize("m", [3, 20, 70])
+def test_matmul_keeps_a_rows_nan_and_infinity_to_itself(m):
+    n, k = 96, 256
+    codes, scales = weight(n, k, seed=11)
+    scales[5, 2] = 255  # a weight row that could not be quantised
+    x = rnd(m, k, seed=5)
+    x[1, 7] = math.nan
+    x[2, k - 1] = math.inf
+    y = K.matmul_mxfp4(x.to(DEV), codes.to(DEV), scales.to(DEV)).cpu()
+    assert torch.isnan(y[:, 5]).all() and torch.isnan(y[1]).all() and not torch.isfinite(y[2]).any()
+    keep = [i for i in range(m) if i not in (1, 2)]
+    ok = [j for j in range(n) if j != 5]
+    check_matmul(y[keep][:, ok], x[keep], codes[ok], scales[ok])
+
+
+# ------------------------------------------------------------------ the cache
+class Cache:
+    """A four-bit cache with random rows; rows at or past lens[b] + used hold NaN scales, which nothing may see."""
+
+    def __init__(self, lens, hkv, cap, d, seed, used=0):
+        B = len(lens)
+        size = torch.exp(0.5 * rnd(d, seed=seed + 2, dtype=torch.float32))
+        self.kc, self.ks = M.quantize((rnd(B, hkv, cap, d, seed=seed, dtype=torch.float32) * size))
+        self.vc, self.vs = M.quantize((rnd(B, hkv, cap, d, seed=seed + 1, dtype=torch.float32) * size))
+        self.lens = torch.tensor(lens, dtype=torch.int32)
+        for b, n in enumerate(lens):
+            self.ks[b, :, n + used:] = 255
+            self.vs[b, :, n + used:] = 255
+
+    def device(self):
+        return tuple(t.to(DEV) for t in (self.kc, self.ks, self.vc, self.vs))
+
+    def values(self):
+        return M.values(self.kc, self.ks), M.values(self.vc, self.vs)
+
+
+def check_attention(o, q, cache, seen, scale):
+    """o, q (B, Hq, Sq, D) against float64 at the bound of the module's docstring."""
+    k, v = cache.values()
+    ref, spread = M.attention(q, k, v, seen, scale)
+    D, rows = q.shape[-1], max(int(seen.max()), 1)
+    G = q.shape[1] // k.shape[1]
+    # sum |q k| of the largest score a query sees (rows behind hold NaN: left out)
+    mag = torch.einsum("bhid,bhkd->bhik", q.double().abs(), k.abs().repeat_interleave(G, 1)).nan_to_num(0.0)
+    for b in range(q.shape[0]):
+        for i in range(q.shape[2]):
+            mag[b, :, i, max(int(seen[b, i]), 0):] = 0
+    mag = mag.amax(-1, keepdim=True) * scale
+    weight_err = HALF + 2 * (D * 2.0 ** -24 * mag + 2.0 ** -22 * (1 + mag)) + rows * 2.0 ** -23
+    tol = weight_err * spread * (1 + HALF) + HALF * ref.abs()
+    d = (o.double().cpu() - ref).abs()
+    assert bool((d <= tol).all()), float((d / tol.clamp(min=1e-300)).max())
+
+
+LENS = [0, 1, 31, 32, 33, 257, 700]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hkv,groups", [(1, 1), (2, 3), (8, 4), (2, 8), (1, 16), (2, 20), (1, 33)])
+def test_decode_matches_float64(hkv, groups, d):
+    c = Cache(LENS, hkv, 700, d, seed=groups)
+    q = rnd(len(LENS), hkv * groups, d, seed=4)
+    lens = c.lens.to(DEV)
+    o = K.decode_attention_mxfp4(q.to(DEV), *c.device(), lens, d ** -0.5)
+    assert torch.equal(lens.cpu(), c.lens)
+    check_attention(o.unsqueeze(2), q.unsqueeze(2), c, c.lens.view(-1, 1), d ** -0.5)
+    assert bool((o[0] == 0).all())
+
+
+def test_decode_one_long_sequence_and_large_scores():
+    c = Cache([5003], 2, 5003, 128, seed=5)
+    q = rnd(1, 8, 128, seed=6) * 6
+    o = K.decode_attention_mxfp4(q.to(DEV), *c.device(), c.lens.to(DEV), 128 ** -0.5)
+    check_attention(o.unsqueeze(2), q.unsqueeze(2), c, c.lens.view(-1, 1), 128 ** -0.5)
+
+
+def test_decode_step_attends_to_the_new_row_and_advances():
+    c = Cache(LENS[:-1] + [699], 2, 700, 128, seed=7, used=1)
+    q, lens = rnd(len(LENS), 8, 128, seed=8), c.lens.to(DEV)
+    out = torch.full((len(LENS), 3, 8, 128), 5.0, dtype=torch.bfloat16, device=DEV)
+    o = K.decode_attention_mxfp4(q.to(DEV).unsqueeze(2), *c.device(), lens, 128 ** -0.5, append=True, out=out[:, 1])
+    assert torch.equal(lens.cpu(), c.lens + 1)
+    check_attention(o.unsqueeze(2), q.unsqueeze(2), c, (c.lens + 1).view(-1, 1), 128 ** -0.5)
+    assert bool((out[:, 0] == 5).all()) and bool((out[:, 2] == 5).all())
+
+
+def test_decode_reads_cache_slices_and_strided_queries():
+    c = Cache([90, 0, 33, 128], 6, 128, 128, seed=9)
+    kc, ks, vc, vs = (t[1:3, 2:5] for t in c.device())
+    q = rnd(2, 128, 12, 2, seed=10)
+    qd = q.to(DEV).permute(3, 2, 0, 1).reshape(2, 24, 128)[:, ::2]  # head rows two apart
+    o = K.decode_attention_mxfp4(qd, kc, ks, vc, vs, c.lens.to(DEV)[1:3].contiguous(), 0.1)
+    sub = Cache([1], 1, 1, 128, seed=0)
+    sub.kc, sub.ks, sub.vc, sub.vs = (t[1:3, 2:5] for t in (c.kc, c.ks, c.vc, c.vs))
+    check_attention(o.unsqueeze(2), qd.cpu().unsqueeze(2), sub, c.lens[1:3].view(-1, 1), 0.1)
+
+
+def test_decode_nan_row_reaches_its_block_of_the_output_only():
+    c = Cache([64, 64], 1, 64, 128, seed=11)
+    c.vs[0, 0, 40, 2] = 255
+    q = rnd(2, 4, 128, seed=12)
+    o = K.decode_attention_mxfp4(q.to(DEV), *c.device(), c.lens.to(DEV), 0.1).cpu()
+    assert torch.isnan(o[0, :, 64:96]).all() and torch.isfinite(o[0, :, :64]).all() and torch.isfinite(o[0, :, 96:]).all()
+    assert torch.isfinite(o[1]).all()
+    c.ks[0, 0, 3, 0] = 255  # a key of NaN: the sequence's softmax is NaN
+    o = K.decode_attention_mxfp4(q.to(DEV), *c.device(), c.lens.to(DEV), 0.1).cpu()
+    assert torch.isnan(o[0]).all() and torch.isfinite(o[1]).all()
+
+
+CHUNKS = [(1, 1, 2), (2, 4, 3), (1, 4, 4), (2, 4, 5), (2, 3, 40), (1, 8, 33), (2, 2, 100), (1, 1, 16), (1, 1, 17)]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hkv,groups,sq", CHUNKS)
+def test_chunk_matches_float64(hkv, groups, sq, d):
+    lens = [0, 1, 30, 63, 200]
+    c = Cache(lens, hkv, 310, d, seed=sq, used=sq)
+    q = rnd(len(lens), sq, hkv * groups, d, seed=13).transpose(1, 2)
+    dl = c.lens.to(DEV)
+    o = K.flash_attention_cache_mxfp4(q.to(DEV), *c.device(), dl, d ** -0.5, groups, advance=True,
+                                      max_len=200 + sq)
+    assert torch.equal(dl.cpu(), c.lens + sq)
+    seen = c.lens.view(-1, 1) + 1 + torch.arange(sq)
+    check_attention(o, q, c, seen, d ** -0.5)
+
+
+def test_chunk_of_one_token_is_the_decode_step():
+    c = Cache([0, 40, 99], 2, 100, 128, seed=14, used=1)
+    q = rnd(3, 8, 1, 128, seed=15).to(DEV)
+    a = K.flash_attention_cache_mxfp4(q, *c.device(), c.lens.to(DEV), 0.1, 4)
+    b = K.decode_attention_mxfp4(q, *c.device(), c.lens.to(DEV), 0.1, append=True)
+    assert torch.equal(a[:, :, 0], b)
+
+
+@pytest.mark.parametrize("groups,sq", [(4, 4), (1, 3)])
+def test_short_chunk_a_later_tokens_nan_is_masked(groups, sq):
+    c = Cache([20, 31], 1, 64, 128, seed=16, used=sq)
+    q = rnd(2, groups, sq, 128, seed=17)
+    for b, n in enumerate((20, 31)):
+        c.ks[b, :, n + sq - 1] = 255
+        c.vs[b, :, n + sq - 1] = 255
+    o = K.flash_attention_cache_mxfp4(q.to(DEV), *c.device(), c.lens.to(DEV), 0.1, groups).cpu()
+    assert torch.isnan(o[:, :, -1]).all()
+    seen = c.lens.view(-1, 1) + 1 + torch.arange(sq - 1)
+    check_attention(o[:, :, :-1], q[:, :, :-1], c, seen, 0.1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+def test_append_writes_its_rows_and_no_other(d, dtype):
+    B, S, H, cap = 4, 5, 3, 40
+    lens = torch.tensor([0, 7, 36, 40], dtype=torch.int32)  # the last two run past the cap
+    kv = rnd(B, S, 2 * H, d, seed=18, dtype=dtype)
+    k, v = kv[:, :, :H], kv[:, :, H:]
+    cache = [torch.full((B, H, cap, w), 0xA5, dtype=torch.uint8) for w in (d // 2, d // 32, d // 2, d // 32)]
+    dev = [t.to(DEV) for t in cache]
+    kvd = kv.to(DEV)
+    K.kv_append_mxfp4(kvd[:, :, :H], kvd[:, :, H:], *dev, lens.to(DEV))
+    for x, c, s in ((k, 0, 1), (v, 2, 3)):
+        qc, qs = M.quantize(x)
+        for b in range(B):
+            for i in range(S):
+                if int(lens[b]) + i < cap:
+                    cache[c][b, :, int(lens[b]) + i] = qc[b, i]
+                    cache[s][b, :, int(lens[b]) + i] = qs[b, i]
+    for got, want in zip(dev, cache):
+        assert torch.equal(got.cpu(), want)
+
+
+def test_append_attend_chunk_and_steps_together_under_a_graph():
+    """A chunk, then steps, as a layer runs them: eager and as a replayed graph, against float64."""
+    B, H, G, D, cap = 2, 2, 4, 128, 80
+    c = Cache([0, 0], H, cap, D, seed=19)
+    cache, lens = c.device(), torch.tensor([3, 0], dtype=torch.int32, device=DEV)
+    k0, v0, q0 = rnd(B, 20, H, D, seed=20), rnd(B, 20, H, D, seed=21), rnd(B, H * G, 20, D, seed=22)
+    K.kv_append_mxfp4(k0.to(DEV)[:1, :3], v0.to(DEV)[:1, :3], *(t[:1] for t in cache),
+                      torch.zeros(1, dtype=torch.int32, device=DEV))  # three rows of the first sequence
+    K.kv_append_mxfp4(k0.to(DEV), v0.to(DEV), *cache, lens)
+    o = K.flash_attention_cache_mxfp4(q0.to(DEV), *cache, lens, 0.1, G, advance=True)
+
+    def host():
+        c.kc, c.ks, c.vc, c.vs = (t.cpu() for t in cache)
+        return c
+    check_attention(o, q0, host(), torch.tensor([[3], [0]]) + 1 + torch.arange(20), 0.1)
+    k, v, q = (torch.empty(B, 1, H, D, dtype=torch.bfloat16, device=DEV) for _ in range(3))
+    q = torch.empty(B, H * G, D, dtype=torch.bfloat16, device=DEV)
+
+    def step():
+        K.kv_append_mxfp4(k, v, *cache, lens)
+        return K.decode_attention_mxfp4(q, *cache, lens, 0.1, append=True)
+
+    start = lens.clone()
+    step()  # once eagerly
+    lens.copy_(start)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        k.copy_(rnd(B, 1, H, D, seed=30 + i))
+        v.copy_(rnd(B, 1, H, D, seed=40 + i))
+        qi = rnd(B, H * G, D, seed=50 + i)
+        q.copy_(qi)
+        before = lens.cpu()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(lens.cpu(), before + 1)
+        check_attention(out.unsqueeze(2), qi.unsqueeze(2), host(), (before + 1).view(-1, 1), 0.1)
+
+
+def test_offsets_past_32_bits():
+    """A cache whose last head starts over 4 GiB into the codes."""
+    B, H, D, cap = 2, 4, 128, 9_000_000
+    assert (B * H - 1) * cap * D // 2 > 2 ** 31
+    cache = [torch.zeros(B, H, cap, w, dtype=torch.uint8, device=DEV) for w in (64, 4, 64, 4)]
+    lens = torch.tensor([5, cap - 40], dtype=torch.int32, device=DEV)
+    k, v = rnd(B, 40, H, D, seed=23), rnd(B, 40, H, D, seed=24)
+    K.kv_append_mxfp4(k.to(DEV), v.to(DEV), *cache, lens)
+    back = K.mxfp4_dequantize(cache[0][:, :, cap - 40:], cache[1][:, :, cap - 40:])
+    assert same_bits(back[1].double(), M.values(*M.quantize(k))[1].transpose(0, 1))
+    q = rnd(1, 4, D, seed=25)  # the last head over its last 40 rows alone
+    o = K.decode_attention_mxfp4(q.to(DEV), *(t[1:, 3:, cap - 40:] for t in cache),
+                                 torch.tensor([40], dtype=torch.int32, device=DEV), 0.1)
+    sub = Cache([40], 1, 40, D, seed=0)
+    sub.kc, sub.ks, sub.vc, sub.vs = (t[1:, 3:, cap - 40:].cpu() for t in cache)
+    check_attention(o.unsqueeze(2), q.unsqueeze(2), sub, torch.tensor([[40]]), 0.1)
+    # all rows but these 40 of the last head: zero values
+    full = K.decode_attention_mxfp4(q.to(DEV).repeat(2, 4, 1), *cache, lens, 0.1)
+    assert bool((full == 0).all())
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals():
+    d = dict(device=DEV)
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, **d)
+    u = lambda *s: torch.zeros(*s, dtype=torch.uint8, **d)  # noqa: E731
+    lens = torch.zeros(2, dtype=torch.int32, **d)
+    cache = (u(2, 2, 32, 64), u(2, 2, 32, 4), u(2, 2, 32, 64), u(2, 2, 32, 4))
+    q = torch.zeros(2, 8, 128, dtype=torch.bfloat16, **d)
+    kv = torch.zeros(2, 1, 2, 128, dtype=torch.bfloat16, **d)
+    for bad, exc in [
+        (lambda: K.mxfp4_quantize(x.cpu()), RuntimeError),
+        (lambda: K.mxfp4_quantize(x[:, :48]), ValueError),
+        (lambda: K.mxfp4_quantize(x.half()), TypeError),
+        (lambda: K.mxfp4_dequantize(u(4, 32), u(4, 1)), ValueError),
+        (lambda: K.mxfp4_dequantize(u(4, 32), u(3, 2)), ValueError),
+        (lambda: K.mxfp4_dequantize(u(4, 32).int(), u(4, 2)), TypeError),
+        (lambda: K.mxfp4_dequantize(u(4, 32), u(4, 2), torch.float16), TypeError),
+        (lambda: K.matmul_mxfp4(x, u(8, 16), u(8, 1)), ValueError),
+        (lambda: K.matmul_mxfp4(x.float(), u(8, 32), u(8, 2)), TypeError),
+        (lambda: K.matmul_mxfp4(x, u(8, 32), u(8, 2), bias=x[0, :7]), ValueError),
+        (lambda: K.matmul_mxfp4(x, u(8, 32), u(8, 2), residual=x[:, :7]), ValueError),
+        (lambda: K.matmul_mxfp4(x, u(8, 32), u(8, 2), out=x[:, :7]), ValueError),
+        (lambda: K.kv_append_mxfp4(kv, kv[:, :, :1], *cache, lens), ValueError),
+        (lambda: K.kv_append_mxfp4(kv, kv, *cache, lens.long()), ValueError),
+        (lambda: K.kv_append_mxfp4(kv, kv, *cache[:3], u(2, 2, 31, 4), lens), ValueError),
+        (lambda: K.kv_append_mxfp4(kv[:, :, :1], kv[:, :, :1], *cache, lens), ValueError),
+        (lambda: K.decode_attention_mxfp4(q.float(), *cache, lens, 1.0), TypeError),
+        (lambda: K.decode_attention_mxfp4(q[:, :7], *cache, lens, 1.0), ValueError),
+        (lambda: K.decode_attention_mxfp4(q, *cache, lens[:1], 1.0), ValueError),
+        (lambda: K.decode_attention_mxfp4(q[..., :64], *cache, lens, 1.0), ValueError),
+        (lambda: K.decode_attention_mxfp4(q, *(t[:, :, ::2] for t in cache), lens, 1.0), ValueError),
+        (lambda: K.flash_attention_cache_mxfp4(q.unsqueeze(2), *cache, lens, 1.0, 2), ValueError),
+        (lambda: K.flash_attention_cache_mxfp4(q.unsqueeze(2), *cache, lens, 1.0, 4, max_len=33), ValueError),
+        (lambda: K.flash_attention_cache_mxfp4(q.unsqueeze(2).expand(2, 8, 40, 128), *cache, lens, 1.0, 4),
+         RuntimeError),  # more tokens than the cache has rows
+    ]:
+        with pytest.raises(exc):
+            bad()
+    w = torch.zeros(4, 64, dtype=torch.bfloat16, requires_grad=True, **d)
+    with torch.enable_grad(), pytest.raises(NotImplementedError):
+        K.matmul_mxfp4(w, u(8, 32), u(8, 2))
+    with pytest.raises(_lib.Q3Error):  # head dim 32: the cache can be written, not attended to
+        K.decode_attention_mxfp4(q[..., :32], u(2, 2, 32, 16), u(2, 2, 32, 1), u(2, 2, 32, 16), u(2, 2, 32, 1), lens, 1.0)

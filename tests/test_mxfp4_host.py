@@ -1,0 +1,99 @@
+"""MXFP4 without a GPU: the float64 oracle against the format's definition, and the C entry points' refusals, which
+come before any device work."""
+import ctypes
+
+import pytest
+import torch
+
+from oracle import mxfp4 as M
+from qwen3_5_vl_cuda_custom_amd import _lib
+
+FAKE = 0x100000  # a non-null, aligned address that validation never dereferences
+
+
+@pytest.fixture(scope="module")
+def L():
+    return _lib.lib()
+
+
+def test_oracle_rounds_to_the_nearest_code_ties_to_even():
+    x = torch.zeros(1, 32, dtype=torch.float64)
+    x[0, :15] = torch.tensor([4.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 5.01, 7.9, -0.2, -0.26, -6.5, 1.0, 3.0])
+    codes, scales = M.quantize(x)
+    want = [4.0, 0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, 6.0, 6.0, -0.0, -0.5, -6.0, 1.0, 3.0]
+    assert int(scales) == 127 and M.values(codes, scales)[0, :15].tolist() == want
+    again = M.quantize(M.values(codes, scales))  # what a code stands for keeps its code
+    assert torch.equal(again[0], codes) and torch.equal(again[1], scales)
+
+
+def test_oracle_scales():
+    x = torch.zeros(6, 32, dtype=torch.float64)
+    x[1, 3], x[2, 0], x[3, 9] = -2.0 ** 20, 2.0 ** -130, 1.999
+    x[4, 1], x[5, 2] = float("inf"), float("nan")
+    codes, scales = M.quantize(x)
+    assert scales.flatten().tolist() == [0, 145, 0, 125, 255, 255]
+    assert torch.isnan(M.values(codes, scales)[4:]).all() and not codes[4:].any()
+
+
+def i64(*v):
+    return (ctypes.c_int64 * len(v))(*v)
+
+
+def test_quantize_refusals(L):
+    q = L.q3_mxfp4_quantize
+    assert q(None, FAKE, FAKE, 4, 64, 64, 1, None) == -1
+    assert q(FAKE, FAKE, FAKE, 4, 48, 48, 1, None) == -2
+    assert q(FAKE, FAKE, FAKE, 4, 64, 32, 1, None) == -2
+    assert q(FAKE, FAKE, FAKE, 4, 64, 64, 2, None) == -3
+    assert q(FAKE + 2, FAKE, FAKE, 4, 64, 64, 1, None) == -4
+    assert q(FAKE, FAKE, FAKE, 4, 64, 68, 1, None) == -4
+    assert q(FAKE, FAKE, FAKE, 0, 64, 64, 1, None) == 0
+    d = L.q3_mxfp4_dequantize
+    assert d(FAKE, FAKE, FAKE, 1, 1, 48, i64(0, 0, 0, 0), 1, None) == -2
+    assert d(FAKE, FAKE, FAKE, 1, 1, 64, None, 1, None) == -1
+    assert d(FAKE, FAKE, FAKE, 300, 300, 64, i64(0, 0, 0, 0), 1, None) == -5
+    assert d(FAKE, FAKE, FAKE, 2, 1, 64, i64(33, 0, 0, 0), 1, None) == -4
+    assert d(FAKE, FAKE, FAKE, 2, 1, 0, i64(0, 0, 0, 0), 1, None) == 0
+
+
+def test_matmul_refusals(L):
+    def mm(M_=4, N=64, K=64, x=FAKE, w=FAKE, ldx=64, ldw=32, lds=2, ldr=0, ldc=64, dt=1, ws=None, nws=0, res=None):
+        return L.q3_matmul_mxfp4(x, w, FAKE, None, res, FAKE, M_, N, K, ldx, ldw, lds, ldr, ldc, dt, ws, nws, None)
+    assert mm(x=None) == -1
+    assert mm(K=48) == -2 and mm(K=0) == -2 and mm(ldw=16) == -2 and mm(lds=1) == -2 and mm(ldc=63) == -2
+    assert mm(res=FAKE, ldr=60) == -2
+    assert mm(dt=0) == -3
+    assert mm(x=FAKE + 2) == -4 and mm(w=FAKE + 4) == -4 and mm(ldw=40) == -4
+    need = L.q3_matmul_mxfp4_workspace_bytes(100, 64, 64)
+    assert need > 0 and mm(M_=100, ws=FAKE, nws=need - 1) == -6 and mm(M_=100) == -6
+    assert mm(M_=0) == 0 and mm(N=0) == 0
+
+
+def test_cache_refusals(L):
+    st = i64(*([128] * 14))
+
+    def append(k=FAKE, lens=FAKE, B=2, S=1, H=2, D=128, cap=32, s=st, dt=1):
+        return L.q3_kv_append_mxfp4(k, FAKE, FAKE, FAKE, FAKE, FAKE, lens, B, S, H, D, cap, s, dt, None)
+    assert append(k=None) == -1 and append(lens=None) == -1 and append(s=None) == -1
+    assert append(B=-1) == -2 and append(H=0) == -2 and append(B=1 << 20, S=1 << 20) == -2
+    assert append(dt=3) == -3
+    assert append(D=48) == -5 and append(D=512) == -5
+    assert append(k=FAKE + 4) == -4 and append(s=i64(4, *([128] * 13))) == -4
+    assert append(B=0) == 0 and append(S=0) == 0
+
+    def decode(q=FAKE, B=2, Hq=8, H=2, D=128, cap=32, s=st, dt=1, nws=1 << 30, ws=FAKE, kc=FAKE):
+        return L.q3_decode_attention_mxfp4(q, kc, FAKE, FAKE, FAKE, FAKE, 0, FAKE, B, Hq, H, D, cap, s, 1.0, dt, ws,
+                                           nws, None)
+    assert decode(q=None) == -1 and decode(s=None) == -1
+    assert decode(Hq=7) == -2 and decode(cap=-1) == -2
+    assert decode(dt=0) == -3
+    assert decode(kc=FAKE + 8) == -4 and decode(s=i64(4, *([128] * 13))) == -4
+    assert decode(D=96) == -5 and decode(B=1025) == -5
+    assert decode(nws=100) == -6 and decode(ws=None) == -6
+    assert decode(B=0) == 0
+
+    def chunk(Sq=64, ml=128, nws=1 << 30, ws=FAKE):
+        return L.q3_flash_attention_cache_mxfp4(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 2, 8, 2, Sq, 128, ml, st,
+                                                1.0, 0, 1, ws, nws, None)
+    assert chunk(Sq=129) == -2 and chunk(nws=0) == -6 and chunk(ws=None) == -6
+    assert chunk(Sq=0) == 0
