@@ -6,39 +6,35 @@ their negatives), each block with one power-of-two scale held as its exponent (E
 255 for NaN). `codes` (..., K / 2) uint8 holds value 2j in the low and 2j + 1 in the high half of byte j, `scales`
 (..., K / 32) uint8 the blocks' scales. Everything a code stands for is exact in bf16, so the products and the
 attention below lose nothing beyond the quantisation itself and the bf16 arithmetic of their unquantised forms.
+
+Inference only. All tensors of a call must be on the current device, whose current stream it uses. The kernels of a
+decode step take a few microseconds each, so the checks here are written for their own time.
 """
 from __future__ import annotations
+
+from struct import Struct
 
 import torch
 
 from .. import _lib
-from ._common import mfma_operand, require_device, require_no_grad, require_same_dtype
+from ._common import mfma_operand, require_device, require_no_grad
 
 MX_BLOCK = 32
+_U8, _BF16, _F32 = torch.uint8, torch.bfloat16, torch.float32
+_i64x4, _i64x14 = Struct("4q").pack, Struct("14q").pack
 
 
-def _one_device(op: str, *tensors: torch.Tensor | None) -> None:
-    """All on the current GPU, whose current stream the call uses."""
-    ts = [t for t in tensors if t is not None]
-    require_device(op, *ts)
-    cur = torch.cuda.current_device()
-    if any(t.device.index != cur for t in ts):
-        raise RuntimeError(f"{op}: tensors must be on the current device (cuda:{cur})")
+def _off_device(op: str, *tensors: torch.Tensor | None) -> None:
+    """Raise for tensors that are not all on the current device."""
+    require_device(op, *tensors)
+    raise RuntimeError(f"{op}: tensors must be on the current device (cuda:{torch.cuda.current_device()})")
 
 
-def _check(op: str, *tensors: torch.Tensor | None) -> None:
-    ts = [t for t in tensors if t is not None]
-    _one_device(op, *ts)
-    require_no_grad(op, *ts)
-
-
-def _check_pair(op: str, codes: torch.Tensor, scales: torch.Tensor) -> None:
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
-        raise TypeError(f"{op}: codes and scales must be uint8, got {codes.dtype} and {scales.dtype}")
-    if (codes.dim() < 1 or codes.dim() != scales.dim() or codes.shape[:-1] != scales.shape[:-1]
-            or codes.shape[-1] != scales.shape[-1] * (MX_BLOCK // 2)):
-        raise ValueError(f"{op}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} must be (..., K / 2) and "
-                         "(..., K / 32)")
+def _pair_error(op: str, codes: torch.Tensor, scales: torch.Tensor) -> Exception:
+    if codes.dtype != _U8 or scales.dtype != _U8:
+        return TypeError(f"{op}: codes and scales must be uint8, got {codes.dtype} and {scales.dtype}")
+    return ValueError(f"{op}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} must be (..., K / 2) and "
+                      "(..., K / 32)")
 
 
 def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -48,44 +44,69 @@ def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     zeros); a value over the scale rounds to the nearest code, ties to the even one, and saturates at 6. A block
     that holds an infinity or a NaN reads back as NaN.
     """
-    _check("mxfp4_quantize", x)
+    dev = x.get_device()
+    if dev < 0 or dev != _lib.current_device():
+        _off_device("mxfp4_quantize", x)
+    require_no_grad("mxfp4_quantize", x)
     dt = _lib.dtype_code(x.dtype)
-    if x.dim() < 1 or x.shape[-1] % MX_BLOCK:
-        raise ValueError(f"mxfp4_quantize: the last dim of {tuple(x.shape)} must be a multiple of {MX_BLOCK}")
-    K = x.shape[-1]
-    codes = torch.empty((*x.shape[:-1], K // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], K // MX_BLOCK), dtype=torch.uint8, device=x.device)
-    if x.numel() == 0:
+    shape = x.shape
+    if not shape or shape[-1] % MX_BLOCK:
+        raise ValueError(f"mxfp4_quantize: the last dim of {tuple(shape)} must be a multiple of {MX_BLOCK}")
+    K = shape[-1]
+    codes = x.new_empty((*shape[:-1], K // 2), dtype=_U8)
+    scales = x.new_empty((*shape[:-1], K // MX_BLOCK), dtype=_U8)
+    n = x.numel()
+    if n == 0:
         return codes, scales
-    x2 = x.reshape(-1, K)
-    if x2.stride(-1) != 1 or x2.data_ptr() % 16 or x2.stride(0) * x2.element_size() % 16:
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    _lib.call("q3_mxfp4_quantize", x2.data_ptr(), codes.data_ptr(), scales.data_ptr(), x2.shape[0], K,
-              max(x2.stride(0), K), dt, _lib.stream())
+    ld = K
+    if x.data_ptr() % 16 or not x.is_contiguous():
+        x = x.reshape(-1, K)
+        ld = x.stride(0) if n > K else K
+        if x.stride(1) != 1 or ld < K or x.data_ptr() % 16 or ld * x.element_size() % 16:
+            x, ld = x.clone(memory_format=torch.contiguous_format), K
+    _lib.call("q3_mxfp4_quantize", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), n // K, K, ld, dt,
+              _lib.raw_stream(dev))
     return codes, scales
 
 
 def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values (..., K) in bf16 or fp32, both exact (blocks of scale 255: NaN). Contiguous tensors
-    and (B, H, rows, ...) slices of a cache are read in place; other views are copied first."""
-    _check("mxfp4_dequantize", codes, scales)
-    _check_pair("mxfp4_dequantize", codes, scales)
+    """The values (..., K) in bf16 or fp32, both exact (blocks of scale 255: NaN; the scales past the type's range,
+    which mxfp4_quantize never makes, give infinities). Contiguous tensors and (B, H, rows, ...) slices of a cache
+    are read in place; other views are copied first."""
+    op = "mxfp4_dequantize"
+    dev = codes.get_device()
+    if dev < 0 or dev != _lib.current_device() or scales.get_device() != dev:
+        _off_device(op, codes, scales)
     dt = _lib.dtype_code(dtype)
-    y = torch.empty((*codes.shape[:-1], codes.shape[-1] * 2), dtype=dtype, device=codes.device)
-    if y.numel() == 0:
+    shape, sshape = codes.shape, scales.shape
+    if (codes.dtype != _U8 or scales.dtype != _U8 or not shape or shape[:-1] != sshape[:-1]
+            or shape[-1] != sshape[-1] * (MX_BLOCK // 2)):
+        raise _pair_error(op, codes, scales)
+    y = codes.new_empty((*shape[:-1], shape[-1] * 2), dtype=dtype)
+    n = y.numel()
+    if n == 0:
         return y
-    n, st = (1, 1), (0, 0, 0, 0)
-    if codes.is_contiguous() and scales.is_contiguous() and codes.data_ptr() % 4 == 0:
-        pass
-    elif (codes.dim() >= 3 and codes[0, 0].is_contiguous() and scales[0, 0].is_contiguous()
-          and codes.shape[0] * codes.shape[1] <= 65535 and codes.data_ptr() % 4 == 0
-          and codes.stride(0) % 4 == 0 and codes.stride(1) % 4 == 0):
-        n, st = codes.shape[:2], (*codes.stride()[:2], *scales.stride()[:2])
-    else:
-        codes, scales = (t.clone(memory_format=torch.contiguous_format) for t in (codes, scales))
-    _lib.call("q3_mxfp4_dequantize", codes.data_ptr(), scales.data_ptr(), y.data_ptr(), *n,
-              y.numel() // (n[0] * n[1]), _lib.i64s(*st), dt, _lib.stream())
+    n0, n1, st = 1, 1, (0, 0, 0, 0)
+    if not (codes.is_contiguous() and scales.is_contiguous() and codes.data_ptr() % 4 == 0):
+        cs = codes.stride()
+        if (len(shape) >= 3 and shape[0] * shape[1] <= 65535 and codes.data_ptr() % 4 == 0 and cs[0] % 4 == 0
+                and cs[1] % 4 == 0 and codes[0, 0].is_contiguous() and scales[0, 0].is_contiguous()):
+            n0, n1, st = shape[0], shape[1], (*cs[:2], *scales.stride()[:2])
+        else:
+            codes, scales = (t.clone(memory_format=torch.contiguous_format) for t in (codes, scales))
+    _lib.call("q3_mxfp4_dequantize", codes.data_ptr(), scales.data_ptr(), y.data_ptr(), n0, n1, n // (n0 * n1),
+              _i64x4(*st), dt, _lib.raw_stream(dev))
     return y
+
+
+def _rows(op: str, t: torch.Tensor, n: int) -> tuple[torch.Tensor, int]:
+    """t (..., n) as rows of contiguous elements and their stride."""
+    if t.is_contiguous():
+        return t, n
+    t = t.reshape(-1, n)
+    if n > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < n:
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else n
 
 
 def matmul_mxfp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None,
@@ -93,65 +114,91 @@ def matmul_mxfp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bia
     """matmul with the weight (N, K) held in MXFP4: x·Wᵀ (+ bias) (+ residual), x (..., K) bf16, one rounding.
 
     `out`, when given: (..., N) whose rows have one stride and contiguous elements, written in place (a column
-    slice of a wider buffer). Inference only.
+    slice of a wider buffer).
     """
     op = "matmul_mxfp4"
-    _check(op, x, codes, scales, bias, residual, out)
-    _check_pair(op, codes, scales)
-    if x.dtype != torch.bfloat16:
+    dev = x.get_device()
+    if dev < 0 or dev != _lib.current_device() or codes.get_device() != dev or scales.get_device() != dev:
+        _off_device(op, x, codes, scales)
+    for t in (bias, residual, out):
+        if t is not None:
+            if t.get_device() != dev:
+                _off_device(op, t)
+            if t.dtype != _BF16:
+                raise TypeError(f"{op}: dtype mismatch ({t.dtype} vs {_BF16})")
+    require_no_grad(op, x, bias, residual, out)
+    if x.dtype != _BF16:
         raise TypeError(f"{op}: x must be bfloat16, got {x.dtype}")
-    require_same_dtype(op, x, bias, residual, out)
-    if codes.dim() != 2 or x.dim() < 1 or codes.shape[1] * 2 != x.shape[-1] or x.shape[-1] == 0:
-        raise ValueError(f"{op}: codes {tuple(codes.shape)} do not match x {tuple(x.shape)}")
-    N, K = codes.shape[0], x.shape[-1]
-    shape = (*x.shape[:-1], N)
+    xs, ws, ss = x.shape, codes.shape, scales.shape
+    if (codes.dtype != _U8 or scales.dtype != _U8 or len(ws) != len(ss) or ws[:-1] != ss[:-1]
+            or ws[-1] != ss[-1] * (MX_BLOCK // 2)):
+        raise _pair_error(op, codes, scales)
+    if len(ws) != 2 or not xs or ws[1] * 2 != xs[-1] or xs[-1] == 0:
+        raise ValueError(f"{op}: codes {tuple(ws)} do not match x {tuple(xs)}")
+    N, K = ws[0], xs[-1]
+    shape = (*xs[:-1], N)
     if bias is not None and bias.shape != (N,):
         raise ValueError(f"{op}: bias {tuple(bias.shape)} != ({N},)")
     if residual is not None and residual.shape != shape:
         raise ValueError(f"{op}: residual {tuple(residual.shape)} != output {shape}")
-    if out is not None and (out.shape != shape or (N > 1 and out.stride(-1) != 1)):
-        raise ValueError(f"{op}: out {tuple(out.shape)} must be {shape} with contiguous elements")
-    y = out if out is not None else torch.empty(shape, dtype=x.dtype, device=x.device)
-    if y.numel() == 0:
+    if out is None:
+        y, ldy = x.new_empty(shape), N
+    else:
+        if out.shape != shape or (N > 1 and out.stride(-1) != 1):
+            raise ValueError(f"{op}: out {tuple(out.shape)} must be {shape} with contiguous elements")
+        y, ldy = out, N
+        if not out.is_contiguous() and out.numel() > N:
+            ldy = out.view(-1, N).stride(0)
+            if ldy < N:
+                raise ValueError(f"{op}: the rows of out overlap")
+    M = x.numel() // K
+    if M == 0 or N == 0:
         return y
-    x2 = x.reshape(-1, K)
-    x2 = mfma_operand(op, x2 if x2.stride(-1) == 1 else x2.contiguous())
-    y2 = y.view(-1, N)
-    r2 = residual.reshape(-1, N) if residual is not None else None
-    if r2 is not None and r2.stride(-1) != 1:
-        r2 = r2.contiguous()
-    M = x2.shape[0]
+    x2, ldx = _rows(op, x, K)
+    if x2.data_ptr() % 16 or ldx % 8:
+        x2, ldx = mfma_operand(op, x2.view(-1, K)), K
+    r2, ldr = _rows(op, residual, N) if residual is not None else (None, 0)
     if not codes.is_contiguous() or codes.data_ptr() % 16:
         codes = codes.clone(memory_format=torch.contiguous_format)
-    scales = scales.contiguous()
-    b = bias.contiguous() if bias is not None else None
-    ws, nws = _lib.workspace(_lib.lib().q3_matmul_mxfp4_workspace_bytes(M, N, K), x.device)
-    _lib.call("q3_matmul_mxfp4", x2.data_ptr(), codes.data_ptr(), scales.data_ptr(), _lib.ptr(b), _lib.ptr(r2),
-              y2.data_ptr(), M, N, K, max(x2.stride(0), K), K // 2, K // MX_BLOCK,
-              max(r2.stride(0), N) if r2 is not None else 0, max(y2.stride(0), N), _lib.Q3_BF16, _lib.ptr(ws), nws,
-              _lib.stream())
+    if not scales.is_contiguous():
+        scales = scales.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    lib = _lib.lib()
+    nws = lib.q3_matmul_mxfp4_workspace_bytes(M, N, K)
+    ws_ = x.new_empty(nws, dtype=_U8) if nws else None
+    _lib.call("q3_matmul_mxfp4", x2.data_ptr(), codes.data_ptr(), scales.data_ptr(), _lib.ptr(bias), _lib.ptr(r2),
+              y.data_ptr(), M, N, K, ldx, K // 2, K // MX_BLOCK, ldr, ldy, _lib.Q3_BF16, _lib.ptr(ws_), nws,
+              _lib.raw_stream(dev))
     return y
 
 
-def _check_cache(op: str, k_codes, k_scales, v_codes, v_scales, kv_lens, B: int, D: int) -> tuple[int, int]:
-    """Checks a (B, Hkv, cap, D) cache in MXFP4 and its lengths; returns (Hkv, cap)."""
+def _check_cache(op: str, dev: int, k_codes, k_scales, v_codes, v_scales, kv_lens, B: int, D: int) -> tuple:
+    """Checks a (B, Hkv, cap, D) cache in MXFP4 and its lengths; returns Hkv, cap and the strides [b, h] of the four
+    tensors."""
+    if dev < 0 or dev != _lib.current_device() or kv_lens.get_device() != dev:
+        _off_device(op, kv_lens, k_codes)
+    shape, lead = k_codes.shape, None
+    st = []
     for c, s in ((k_codes, k_scales), (v_codes, v_scales)):
-        _check_pair(op, c, s)
-        if c.dim() != 4 or c.shape[0] != B or c.shape[3] * 2 != D or c.shape != k_codes.shape:
+        if c.get_device() != dev or s.get_device() != dev:
+            _off_device(op, c, s)
+        cs, ss = c.shape, s.shape
+        if (c.dtype != _U8 or s.dtype != _U8 or len(cs) != 4 or len(ss) != 4 or cs[:3] != ss[:3]
+                or cs[3] != ss[3] * (MX_BLOCK // 2)):
+            raise _pair_error(op, c, s)
+        if cs != shape or cs[0] != B or cs[3] * 2 != D:
             raise ValueError(f"{op}: cache codes {tuple(k_codes.shape)} and {tuple(v_codes.shape)} must be "
                              f"({B}, Hkv, cap, {D // 2})")
-        for t in (c, s):
-            if t.numel() and (t.stride(3) != 1 or (t.shape[2] > 1 and t.stride(2) != t.shape[3])):
-                raise ValueError(f"{op}: the rows of a cache head must be packed")
-        if c.numel() and (c.data_ptr() % 16 or c.stride(0) % 16 or c.stride(1) % 16):
+        ct, s_t = c.stride(), s.stride()
+        if cs[2] > 1 and (ct[2] != cs[3] or s_t[2] != ss[3]) or ct[3] != 1 or ss[3] > 1 and s_t[3] != 1:
+            raise ValueError(f"{op}: the rows of a cache head must be packed")
+        if c.data_ptr() % 16 or ct[0] % 16 or ct[1] % 16:
             raise ValueError(f"{op}: the cache codes must be 16-byte aligned")
+        st += (ct[0], ct[1], s_t[0], s_t[1])
     if kv_lens.dtype != torch.int32 or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
         raise ValueError(f"{op}: kv_lens must be a contiguous int32 ({B},) device tensor")
-    return k_codes.shape[1], k_codes.shape[2]
-
-
-def _cache_strides(*ts: torch.Tensor) -> list[int]:
-    return [s for t in ts for s in (t.stride(0), t.stride(1))]
+    return shape[1], shape[2], st
 
 
 def kv_append_mxfp4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
@@ -163,39 +210,48 @@ def kv_append_mxfp4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_s
     dropped at or past cap. kv_lens is left as it is (the attention that follows advances it).
     """
     op = "kv_append_mxfp4"
-    _check(op, k, v, k_codes, k_scales, v_codes, v_scales, kv_lens)
+    dev, shape = k.get_device(), k.shape
+    if v.get_device() != dev:
+        _off_device(op, k, v)
+    require_no_grad(op, k, v)
     dt = _lib.dtype_code(k.dtype)
-    require_same_dtype(op, k, v)
-    if k.dim() != 4 or k.shape != v.shape:
-        raise ValueError(f"{op}: k {tuple(k.shape)} and v {tuple(v.shape)} must be (B, S, Hkv, D)")
-    B, S, Hkv, D = k.shape
-    heads, cap = _check_cache(op, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D)
+    if k.dtype != v.dtype:
+        raise TypeError(f"{op}: dtype mismatch ({v.dtype} vs {k.dtype})")
+    if len(shape) != 4 or shape != v.shape:
+        raise ValueError(f"{op}: k {tuple(shape)} and v {tuple(v.shape)} must be (B, S, Hkv, D)")
+    B, S, Hkv, D = shape
+    heads, cap, st = _check_cache(op, dev, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D)
     if heads != Hkv:
         raise ValueError(f"{op}: {Hkv} KV heads for a cache of {heads}")
     if k.numel() == 0 or cap == 0:
         return
-    es = k.element_size()
-    k, v = (t if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(t.stride(i) * es % 16 == 0 for i in range(3))
-            else t.clone(memory_format=torch.contiguous_format) for t in (k, v))
+    unit = 16 // k.element_size()
+    ks, vs = k.stride(), v.stride()
+    if k.data_ptr() % 16 or ks[3] != 1 or ks[0] % unit or ks[1] % unit or ks[2] % unit:
+        k = k.clone(memory_format=torch.contiguous_format)
+        ks = k.stride()
+    if v.data_ptr() % 16 or vs[3] != 1 or vs[0] % unit or vs[1] % unit or vs[2] % unit:
+        v = v.clone(memory_format=torch.contiguous_format)
+        vs = v.stride()
     _lib.call("q3_kv_append_mxfp4", k.data_ptr(), v.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(),
               v_codes.data_ptr(), v_scales.data_ptr(), kv_lens.data_ptr(), B, S, Hkv, D, cap,
-              _lib.i64s(*k.stride()[:3], *v.stride()[:3], *_cache_strides(k_codes, k_scales, v_codes, v_scales)), dt,
-              _lib.stream())
+              _i64x14(*ks[:3], *vs[:3], *st), dt, _lib.raw_stream(dev))
 
 
-def _query(op: str, q: torch.Tensor) -> torch.Tensor:
-    if q.dtype != torch.bfloat16:
+def _query(op: str, q: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
+    """q as the kernels read it, and the output."""
+    require_no_grad(op, q, out)
+    if q.dtype != _BF16:
         raise TypeError(f"{op}: q must be bfloat16, got {q.dtype}")
-    return mfma_operand(op, q if q.stride(-1) == 1 else q.contiguous())
-
-
-def _output(op: str, q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = mfma_operand(op, q if q.stride(-1) == 1 else q.contiguous())
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if (out.shape != q.shape or out.dtype != q.dtype or out.data_ptr() % 16 or out.stride(-1) != 1
-            or any(out.stride(i) % 8 for i in range(out.dim() - 1))):
-        raise ValueError(f"{op}: out must be {tuple(q.shape)} {q.dtype} with a contiguous head dim, 16-byte aligned")
-    return out
+        return q, q.new_empty(q.shape)
+    if (out.get_device() != q.get_device() or out.shape != q.shape or out.dtype != _BF16 or out.data_ptr() % 16
+            or out.stride(-1) != 1 or any(out.stride(i) % 8 for i in range(out.dim() - 1))):
+        raise ValueError(f"{op}: out must be {tuple(q.shape)} {_BF16} on q's device with a contiguous head dim, 16-byte "
+                         "aligned")
+    return q, out
 
 
 def decode_attention_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
@@ -209,23 +265,23 @@ def decode_attention_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: tor
     Hq, D); an empty sequence gives zeros.
     """
     op = "decode_attention_mxfp4"
-    _check(op, q, k_codes, k_scales, v_codes, v_scales, kv_lens, out)
     if q.dim() == 4 and q.shape[2] == 1:
         q = q[:, :, 0]
     if q.dim() != 3:
         raise ValueError(f"{op}: q must be (B, Hq, D), got {tuple(q.shape)}")
-    q = _query(op, q)
+    dev = q.get_device()
     B, Hq, D = q.shape
-    Hkv, cap = _check_cache(op, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D)
+    Hkv, cap, st = _check_cache(op, dev, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D)
     if Hkv == 0 or Hq % Hkv:
         raise ValueError(f"{op}: {Hq} query heads for {Hkv} KV heads")
-    o = _output(op, q, out)
-    ws, nws = _lib.workspace(_lib.lib().q3_decode_attention_mxfp4_workspace_bytes(B, Hq, Hkv, D), q.device)
+    q, o = _query(op, q, out)
+    nws = _lib.lib().q3_decode_attention_mxfp4_workspace_bytes(B, Hq, Hkv, D)
+    ws = q.new_empty(nws, dtype=_U8)
+    qs, os = q.stride(), o.stride()
     _lib.call("q3_decode_attention_mxfp4", q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
-              v_scales.data_ptr(), kv_lens.data_ptr(), int(bool(append)), o.data_ptr(), B, Hq, Hkv, D, cap,
-              _lib.i64s(q.stride(0), q.stride(1), 0, o.stride(0), o.stride(1), 0,
-                        *_cache_strides(k_codes, k_scales, v_codes, v_scales)), float(scale), _lib.Q3_BF16,
-              _lib.ptr(ws), nws, _lib.stream())
+              v_scales.data_ptr(), kv_lens.data_ptr(), 1 if append else 0, o.data_ptr(), B, Hq, Hkv, D, cap,
+              _i64x14(qs[0], qs[1], 0, os[0], os[1], 0, *st), scale, _lib.Q3_BF16, ws.data_ptr(), nws,
+              _lib.raw_stream(dev))
     return o
 
 
@@ -240,22 +296,22 @@ def flash_attention_cache_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales
     `max_len` bounds every kv_lens[b] + Sq (default: cap) and sizes the workspace of a longer chunk.
     """
     op = "flash_attention_cache_mxfp4"
-    _check(op, q, k_codes, k_scales, v_codes, v_scales, kv_lens, out)
     if q.dim() != 4:
         raise ValueError(f"{op}: q must be (B, Hq, Sq, D), got {tuple(q.shape)}")
-    q = _query(op, q)
+    dev = q.get_device()
     B, Hq, Sq, D = q.shape
-    Hkv, cap = _check_cache(op, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D)
+    Hkv, cap, st = _check_cache(op, dev, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D)
     if Hkv * num_kv_groups != Hq:
         raise ValueError(f"{op}: Hq={Hq} != Hkv={Hkv} * num_kv_groups={num_kv_groups}")
     ml = cap if max_len is None else int(max_len)
     if not 0 <= ml <= cap:
         raise ValueError(f"{op}: max_len {ml} must lie in [0, {cap}]")
-    o = _output(op, q, out)
-    ws, nws = _lib.workspace(_lib.lib().q3_flash_attention_cache_mxfp4_workspace_bytes(B, Hq, Hkv, Sq, D, ml), q.device)
+    q, o = _query(op, q, out)
+    nws = _lib.lib().q3_flash_attention_cache_mxfp4_workspace_bytes(B, Hq, Hkv, Sq, D, ml)
+    ws = q.new_empty(nws, dtype=_U8)
+    qs, os = q.stride(), o.stride()
     _lib.call("q3_flash_attention_cache_mxfp4", q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(),
               v_codes.data_ptr(), v_scales.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), B, Hq, Hkv, Sq, D, ml,
-              _lib.i64s(q.stride(0), q.stride(1), q.stride(2), o.stride(0), o.stride(1), o.stride(2),
-                        *_cache_strides(k_codes, k_scales, v_codes, v_scales)), float(scale), int(bool(advance)),
-              _lib.Q3_BF16, _lib.ptr(ws), nws, _lib.stream())
+              _i64x14(*qs[:3], *os[:3], *st), scale, 1 if advance else 0, _lib.Q3_BF16, ws.data_ptr(), nws,
+              _lib.raw_stream(dev))
     return o
