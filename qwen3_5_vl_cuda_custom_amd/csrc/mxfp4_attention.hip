@@ -38,8 +38,9 @@ using namespace q3;
 constexpr int kUnit = 32;        // rows of a unit
 constexpr int kMaxBatch = 1024;  // sequences (their unit counts live in LDS)
 constexpr int kCols = 16;        // MFMA columns
-constexpr int kWavesPerBlock = 8;
-constexpr int kBlocks = 512;
+constexpr int kWavesPerBlock = 12;  // three per SIMD, one block per CU
+constexpr int kBlocks = 256;
+constexpr int kSlots = 2;  // ring slots of a wave: the unit at hand and the next
 constexpr int kWaves = kBlocks * kWavesPerBlock;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.0f;  // log2 units the running max may lag behind
@@ -74,129 +75,163 @@ __device__ __forceinline__ int rows_of(const MxAttn& p, int b) {
   return (int)min(max((int64_t)p.lens[b] + p.len_add + p.Sq - 1, (int64_t)0), (int64_t)p.cap);
 }
 
-// Exclusive prefix of the sequences' unit counts in s_pre[0..B], their rows in s_len.
-__device__ void unit_prefix(const MxAttn& p, int* s_pre, int* s_len, int* s_sum) {
-  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, wv = tid >> 6;
-  const int per = (p.B + nt - 1) / nt;
-  int local = 0;
-  for (int i = 0; i < per; ++i) {
-    const int b = tid * per + i;
-    if (b < p.B) {
-      const int n = rows_of(p, b);
-      s_len[b] = n;
-      local += (n + kUnit - 1) / kUnit;
-    }
-  }
-  int incl = local;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int v = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 63) s_sum[wv] = incl;
-  __syncthreads();
-  int run = incl - local;
-  for (int i = 0; i < wv; ++i) run += s_sum[i];
-  for (int i = 0; i < per; ++i) {
-    const int b = tid * per + i;
-    if (b < p.B) {
-      s_pre[b] = run;
-      run += (s_len[b] + kUnit - 1) / kUnit;
-    }
-  }
-  if (tid == nt - 1) s_pre[p.B] = run;
-  __syncthreads();
-}
+__device__ __forceinline__ int units_of(const MxAttn& p, int b) { return (rows_of(p, b) + kUnit - 1) / kUnit; }
 
-// Unit u belongs to active wave ((u + 1) * n - 1) / U, n = min(U, waves) of them.
-__device__ __forceinline__ int wave_of(int64_t u, int64_t U) {
-  const int64_t n = min<int64_t>(U, kWaves);
-  return (int)(((u + 1) * n - 1) / U);
-}
+// U units over n = min(U, kWaves) waves: the first U % n take one more than the others.
+struct Split {
+  int n, q, r;
+  __device__ __forceinline__ explicit Split(int U) : n(min(U, kWaves)), q(U <= kWaves ? 1 : U / kWaves), r(U <= kWaves ? 0 : U % kWaves) {}
+  __device__ __forceinline__ int first(int w) const { return w * q + min(w, r); }
+  __device__ __forceinline__ int wave_of(int u) const {
+    const int big = r * (q + 1);
+    return u < big ? u / (q + 1) : r + (u - big) / q;
+  }
+};
 
 struct Cursor {
   int b, hs, tile, nb;  // sequence, KV head and column set, tile, tiles of the sequence
 };
 
-// LDS element of value d of row r (0..31) in a wave's V tile. A row's 16-byte
-// chunk c sits at slot c ^ swizzle(r), so that the 16 rows of a write (one chunk
-// each) and of a transposed read (two neighbouring chunks each) use all banks.
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(v, o, 64);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+
+// Over the lanes l % 16 = c, whose l / 16 hold the same column.
+__device__ __forceinline__ float max4(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  x = fmaxf(__builtin_bit_cast(float, a[0]), __builtin_bit_cast(float, a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, b[0]), __builtin_bit_cast(float, b[1]));
+}
+
+// LDS element of value d of row r (0..15) of the V rows being transposed. A row's
+// 16-byte chunk c sits at slot c ^ swizzle(r), so that the 16 rows of a write (one
+// chunk each) and of a transposed read (two neighbouring chunks each) use all banks.
 template <int D>
 __device__ __forceinline__ int v_at(int r, int d) {
-  const int sw = D == 128 ? (((r & 7) << 1) | ((r >> 3) & 1)) : (r & 7);
+  const int sw = D == 128 ? (((r & 7) << 1) | (r >> 3)) : (r & 7);
   return r * D + ((((d >> 3) ^ sw) << 3) | (d & 7));
 }
 
+__device__ __forceinline__ short4v read_tr16(const bf16* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (short4v __attribute__((address_space(3)))*)(reinterpret_cast<uintptr_t>(p)));
+}
+
+// LDS of a wave: kSlots slots, each the unit's codes as the lanes read them (K then
+// V, 32 rows) and a word with the scales of each K and each V row. Once those are in
+// registers, the slot holds 16 rows of V in bf16 at a time.
 template <int D>
-__global__ __launch_bounds__(64 * kWavesPerBlock, 2) void mx_decode_kernel(const MxAttn p) {
+struct WaveLds {
+  static constexpr int kCodes = kUnit * D / 2;  // bytes of K's codes
+  static constexpr int kSlot = 2 * kCodes + 256;
+  static constexpr int kBytes = kSlots * kSlot;
+  static_assert(16 * D * 2 <= 2 * kCodes, "the rows of V being transposed");
+};
+
+template <int D, bool ONCE>
+__global__ __launch_bounds__(64 * kWavesPerBlock) void mx_decode_kernel(const MxAttn p) {
   constexpr int LB = D / 8;         // bytes of codes a lane takes of a row
   constexpr int LW = LB / 4;        // the same in words: A fragments of 8 values
   constexpr int DT = D / 16;        // output tiles along the head dim
   constexpr int NB = D / kMxBlock;  // blocks of a row
+  constexpr int PIECES = D / 64;    // 16-byte loads per lane of a unit's K (or V) codes
+  constexpr int LOADS = 2 * PIECES + 1;
+  typedef WaveLds<D> Lds;
   typedef uint32_t words __attribute__((ext_vector_type(LW)));
-  __shared__ int s_pre[kMaxBatch + 1];
-  __shared__ int s_len[kMaxBatch];
-  __shared__ int s_sum[kWavesPerBlock];
-  __shared__ __attribute__((aligned(16))) bf16 s_v[kWavesPerBlock * kUnit * D];
-
-  unit_prefix(p, s_pre, s_len, s_sum);
-  if (blockIdx.x == 0)  // for the merge, which must not read the lengths
-    for (int i = threadIdx.x; i <= p.B; i += blockDim.x) p.hdr[i] = s_pre[i];
+  __shared__ __attribute__((aligned(1024))) char s_mem[kWavesPerBlock * Lds::kBytes];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int HS = p.Hkv * p.nset;
-  const int64_t U = (int64_t)HS * s_pre[p.B];
-  const int64_t nw = min<int64_t>(U, kWaves);
-  const int w = blockIdx.x * kWavesPerBlock + wave;
-  if (w >= nw) return;
-  const int64_t u0 = (int64_t)w * U / nw, u1 = (int64_t)(w + 1) * U / nw;
-  bf16* tile = s_v + wave * kUnit * D;
+  // Few units go one to a CU; waves that read the same rows (several column sets) share an XCD's L2.
+  const int w = ONCE ? wave * kBlocks + (int)blockIdx.x : xcd_remap(blockIdx.x, kBlocks) * kWavesPerBlock + wave;
 
-  Cursor cc;
-  {
-    int lo = 0, hi = p.B - 1;  // the largest b with HS * s_pre[b] <= u0
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((int64_t)HS * s_pre[mid] <= u0) lo = mid;
-      else hi = mid - 1;
-    }
-    cc.b = lo;
-    cc.nb = s_pre[lo + 1] - s_pre[lo];
-    const int r = (int)(u0 - (int64_t)HS * s_pre[lo]);
-    cc.hs = r / cc.nb;
-    cc.tile = r - cc.hs * cc.nb;
+  // The wave's units: every wave sums the sequences' unit counts by itself (64 a
+  // round), so nothing waits at a barrier.
+  int total = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const int incl = wave_scan(b0 + lane < p.B ? units_of(p, b0 + lane) : 0, lane);
+    if (w == 0 && b0 + lane < p.B) p.hdr[b0 + lane + 1] = total + incl;  // for the merge, which must not read the lengths
+    total += __builtin_amdgcn_readlane(incl, 63);
   }
-  auto advance = [&](Cursor& x) {
-    if (++x.tile < x.nb) return;
+  if (w == 0 && lane == 0) p.hdr[0] = 0;
+  const Split split(total * HS);
+  if (w >= split.n) return;
+  const int u0 = split.first(w), count = split.first(w + 1) - u0;
+  Cursor cc{};
+  for (int b0 = 0, before = 0; b0 < p.B; b0 += 64) {
+    const int n = b0 + lane < p.B ? units_of(p, b0 + lane) : 0;
+    const int incl = before + wave_scan(n, lane);
+    const int at = __popcll(__builtin_amdgcn_ballot_w64(incl * HS <= u0));  // sequences that end at or before u0
+    if (at < 64) {
+      cc.b = b0 + at;
+      cc.nb = __builtin_amdgcn_readlane(n, at);
+      const int r = u0 - (__builtin_amdgcn_readlane(incl, at) - cc.nb) * HS;
+      cc.hs = r / cc.nb;
+      cc.tile = r - cc.hs * cc.nb;
+      break;
+    }
+    before = __builtin_amdgcn_readlane(incl, 63);
+  }
+  char* mem = s_mem + wave * Lds::kBytes;
+  const uint32_t lmem = lds_addr(mem);
+
+  auto advance = [&](Cursor& x) {  // to the next pair
     x.tile = 0;
     if (++x.hs < HS) return;
     x.hs = 0;
     do {
       ++x.b;
-    } while (x.b < p.B && s_pre[x.b + 1] == s_pre[x.b]);
-    x.nb = x.b < p.B ? s_pre[x.b + 1] - s_pre[x.b] : 0;
+      x.nb = x.b < p.B ? units_of(p, x.b) : 1;
+    } while (x.nb == 0);
   };
 
-  struct Tile {
-    words k[2], v[2];
-    uint32_t sk[2], sv[2];
+  // The pair whose units are being loaded. The codes' buffers end after the sequence's
+  // rows: what lies behind (and, past the wave's range, everything) reads as zeros
+  // without memory traffic; scales behind repeat the last row's.
+  Cursor ic = cc;
+  __amdgpu_buffer_rsrc_t rk, rv;
+  const uint8_t* sp;  // lanes 0-31 the K, 32-63 the V scales of the pair
+  int last = 0;       // last row
+  auto open = [&](const Cursor& x) {
+    const int kvh = __builtin_amdgcn_readfirstlane(x.hs / p.nset), b = __builtin_amdgcn_readfirstlane(x.b);
+    const int64_t n = __builtin_amdgcn_readfirstlane(rows_of(p, b));
+    rk = make_rsrc(p.kc + b * p.kcb + kvh * p.kch, n * (D / 2));
+    rv = make_rsrc(p.vc + b * p.vcb + kvh * p.vch, n * (D / 2));
+    sp = lane < 32 ? p.ks + b * p.ksb + kvh * p.ksh : p.vs + b * p.vsb + kvh * p.vsh;
+    last = (int)n - 1;
   };
-  // Rows past the sequence's end repeat its last row: read in bounds, masked below.
-  auto load = [&](const Cursor& x, Tile& t) {
-    const int n = s_len[x.b], kvh = x.hs / p.nset;
-    const uint8_t* kc = p.kc + x.b * p.kcb + kvh * p.kch;
-    const uint8_t* ks = p.ks + x.b * p.ksb + kvh * p.ksh;
-    const uint8_t* vc = p.vc + x.b * p.vcb + kvh * p.vch;
-    const uint8_t* vs = p.vs + x.b * p.vsb + kvh * p.vsh;
+  // Piece of the codes a lane fetches: with D = 128 the one it will use itself (16
+  // bytes of row c), with D = 64 chunk g / 2 of row l % 32.
+  const uint32_t c_off = D == 128 ? c * 64 + g * 16 : (lane & 31) * 32 + (lane >> 5) * 16;
+  auto issue = [&](bool live, int slot) {
+    const uint32_t at = lmem + slot;
+    const uint32_t row = ic.tile * kUnit;
+    auto codes = [&](__amdgpu_buffer_rsrc_t r, uint32_t to) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int64_t row = min(x.tile * kUnit + 16 * i + c, n - 1);
-      t.k[i] = __builtin_nontemporal_load(reinterpret_cast<const words*>(kc + row * (D / 2) + g * LB));
-      t.v[i] = __builtin_nontemporal_load(reinterpret_cast<const words*>(vc + row * (D / 2) + g * LB));
-      t.sk[i] = ks[row * NB + g * NB / 4];
-      t.sv[i] = vs[row * NB + g * NB / 4];
-    }
+      for (int i = 0; i < PIECES; ++i) {
+        const uint32_t off = live ? (row + 16 * i) * (D / 2) + c_off : kOOB;
+        if constexpr (ONCE) dma16_nt(r, off, to + 1024 * i);
+        else dma16(r, off, to + 1024 * i);
+      }
+    };
+    codes(rk, at);
+    codes(rv, at + Lds::kCodes);
+    const uint8_t* from = sp + (int64_t)min((int)row + (lane & 31), last) * NB;
+    if constexpr (D == 128) dma4_at(from, at + 2 * Lds::kCodes);
+    else dma2_at(from, at + 2 * Lds::kCodes);
+  };
+  // Lane's codes of row 16 i + c, and its block's scale, from a slot.
+  auto codes_at = [&](const char* slot, int i) {
+    const int off = D == 128 ? 1024 * i + 16 * lane : ((g >> 1) * 32 + 16 * i + c) * 16 + (g & 1) * 8;
+    return *reinterpret_cast<const words*>(slot + off);
   };
 
   bf16x8 qf[LW];
@@ -204,15 +239,15 @@ __global__ __launch_bounds__(64 * kWavesPerBlock, 2) void mx_decode_kernel(const
   float m = -INFINITY, lsum = 0.f;
   int vis = 0;  // rows this lane's column sees
   bool valid = false;
-  bf16* orow = nullptr;
+  int64_t o_off = 0;
   auto start = [&](const Cursor& x) {  // the query columns of a pair, and empty statistics
     const int kvh = x.hs / p.nset, col = (x.hs - kvh * p.nset) * kCols + c;
-    const int tok = col / p.groups, hd = col - tok * p.groups;  // Sq = 1 or groups * Sq <= kCols
+    const int tok = col / p.groups, hd = col - tok * p.groups;
     valid = tok < p.Sq;
     const int64_t head = (int64_t)kvh * p.groups + hd;
     const bf16* q = p.q + x.b * p.qb + head * p.qh + tok * p.qs;
-    orow = p.o + x.b * p.ob + head * p.oh + tok * p.os;
-    vis = min((int)min((int64_t)p.lens[x.b] + p.len_add + tok, (int64_t)p.cap), s_len[x.b]);
+    o_off = x.b * p.ob + head * p.oh + tok * p.os;
+    vis = (int)min((int64_t)p.lens[x.b] + p.len_add + tok, (int64_t)p.cap);
 #pragma unroll
     for (int t = 0; t < LW; ++t) {
       qf[t] = bf16x8{};
@@ -223,18 +258,18 @@ __global__ __launch_bounds__(64 * kWavesPerBlock, 2) void mx_decode_kernel(const
     m = -INFINITY;
     lsum = 0.f;
   };
-  auto flush = [&](const Cursor& x, int64_t pair_u0) {
+  auto flush = [&](const Cursor& x, bool whole) {
     lsum += __shfl_xor(lsum, 16, 64);
     lsum += __shfl_xor(lsum, 32, 64);
-    if (pair_u0 >= u0 && pair_u0 + x.nb <= u1) {
-      if (!valid) return;
+    if (!valid) return;
+    if (whole) {
       const float inv = lsum != 0.f ? 1.0f / lsum : 0.f;  // a NaN sum stays one
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
         bf16x4 r;
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[e] = f2bf(o[t][e] * inv);
-        *reinterpret_cast<bf16x4*>(orow + 16 * t + 4 * g) = r;
+        *reinterpret_cast<bf16x4*>(p.o + o_off + 16 * t + 4 * g) = r;
       }
     } else {
       float* rec = p.rec + ((int64_t)w + (int64_t)x.b * HS + x.hs) * rec_floats(D);
@@ -247,49 +282,70 @@ __global__ __launch_bounds__(64 * kWavesPerBlock, 2) void mx_decode_kernel(const
     }
   };
 
-  int64_t pair_u0 = u0 - cc.tile;
-  Tile cur, nxt;
-  load(cc, cur);
-  start(cc);
-  for (int64_t u = u0; u < u1; ++u) {
-    Cursor nc = cc;
-    if (u + 1 < u1) advance(nc);
-    load(nc, nxt);  // the last one's again past the range
+  start(cc);  // its loads before the ring's: loads retire in order
+  open(ic);
+  int issued = 0, islot = 0, slot_at = 0;
+  auto issue_next = [&]() {
+    issue(issued < count, islot);
+    islot = islot == (kSlots - 1) * Lds::kSlot ? 0 : islot + Lds::kSlot;
+    if (++issued < count && ++ic.tile == ic.nb) {
+      advance(ic);
+      open(ic);
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < kSlots - 1; ++i) issue_next();
+  int first = cc.tile;  // tile of the current pair at which this wave began
+  for (int u = 0; u < count; ++u) {
+    issue_next();
+    vm_wait<(kSlots - 1) * LOADS>();  // this unit's loads have landed
+    char* slot = mem + slot_at;
+    slot_at = slot_at == (kSlots - 1) * Lds::kSlot ? 0 : slot_at + Lds::kSlot;
+    const uint8_t* sc = reinterpret_cast<const uint8_t*>(slot + 2 * Lds::kCodes) + 4 * c + g * NB / 4;
+    const words kw[2] = {codes_at(slot, 0), codes_at(slot, 1)};
+    const words vw[2] = {codes_at(slot + Lds::kCodes, 0), codes_at(slot + Lds::kCodes, 1)};
+    const uint32_t kb[2] = {sc[0], sc[64]}, vb[2] = {sc[128], sc[192]};
+    asm volatile("" ::: "memory");  // read before V's rows take their place (the LDS works in a wave's order)
+    bf16* tile = reinterpret_cast<bf16*>(slot);
 
     floatx4 s[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       s[i] = floatx4{};
-      const float ks = mx_scale(cur.sk[i]);
+      const float ks = mx_scale(kb[i]);
 #pragma unroll
-      for (int t = 0; t < LW; ++t) s[i] = mfma16x16x32(mx_bf16x8(cur.k[i][t], ks), qf[t], s[i]);
+      for (int t = 0; t < LW; ++t) s[i] = mfma16x16x32(mx_bf16x8(kw[i][t], ks), qf[t], s[i]);
     }
-    const int k0 = cc.tile * kUnit + 4 * g;
+    const int seen = vis - cc.tile * kUnit - 4 * g;  // this lane's rows are 16 i + e
+    if (__builtin_amdgcn_ballot_w64(seen < 20) != 0) {  // a unit that some column sees in part
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (k0 + 16 * i + e >= vis) s[i][e] = -INFINITY;
-    // V rows whose block holds a NaN (scale 255) count as zeros in the product, and
-    // the blocks become NaN in the columns that see such a row: a masked one must not
-    // reach a column through 0 * NaN.
+        for (int e = 0; e < 4; ++e)
+          if (16 * i + e >= seen) s[i][e] = -INFINITY;
+    }
+
+    // V^T fragments: rows 0-15, then 16-31 (the LDS of a wave works in order). A NaN
+    // block (scale 255) counts as zeros here: a masked one must not reach a column
+    // through 0 * NaN.
+    const int rr = c >> 2, qq = c & 3;
     uint64_t bad[2];
+    short4v vf[DT][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      bad[i] = __builtin_amdgcn_ballot_w64(cur.sv[i] == 255);
-      const float vs = mx_scale(cur.sv[i]);
+      bad[i] = __builtin_amdgcn_ballot_w64(vb[i] == 255);
+      const float vs = mx_scale(vb[i] == 255 ? 0 : vb[i]);
 #pragma unroll
-      for (int t = 0; t < LW; ++t) {
-        bf16x8 v = mx_bf16x8(cur.v[i][t], vs);
-        if (bad[i] != 0 && cur.sv[i] == 255) v = bf16x8{};
-        *reinterpret_cast<bf16x8*>(tile + v_at<D>(16 * i + c, g * (2 * LB) + 8 * t)) = v;
-      }
+      for (int t = 0; t < LW; ++t)
+        *reinterpret_cast<bf16x8*>(tile + v_at<D>(c, g * (2 * LB) + 8 * t)) = mx_bf16x8(vw[i][t], vs);
+#pragma unroll
+      for (int t = 0; t < DT; ++t) vf[t][i] = read_tr16(tile + v_at<D>(4 * g + rr, 16 * t + 4 * qq));
     }
+
     float top = s[0][0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, s[i >> 2][i & 3]);
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64)) * p.scale_log2;
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i >> 2][i & 3]);
+    top = max4(top) * p.scale_log2;
     const bool raise = top > m + kRescale;
     if (__builtin_amdgcn_ballot_w64(raise) != 0) {
       const float mn = raise ? top : m;
@@ -307,27 +363,20 @@ __global__ __launch_bounds__(64 * kWavesPerBlock, 2) void mx_decode_kernel(const
       lsum += e;
       pb[i] = f2bf(e);
     }
-    const int rr = c >> 2, qq = c & 3;
 #pragma unroll
     for (int t = 0; t < DT; ++t) {
-      const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4v __attribute__((address_space(3)))*)(
-          reinterpret_cast<uintptr_t>(tile + v_at<D>(4 * g + rr, 16 * t + 4 * qq))));
-      const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4v __attribute__((address_space(3)))*)(
-          reinterpret_cast<uintptr_t>(tile + v_at<D>(16 + 4 * g + rr, 16 * t + 4 * qq))));
+      const short4v lo = vf[t][0], hi = vf[t][1];
       const short8v a8 = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       o[t] = mfma16x16x32(__builtin_bit_cast(bf16x8, a8), pb, o[t]);
     }
-    if ((bad[0] | bad[1]) != 0) {
+    if ((bad[0] | bad[1]) != 0) {  // rare: the NaN blocks of rows that a column sees
+      uint32_t see[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) see[i] = (1u << min(max(seen - 16 * i, 0), 4)) - 1;
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        bool hit = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = 4 * g + (i & 3);
-          // the lanes of block n of row r: l % 16 = r, l / 16 = 4 n / NB
-          const bool nan = (bad[i >> 2] >> (r + 16 * (4 * n / NB))) & 1;
-          hit = hit || (nan && k0 + 16 * (i >> 2) + (i & 3) < vis);
-        }
+        const int at = 16 * (4 * n / NB) + 4 * g;  // bit of row 4 g in the ballot, among the lanes of block n
+        const uint32_t hit = ((uint32_t)(bad[0] >> at) & see[0]) | ((uint32_t)(bad[1] >> at) & see[1]);
         float add = hit ? NAN : 0.f;
         add += __shfl_xor(add, 16, 64);
         add += __shfl_xor(add, 32, 64);
@@ -336,102 +385,138 @@ __global__ __launch_bounds__(64 * kWavesPerBlock, 2) void mx_decode_kernel(const
       }
     }
 
-    const bool pair_end = cc.tile == cc.nb - 1;
-    if (pair_end || u == u1 - 1) {
-      flush(cc, pair_u0);
-      if (pair_end) pair_u0 += cc.nb;
-      if (u + 1 < u1) start(nc);
+    if (cc.tile + 1 == cc.nb || u + 1 == count) {
+      flush(cc, first == 0 && cc.tile + 1 == cc.nb);
+      if (u + 1 < count) {
+        advance(cc);
+        start(cc);
+        first = 0;
+      }
+    } else {
+      ++cc.tile;
     }
-    cc = nc;
-    cur = nxt;
   }
+  vm_wait<0>();  // no load may still target this block's LDS when the wave retires
 }
 
-// Merges the records of the pairs split between waves: a block per pair and
-// column, its four waves every fourth record each, merged in wave order.
-template <int D>
-__global__ __launch_bounds__(256) void mx_decode_combine(const MxAttn p) {
+// Merges the records of the pairs split between waves: a block per pair and column,
+// its NW waves every NW-th record each, kBatch of them in flight together (the merge
+// is bound by latency), and the waves' sums in wave order.
+constexpr int kBatch = 4;
+
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) void mx_decode_combine(const MxAttn p) {
   constexpr int N = D / 64;  // outputs per lane
-  __shared__ float s_m[4], s_l[4], s_o[4][D];
+  typedef float outs __attribute__((ext_vector_type(N)));
+  __shared__ float s_m[NW], s_l[NW];
+  __shared__ outs s_o[NW][64];
   const int HS = p.Hkv * p.nset, pair = blockIdx.x, col = blockIdx.y;
   const int b = pair / HS, hs = pair - b * HS;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (p.lens_inc && hs == 0 && col == 0 && threadIdx.x == 0) p.lens_inc[b] += p.inc;
+  const int u0 = p.hdr[b], u1 = p.hdr[b + 1], units = p.hdr[p.B];
   const int kvh = hs / p.nset, gc = (hs - kvh * p.nset) * kCols + col;
   const int tok = gc / p.groups, hd = gc - tok * p.groups;
   if (tok >= p.Sq) return;
-  bf16* orow = p.o + b * p.ob + ((int64_t)kvh * p.groups + hd) * p.oh + tok * p.os;
-  const int nb = p.hdr[b + 1] - p.hdr[b];
-  if (nb == 0) {  // an empty sequence: zeros
-    if (wv == 0)
+  bf16* orow = p.o + b * p.ob + ((int64_t)kvh * p.groups + hd) * p.oh + tok * p.os + N * lane;
+  auto store = [&](outs o) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) orow[N * lane + e] = f2bf(0.f);
+    for (int e = 0; e < N; ++e) orow[e] = f2bf(o[e]);
+  };
+  if (u0 == u1) {  // an empty sequence: zeros
+    if (wv == 0) store(outs{});
     return;
   }
-  const int64_t U = (int64_t)HS * p.hdr[p.B], first = (int64_t)HS * p.hdr[b] + (int64_t)hs * nb;
-  const int w0 = wave_of(first, U), w1 = wave_of(first + nb - 1, U);
+  const Split split(HS * units);
+  const int first = HS * u0 + hs * (u1 - u0);
+  const int w0 = split.wave_of(first), w1 = split.wave_of(first + (u1 - u0) - 1);
   if (w0 == w1) return;  // stored by its wave
-  float m = -INFINITY, l = 0.f, o[N] = {};
-  for (int w = w0 + wv; w <= w1; w += 4) {
-    const float* rec = p.rec + ((int64_t)w + pair) * rec_floats(D);
-    const float mr = rec[col], lr = rec[kCols + col];
-    const float mn = fmaxf(m, mr), base = mn == -INFINITY ? 0.f : mn;
-    const float a = exp2_(m - base), r = exp2_(mr - base);
-    l = l * a + lr * r;
+  float m = -INFINITY, l = 0.f;
+  outs o{};
+  for (int wb = w0 + wv; wb <= w1; wb += NW * kBatch) {
+    float mr[kBatch], lr[kBatch];
+    outs orr[kBatch];
 #pragma unroll
-    for (int e = 0; e < N; ++e) o[e] = o[e] * a + rec[2 * kCols + col * D + N * lane + e] * r;
+    for (int i = 0; i < kBatch; ++i) {
+      const int w = min(wb + NW * i, w1);
+      const float* rec = p.rec + (int64_t)(w + pair) * rec_floats(D);
+      mr[i] = rec[col];
+      lr[i] = rec[kCols + col];
+      orr[i] = *reinterpret_cast<const outs*>(rec + 2 * kCols + col * D + N * lane);
+    }
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (wb + NW * i <= w1) mn = fmaxf(mn, mr[i]);
+    const float base = mn == -INFINITY ? 0.f : mn;  // no row seen yet: weights 0, not NaN
+    const float a = exp2_(m - base);
+    l *= a;
+    o *= a;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (wb + NW * i > w1) break;
+      const float r = exp2_(mr[i] - base);
+      l += lr[i] * r;
+      o += orr[i] * r;
+    }
     m = mn;
   }
   if (lane == 0) {
     s_m[wv] = m;
     s_l[wv] = l;
   }
-#pragma unroll
-  for (int e = 0; e < N; ++e) s_o[wv][N * lane + e] = o[e];
+  s_o[wv][lane] = o;
   __syncthreads();
   if (wv != 0) return;
-  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+#pragma unroll
+  for (int i = 1; i < NW; ++i) m = fmaxf(m, s_m[i]);
   if (m == -INFINITY) m = 0.f;
   l = 0.f;
+  o = outs{};
 #pragma unroll
-  for (int e = 0; e < N; ++e) o[e] = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < NW; ++i) {
     const float r = exp2_(s_m[i] - m);
     l += s_l[i] * r;
-#pragma unroll
-    for (int e = 0; e < N; ++e) o[e] += s_o[i][N * lane + e] * r;
+    o += s_o[i][lane] * r;
   }
-  const float inv = l != 0.f ? 1.0f / l : 0.f;
-#pragma unroll
-  for (int e = 0; e < N; ++e) orow[N * lane + e] = f2bf(o[e] * inv);
+  store(o * (l != 0.f ? 1.0f / l : 0.f));
 }
 
 int64_t header_bytes(int64_t B) { return (B + 1 + 63) / 64 * 256; }
 
 int64_t sets_of(int64_t groups, int64_t Sq) { return q3_cdiv(groups * Sq, kCols); }
 
+#ifndef STREAM_SETS
+#define STREAM_SETS 24
+#endif
 // The streaming kernel takes one token of any group, or a short chunk whose tokens and heads share the columns.
-bool streams(int64_t groups, int64_t Sq) { return Sq == 1 || groups * Sq <= kCols; }
+bool streams(int64_t groups, int64_t Sq) { return Sq == 1 || sets_of(groups, Sq) <= STREAM_SETS; }
 
 int64_t stream_ws_bytes(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq, int64_t D) {
   return header_bytes(B) + (kWaves + B * Hkv * sets_of(groups, Sq)) * (int64_t)rec_floats((int)D) * 4;
 }
 
-int launch_stream(const MxAttn& p, int64_t D, hipStream_t st) {
+template <int D>
+int launch_stream(const MxAttn& p, hipStream_t st) {
   const dim3 grid(kBlocks), block(64 * kWavesPerBlock);
-  const dim3 merge((unsigned)(p.B * p.Hkv * p.nset), (unsigned)std::min(kCols, p.groups * p.Sq));
-  if (D == 128) {
-    hipLaunchKernelGGL((mx_decode_kernel<128>), grid, block, 0, st, p);
-    Q3_LAUNCH_CHECK();
-    hipLaunchKernelGGL((mx_decode_combine<128>), merge, dim3(256), 0, st, p);
-  } else {
-    hipLaunchKernelGGL((mx_decode_kernel<64>), grid, block, 0, st, p);
-    Q3_LAUNCH_CHECK();
-    hipLaunchKernelGGL((mx_decode_combine<64>), merge, dim3(256), 0, st, p);
-  }
+  if (p.nset == 1)  // every row is read once
+    hipLaunchKernelGGL((mx_decode_kernel<D, true>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((mx_decode_kernel<D, false>), grid, block, 0, st, p);
+  Q3_LAUNCH_CHECK();
+  const int pairs = p.B * p.Hkv * p.nset;
+  const dim3 merge((unsigned)pairs, (unsigned)std::min(kCols, p.groups * p.Sq));
+  // A pair has about kWaves / pairs records: with more than 16 of them all are in flight at once on 16 waves.
+  if (kWaves / pairs > 16)
+    hipLaunchKernelGGL((mx_decode_combine<D, 16>), merge, dim3(64 * 16), 0, st, p);
+  else
+    hipLaunchKernelGGL((mx_decode_combine<D, 4>), merge, dim3(64 * 4), 0, st, p);
   Q3_LAUNCH_CHECK();
   return Q3_OK;
+}
+
+int launch_stream(const MxAttn& p, int64_t D, hipStream_t st) {
+  return D == 128 ? launch_stream<128>(p, st) : launch_stream<64>(p, st);
 }
 
 // Arguments that both entry points take; strides = [qb, qh, qs, ob, oh, os] in
@@ -442,12 +527,15 @@ int check(const void* q, const void* kc, const void* ks, const void* vc, const v
   Q3_REQUIRE(q && kc && ks && vc && vs && lens && o && strides, Q3_ERR_NULL);
   Q3_REQUIRE(B >= 0 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Sq >= 0 && D >= 1 && cap >= 0, Q3_ERR_SHAPE);
   Q3_REQUIRE(dtype == Q3_BF16, Q3_ERR_DTYPE);
-  Q3_REQUIRE((D == 64 || D == 128) && B <= kMaxBatch && cap < (1ll << 31) - kUnit && Sq < (1ll << 31) &&
-                 Hq < (1ll << 16) && B * Hkv * q3_cdiv(Hq / Hkv, kCols) < (1ll << 31),
+  Q3_REQUIRE((D == 64 || D == 128) && B <= kMaxBatch && (cap + kUnit) * D / 2 < (1ll << 31) && Sq < (1ll << 31) &&
+                 Hq < (1ll << 16) && B * Hkv * sets_of(Hq / Hkv, streams(Hq / Hkv, Sq) ? Sq : 1) * q3_cdiv(cap, kUnit) < (1ll << 31),
              Q3_ERR_UNSUPPORTED);
   bool ok = q3_aligned(q, 16) && q3_aligned(kc, 16) && q3_aligned(vc, 16) && q3_aligned(o, 8);
   for (int i = 0; i < 6; ++i) ok = ok && strides[i] % 8 == 0;
   for (int i : {6, 7, 10, 11}) ok = ok && strides[i] % 16 == 0;
+  const int64_t row = D / kMxBlock;  // a row's scales are read at once
+  ok = ok && q3_aligned(ks, row) && q3_aligned(vs, row);
+  for (int i : {8, 9, 12, 13}) ok = ok && strides[i] % row == 0;
   return ok ? Q3_OK : Q3_ERR_ALIGN;
 }
 

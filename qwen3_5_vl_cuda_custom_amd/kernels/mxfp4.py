@@ -195,6 +195,8 @@ def _check_cache(op: str, dev: int, k_codes, k_scales, v_codes, v_scales, kv_len
             raise ValueError(f"{op}: the rows of a cache head must be packed")
         if c.data_ptr() % 16 or ct[0] % 16 or ct[1] % 16:
             raise ValueError(f"{op}: the cache codes must be 16-byte aligned")
+        if ss[3] and (s.data_ptr() % ss[3] or s_t[0] % ss[3] or s_t[1] % ss[3]):
+            raise ValueError(f"{op}: the cache scales must be whole rows apart and aligned to one")
         st += (ct[0], ct[1], s_t[0], s_t[1])
     if kv_lens.dtype != torch.int32 or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
         raise ValueError(f"{op}: kv_lens must be a contiguous int32 ({B},) device tensor")
