@@ -80,13 +80,14 @@ __device__ __forceinline__ void mx_load8(const T* p, float (&v)[8]) {
   }
 }
 
-// Codes and scales of n0 x n1 planes, each `run` consecutive values; plane
-// (i, j) at strides[0] i + strides[1] j (codes) and strides[2] i + strides[3] j
-// (scales) bytes, to (n0, n1, run) in y. With lens, plane (i, j) ends after lens[i] +
-// len_add rows of `row` values: nothing behind them is read, the rows up to the next
-// multiple of 64 become zeros (a consumer's tile may reach there) and those behind
-// are not written.
-int mx_expand(const void* codes, const void* scales, void* y, int64_t n0, int64_t n1, int64_t run,
-              const int64_t* strides, const int* lens, int len_add, int64_t row, int dtype, hipStream_t st);
+// n consecutive values (a multiple of 32) to bf16.
+int mx_expand(const void* codes, const void* scales, bf16* y, int64_t n, hipStream_t st);
+
+// The rows in use of a 4-bit cache to bf16: y holds K, then V, (B, Hkv, rows, D) each. Rows at or past lens[b] +
+// len_add are not read; those up to the next multiple of 64 become zeros (a consumer's tile may reach there), those
+// behind are not written. V's NaN blocks in rows from lens[b] on become zeros as well. cst / sst: (b, h) strides of K's, then V's codes / scales in bytes.
+int mx_expand_cache(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, bf16* y,
+                    int64_t B, int64_t Hkv, int64_t rows, int64_t D, const int64_t* cst, const int64_t* sst,
+                    const int* lens, int len_add, hipStream_t st);
 
 }  // namespace q3

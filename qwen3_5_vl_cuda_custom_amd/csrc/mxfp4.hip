@@ -39,25 +39,36 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
   }
 }
 
+struct ExpandArgs {
+  const uint8_t* codes[2];
+  const uint8_t* scales[2];
+  void* y;
+  int n0, n1;           // planes (i, j) of each source, at i * stride + j * stride bytes
+  int64_t cst[2][2], sst[2][2];
+  int64_t run;          // values of a plane; y is (source, n0, n1, run)
+  const int* lens;      // if set: plane (i, j) of `run` values has lens[i] + len_add rows of `row` values in use
+  int len_add;
+  int64_t row;
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void mx_expand_kernel(const uint8_t* __restrict__ codes,
-                                                        const uint8_t* __restrict__ scales, T* __restrict__ y,
-                                                        int n1, int64_t run, int64_t c0, int64_t c1, int64_t s0,
-                                                        int64_t s1, const int* __restrict__ lens, int len_add,
-                                                        int64_t row) {
-  const int plane = blockIdx.y, i0 = plane / n1, i1 = plane % n1;
-  int64_t rows = 0, end = run, used = run;
-  if (lens) {
-    rows = max((int64_t)lens[i0] + len_add, (int64_t)0);
-    used = min(run, rows * row);
-    end = min(run, (rows + 63) / 64 * 64 * row);
+__global__ __launch_bounds__(256) void mx_expand_kernel(const ExpandArgs a) {
+  const int plane = blockIdx.y, i0 = plane / a.n1, i1 = plane - i0 * a.n1, kv = blockIdx.z;
+  int64_t end = a.run, used = a.run, fresh = a.run;
+  if (a.lens) {
+    fresh = max((int64_t)a.lens[i0], (int64_t)0) * a.row >> 3;
+    const int64_t rows = max((int64_t)a.lens[i0] + a.len_add, (int64_t)0);
+    used = min(a.run, rows * a.row);
+    end = min(a.run, (rows + 63) / 64 * 64 * a.row);
   }
   const int64_t pieces = end >> 3, last = (used >> 3) - 1;
   const int64_t base = (int64_t)blockIdx.x * (256 * kPieces) + threadIdx.x;
-  const uint32_t* c = reinterpret_cast<const uint32_t*>(codes + i0 * c0 + i1 * c1);
-  const uint8_t* s = scales + i0 * s0 + i1 * s1;
-  T* o = y + (int64_t)plane * run;
   if (base - threadIdx.x >= pieces) return;
+  const uint32_t* c = reinterpret_cast<const uint32_t*>((kv ? a.codes[1] : a.codes[0]) + i0 * (kv ? a.cst[1][0] : a.cst[0][0]) +
+                                                        i1 * (kv ? a.cst[1][1] : a.cst[0][1]));
+  const uint8_t* s = (kv ? a.scales[1] : a.scales[0]) + i0 * (kv ? a.sst[1][0] : a.sst[0][0]) +
+                     i1 * (kv ? a.sst[1][1] : a.sst[0][1]);
+  T* o = static_cast<T*>(a.y) + ((int64_t)kv * a.n0 * a.n1 + plane) * a.run;
   uint32_t w[kPieces], b[kPieces];
 #pragma unroll
   for (int u = 0; u < kPieces; ++u) {
@@ -66,6 +77,7 @@ __global__ __launch_bounds__(256) void mx_expand_kernel(const uint8_t* __restric
     if (i <= last) {
       w[u] = c[i];
       b[u] = s[i >> 2];
+      if (kv && b[u] == 255 && i >= fresh) w[u] = b[u] = 0;
     }
   }
 #pragma unroll
@@ -86,6 +98,16 @@ __global__ __launch_bounds__(256) void mx_expand_kernel(const uint8_t* __restric
       reinterpret_cast<floatx4*>(o)[2 * i + 1] = hi;
     }
   }
+}
+
+int launch_expand(const ExpandArgs& a, int sources, int dtype, hipStream_t st) {
+  const dim3 grid((unsigned)q3_cdiv(a.run / 8, 256 * kPieces), (unsigned)(a.n0 * a.n1), (unsigned)sources);
+  if (dtype == Q3_BF16)
+    hipLaunchKernelGGL((mx_expand_kernel<bf16>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((mx_expand_kernel<float>), grid, dim3(256), 0, st, a);
+  Q3_LAUNCH_CHECK();
+  return Q3_OK;
 }
 
 struct AppendArgs {
@@ -149,19 +171,36 @@ void launch_quantize(const void* x, void* codes, void* scales, int64_t rows, int
 
 namespace q3 {
 
-int mx_expand(const void* codes, const void* scales, void* y, int64_t n0, int64_t n1, int64_t run,
-              const int64_t* strides, const int* lens, int len_add, int64_t row, int dtype, hipStream_t st) {
-  const dim3 grid((unsigned)q3_cdiv(run / 8, 256 * kPieces), (unsigned)(n0 * n1));
-  auto* c = static_cast<const uint8_t*>(codes);
-  auto* s = static_cast<const uint8_t*>(scales);
-  if (dtype == Q3_BF16)
-    hipLaunchKernelGGL((mx_expand_kernel<bf16>), grid, dim3(256), 0, st, c, s, static_cast<bf16*>(y), (int)n1, run,
-                       strides[0], strides[1], strides[2], strides[3], lens, len_add, row);
-  else
-    hipLaunchKernelGGL((mx_expand_kernel<float>), grid, dim3(256), 0, st, c, s, static_cast<float*>(y), (int)n1, run,
-                       strides[0], strides[1], strides[2], strides[3], lens, len_add, row);
-  Q3_LAUNCH_CHECK();
-  return Q3_OK;
+int mx_expand(const void* codes, const void* scales, bf16* y, int64_t n, hipStream_t st) {
+  ExpandArgs a{};
+  a.codes[0] = static_cast<const uint8_t*>(codes);
+  a.scales[0] = static_cast<const uint8_t*>(scales);
+  a.y = y;
+  a.n0 = a.n1 = 1;
+  a.run = n;
+  return launch_expand(a, 1, Q3_BF16, st);
+}
+
+int mx_expand_cache(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, bf16* y,
+                    int64_t B, int64_t Hkv, int64_t rows, int64_t D, const int64_t* cst, const int64_t* sst,
+                    const int* lens, int len_add, hipStream_t st) {
+  ExpandArgs a{};
+  a.codes[0] = static_cast<const uint8_t*>(k_codes);
+  a.codes[1] = static_cast<const uint8_t*>(v_codes);
+  a.scales[0] = static_cast<const uint8_t*>(k_scales);
+  a.scales[1] = static_cast<const uint8_t*>(v_scales);
+  a.y = y;
+  a.n0 = (int)B;
+  a.n1 = (int)Hkv;
+  for (int i = 0; i < 4; ++i) {
+    a.cst[i / 2][i % 2] = cst[i];
+    a.sst[i / 2][i % 2] = sst[i];
+  }
+  a.run = rows * D;
+  a.lens = lens;
+  a.len_add = len_add;
+  a.row = D;
+  return launch_expand(a, 2, Q3_BF16, st);
 }
 
 }  // namespace q3
@@ -194,8 +233,18 @@ int q3_mxfp4_dequantize(const void* codes, const void* scales, void* y, int64_t 
   if (n0 == 0 || n1 == 0 || run == 0) return Q3_OK;
   Q3_REQUIRE(n0 <= 65535 && n1 <= 65535 && n0 * n1 <= 65535, Q3_ERR_UNSUPPORTED);
   Q3_REQUIRE(q3_aligned(codes, 4) && q3_aligned(y, 16) && strides[0] % 4 == 0 && strides[1] % 4 == 0, Q3_ERR_ALIGN);
-  return q3::mx_expand(codes, scales, y, n0, n1, run, strides, nullptr, 0, 0, dtype,
-                       static_cast<hipStream_t>(stream));
+  ExpandArgs a{};
+  a.codes[0] = static_cast<const uint8_t*>(codes);
+  a.scales[0] = static_cast<const uint8_t*>(scales);
+  a.y = y;
+  a.n0 = (int)n0;
+  a.n1 = (int)n1;
+  for (int i = 0; i < 2; ++i) {
+    a.cst[0][i] = strides[i];
+    a.sst[0][i] = strides[2 + i];
+  }
+  a.run = run;
+  return launch_expand(a, 1, dtype, static_cast<hipStream_t>(stream));
 }
 
 int q3_kv_append_mxfp4(const void* k, const void* v, void* k_codes, void* k_scales, void* v_codes, void* v_scales,

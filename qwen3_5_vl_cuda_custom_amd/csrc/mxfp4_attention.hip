@@ -27,6 +27,7 @@
 //    over the rows: the output's own rounding to bf16 is larger); q, K and V enter
 //    exactly; m, the sum and o are fp32.
 #include <algorithm>
+#include <type_traits>
 
 #include "gemm_tile.h"
 #include "mxfp4.h"
@@ -36,7 +37,7 @@ namespace {
 using namespace q3;
 
 constexpr int kUnit = 32;        // rows of a unit
-constexpr int kMaxBatch = 1024;  // sequences (their unit counts live in LDS)
+constexpr int kMaxBatch = 1024;  // sequences
 constexpr int kCols = 16;        // MFMA columns
 constexpr int kWavesPerBlock = 12;  // three per SIMD, one block per CU
 constexpr int kBlocks = 256;
@@ -410,9 +411,9 @@ __global__ __launch_bounds__(64 * NW) void mx_decode_combine(const MxAttn p) {
   typedef float outs __attribute__((ext_vector_type(N)));
   __shared__ float s_m[NW], s_l[NW];
   __shared__ outs s_o[NW][64];
-  const int HS = p.Hkv * p.nset, pair = blockIdx.x, col = blockIdx.y;
+  const int HS = p.Hkv * p.nset, pair = blockIdx.x;
   const int b = pair / HS, hs = pair - b * HS;
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = blockIdx.y;
   if (p.lens_inc && hs == 0 && col == 0 && threadIdx.x == 0) p.lens_inc[b] += p.inc;
   const int u0 = p.hdr[b], u1 = p.hdr[b + 1], units = p.hdr[p.B];
   const int kvh = hs / p.nset, gc = (hs - kvh * p.nset) * kCols + col;
@@ -486,11 +487,17 @@ int64_t header_bytes(int64_t B) { return (B + 1 + 63) / 64 * 256; }
 
 int64_t sets_of(int64_t groups, int64_t Sq) { return q3_cdiv(groups * Sq, kCols); }
 
-#ifndef STREAM_SETS
-#define STREAM_SETS 24
-#endif
-// The streaming kernel takes one token of any group, or a short chunk whose tokens and heads share the columns.
-bool streams(int64_t groups, int64_t Sq) { return Sq == 1 || sets_of(groups, Sq) <= STREAM_SETS; }
+// The streaming kernel takes single tokens and chunks of up to 1024 pairs; a longer
+// chunk expands the cache to bf16 once and runs the chunk kernel of the bf16 cache, which
+// shares each row among 256 columns but does not split the rows. Microseconds, streaming
+// / expanding (8 KV heads of 4 query heads unless said otherwise): 8192 rows, 32 tokens
+// (64 pairs) 36 / 206, 128 (256) 60 / 210, 512 (1024) 166 / 211, 1024 (2048) 323 / 207;
+// 1024 rows, 256 tokens (512) 35 / 40, 512 (1024) 45 / 40; 8 sequences of 300 rows x 4 x
+// 8 heads, 100 tokens (1600) 37 / 26.
+constexpr int64_t kStreamPairs = 1024;
+bool streams(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq) {
+  return Sq == 1 || B * Hkv * sets_of(groups, Sq) <= kStreamPairs;
+}
 
 int64_t stream_ws_bytes(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq, int64_t D) {
   return header_bytes(B) + (kWaves + B * Hkv * sets_of(groups, Sq)) * (int64_t)rec_floats((int)D) * 4;
@@ -506,7 +513,8 @@ int launch_stream(const MxAttn& p, hipStream_t st) {
   Q3_LAUNCH_CHECK();
   const int pairs = p.B * p.Hkv * p.nset;
   const dim3 merge((unsigned)pairs, (unsigned)std::min(kCols, p.groups * p.Sq));
-  // A pair has about kWaves / pairs records: with more than 16 of them all are in flight at once on 16 waves.
+  // A pair has about kWaves / pairs records: with more than 16 of them all are in flight at once on 16 waves (8
+  // pairs of one sequence's 1500 rows: 4.9 us against 6.3 on 4; 256 pairs of 32 sequences 5.5 on 4, 8.5 on 16).
   if (kWaves / pairs > 16)
     hipLaunchKernelGGL((mx_decode_combine<D, 16>), merge, dim3(64 * 16), 0, st, p);
   else
@@ -528,7 +536,7 @@ int check(const void* q, const void* kc, const void* ks, const void* vc, const v
   Q3_REQUIRE(B >= 0 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Sq >= 0 && D >= 1 && cap >= 0, Q3_ERR_SHAPE);
   Q3_REQUIRE(dtype == Q3_BF16, Q3_ERR_DTYPE);
   Q3_REQUIRE((D == 64 || D == 128) && B <= kMaxBatch && (cap + kUnit) * D / 2 < (1ll << 31) && Sq < (1ll << 31) &&
-                 Hq < (1ll << 16) && B * Hkv * sets_of(Hq / Hkv, streams(Hq / Hkv, Sq) ? Sq : 1) * q3_cdiv(cap, kUnit) < (1ll << 31),
+                 Hq < (1ll << 16) && B * Hkv * sets_of(Hq / Hkv, streams(B, Hkv, Hq / Hkv, Sq) ? Sq : 1) * q3_cdiv(cap, kUnit) < (1ll << 31),
              Q3_ERR_UNSUPPORTED);
   bool ok = q3_aligned(q, 16) && q3_aligned(kc, 16) && q3_aligned(vc, 16) && q3_aligned(o, 8);
   for (int i = 0; i < 6; ++i) ok = ok && strides[i] % 8 == 0;
@@ -567,6 +575,38 @@ void workspace_of(MxAttn& p, void* ws) {
   p.rec = reinterpret_cast<float*>(static_cast<char*>(ws) + header_bytes(p.B));
 }
 
+// A NaN block of V in one of the chunk's own rows (the expansion made zeros of it, so
+// that it does not reach the earlier tokens' 0 * NaN) into the outputs of the tokens
+// from that row's on. lens[b] - off is the sequence's length before the chunk.
+template <int D>
+__global__ __launch_bounds__(256) void mx_chunk_nan_kernel(const MxAttn p, int off) {
+  constexpr int NB = D / kMxBlock;
+  __shared__ int s_first[NB];
+  const int b = blockIdx.x / p.Hkv, kvh = blockIdx.x - b * p.Hkv;
+  const int64_t len = max((int64_t)p.lens[b] - off, (int64_t)0);
+  if (threadIdx.x < NB) s_first[threadIdx.x] = p.Sq;
+  __syncthreads();
+  typedef typename std::conditional<NB == 4, uint32_t, uint16_t>::type word;  // a row's scales
+  const word* s = reinterpret_cast<const word*>(p.vs + b * p.vsb + kvh * p.vsh + len * NB);
+  const int n = (int)max(min((int64_t)p.Sq, p.cap - len), (int64_t)0);
+  for (int r0 = threadIdx.x; r0 < n; r0 += 4 * 256) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = s[min(r0 + 256 * i, n - 1)];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < NB; ++k)
+        if ((w[i] >> (8 * k) & 255) == 255) atomicMin(&s_first[k], min(r0 + 256 * i, n - 1));
+  }
+  __syncthreads();
+  for (int k = 0; k < NB; ++k)
+    for (int64_t i = (int64_t)s_first[k] * p.groups + threadIdx.x / kMxBlock; i < (int64_t)p.Sq * p.groups;
+         i += 256 / kMxBlock)
+      p.o[b * p.ob + ((int64_t)kvh * p.groups + i % p.groups) * p.oh + (i / p.groups) * p.os + k * kMxBlock +
+          threadIdx.x % kMxBlock] = f2bf(NAN);
+}
+
 }  // namespace
 
 extern "C" {
@@ -596,7 +636,7 @@ int q3_decode_attention_mxfp4(const void* q, const void* k_codes, const void* k_
 int64_t q3_flash_attention_cache_mxfp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
                                                        int64_t max_len) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || D <= 0 || max_len < 0) return 0;
-  if (streams(Hq / Hkv, Sq)) return stream_ws_bytes(B, Hkv, Hq / Hkv, Sq, D);
+  if (streams(B, Hkv, Hq / Hkv, Sq)) return stream_ws_bytes(B, Hkv, Hq / Hkv, Sq, D);
   return 2 * B * Hkv * max_len * D * 2;  // K and V in bf16
 }
 
@@ -604,7 +644,7 @@ int q3_flash_attention_cache_mxfp4(const void* q, const void* k_codes, const voi
                                    const void* v_scales, int* kv_lens, void* o, int64_t B, int64_t Hq, int64_t Hkv,
                                    int64_t Sq, int64_t D, int64_t max_len, const int64_t* strides, float scale,
                                    int advance, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
-  const int rc =
+  int rc =
       check(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, Sq, D, max_len, strides, dtype);
   if (rc != Q3_OK || B == 0 || Sq == 0) return rc;
   Q3_REQUIRE(Sq <= max_len, Q3_ERR_SHAPE);
@@ -613,7 +653,7 @@ int q3_flash_attention_cache_mxfp4(const void* q, const void* k_codes, const voi
              Q3_ERR_WORKSPACE);
   Q3_REQUIRE(q3_aligned(workspace, 16), Q3_ERR_ALIGN);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (streams(Hq / Hkv, Sq)) {
+  if (streams(B, Hkv, Hq / Hkv, Sq)) {
     MxAttn p = arguments(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, Sq, max_len, strides, scale);
     p.len_add = 1;
     p.lens_inc = advance ? kv_lens : nullptr;
@@ -625,16 +665,26 @@ int q3_flash_attention_cache_mxfp4(const void* q, const void* k_codes, const voi
   // bf16 once (exact) and the chunk kernel of the bf16 cache runs on them.
   Q3_REQUIRE(B * Hkv <= 65535 && (max_len + 1) * D * 2 < 0x7fffffffLL, Q3_ERR_UNSUPPORTED);
   bf16* kx = static_cast<bf16*>(workspace);
-  bf16* vx = kx + B * Hkv * max_len * D;
-  int r = mx_expand(k_codes, k_scales, kx, B, Hkv, max_len * D, strides + 6, kv_lens, (int)Sq, D, Q3_BF16, st);
-  if (r != Q3_OK) return r;
-  const int64_t vst[4] = {strides[10], strides[11], strides[12], strides[13]};
-  r = mx_expand(v_codes, v_scales, vx, B, Hkv, max_len * D, vst, kv_lens, (int)Sq, D, Q3_BF16, st);
-  if (r != Q3_OK) return r;
+  const bf16* vx = kx + B * Hkv * max_len * D;
+  const int64_t cst[4] = {strides[6], strides[7], strides[10], strides[11]};
+  const int64_t sst[4] = {strides[8], strides[9], strides[12], strides[13]};
+  rc = mx_expand_cache(k_codes, k_scales, v_codes, v_scales, kx, B, Hkv, max_len, D, cst, sst, kv_lens,
+                                (int)Sq, st);
+  if (rc != Q3_OK) return rc;
   const int64_t rows[12] = {strides[0], strides[1], strides[2], Hkv * max_len * D, max_len * D, D,
                             Hkv * max_len * D, max_len * D, D, strides[3], strides[4], strides[5]};
-  return q3_flash_attention_cache(q, kx, vx, kv_lens, o, B, Hq, Hkv, Sq, max_len, D, rows, scale, advance, dtype,
-                                  stream);
+  rc = q3_flash_attention_cache(q, kx, vx, kv_lens, o, B, Hq, Hkv, Sq, max_len, D, rows, scale, advance,
+                                           dtype, stream);
+  if (rc != Q3_OK) return rc;
+  const MxAttn p =
+      arguments(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, Sq, max_len, strides, scale);
+  const dim3 heads((unsigned)(B * Hkv));
+  if (D == 128)
+    hipLaunchKernelGGL((mx_chunk_nan_kernel<128>), heads, dim3(256), 0, st, p, advance ? (int)Sq : 0);
+  else
+    hipLaunchKernelGGL((mx_chunk_nan_kernel<64>), heads, dim3(256), 0, st, p, advance ? (int)Sq : 0);
+  Q3_LAUNCH_CHECK();
+  return Q3_OK;
 }
 
 }  // extern "C"

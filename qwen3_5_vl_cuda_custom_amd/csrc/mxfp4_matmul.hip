@@ -167,8 +167,7 @@ int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, co
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (M > kGemvMaxRows) {
     Q3_REQUIRE(ldw == K / 2 && lds == K / kMxBlock, Q3_ERR_UNSUPPORTED);
-    const int64_t strides[4] = {0, 0, 0, 0};
-    const int rc = mx_expand(w_codes, w_scales, workspace, 1, 1, N * K, strides, nullptr, 0, 0, Q3_BF16, st);
+    const int rc = mx_expand(w_codes, w_scales, static_cast<bf16*>(workspace), N * K, st);
     if (rc != Q3_OK) return rc;
     return q3_matmul(x, workspace, bias, residual, y, M, N, K, ldx, K, ldr, ldc, dtype, nullptr, 0, stream);
   }

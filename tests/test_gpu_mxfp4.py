@@ -254,7 +254,9 @@ def test_decode_nan_row_reaches_its_block_of_the_output_only():
     assert torch.isnan(o[0]).all() and torch.isfinite(o[1]).all()
 
 
-CHUNKS = [(1, 1, 2), (2, 4, 3), (1, 4, 4), (2, 4, 5), (2, 3, 40), (1, 8, 33), (2, 2, 100), (1, 1, 16), (1, 1, 17)]
+# (KV heads, group, tokens): the last ones past the streaming kernel's 1024 pairs
+CHUNKS = [(1, 1, 2), (2, 4, 3), (1, 4, 4), (2, 4, 5), (2, 3, 40), (1, 8, 33), (2, 2, 100), (1, 1, 16), (1, 1, 17), (9, 5, 75),
+          (13, 4, 65)]
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -290,6 +292,31 @@ def test_short_chunk_a_later_tokens_nan_is_masked(groups, sq):
     assert torch.isnan(o[:, :, -1]).all()
     seen = c.lens.view(-1, 1) + 1 + torch.arange(sq - 1)
     check_attention(o[:, :, :-1], q[:, :, :-1], c, seen, 0.1)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("advance", [False, True])
+def test_long_chunk_a_nan_row_reaches_the_tokens_that_see_it(d, advance):
+    """Past the streaming kernel's pairs, over expanded rows."""
+    B, hkv, groups, sq = 2, 15, 8, 80
+    assert B * hkv * groups * sq / 16 > 1024
+    c = Cache([20, 31], hkv, 120, d, seed=26, used=sq)
+    q = rnd(B, hkv * groups, sq, d, seed=27)
+    c.vs[0, 0, 20 + 50, 1] = 255  # token 50's value
+    c.vs[1, 3, 31 + 7, 0] = 255
+    c.ks[1, 4, 31 + 60, 0] = 255  # token 60's key
+    clean = Cache([20, 31], hkv, 120, d, seed=26, used=sq)
+    lens = c.lens.to(DEV)
+    o = K.flash_attention_cache_mxfp4(q.to(DEV), *c.device(), lens, 0.1, groups, advance=advance).cpu()
+    ref = K.flash_attention_cache_mxfp4(q.to(DEV), *clean.device(), c.lens.to(DEV), 0.1, groups).cpu()
+    bad = torch.zeros(o.shape, dtype=torch.bool)
+    bad[0, :groups, 50:, 32:64] = True
+    bad[1, 3 * groups:4 * groups, 7:, :32] = True
+    bad[1, 4 * groups:5 * groups, 60:] = True
+    assert torch.equal(torch.isnan(o), bad)
+    # a masked row's weight is zero whatever it holds: the other outputs are the clean cache's to the bit
+    assert torch.equal(o[~bad], ref[~bad]) and torch.isfinite(ref).all()
+    assert torch.equal(lens.cpu(), c.lens + (sq if advance else 0))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
