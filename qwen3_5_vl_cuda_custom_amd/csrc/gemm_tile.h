@@ -48,6 +48,16 @@ __device__ __forceinline__ void dma16_nt(__amdgpu_buffer_rsrc_t r, uint32_t voff
   asm volatile("s_mov_b32 m0, %1\n\tbuffer_load_dwordx4 %0, %2, 0 offen nt lds" ::"v"(voff), "s"(m0v), "s"(r)
                : "memory");
 }
+// One byte per lane, zero-extended to a word at `lds_byte` + 4 * lane.
+__device__ __forceinline__ void dma1(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t lds_byte) {
+  const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds_byte);
+  asm volatile("s_mov_b32 m0, %1\n\tbuffer_load_ubyte %0, %2, 0 offen lds" ::"v"(voff), "s"(m0v), "s"(r) : "memory");
+}
+// Four bytes per lane, at `lds_byte` + 4 * lane.
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t lds_byte) {
+  const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds_byte);
+  asm volatile("s_mov_b32 m0, %1\n\tbuffer_load_dword %0, %2, 0 offen lds" ::"v"(voff), "s"(m0v), "s"(r) : "memory");
+}
 // 4 (2) bytes per lane from `p`, which may differ between the lanes by any distance,
 // into the word at `lds_byte` + 4 * lane (2 bytes: zero-extended).
 __device__ __forceinline__ void dma4_at(const void* p, uint32_t lds_byte) {

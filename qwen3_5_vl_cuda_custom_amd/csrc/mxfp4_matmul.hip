@@ -20,6 +20,7 @@ struct MxGemm {
   float* part;  // (gridDim.y, M, N) sums, or null: the block writes y
   int M, N, K;
   int64_t ldx, ldw, lds, ldr, ldc;  // ldw, lds in bytes
+  int vec;  // N a multiple of 4, the rows of y, bias and residual in 8-byte pieces
 };
 
 __device__ __forceinline__ void store_y(const MxGemm& p, int m, int n, float v) {
@@ -27,117 +28,293 @@ __device__ __forceinline__ void store_y(const MxGemm& p, int m, int n, float v) 
   if (p.res) v += bf2f(p.res[m * p.ldr + n]);
   p.y[m * p.ldc + n] = f2bf(v);
 }
+// Four columns at once (p.vec: every row of y, bias and residual in 8-byte pieces).
+__device__ __forceinline__ void store_y4(const MxGemm& p, int m, int n, floatx4 v) {
+  if (p.bias) {
+    const bf16x4 b = *reinterpret_cast<const bf16x4*>(p.bias + n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += bf2f(b[e]);
+  }
+  if (p.res) {
+    const bf16x4 b = *reinterpret_cast<const bf16x4*>(p.res + m * p.ldr + n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += bf2f(b[e]);
+  }
+  bf16x4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = f2bf(v[e]);
+  *reinterpret_cast<bf16x4*>(p.y + m * p.ldc + n) = o;
+}
 
 // ------------------------------------------------------------------ few rows (decode)
-// Bound by the weight stream. A wave takes RT groups of 16 weight rows and every
-// eighth 128-value step of its block's k range: lane (r = l % 16, g = l / 16) loads
-// the 16 bytes of block 4 step + g of weight row r, one scale, and the 32 values of
-// x's row r at the same k (MT tiles of 16 rows), and forms 4 products of 16x16x32
-// per tile pair (k permuted alike in both). The eight waves' sums meet in LDS, in
-// wave order.
+// Bound by the weight stream (N=K=4096, one row: 6.1 us, 8.9 MB; an empty kernel takes
+// 2). A block takes 16 weight rows, a wave every eighth 128-value step of k: lane (r = l %
+// 16, g = l / 16) loads the 16 bytes of block 4 step + g of weight row r, its scale, and
+// the 32 values of x's row r at the same k, and forms 4 products of 16x16x32 (k permuted
+// alike in both). The eight waves' sums meet in LDS, in wave order.
 constexpr int kGemvWaves = 8;
 
-template <int MT, int RT>
 __global__ __launch_bounds__(64 * kGemvWaves) void mx_gemv_kernel(const MxGemm p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * (16 * RT);
+  const int n0 = blockIdx.x * 16;
   const int blocks = p.K / kMxBlock, steps = (blocks + 3) / 4;
-  const int t0 = (int)((int64_t)steps * blockIdx.y / gridDim.y), t1 = (int)((int64_t)steps * (blockIdx.y + 1) / gridDim.y);
 
   struct Step {
-    u32x4 w[RT];
-    uint32_t s[RT];
-    bf16x8 x[MT][4];
+    u32x4 w;
+    uint32_t s;
+    bf16x8 x[4];
   };
+  const int64_t row = min(n0 + r, p.N - 1);
   auto load = [&](int t, Step& d) {
     const int kb = 4 * t + g;
-    const bool in = kb < blocks && t < t1;
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const int64_t n = min(n0 + 16 * i + r, p.N - 1);
-      d.w[i] = u32x4{};
-      d.s[i] = 0;
-      if (in) {
-        d.w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p.w + n * p.ldw + kb * 16));
-        d.s[i] = p.s[n * p.lds + kb];
-      }
+    const bool in = kb < blocks;
+    d.w = u32x4{};
+    d.s = 0;
+    if (in) {
+      d.w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p.w + row * p.ldw + kb * 16));
+      d.s = p.s[row * p.lds + kb];
     }
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      const int m = 16 * j + r;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        d.x[j][e] = bf16x8{};
-        if (in && m < p.M) d.x[j][e] = *reinterpret_cast<const bf16x8*>(p.x + m * p.ldx + kb * 32 + 8 * e);
-      }
+    for (int e = 0; e < 4; ++e) {
+      d.x[e] = bf16x8{};
+      if (in && r < p.M) d.x[e] = *reinterpret_cast<const bf16x8*>(p.x + r * p.ldx + kb * 32 + 8 * e);
     }
   };
+  floatx4 acc{};
+  Step cur, nxt;
+  load(wave, cur);
+  for (int t = wave; t < steps; t += kGemvWaves) {
+    load(t + kGemvWaves, nxt);
+    const float s = mx_scale(cur.s);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = mfma16x16x32(mx_bf16x8(cur.w[e], s), cur.x[e], acc);
+    cur = nxt;
+  }
+
+  __shared__ floatx4 s_acc[kGemvWaves][64];
+  s_acc[wave][lane] = acc;
+  __syncthreads();
+  if (wave != 0 || r >= p.M) return;
+#pragma unroll
+  for (int k = 1; k < kGemvWaves; ++k) acc += s_acc[k][lane];
+  const int n = n0 + 4 * g;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < p.N) store_y(p, r, n + e, acc[e]);
+}
+
+// ------------------------------------------------------------------ more rows
+// x through LDS. A block of eight waves, WM along m and 8 / WM along n, forms a tile
+// of BN = 16 RT (8 / WM) columns and BM rows over its k range, in stages of BK: every
+// load goes global -> LDS past the registers, a ring of NST stages keeps NST - 1 in
+// flight, one barrier per stage. Row r of a 16-row group of codes is BK / 2 bytes, row
+// m of x 2 BK; their 16-byte chunk c lies at slot c ^ wswz(r), c ^ (m & 15), so that the
+// 16 rows of a fragment read use all banks. Scales are loaded as words of four (ALIGNED:
+// the rows of scales start at multiples of four bytes), else byte by byte (a load of
+// one byte per lane costs as much as one of sixteen: M=32 N=151936 158 -> 113 us without).
+// 128 rows run at 1.1 PFLOP/s of the CUs they fill (M=512 N=12288 K=4096: 192 tiles, 67
+// us), 32 rows at the loads into LDS (N=4096 K=12288: 11 us for 26.7 MB of weights and
+// 98 KB of x per CU, and 4 for the sum over 8 ranges).
+template <int RT, int BM, int WM, int BK, int NST, bool ALIGNED>
+__global__ __launch_bounds__(512) void mx_tile_kernel(const MxGemm p) {
+  constexpr int NW = 8, WN = NW / WM, BN = 16 * RT * WN, MT = BM / 16 / WM;
+  constexpr int CW = BK / 32, CX = BK / 8;       // 16-byte chunks of a row of codes, of x
+  constexpr int WPT = CW / 4, TPW = RT / WM;     // loads of a 16-row group's codes; groups a wave loads
+  constexpr int PX = BM * CX / 64 / NW, PW = TPW * WPT;
+  constexpr int SB = TPW * 16 * CW;              // scales a wave loads
+  constexpr int PS = ALIGNED ? 1 : SB / 64;
+  constexpr int PER = PX + PW + PS;
+  constexpr int kX = BM * BK * 2, kW = BN * BK / 2, kS = 256 * PS, kStage = kX + kW + NW * kS;  // bytes
+  static_assert(BM * CX % (64 * NW) == 0 && RT % WM == 0 && SB <= 256 && SB % 64 == 0, "whole loads per wave");
+  __shared__ __attribute__((aligned(1024))) char smem[NST * kStage];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wave % WN, wm = wave / WN;
+  const int r = lane & 15, g = lane >> 4;
+  const int tiles_n = (p.N + BN - 1) / BN;
+  const int tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
+  const int n0 = tn * BN, m0 = tm * BM;
+  const int blocks = p.K / kMxBlock, steps = (blocks + CW - 1) / CW;
+  const int t0 = (int)((int64_t)steps * blockIdx.y / gridDim.y), t1 = (int)((int64_t)steps * (blockIdx.y + 1) / gridDim.y);
+  const uint32_t lbase = lds_addr(smem);
+  auto wswz = [](int row) { return row / (16 / CW) & (CW - 1); };
+
+  // This wave's loads, as byte offsets of stage 0 from the tile's first row.
+  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x + (int64_t)m0 * p.ldx, ((int64_t)(min(BM, p.M - m0) - 1) * p.ldx + p.K) * 2);
+  const int nrows = min(BN, p.N - n0);
+  const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w + (int64_t)n0 * p.ldw, (int64_t)(nrows - 1) * p.ldw + p.K / 2);
+  const __amdgpu_buffer_rsrc_t rs = make_rsrc(p.s + (int64_t)n0 * p.lds, (int64_t)(nrows - 1) * p.lds + blocks);
+  const int group0 = RT * wn + TPW * wm;  // first 16-row group it loads
+  uint32_t xoff[PX], woff[PW], soff[PS];
+  int xc[PX], wc[PW], sb[PS];  // and their first chunk, code chunk (= block), scale
+#pragma unroll
+  for (int i = 0; i < PX; ++i) {
+    const int at = (wave * PX + i) * 64 + lane, m = at / CX;
+    xc[i] = at % CX ^ (m & 15);
+    xoff[i] = m0 + m < p.M ? (uint32_t)(m * p.ldx * 2 + xc[i] * 16) : kOOB;
+  }
+#pragma unroll
+  for (int i = 0; i < PW; ++i) {
+    const int at = i % WPT * 64 + lane, row = at / CW, n = 16 * (group0 + i / WPT) + row;
+    wc[i] = at % CW ^ wswz(row);
+    woff[i] = n < nrows ? (uint32_t)(n * p.ldw + wc[i] * 16) : kOOB;
+  }
+#pragma unroll
+  for (int i = 0; i < PS; ++i) {
+    const int at = ALIGNED ? 4 * lane : 64 * i + lane, n = 16 * group0 + at / CW;
+    sb[i] = at % CW;
+    soff[i] = at < SB && n < nrows ? (uint32_t)(n * p.lds + sb[i]) : kOOB;
+  }
+  auto issue = [&](int t) {
+    const uint32_t at = lbase + (uint32_t)((t - t0) % NST) * kStage;
+    const int left = t < t1 ? blocks - t * CW : 0;  // blocks from this stage's first on
+#pragma unroll
+    for (int i = 0; i < PX; ++i)
+      dma16(rx, xoff[i] != kOOB && xc[i] < 4 * left ? xoff[i] + (uint32_t)t * (BK * 2) : kOOB,
+            at + (wave * PX + i) * 1024);
+#pragma unroll
+    for (int i = 0; i < PW; ++i)
+      dma16(rw, woff[i] != kOOB && wc[i] < left ? woff[i] + (uint32_t)t * (BK / 2) : kOOB,
+            at + kX + (group0 * WPT + i) * 1024);
+#pragma unroll
+    for (int i = 0; i < PS; ++i) {
+      // a word's scales past the row's last are the next row's: their codes are not loaded (zeros)
+      const uint32_t off = soff[i] != kOOB && sb[i] < left ? soff[i] + (uint32_t)t * CW : kOOB;
+      if constexpr (ALIGNED) dma4(rs, off, at + kX + kW + wave * kS);
+      else dma1(rs, off, at + kX + kW + wave * kS + 256 * i);
+    }
+  };
+
   floatx4 acc[RT][MT];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = floatx4{};
-  Step cur, nxt;
-  load(t0 + wave, cur);
-  for (int t = t0 + wave; t < t1; t += kGemvWaves) {
-    load(t + kGemvWaves, nxt);
+#pragma unroll 1
+  for (int i = 0; i < NST - 1; ++i) issue(t0 + i);
+  for (int t = t0; t < t1; ++t) {
+    vm_wait<(NST - 2) * PER>();                                       // this wave's part of stage t has landed
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // every wave's; nobody reads stage t - 1 any more
+    issue(t + NST - 1);
+    const char* st = smem + ((t - t0) % NST) * kStage;
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const float s = mx_scale(cur.s[i]);
+    for (int h = 0; h < CW / 4; ++h) {  // 128 k
+      u32x4 w[RT];
+      float s[RT];
+      const int c = 4 * h + g;  // this lane's block
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int from = wn + WN * (i / TPW), at = (i % TPW * 16 + r) * CW + c;  // the wave that loaded it, and where
+        w[i] = *reinterpret_cast<const u32x4*>(st + kX + (RT * wn + i) * (16 * BK / 2) + r * (BK / 2) +
+                                               ((c ^ wswz(r)) << 4));
+        const char* sp = st + kX + kW + from * kS;
+        s[i] = mx_scale(ALIGNED ? *reinterpret_cast<const uint8_t*>(sp + at) : *reinterpret_cast<const uint32_t*>(sp + 4 * at));
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const bf16x8 w = mx_bf16x8(cur.w[i][e], s);
+        bf16x8 x[MT];
 #pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = mfma16x16x32(w, cur.x[j][e], acc[i][j]);
+        for (int j = 0; j < MT; ++j) {
+          const int m = 16 * (MT * wm + j) + r;
+          x[j] = *reinterpret_cast<const bf16x8*>(st + m * (BK * 2) + (((4 * c + e) ^ r) << 4));
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          const bf16x8 a = mx_bf16x8(w[i][e], s[i]);
+#pragma unroll
+          for (int j = 0; j < MT; ++j) acc[i][j] = mfma16x16x32(a, x[j], acc[i][j]);
+        }
       }
     }
-    cur = nxt;
   }
-
-  __shared__ floatx4 s_acc[kGemvWaves][RT * MT][64];
+  vm_wait<0>();  // the ring's last loads (zeros) have landed, and every wave has read its last stage
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  // The sums through LDS, so that a wave stores runs of a row.
+  constexpr int LD = BN + 4;
+  static_assert(BM * LD * 4 <= NST * kStage, "the tile's sums");
+  float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int j = 0; j < MT; ++j) s_acc[wave][i * MT + j][lane] = acc[i][j];
+    for (int j = 0; j < MT; ++j)
+      *reinterpret_cast<floatx4*>(sums + (16 * (MT * wm + j) + r) * LD + 16 * (RT * wn + i) + 4 * g) = acc[i][j];
   __syncthreads();
-  for (int q = wave; q < RT * MT; q += kGemvWaves) {
-    floatx4 v = s_acc[0][q][lane];
-#pragma unroll
-    for (int k = 1; k < kGemvWaves; ++k) v += s_acc[k][q][lane];
-    const int m = 16 * (q % MT) + r, n = n0 + 16 * (q / MT) + 4 * g;
-    if (m >= p.M) continue;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (n + e >= p.N) break;
-      if (p.part)
-        p.part[((int64_t)blockIdx.y * p.M + m) * p.N + n + e] = v[e];
-      else
-        store_y(p, m, n + e, v[e]);
+  float* part = p.part ? p.part + (int64_t)blockIdx.y * p.M * p.N : nullptr;
+  if (p.vec) {
+    for (int at = threadIdx.x; at < BM * BN / 4; at += 64 * NW) {
+      const int m = m0 + at / (BN / 4), n = n0 + at % (BN / 4) * 4;
+      if (m >= p.M || n >= p.N) continue;
+      const floatx4 v = *reinterpret_cast<const floatx4*>(sums + (m - m0) * LD + n - n0);
+      if (part) *reinterpret_cast<floatx4*>(part + (int64_t)m * p.N + n) = v;
+      else store_y4(p, m, n, v);
+    }
+  } else {
+    for (int at = threadIdx.x; at < BM * BN; at += 64 * NW) {
+      const int m = m0 + at / BN, n = n0 + at % BN;
+      if (m >= p.M || n >= p.N) continue;
+      const float v = sums[(m - m0) * LD + n - n0];
+      if (part) part[(int64_t)m * p.N + n] = v;
+      else store_y(p, m, n, v);
     }
   }
 }
 
 // y from the k ranges' sums, added in their order.
-__global__ __launch_bounds__(256) void mx_gemv_sum_kernel(const MxGemm p, int parts) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, mn = (int64_t)p.M * p.N;
-  if (i >= mn) return;
-  float v = 0.f;
-  for (int k = 0; k < parts; ++k) v += p.part[k * mn + i];
-  store_y(p, (int)(i / p.N), (int)(i % p.N), v);
+__global__ __launch_bounds__(256) void mx_sum_kernel(const MxGemm p, int parts) {
+  const int64_t mn = (int64_t)p.M * p.N, t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (p.vec) {
+    if (4 * t >= mn) return;
+    floatx4 v{};
+#pragma unroll 8
+    for (int k = 0; k < parts; ++k) v += *reinterpret_cast<const floatx4*>(p.part + k * mn + 4 * t);
+    store_y4(p, (int)(4 * t / p.N), (int)(4 * t % p.N), v);
+  } else {
+    if (t >= mn) return;
+    float v = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < parts; ++k) v += p.part[k * mn + t];
+    store_y(p, (int)(t / p.N), (int)(t % p.N), v);
+  }
 }
 
-constexpr int64_t kGemvMaxRows = 32;
+// How a product runs: one 16-row weight group per block (kRows), x through LDS in tiles
+// of 32, 64 or 128 rows, or the weights expanded to bf16 for the bf16 GEMM.
+enum Form { kRows, kTile32, kTile64, kTile128, kExpand };
 
-struct GemvPlan {
-  int rt, parts;
+struct Plan {
+  Form form;
+  int bn, bm, parts;  // tile, and ranges of k whose sums are added by mx_sum_kernel
 };
 
-GemvPlan gemv_plan(int64_t M, int64_t N, int64_t K) {
-  GemvPlan g{M > 4 ? 4 : 1, 1};
-  const int64_t tiles = q3_cdiv(N, 16 * g.rt), steps = q3_cdiv(K, 128);
-  while (tiles * g.parts < 256 && steps / (2 * g.parts) >= kGemvWaves && g.rt > 1) g.parts *= 2;
+// kRows up to 4 rows, where x is next to nothing. Up to 64 rows always tiles. Above,
+// tiles unless the expansion is estimated faster: 128 x 256 tiles run in rounds of 256
+// at 1.1 PFLOP/s; expanding costs 2.53 bytes a weight at 5.5 TB/s, 16 us, and the
+// product at 1.3 PFLOP/s. Microseconds, tiles / expanded: N=12288 K=4096 M=64 21 / 69,
+// M=256 45 / 77, M=512 (192 tiles) 67 / 98, M=777 (336) 126 / 115; N=4096 K=12288 M=777 95
+// / 144; N=K=4096 M=777 43 / 55, M=1500 66 / 77; N=K=1024 M=1500 19 / 18. With fewer tiles
+// than CUs, k is split until they fill them (ranges of at least 512 k).
+Plan plan_of(int64_t M, int64_t N, int64_t K) {
+  if (M <= 4) return {kRows, 16, 16, 1};
+  Plan g = M <= 32 ? Plan{kTile32, 128, 32, 1} : M <= 64 ? Plan{kTile64, 256, 64, 1} : Plan{kTile128, 256, 128, 1};
+  const int64_t tiles = q3_cdiv(N, g.bn) * q3_cdiv(M, g.bm);
+  if (g.form == kTile128) {
+    const double nk = (double)N * (double)K;
+    const double tile_us = (double)q3_cdiv(tiles, 256) * 256 * 128 * 256 * 2 * (double)K / 1.1e9;
+    const double expand_us = 2 * (double)M * nk / 1.3e9 + nk * 2.53 / 5.5e6 + 16;
+    if (tiles > 256 && expand_us < tile_us) return {kExpand, 0, 0, 1};
+  }
+  g.parts = (int)std::max<int64_t>(1, std::min<int64_t>(256 / tiles, q3_cdiv(K, 256) / 2));
   return g;
+}
+
+template <int RT, int BM, int WM, int BK, int NST>
+void launch_tile(const MxGemm& p, const Plan& g, hipStream_t st) {
+  const dim3 grid((unsigned)(q3_cdiv(p.N, g.bn) * q3_cdiv(p.M, g.bm)), (unsigned)g.parts);
+  if (p.K % 128 == 0 && p.lds % 4 == 0 && q3_aligned(p.s, 4))  // whole words of scales
+    hipLaunchKernelGGL((mx_tile_kernel<RT, BM, WM, BK, NST, true>), grid, dim3(512), 0, st, p);
+  else
+    hipLaunchKernelGGL((mx_tile_kernel<RT, BM, WM, BK, NST, false>), grid, dim3(512), 0, st, p);
 }
 
 }  // namespace
@@ -146,8 +323,8 @@ extern "C" {
 
 int64_t q3_matmul_mxfp4_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  if (M > kGemvMaxRows) return N * K * 2;  // the weights in bf16
-  const GemvPlan g = gemv_plan(M, N, K);
+  const Plan g = plan_of(M, N, K);
+  if (g.form == kExpand) return N * K * 2;  // the weights in bf16
   return g.parts > 1 ? g.parts * M * N * (int64_t)sizeof(float) : 0;
 }
 
@@ -156,7 +333,9 @@ int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, co
                     int64_t ldc, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   Q3_REQUIRE(x && w_codes && w_scales && y, Q3_ERR_NULL);
   Q3_REQUIRE(M >= 0 && N >= 0 && K >= kMxBlock && K % kMxBlock == 0, Q3_ERR_SHAPE);
-  Q3_REQUIRE(M < (1ll << 31) && N < (1ll << 31) - 256 && K < (1ll << 30), Q3_ERR_SHAPE);
+  Q3_REQUIRE(M < (1ll << 31) && N < (1ll << 31) - 256, Q3_ERR_SHAPE);
+  // The rows of a tile are addressed with 32-bit offsets.
+  Q3_REQUIRE(ldw < (1ll << 22) && lds < (1ll << 22) && ldx < (1ll << 22), Q3_ERR_UNSUPPORTED);
   Q3_REQUIRE(ldx >= K && ldw >= K / 2 && lds >= K / kMxBlock && ldc >= N && (!residual || ldr >= N), Q3_ERR_SHAPE);
   Q3_REQUIRE(dtype == Q3_BF16, Q3_ERR_DTYPE);
   if (M == 0 || N == 0) return Q3_OK;
@@ -165,26 +344,30 @@ int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, co
   Q3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Q3_ERR_WORKSPACE);
   Q3_REQUIRE(need == 0 || q3_aligned(workspace, 16), Q3_ERR_ALIGN);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (M > kGemvMaxRows) {
+  const Plan g = plan_of(M, N, K);
+  if (g.form == kExpand) {
     Q3_REQUIRE(ldw == K / 2 && lds == K / kMxBlock, Q3_ERR_UNSUPPORTED);
     const int rc = mx_expand(w_codes, w_scales, static_cast<bf16*>(workspace), N * K, st);
     if (rc != Q3_OK) return rc;
     return q3_matmul(x, workspace, bias, residual, y, M, N, K, ldx, K, ldr, ldc, dtype, nullptr, 0, stream);
   }
-  const GemvPlan g = gemv_plan(M, N, K);
   MxGemm p{static_cast<const bf16*>(x), static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales),
            static_cast<const bf16*>(bias), static_cast<const bf16*>(residual), static_cast<bf16*>(y),
-           g.parts > 1 ? static_cast<float*>(workspace) : nullptr, (int)M, (int)N, (int)K, ldx, ldw, lds, ldr, ldc};
-  const dim3 grid((unsigned)q3_cdiv(N, 16 * g.rt), (unsigned)g.parts), block(64 * kGemvWaves);
-  if (g.rt == 1)
-    hipLaunchKernelGGL((mx_gemv_kernel<1, 1>), grid, block, 0, st, p);
-  else if (M <= 16)
-    hipLaunchKernelGGL((mx_gemv_kernel<1, 4>), grid, block, 0, st, p);
+           g.parts > 1 ? static_cast<float*>(workspace) : nullptr, (int)M, (int)N, (int)K, ldx, ldw, lds, ldr, ldc, 0};
+  p.vec = N % 4 == 0 && q3_aligned(y, 8) && ldc % 4 == 0 && (!bias || q3_aligned(bias, 8)) &&
+          (!residual || (q3_aligned(residual, 8) && ldr % 4 == 0));
+  if (g.form == kRows)
+    hipLaunchKernelGGL(mx_gemv_kernel, dim3((unsigned)q3_cdiv(N, 16)), dim3(64 * kGemvWaves), 0, st, p);
+  else if (g.form == kTile32)
+    launch_tile<1, 32, 1, 256, 2>(p, g, st);
+  else if (g.form == kTile64)
+    launch_tile<2, 64, 1, 256, 2>(p, g, st);
   else
-    hipLaunchKernelGGL((mx_gemv_kernel<2, 4>), grid, block, 0, st, p);
+    launch_tile<4, 128, 2, 128, 3>(p, g, st);
   Q3_LAUNCH_CHECK();
   if (g.parts > 1) {
-    hipLaunchKernelGGL(mx_gemv_sum_kernel, dim3((unsigned)q3_cdiv(M * N, 256)), dim3(256), 0, st, p, g.parts);
+    hipLaunchKernelGGL(mx_sum_kernel, dim3((unsigned)q3_cdiv(p.vec ? M * N / 4 : M * N, 256)), dim3(256), 0, st, p,
+                       g.parts);
     Q3_LAUNCH_CHECK();
   }
   return Q3_OK;

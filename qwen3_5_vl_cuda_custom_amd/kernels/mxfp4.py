@@ -155,6 +155,8 @@ def matmul_mxfp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bia
     if M == 0 or N == 0:
         return y
     x2, ldx = _rows(op, x, K)
+    if ldx >= 1 << 22 and K < 1 << 22:  # farther apart than the kernels address
+        x2, ldx = x2.contiguous(), K
     if x2.data_ptr() % 16 or ldx % 8:
         x2, ldx = mfma_operand(op, x2.view(-1, K)), K
     r2, ldr = _rows(op, residual, N) if residual is not None else (None, 0)

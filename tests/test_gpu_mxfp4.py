@@ -126,6 +126,14 @@ def test_matmul_matches_float64(m, n, k):
     check_matmul(y, x, codes, scales)
 
 
+@pytest.mark.parametrize("m,n,k", [(1100, 8000, 96), (200, 66000, 64), (2500, 4100, 128), (900, 1001, 2080)])
+def test_matmul_many_tiles_and_expanded_weights(m, n, k):
+    codes, scales = weight(n, k, seed=n)
+    x, b, r = rnd(m, k, seed=m), rnd(n, seed=1), rnd(m, n, seed=2)
+    y = K.matmul_mxfp4(x.to(DEV), codes.to(DEV), scales.to(DEV), b.to(DEV), r.to(DEV))
+    check_matmul(y, x, codes, scales, b, r)
+
+
 @pytest.mark.parametrize("m", [1, 3, 20, 70])
 def test_matmul_bias_residual_out_and_strides(m):
     n, k = 136, 320
@@ -145,7 +153,7 @@ def test_matmul_bias_residual_out_and_strides(m):
     assert K.matmul_mxfp4(x3.to(DEV)[:0], codes.to(DEV), scales.to(DEV)).shape == (0, m, n)
 
 
-@pytest.mark.parametrize("m", [3, 20, 70])
+@pytest.mark.parametrize("m", [3, 20, 50, 70])
 def test_matmul_keeps_a_rows_nan_and_infinity_to_itself(m):
     n, k = 96, 256
     codes, scales = weight(n, k, seed=11)

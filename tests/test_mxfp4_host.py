@@ -64,8 +64,9 @@ def test_matmul_refusals(L):
     assert mm(res=FAKE, ldr=60) == -2
     assert mm(dt=0) == -3
     assert mm(x=FAKE + 2) == -4 and mm(w=FAKE + 4) == -4 and mm(ldw=40) == -4
-    need = L.q3_matmul_mxfp4_workspace_bytes(100, 64, 64)
-    assert need > 0 and mm(M_=100, ws=FAKE, nws=need - 1) == -6 and mm(M_=100) == -6
+    big = dict(M_=5000, N=4096, K=12288, ldx=12288, ldw=6144, lds=384, ldc=4096)  # expands its weights
+    need = L.q3_matmul_mxfp4_workspace_bytes(5000, 4096, 12288)
+    assert need > 0 and mm(**big, ws=FAKE, nws=need - 1) == -6 and mm(**big) == -6
     assert mm(M_=0) == 0 and mm(N=0) == 0
 
 
