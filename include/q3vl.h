@@ -583,8 +583,8 @@ int q3_mxfp4_dequantize(const void* codes, const void* scales, void* y, int64_t 
                         const int64_t* strides, int dtype, void* stream);
 
 /* y = x w^T (+ bias) (+ residual), one rounding: q3_matmul with w (N, K) in MXFP4, code rows ldw and scale rows lds
- * bytes apart. bf16; K a multiple of 32; x and the code rows 16-byte aligned. Up to 32 rows stream the weights;
- * more rows need packed weights (ldw = K / 2, lds = K / 32). */
+ * bytes apart. bf16; K a multiple of 32; x and the code rows 16-byte aligned; row strides below 2^22. Where the
+ * weights are expanded first (many rows), they have to be packed (ldw = K / 2, lds = K / 32). */
 int64_t q3_matmul_mxfp4_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, const void* bias, const void* residual,
                     void* y, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t lds, int64_t ldr,
@@ -598,6 +598,16 @@ int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, co
 int q3_kv_append_mxfp4(const void* k, const void* v, void* k_codes, void* k_scales, void* v_codes, void* v_scales,
                        const int* kv_lens, int64_t B, int64_t S, int64_t Hkv, int64_t D, int64_t cap,
                        const int64_t* strides, int dtype, void* stream);
+
+/* q3_qk_norm_rope whose k and v rows go into the four-bit cache, at rows kv_lens[b] + s (below cap): each is rounded
+ * to bf16, as a bf16 cache holds it, and quantised, so the cache equals q3_qk_norm_rope followed by
+ * q3_kv_append_mxfp4 to the bit. bf16, D = 64, 128 or 256; every row 16-byte aligned. strides = q3_qk_norm_rope's of
+ * q_in, k_in, v_in, q_out, then [b, h] of k_codes, k_scales, v_codes, v_scales in bytes. */
+int q3_qk_norm_rope_mxfp4(const void* q_in, const void* k_in, const void* v_in, void* q_out, void* k_codes,
+                          void* k_scales, void* v_codes, void* v_scales, const void* q_weight, const void* k_weight,
+                          const int* positions, const float* inv_freq, const int* kv_lens, int64_t cap, int64_t B,
+                          int64_t S, int64_t Hq, int64_t Hkv, int64_t D, const int64_t* section, float eps,
+                          const int64_t* strides, int dtype, void* stream);
 
 /* q3_decode_attention over a four-bit cache: sequence b attends to rows [0, kv_lens[b] + advance) (advance = 1: the
  * step, whose row is already written; kv_lens[b] is then incremented in place), at most cap. q, o (B, Hq, D);

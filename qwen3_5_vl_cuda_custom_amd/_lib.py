@@ -119,6 +119,8 @@ _SIGS: dict[str, tuple] = {
     "q3_matmul_mxfp4_workspace_bytes": (c_int64, [_I, _I, _I]),
     "q3_matmul_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, _I, _I, _I, c_int, _V, _I, _V]),
     "q3_kv_append_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, _V, c_int, _V]),
+    "q3_qk_norm_rope_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, _I, _i64p,
+                                      c_float, _V, c_int, _V]),
     "q3_decode_attention_mxfp4_workspace_bytes": (c_int64, [_I, _I, _I, _I]),
     "q3_decode_attention_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, c_int, _V, _I, _I, _I, _I, _I, _V, c_float, c_int,
                                           _V, _I, _V]),

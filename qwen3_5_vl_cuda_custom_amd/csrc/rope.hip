@@ -10,6 +10,8 @@
 //                   projection outputs in (B, S, H, D) layout and written to any
 //                   strided destination (e.g. straight into a KV cache)
 //  q3_qk_norm_rope_backward  its gradients, for training
+//  q3_qk_norm_rope_mxfp4  the same prologue with the k and v rows written into a
+//                   4-bit cache
 //
 // Rotate-half on pairs (i, i + Dr/2) with c = cos[i], s = sin[i], i < Dr/2:
 //   y[i] = x[i] c - x[i + Dr/2] s,   y[i + Dr/2] = x[i + Dr/2] c + x[i] s
@@ -17,6 +19,7 @@
 #include <type_traits>
 
 #include "gemm_bwd.h"
+#include "mxfp4.h"
 #include "q3_common.h"
 
 namespace {
@@ -211,6 +214,11 @@ struct QKNormRopeArgs {
   // cos of the D/2 angles then their sin (for a consumer that rotates q
   // itself). q_in == null: the q rows are not processed (k and v only).
   float* rope_tab;
+  // Four-bit k_out / v_out (MX kernels, instead of the pointers above): codes and
+  // scales of k, then v, with packed rows and (b, h) strides in bytes.
+  uint8_t* codes[2];
+  uint8_t* scales[2];
+  int64_t cst[2][2], sst[2][2];
 };
 
 // One block per (b, s) token. The D/2 rotary angles of the token (pos[axis]
@@ -287,8 +295,10 @@ __device__ __forceinline__ const T* qk_in_row(const QKNormRopeArgs& a, int64_t b
 // One head row of token (b, s), held by a group of G lanes (lane j: elements
 // [8j, 8j+8) in x): RMSNorm (with weights) and mRoPE for q and k rows, then the
 // store (k / v rows at sequence offset so_b, through the block table when
-// paged; rows past dst_seq_cap or on a rejected page are not written).
-template <typename T, int G, bool VEC>
+// paged; rows past dst_seq_cap or on a rejected page are not written). MX: k and
+// v rows are rounded to T, as a cache of T holds them, then quantised; the four
+// lanes of a block are neighbours in the group.
+template <typename T, int G, bool VEC, bool MX = false>
 __device__ __forceinline__ void qk_row(const QKNormRopeArgs& a, int64_t b, int64_t s, int row, int j, int so_b,
                                        float (&x)[8], const float (&cs)[8], const float (&sn)[8],
                                        const float (&wq)[8], const float (&wk)[8]) {
@@ -299,7 +309,7 @@ __device__ __forceinline__ void qk_row(const QKNormRopeArgs& a, int64_t b, int64
   const int so = kind > 0 ? so_b : 0;
   bool skip_store = kind > 0 && (s + (int64_t)so >= a.dst_seq_cap || s + so < 0);
   int64_t ob = b, orow = s + so;  // k / v: page and row within it when paged
-  if (kind > 0 && a.block_table && !skip_store) {
+  if (!MX && kind > 0 && a.block_table && !skip_store) {
     const int pg = a.block_table[b * a.max_pages + orow / a.page_rows];
     if ((unsigned)pg >= (unsigned)a.num_pages) {
       if (a.status && j == 0) atomicOr(a.status, 2);
@@ -331,11 +341,27 @@ __device__ __forceinline__ void qk_row(const QKNormRopeArgs& a, int64_t b, int64
       // lo half: x1*c - x2*s  (partner holds x2); hi half: x2*c + x1*s (partner holds x1).
       x[e] = lo ? (x[e] * cs[e] - p[e] * sn[e]) : (x[e] * cs[e] + p[e] * sn[e]);
   }
+  if constexpr (MX) {
+    if (kind > 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = to_f<T>(from_f<T>(x[e]));
+      uint32_t byte;
+      const uint32_t c = q3::mx_quantize8(x, byte);
+      if (skip_store) return;
+      const bool v = kind == 2;
+      uint8_t* cp = (v ? a.codes[1] : a.codes[0]) + b * (v ? a.cst[1][0] : a.cst[0][0]) + h * (v ? a.cst[1][1] : a.cst[0][1]);
+      uint8_t* sp = (v ? a.scales[1] : a.scales[0]) + b * (v ? a.sst[1][0] : a.sst[0][0]) +
+                    h * (v ? a.sst[1][1] : a.sst[0][1]);
+      reinterpret_cast<uint32_t*>(cp)[orow * G + j] = c;
+      if ((j & 3) == 0) sp[orow * (G / 4) + j / 4] = (uint8_t)byte;
+      return;
+    }
+  }
   if (skip_store) return;
   store8<T, VEC>(out + 8 * j, x);
 }
 
-template <typename T, int G, bool VEC, int BATCH = kQKBatch, int MINB = 1>
+template <typename T, int G, bool VEC, int BATCH = kQKBatch, int MINB = 1, bool MX = false>
 __global__ __launch_bounds__(256, MINB) void qk_norm_rope_kernel(const QKNormRopeArgs a) {
   constexpr int D = G * 8;
   constexpr int HALF = D / 2;
@@ -344,7 +370,7 @@ __global__ __launch_bounds__(256, MINB) void qk_norm_rope_kernel(const QKNormRop
   const int tid = threadIdx.x;
   const int b = blockIdx.x / a.S, s = blockIdx.x % a.S;
   const int j = tid % G;
-  const int nrows = a.Hq + a.Hkv + (a.v_out ? a.Hkv : 0);
+  const int nrows = a.Hq + a.Hkv + (MX || a.v_out ? a.Hkv : 0);
 
   // The token's angles: thread i < HALF loads its position and frequency.
   int posv = 0;
@@ -394,7 +420,7 @@ __global__ __launch_bounds__(256, MINB) void qk_norm_rope_kernel(const QKNormRop
     for (int u = 0; u < BATCH; ++u) {
       const int row = r0 + u * RPP;
       if (row >= nrows) break;
-      qk_row<T, G, VEC>(a, b, s, row, j, so_b, v[u], cs, sn, wq, wk);
+      qk_row<T, G, VEC, MX>(a, b, s, row, j, so_b, v[u], cs, sn, wq, wk);
     }
   }
 }
@@ -503,6 +529,25 @@ int launch_qk(const QKNormRopeArgs& a, hipStream_t st) {
       break;
     default:
       return Q3_ERR_UNSUPPORTED;
+  }
+  Q3_LAUNCH_CHECK();
+  return Q3_OK;
+}
+
+// The k and v rows into a 4-bit cache: bf16, every row start 16-byte aligned.
+int launch_qk_mx(const QKNormRopeArgs& a, hipStream_t st) {
+  const int64_t tokens = (int64_t)a.B * a.S;
+  const int passes = (int)q3_cdiv(a.Hq + 2 * a.Hkv, kQKBatch * (256 / (a.D / 8)));
+  const dim3 grid((unsigned)tokens, tokens <= 256 ? (unsigned)passes : 1u);
+  switch (a.D) {
+    case 64:
+      hipLaunchKernelGGL((qk_norm_rope_kernel<bf16, 8, true, kQKBatch, 1, true>), grid, dim3(256), 0, st, a);
+      break;
+    case 128:
+      hipLaunchKernelGGL((qk_norm_rope_kernel<bf16, 16, true, kQKBatch, 1, true>), grid, dim3(256), 0, st, a);
+      break;
+    default:
+      hipLaunchKernelGGL((qk_norm_rope_kernel<bf16, 32, true, kQKBatch, 1, true>), grid, dim3(256), 0, st, a);
   }
   Q3_LAUNCH_CHECK();
   return Q3_OK;
@@ -778,6 +823,59 @@ int q3_qk_norm_rope_paged(const void* q_in, const void* k_in, const void* v_in, 
   return qk_impl(q_in, k_in, v_in, q_out, k_pages, v_pages, q_weight, k_weight, positions, inv_freq, kv_lens,
                  max_pages * page_rows, B, S, Hq, Hkv, D, section, eps, strides, dtype, block_table, max_pages,
                  page_rows, num_pages, status, stream);
+}
+
+int q3_qk_norm_rope_mxfp4(const void* q_in, const void* k_in, const void* v_in, void* q_out, void* k_codes,
+                          void* k_scales, void* v_codes, void* v_scales, const void* q_weight, const void* k_weight,
+                          const int* positions, const float* inv_freq, const int* kv_lens, int64_t cap, int64_t B,
+                          int64_t S, int64_t Hq, int64_t Hkv, int64_t D, const int64_t* section, float eps,
+                          const int64_t* strides, int dtype, void* stream) {
+  Q3_REQUIRE(q_in && k_in && v_in && q_out && k_codes && k_scales && v_codes && v_scales && positions && inv_freq &&
+                 kv_lens && section && strides,
+             Q3_ERR_NULL);
+  Q3_REQUIRE((q_weight == nullptr) == (k_weight == nullptr), Q3_ERR_NULL);
+  Q3_REQUIRE(B >= 0 && S >= 0 && Hq >= 1 && Hkv >= 1 && D >= 16 && cap >= 0, Q3_ERR_SHAPE);
+  Q3_REQUIRE(section[0] >= 0 && section[1] >= 0 && section[2] >= 0 && section[0] + section[1] + section[2] == D / 2,
+             Q3_ERR_SHAPE);
+  Q3_REQUIRE(dtype == Q3_BF16, Q3_ERR_DTYPE);
+  Q3_REQUIRE(D == 64 || D == 128 || D == 256, Q3_ERR_UNSUPPORTED);
+  if (B == 0 || S == 0) return Q3_OK;
+  Q3_REQUIRE(B < (1ll << 31) && S < (1ll << 31) / B && Hq < (1 << 20) && Hkv < (1 << 20), Q3_ERR_SHAPE);
+  bool ok = q3_aligned(q_in, 16) && q3_aligned(k_in, 16) && q3_aligned(v_in, 16) && q3_aligned(q_out, 16) &&
+            q3_aligned(q_weight, 16) && q3_aligned(k_weight, 16) && q3_aligned(k_codes, 4) && q3_aligned(v_codes, 4);
+  for (int i = 0; i < 12; ++i) ok = ok && strides[i] % 8 == 0;
+  for (int i : {12, 13, 16, 17}) ok = ok && strides[i] % 4 == 0;
+  Q3_REQUIRE(ok, Q3_ERR_ALIGN);
+  QKNormRopeArgs a{};
+  a.q_in = q_in;
+  a.k_in = k_in;
+  a.v_in = v_in;
+  a.q_out = q_out;
+  a.q_w = q_weight;
+  a.k_w = k_weight;
+  a.pos = positions;
+  a.inv_freq = inv_freq;
+  a.dst_seq_off = kv_lens;
+  a.dst_seq_cap = cap;
+  a.B = (int)B;
+  a.S = (int)S;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.D = (int)D;
+  a.s0 = (int)section[0];
+  a.s1 = (int)section[1];
+  a.eps = eps;
+  for (int i = 0; i < 12; ++i) a.st[i] = strides[i];
+  a.codes[0] = static_cast<uint8_t*>(k_codes);
+  a.codes[1] = static_cast<uint8_t*>(v_codes);
+  a.scales[0] = static_cast<uint8_t*>(k_scales);
+  a.scales[1] = static_cast<uint8_t*>(v_scales);
+  for (int kv = 0; kv < 2; ++kv)
+    for (int i = 0; i < 2; ++i) {
+      a.cst[kv][i] = strides[12 + 4 * kv + i];
+      a.sst[kv][i] = strides[14 + 4 * kv + i];
+    }
+  return launch_qk_mx(a, static_cast<hipStream_t>(stream));
 }
 
 int64_t q3_qk_norm_rope_backward_workspace_bytes(int64_t B, int64_t S, int64_t D) {

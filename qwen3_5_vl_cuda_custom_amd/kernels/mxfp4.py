@@ -21,7 +21,7 @@ from ._common import mfma_operand, require_device, require_no_grad
 
 MX_BLOCK = 32
 _U8, _BF16, _F32 = torch.uint8, torch.bfloat16, torch.float32
-_i64x4, _i64x14 = Struct("4q").pack, Struct("14q").pack
+_i64x4, _i64x14, _i64x20 = Struct("4q").pack, Struct("14q").pack, Struct("20q").pack
 
 
 def _off_device(op: str, *tensors: torch.Tensor | None) -> None:
@@ -240,6 +240,56 @@ def kv_append_mxfp4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_s
     _lib.call("q3_kv_append_mxfp4", k.data_ptr(), v.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(),
               v_codes.data_ptr(), v_scales.data_ptr(), kv_lens.data_ptr(), B, S, Hkv, D, cap,
               _i64x14(*ks[:3], *vs[:3], *st), dt, _lib.raw_stream(dev))
+
+
+def qk_norm_rope_mxfp4(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torch.Tensor, q_out: torch.Tensor,
+                       k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
+                       q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, positions: torch.Tensor,
+                       inv_freq: torch.Tensor, mrope_section, eps: float, kv_lens: torch.Tensor) -> None:
+    """qk_norm_rope with the k/v rows quantised into a four-bit cache at rows kv_lens[b] + s, in one launch.
+
+    q_in, q_out (B, S, Hq, D), k_in, v_in (B, S, Hkv, D) bf16 views with 16-byte aligned rows (q_out may be q_in); D
+    64, 128 or 256. The rows are rounded to bf16 first, so the cache equals qk_norm_rope followed by kv_append_mxfp4
+    to the bit.
+    """
+    op = "qk_norm_rope_mxfp4"
+    ts = (q_in, k_in, v_in, q_out)
+    require_no_grad(op, *ts, q_weight, k_weight)
+    if any(t.dim() != 4 for t in ts):
+        raise ValueError(f"{op}: q, k and v must be (B, S, H, D)")
+    B, S, Hq, D = q_in.shape
+    dev = q_in.get_device()
+    Hkv, cap, st = _check_cache(op, dev, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D)
+    if k_in.shape != (B, S, Hkv, D) or v_in.shape != k_in.shape or q_out.shape != q_in.shape:
+        raise ValueError(f"{op}: q {tuple(q_in.shape)} -> {tuple(q_out.shape)}, k {tuple(k_in.shape)}, v "
+                         f"{tuple(v_in.shape)} for a cache of {Hkv} heads")
+    strides = []
+    for t in ts:
+        s = t.stride()
+        if t.get_device() != dev:
+            _off_device(op, t)
+        if t.dtype != _BF16:
+            raise TypeError(f"{op}: bfloat16 only, got {t.dtype}")
+        if s[3] != 1 or t.data_ptr() % 16 or s[0] % 8 or s[1] % 8 or s[2] % 8:
+            raise ValueError(f"{op}: every row must be 16-byte aligned with a contiguous head dim")
+        strides += s[:3]
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError(f"{op}: give both norm weights or none")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.get_device() != dev or w.dtype != _BF16 or w.shape != (D,) or not w.is_contiguous()
+                              or w.data_ptr() % 16):
+            raise ValueError(f"{op}: norm weights must be contiguous, 16-byte aligned bfloat16 ({D},) device tensors")
+    if (positions.dtype != torch.int32 or positions.get_device() != dev or positions.shape != (3, B, S)
+            or not positions.is_contiguous()):
+        raise ValueError(f"{op}: positions must be a contiguous int32 (3, {B}, {S}) device tensor")
+    if inv_freq.dtype != _F32 or inv_freq.get_device() != dev or inv_freq.numel() != D // 2:
+        raise ValueError(f"{op}: inv_freq must be a float32 ({D // 2},) device tensor")
+    if len(mrope_section) != 3 or sum(mrope_section) * 2 != D:
+        raise ValueError(f"{op}: mrope_section {list(mrope_section)} must be three counts that sum to D/2 = {D // 2}")
+    _lib.call("q3_qk_norm_rope_mxfp4", q_in.data_ptr(), k_in.data_ptr(), v_in.data_ptr(), q_out.data_ptr(),
+              k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), _lib.ptr(q_weight),
+              _lib.ptr(k_weight), positions.data_ptr(), inv_freq.data_ptr(), kv_lens.data_ptr(), cap, B, S, Hq, Hkv, D,
+              _lib.i64s(*mrope_section), eps, _i64x20(*strides, *st), _lib.Q3_BF16, _lib.raw_stream(dev))
 
 
 def _query(op: str, q: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:

@@ -16,9 +16,8 @@ from torch import nn
 
 from ..configs import Qwen3VLConfig
 from ..kernels import cuda_index_add
-from ..modules import (CudaEmbedding, CudaLinear, CudaRMSNorm, CudaTextDecoderLayer, PagedKVCache, StaticKVCache,
-                       StepGraph,
-                       TextMRoPE)
+from ..modules import (CudaEmbedding, CudaLinear, CudaRMSNorm, CudaTextDecoderLayer, MXFP4KVCache, PagedKVCache,
+                       StaticKVCache, StepGraph, TextMRoPE)
 from .common import CudaVisionTower
 
 
@@ -86,15 +85,28 @@ class _TextLM(nn.Module):
                 x = self._deepstack_process(x, visual_pos_masks, deepstack_visual_embeds[i])
         return self.norm(x), new_kvs
 
+    def _head_weight(self) -> torch.Tensor:
+        """The tensor whose device and type the serving path goes by: lm_head's weight, or where that is in four bits
+        the final norm's."""
+        return self.lm_head.weight if isinstance(self.lm_head, CudaLinear) else self.norm.weight
+
     # ------------------------------------------------------------ KV-cache serving path
     def new_caches(self, batch: int, capacity: int, device=None, dtype=None, *, page_rows: int = 0,
-                   num_pages: int | None = None) -> list[StaticKVCache] | list[PagedKVCache]:
+                   num_pages: int | None = None, kv_format: str | None = None
+                   ) -> list[StaticKVCache] | list[PagedKVCache] | list[MXFP4KVCache]:
         """One cache per layer, empty, for `batch` sequences of up to `capacity` tokens: a StaticKVCache,
-        or with page_rows > 0 a PagedKVCache of `num_pages` pages (default: enough for every sequence
-        to reach `capacity`)."""
+        with page_rows > 0 a PagedKVCache of `num_pages` pages (default: enough for every sequence
+        to reach `capacity`), or with kv_format="mxfp4" an MXFP4KVCache (bf16 models)."""
         t = self.cfg.text
-        dev = device if device is not None else self.lm_head.weight.device
-        dt = dtype if dtype is not None else self.lm_head.weight.dtype
+        head = self._head_weight()
+        dev = device if device is not None else head.device
+        dt = dtype if dtype is not None else head.dtype
+        if kv_format not in (None, "mxfp4"):
+            raise ValueError(f"new_caches: kv_format must be None or 'mxfp4', got {kv_format!r}")
+        if kv_format == "mxfp4":
+            if page_rows > 0 or dt != torch.bfloat16:
+                raise ValueError("new_caches: kv_format='mxfp4' takes bfloat16 and no pages")
+            return [MXFP4KVCache(batch, t.num_kv_heads, capacity, t.head_dim, device=dev) for _ in range(t.num_layers)]
         if page_rows > 0:
             per_seq = -(-capacity // page_rows)
             n = num_pages if num_pages is not None else batch * per_seq
@@ -109,7 +121,7 @@ class _TextLM(nn.Module):
                  deepstack_visual_embeds: list[torch.Tensor] | None = None,
                  inputs_embeds: torch.Tensor | None = None, *, prompt_lens=None,
                  rope_deltas: torch.Tensor | None = None, use_graph: bool = True,
-                 page_rows: int = 0) -> torch.Tensor:
+                 page_rows: int = 0, kv_format: str | None = None) -> torch.Tensor:
         """Greedy decoding (reference models/dense.py:123-162). Returns (B, S + new tokens):
         each row's prompt (as given, padding included) followed by its generated tokens.
 
@@ -119,14 +131,16 @@ class _TextLM(nn.Module):
         Generation stops early only when every sequence has just produced
         `eos_token_id`, as in the reference. page_rows > 0 keeps the KV cache
         in pages of that many rows (a multiple of 32) instead of one
-        preallocated block per sequence.
+        preallocated block per sequence; kv_format="mxfp4" keeps it in four
+        bits (the prompt attends to its unquantised rows, the new tokens to the
+        quantised ones).
         """
         B, S = input_ids.shape
-        dev = self.lm_head.weight.device
+        dev = self._head_weight().device
         lens = [int(v) for v in prompt_lens] if prompt_lens is not None else [S] * B
         if len(lens) != B or min(lens) < 1 or max(lens) > S:
             raise ValueError("generate: prompt_lens must give 1..S tokens for every sequence")
-        caches = self.new_caches(B, S + max_new_tokens, dev, page_rows=page_rows)
+        caches = self.new_caches(B, S + max_new_tokens, dev, page_rows=page_rows, kv_format=kv_format)
         emb = inputs_embeds if inputs_embeds is not None else self.embed_tokens(input_ids.to(dev))
         pos3 = text_positions(position_ids, B, S, 0, dev)
         h, _ = self._run_layers(emb, self.rotary.bind(pos3), visual_pos_masks, deepstack_visual_embeds,

@@ -3,11 +3,12 @@
 from .attention import CudaFullAttention, CudaVisionAttention
 from .embedding import CudaEmbedding
 from .graph import StepGraph
-from .kv_cache import PagedKVCache, StaticKVCache
+from .kv_cache import MXFP4KVCache, PagedKVCache, StaticKVCache
 from .linear import CudaLinear
 from .mlp import CudaSwiGLUMLP, CudaVisionMLP
 from .moe import CudaSparseMoE
 from .norms import CudaLayerNorm, CudaRMSNorm
+from .quantized import CudaLinearMXFP4, quantize_text_linears
 from .rotary import MRoPEBinding, TextMRoPE, Vision2DRoPE
 from .text_decoder import CudaTextDecoderLayer
 from .vision_block import CudaVisionBlock
@@ -32,5 +33,8 @@ __all__ = [
     "CudaVisionPatchMerger",
     "PagedKVCache",
     "StaticKVCache",
+    "MXFP4KVCache",
+    "CudaLinearMXFP4",
+    "quantize_text_linears",
     "StepGraph",
 ]

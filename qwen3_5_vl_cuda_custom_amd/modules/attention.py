@@ -7,11 +7,12 @@ from torch.nn.modules import module as nn_module
 
 from ..kernels.backward import (FlashAttentionFunction, QKNormRopeFunction, RopeAttentionFunction, attention_bshd_ok,
                                 needs_grad)
-from ..kernels import (apply_rope, decode_attention, decode_attention_paged, flash_attention, flash_attention_cache,
-                       flash_attention_cache_paged,
-                       flash_attention_varlen, matmul_segments, qk_norm_rope, qk_norm_rope_attention,
-                       qk_norm_rope_attention_ok, qk_norm_rope_paged, rmsnorm_matmul_segments)
-from .kv_cache import PagedKVCache, StaticKVCache
+from ..kernels import (apply_rope, decode_attention, decode_attention_mxfp4, decode_attention_paged, flash_attention,
+                       flash_attention_cache, flash_attention_cache_mxfp4, flash_attention_cache_paged,
+                       flash_attention_varlen, kv_append_mxfp4, matmul, matmul_segments, qk_norm_rope,
+                       qk_norm_rope_attention, qk_norm_rope_attention_ok, qk_norm_rope_mxfp4, qk_norm_rope_paged,
+                       rmsnorm_matmul_segments)
+from .kv_cache import MXFP4KVCache, PagedKVCache, StaticKVCache
 from .linear import CudaLinear
 from .norms import CudaRMSNorm, fused_norm_ok
 from .rotary import MRoPEBinding, TextMRoPE
@@ -95,6 +96,10 @@ class CudaFullAttention(nn.Module):
       kv_cache=PagedKVCache   the same over a paged cache: decode and prefill
                               chunks read the pages in place through the
                               block table; returns (k_pages, v_pages)
+      kv_cache=MXFP4KVCache   the same over a four-bit cache: rows are quantised
+                              as they are written and read in place; a prefill
+                              into an empty cache attends to its unquantised
+                              rows; returns the cache's (k_codes, v_codes)
       residual=tensor         added to o_proj's output in the GEMM epilogue
       input_norm=CudaRMSNorm  x is the layer input before this RMSNorm; for
                               decode shapes (at most 32 tokens, bf16) the norm
@@ -133,14 +138,18 @@ class CudaFullAttention(nn.Module):
             return self._forward_autograd(x, mrope_apply, past_kv, kv_cache, residual, input_norm)
         # q/k/v projections in one GEMM over the three weights (no concatenated
         # copy); q, k, v are column views of its output.
-        weights = (self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
-        biases = (self.q_proj.bias, self.k_proj.bias, self.v_proj.bias)
-        if input_norm is not None and fused_norm_ok(x, input_norm):
-            qkv = rmsnorm_matmul_segments(x, input_norm.weight, input_norm.eps, weights, biases)
+        projs = (self.q_proj, self.k_proj, self.v_proj)
+        if not all(isinstance(p, CudaLinear) for p in projs):
+            qkv = self._project_apart(x if input_norm is None else input_norm(x), projs)
         else:
-            if input_norm is not None:
-                x = input_norm(x)
-            qkv = matmul_segments(x, weights, biases)
+            weights = tuple(p.weight for p in projs)
+            biases = tuple(p.bias for p in projs)
+            if input_norm is not None and fused_norm_ok(x, input_norm):
+                qkv = rmsnorm_matmul_segments(x, input_norm.weight, input_norm.eps, weights, biases)
+            else:
+                if input_norm is not None:
+                    x = input_norm(x)
+                qkv = matmul_segments(x, weights, biases)
         q = qkv[..., :Hq * D].view(B, S, Hq, D)
         k = qkv[..., Hq * D:(Hq + Hkv) * D].view(B, S, Hkv, D)
         v = qkv[..., (Hq + Hkv) * D:].view(B, S, Hkv, D)
@@ -157,9 +166,13 @@ class CudaFullAttention(nn.Module):
             pos = mrope_apply.positions_int32(x.device, B, S)
             if isinstance(kv_cache, PagedKVCache):
                 kv_cache.check_kernels(self.num_kv_groups)
+            elif isinstance(kv_cache, MXFP4KVCache):
+                kv_cache.check_kernels(self.q_norm.weight.dtype if x.dtype == torch.bfloat16 else x.dtype, Hkv, D)
             kv_cache.reserve(S)  # raises, before any launch, if a sequence would overflow the cache
             if isinstance(kv_cache, PagedKVCache):
                 return self._forward_paged(q, k, v, o, pos, rope, kv_cache, residual)
+            if isinstance(kv_cache, MXFP4KVCache):
+                return self._forward_mxfp4(q, k, v, o, pos, rope, kv_cache, residual)
             kc, vc = kv_cache.k.transpose(1, 2), kv_cache.v.transpose(1, 2)  # (B, cap, Hkv, D) views
             # The new tokens' K/V rows go to cache rows [lens[b], lens[b] + S).
             qk_norm_rope(q, k, v, q, kc, vc, self.q_norm.weight, self.k_norm.weight, pos, rope.inv_freq,
@@ -200,6 +213,21 @@ class CudaFullAttention(nn.Module):
         flash_attention(qh, kh, vh, scale=self.scale, is_causal=is_causal, num_kv_groups=self.num_kv_groups,
                         out=o.transpose(1, 2))
         return self.o_proj(o.view(B, S, Hq * D), residual=residual), (kh, vh)
+
+    @staticmethod
+    def _project_apart(x, projs) -> torch.Tensor:
+        """The q/k/v rows side by side where some projections hold four-bit weights: one product each, into its
+        columns."""
+        qkv = torch.empty((*x.shape[:-1], sum(p.out_features for p in projs)), dtype=x.dtype, device=x.device)
+        at = 0
+        for p in projs:
+            out = qkv[..., at:at + p.out_features]
+            if isinstance(p, CudaLinear):
+                matmul(x, p.weight, p.bias, out=out)
+            else:
+                p(x, out=out)
+            at += p.out_features
+        return qkv
 
     def _forward_autograd(self, x, mrope_apply, past_kv, kv_cache, residual, input_norm):
         """Training: the reference composition (modules/attention.py:75-98) on the differentiable ops
@@ -257,6 +285,36 @@ class CudaFullAttention(nn.Module):
                 or rope.inv_freq.dtype != torch.float32 or rope.inv_freq.numel() * 2 != self.head_dim):
             return None
         return pid.to(torch.int32, copy=True).expand(3, B, S).contiguous()
+
+    def _forward_mxfp4(self, q, k, v, o, pos, rope, kv_cache: MXFP4KVCache, residual):
+        B, S, Hq, D = q.shape
+        oh = o.transpose(1, 2)
+        # kv_cache.reserve has counted the S new rows already
+        capturing = torch.cuda.is_current_stream_capturing()
+        if S > 1 and kv_cache.max_len == S and not capturing:
+            # A prefill into an empty cache: attention over the rows as they are, then into the cache. A captured
+            # chunk takes the other path: its replays find the cache filled.
+            if self.q_norm.weight.dtype == q.dtype and qk_norm_rope_attention_ok(q, k, self.num_kv_groups, v):
+                qk_norm_rope_attention(q, k, v, self.q_norm.weight, self.k_norm.weight, pos, rope.inv_freq,
+                                       rope.mrope_section, self.q_norm.eps, self.scale, True, out=o)
+            else:
+                qk_norm_rope(q, k, None, q, k, None, self.q_norm.weight, self.k_norm.weight, pos, rope.inv_freq,
+                             rope.mrope_section, self.q_norm.eps)
+                flash_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), self.scale, True,
+                                self.num_kv_groups, out=oh)
+            kv_append_mxfp4(k, v, *kv_cache.tensors, kv_cache.lens)
+            kv_cache.lens.add_(S)
+        else:
+            qk_norm_rope_mxfp4(q, k, v, q, *kv_cache.tensors, self.q_norm.weight, self.k_norm.weight, pos,
+                               rope.inv_freq, rope.mrope_section, self.q_norm.eps, kv_cache.lens)
+            if S == 1:
+                decode_attention_mxfp4(q[:, 0], *kv_cache.tensors, kv_cache.lens, self.scale, out=o[:, 0], append=True)
+            else:
+                # a captured chunk is replayed over longer caches than the host knows of now
+                flash_attention_cache_mxfp4(q.transpose(1, 2), *kv_cache.tensors, kv_cache.lens, self.scale,
+                                            self.num_kv_groups, out=oh, advance=True,
+                                            max_len=kv_cache.capacity if capturing else kv_cache.max_len)
+        return self.o_proj(o.view(B, S, Hq * D), residual=residual), (kv_cache.k_codes, kv_cache.v_codes)
 
     def _forward_paged(self, q, k, v, o, pos, rope, kv_cache: PagedKVCache, residual):
         B, S, Hq, D = q.shape

@@ -7,6 +7,9 @@ from __future__ import annotations
 
 import torch
 
+from ..kernels import kv_append_mxfp4, mxfp4_dequantize
+from ..kernels.mxfp4 import MX_BLOCK
+
 
 class StaticKVCache:
     """k, v: (B, Hkv, capacity, D); lens: (B,) int32 on the device (valid rows per sequence).
@@ -43,9 +46,9 @@ class StaticKVCache:
         """Overwrite the per-sequence lengths (one host read of the new values)."""
         host = torch.as_tensor(lens, dtype=torch.int64).cpu().reshape(-1)
         if host.numel() != self.batch:
-            raise ValueError(f"StaticKVCache: {host.numel()} lengths for a batch of {self.batch}")
+            raise ValueError(f"{type(self).__name__}: {host.numel()} lengths for a batch of {self.batch}")
         if host.numel() and (int(host.min()) < 0 or int(host.max()) > self.capacity):
-            raise ValueError(f"StaticKVCache: lengths must lie in [0, {self.capacity}]")
+            raise ValueError(f"{type(self).__name__}: lengths must lie in [0, {self.capacity}]")
         self.lens.copy_(host.to(torch.int32))
         self.min_len = int(host.min()) if host.numel() else 0
         self.max_len = int(host.max()) if host.numel() else 0
@@ -53,7 +56,7 @@ class StaticKVCache:
     def check_reserve(self, n: int) -> None:
         """Raise if appending `n` rows to every sequence would overflow (nothing changes)."""
         if self.max_len + n > self.capacity:
-            raise ValueError(f"StaticKVCache overflow: appending {n} row(s) to a sequence of length "
+            raise ValueError(f"{type(self).__name__} overflow: appending {n} row(s) to a sequence of length "
                              f"{self.max_len} exceeds the capacity {self.capacity}")
 
     def reserve(self, n: int) -> None:
@@ -71,6 +74,67 @@ class StaticKVCache:
 
     def set_host_state(self, state: tuple[int, int]) -> None:
         self.min_len, self.max_len = state
+
+
+class MXFP4KVCache(StaticKVCache):
+    """StaticKVCache held in four bits (MXFP4, blocks of 32 along the head dim): 4.25 bits a value, an eighth more
+    than a quarter of a bf16 cache (no reference counterpart).
+
+    k_codes, v_codes: (B, Hkv, capacity, D / 2), k_scales, v_scales: (B, Hkv, capacity, D / 32), uint8; `lens` and the
+    host's lengths as in StaticKVCache. Rows are quantised from bf16 as they are written and read in place by the
+    attention kernels (bf16 queries, head_dim 64 or 128, up to 1024 sequences).
+    """
+
+    def __init__(self, batch: int, num_kv_heads: int, capacity: int, head_dim: int, *,
+                 device: torch.device | str = "cuda", lens: torch.Tensor | None = None) -> None:
+        if head_dim not in (64, 128):
+            raise ValueError(f"MXFP4KVCache: head_dim must be 64 or 128, got {head_dim}")
+        if batch > PAGED_MAX_BATCH:
+            raise ValueError(f"MXFP4KVCache: at most {PAGED_MAX_BATCH} sequences, got {batch}")
+        self.capacity = capacity
+        rows = batch, num_kv_heads, capacity
+        self.k_codes = torch.zeros(*rows, head_dim // 2, dtype=torch.uint8, device=device)
+        self.v_codes = torch.zeros_like(self.k_codes)
+        self.k_scales = torch.zeros(*rows, head_dim // MX_BLOCK, dtype=torch.uint8, device=device)
+        self.v_scales = torch.zeros_like(self.k_scales)
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.min_len = self.max_len = 0
+        if lens is not None:
+            self.set_lens(lens)
+
+    @classmethod
+    def from_static(cls, cache: StaticKVCache) -> "MXFP4KVCache":
+        """The rows and lengths of a bf16 (or fp32) cache, quantised."""
+        B, Hkv, cap, D = cache.k.shape
+        new = cls(B, Hkv, cap, D, device=cache.k.device)
+        kv_append_mxfp4(cache.k.transpose(1, 2), cache.v.transpose(1, 2), *new.tensors, new.lens)  # from row 0
+        new.lens.copy_(cache.lens)
+        new.set_host_state(cache.host_state())
+        return new
+
+    def check_kernels(self, dtype: torch.dtype, num_kv_heads: int, head_dim: int) -> None:
+        """Raise unless the attention of these rows can use this cache. Checked before a step changes any state."""
+        have = self.k_codes.shape[1], self.k_codes.shape[3] * 2
+        if dtype != torch.bfloat16 or have != (num_kv_heads, head_dim):
+            raise ValueError(f"MXFP4KVCache: holds bfloat16 rows of {have[0]} heads x {have[1]}, got {dtype} of "
+                             f"{num_kv_heads} x {head_dim}")
+
+    @property
+    def batch(self) -> int:
+        return self.k_codes.shape[0]
+
+    @property
+    def tensors(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+        """(k_codes, k_scales, v_codes, v_scales), as the four-bit cache ops take them."""
+        return self.k_codes, self.k_scales, self.v_codes, self.v_scales
+
+    def gather(self, rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The first `rows` rows of every sequence as (B, Hkv, rows, D) bf16 keys and values (rows past a sequence's
+        length: whatever the cache holds there)."""
+        if not 0 <= rows <= self.capacity:
+            raise ValueError(f"MXFP4KVCache: rows must lie in [0, {self.capacity}]")
+        return (mxfp4_dequantize(self.k_codes[:, :, :rows], self.k_scales[:, :, :rows]),
+                mxfp4_dequantize(self.v_codes[:, :, :rows], self.v_scales[:, :, :rows]))
 
 
 PAGED_MAX_BATCH = 1024  # the paged decode kernel's batch bound

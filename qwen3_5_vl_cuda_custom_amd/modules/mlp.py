@@ -35,6 +35,11 @@ class CudaSwiGLUMLP(nn.Module):
             if input_norm is not None:
                 x = input_norm(x)
             return self.down_proj(swiglu(self.gate_proj(x), self.up_proj(x)), residual=residual)
+        if not all(isinstance(p, CudaLinear) for p in (self.gate_proj, self.up_proj)):
+            # four-bit weights (CudaLinearMXFP4): each projection by its own forward
+            if input_norm is not None:
+                x = input_norm(x)
+            return self.down_proj(swiglu(self.gate_proj(x), self.up_proj(x)), residual=residual)
         no_bias = self.gate_proj.bias is None and self.up_proj.bias is None
         if input_norm is not None and no_bias and fused_norm_ok(x, input_norm):
             act = rmsnorm_matmul_swiglu(x, input_norm.weight, input_norm.eps, self.gate_proj.weight,

@@ -98,3 +98,36 @@ def test_cache_refusals(L):
                                                 1.0, 0, 1, ws, nws, None)
     assert chunk(Sq=129) == -2 and chunk(nws=0) == -6 and chunk(ws=None) == -6
     assert chunk(Sq=0) == 0
+
+
+def test_fused_append_refusals(L):
+    st, sec = i64(*([128] * 20)), i64(24, 20, 20)
+
+    def f(q=FAKE, w=FAKE, kw=FAKE, D=128, s=st, sec=sec, dt=1, B=2, S=1, kc=FAKE):
+        return L.q3_qk_norm_rope_mxfp4(q, FAKE, FAKE, FAKE, kc, FAKE, FAKE, FAKE, w, kw, FAKE, FAKE, FAKE, 32, B, S, 8,
+                                       2, D, sec, 1e-6, bytes(s), dt, None)
+    assert f(q=None) == -1 and f(kw=None) == -1
+    assert f(sec=i64(24, 20, 21)) == -2 and f(B=1 << 20, S=1 << 20) == -2
+    assert f(dt=0) == -3
+    assert f(D=96, sec=i64(16, 16, 16)) == -5
+    assert f(q=FAKE + 8) == -4 and f(kc=FAKE + 2) == -4 and f(s=i64(4, *([128] * 19))) == -4
+    assert f(B=0) == 0 and f(S=0) == 0
+
+
+def test_cache_lengths_on_the_host():
+    from qwen3_5_vl_cuda_custom_amd.modules import MXFP4KVCache
+    c = MXFP4KVCache(3, 2, 40, 64, device="cpu")
+    assert c.batch == 3 and c.empty and [t.shape[-1] for t in c.tensors] == [32, 2, 32, 2]
+    c.set_lens([5, 0, 33])
+    assert (c.min_len, c.max_len, c.lens.tolist()) == (0, 33, [5, 0, 33])
+    c.reserve(7)
+    with pytest.raises(ValueError, match="MXFP4KVCache overflow"):
+        c.reserve(1)
+    assert c.host_state() == (7, 40)
+    for bad in (lambda: c.set_lens([41, 0, 0]), lambda: c.set_lens([1]), lambda: MXFP4KVCache(1, 1, 8, 96, device="cpu"),
+                lambda: MXFP4KVCache(1025, 1, 8, 64, device="cpu"), lambda: c.gather(41),
+                lambda: c.check_kernels(torch.float32, 2, 64), lambda: c.check_kernels(torch.bfloat16, 2, 128),
+                lambda: c.check_kernels(torch.bfloat16, 4, 64)):
+        with pytest.raises(ValueError):
+            bad()
+    c.check_kernels(torch.bfloat16, 2, 64)
