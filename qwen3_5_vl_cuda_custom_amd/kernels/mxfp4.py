@@ -12,6 +12,7 @@ decode step take a few microseconds each, so the checks here are written for the
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from struct import Struct
 
 import torch
@@ -22,6 +23,16 @@ from ._common import mfma_operand, require_device, require_no_grad
 MX_BLOCK = 32
 _U8, _BF16, _F32 = torch.uint8, torch.bfloat16, torch.float32
 _i64x4, _i64x14, _i64x20 = Struct("4q").pack, Struct("14q").pack, Struct("20q").pack
+
+
+@lru_cache(maxsize=4096)
+def _matmul_workspace(M: int, N: int, K: int) -> int:
+    return _lib.lib().q3_matmul_mxfp4_workspace_bytes(M, N, K)
+
+
+@lru_cache(maxsize=1024)
+def _decode_workspace(B: int, Hq: int, Hkv: int, D: int) -> int:
+    return _lib.lib().q3_decode_attention_mxfp4_workspace_bytes(B, Hq, Hkv, D)
 
 
 def _off_device(op: str, *tensors: torch.Tensor | None) -> None:
@@ -47,14 +58,15 @@ def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     dev = x.get_device()
     if dev < 0 or dev != _lib.current_device():
         _off_device("mxfp4_quantize", x)
-    require_no_grad("mxfp4_quantize", x)
+    if x.requires_grad:
+        require_no_grad("mxfp4_quantize", x)
     dt = _lib.dtype_code(x.dtype)
     shape = x.shape
     if not shape or shape[-1] % MX_BLOCK:
         raise ValueError(f"mxfp4_quantize: the last dim of {tuple(shape)} must be a multiple of {MX_BLOCK}")
     K = shape[-1]
     codes = x.new_empty((*shape[:-1], K // 2), dtype=_U8)
-    scales = x.new_empty((*shape[:-1], K // MX_BLOCK), dtype=_U8)
+    scales = codes.new_empty((*shape[:-1], K // MX_BLOCK))
     n = x.numel()
     if n == 0:
         return codes, scales
@@ -126,7 +138,10 @@ def matmul_mxfp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bia
                 _off_device(op, t)
             if t.dtype != _BF16:
                 raise TypeError(f"{op}: dtype mismatch ({t.dtype} vs {_BF16})")
-    require_no_grad(op, x, bias, residual, out)
+            if t.requires_grad:
+                require_no_grad(op, t)
+    if x.requires_grad:
+        require_no_grad(op, x)
     if x.dtype != _BF16:
         raise TypeError(f"{op}: x must be bfloat16, got {x.dtype}")
     xs, ws, ss = x.shape, codes.shape, scales.shape
@@ -166,9 +181,8 @@ def matmul_mxfp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bia
         scales = scales.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    lib = _lib.lib()
-    nws = lib.q3_matmul_mxfp4_workspace_bytes(M, N, K)
-    ws_ = x.new_empty(nws, dtype=_U8) if nws else None
+    nws = _matmul_workspace(M, N, K)
+    ws_ = codes.new_empty(nws) if nws else None
     _lib.call("q3_matmul_mxfp4", x2.data_ptr(), codes.data_ptr(), scales.data_ptr(), _lib.ptr(bias), _lib.ptr(r2),
               y.data_ptr(), M, N, K, ldx, K // 2, K // MX_BLOCK, ldr, ldy, _lib.Q3_BF16, _lib.ptr(ws_), nws,
               _lib.raw_stream(dev))
@@ -180,7 +194,21 @@ def _check_cache(op: str, dev: int, k_codes, k_scales, v_codes, v_scales, kv_len
     tensors."""
     if dev < 0 or dev != _lib.current_device() or kv_lens.get_device() != dev:
         _off_device(op, kv_lens, k_codes)
-    shape, lead = k_codes.shape, None
+    if kv_lens.dtype != torch.int32 or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
+        raise ValueError(f"{op}: kv_lens must be a contiguous int32 ({B},) device tensor")
+    shape = k_codes.shape
+    if len(shape) == 4:
+        _, Hkv, cap, W = shape
+        n = W // 16
+        if (W * 2 == D and shape[0] == B and W == n * 16 and v_codes.shape == shape
+                and k_scales.shape == v_scales.shape == (B, Hkv, cap, n)
+                and k_codes.dtype == k_scales.dtype == v_codes.dtype == v_scales.dtype == _U8
+                and k_codes.get_device() == k_scales.get_device() == v_codes.get_device() == v_scales.get_device() == dev
+                and k_codes.is_contiguous() and k_scales.is_contiguous() and v_codes.is_contiguous()
+                and v_scales.is_contiguous() and (k_codes.data_ptr() | v_codes.data_ptr()) % 16 == 0
+                and (k_scales.data_ptr() | v_scales.data_ptr()) % n == 0):
+            c, s = (Hkv * cap * W, cap * W), (Hkv * cap * n, cap * n)  # whole caches: the usual call
+            return Hkv, cap, (*c, *s, *c, *s)
     st = []
     for c, s in ((k_codes, k_scales), (v_codes, v_scales)):
         if c.get_device() != dev or s.get_device() != dev:
@@ -200,8 +228,6 @@ def _check_cache(op: str, dev: int, k_codes, k_scales, v_codes, v_scales, kv_len
         if ss[3] and (s.data_ptr() % ss[3] or s_t[0] % ss[3] or s_t[1] % ss[3]):
             raise ValueError(f"{op}: the cache scales must be whole rows apart and aligned to one")
         st += (ct[0], ct[1], s_t[0], s_t[1])
-    if kv_lens.dtype != torch.int32 or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
-        raise ValueError(f"{op}: kv_lens must be a contiguous int32 ({B},) device tensor")
     return shape[1], shape[2], st
 
 
@@ -217,7 +243,8 @@ def kv_append_mxfp4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_s
     dev, shape = k.get_device(), k.shape
     if v.get_device() != dev:
         _off_device(op, k, v)
-    require_no_grad(op, k, v)
+    if k.requires_grad or v.requires_grad:
+        require_no_grad(op, k, v)
     dt = _lib.dtype_code(k.dtype)
     if k.dtype != v.dtype:
         raise TypeError(f"{op}: dtype mismatch ({v.dtype} vs {k.dtype})")
@@ -294,7 +321,8 @@ def qk_norm_rope_mxfp4(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torch.Tenso
 
 def _query(op: str, q: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
     """q as the kernels read it, and the output."""
-    require_no_grad(op, q, out)
+    if q.requires_grad or out is not None and out.requires_grad:
+        require_no_grad(op, q, out)
     if q.dtype != _BF16:
         raise TypeError(f"{op}: q must be bfloat16, got {q.dtype}")
     if not q.is_contiguous() or q.data_ptr() % 16:
@@ -329,8 +357,8 @@ def decode_attention_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: tor
     if Hkv == 0 or Hq % Hkv:
         raise ValueError(f"{op}: {Hq} query heads for {Hkv} KV heads")
     q, o = _query(op, q, out)
-    nws = _lib.lib().q3_decode_attention_mxfp4_workspace_bytes(B, Hq, Hkv, D)
-    ws = q.new_empty(nws, dtype=_U8)
+    nws = _decode_workspace(B, Hq, Hkv, D)
+    ws = k_codes.new_empty(nws)
     qs, os = q.stride(), o.stride()
     _lib.call("q3_decode_attention_mxfp4", q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
               v_scales.data_ptr(), kv_lens.data_ptr(), 1 if append else 0, o.data_ptr(), B, Hq, Hkv, D, cap,
@@ -362,7 +390,7 @@ def flash_attention_cache_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales
         raise ValueError(f"{op}: max_len {ml} must lie in [0, {cap}]")
     q, o = _query(op, q, out)
     nws = _lib.lib().q3_flash_attention_cache_mxfp4_workspace_bytes(B, Hq, Hkv, Sq, D, ml)
-    ws = q.new_empty(nws, dtype=_U8)
+    ws = k_codes.new_empty(nws)
     qs, os = q.stride(), o.stride()
     _lib.call("q3_flash_attention_cache_mxfp4", q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(),
               v_codes.data_ptr(), v_scales.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), B, Hq, Hkv, Sq, D, ml,
