@@ -78,10 +78,19 @@ __device__ __forceinline__ int rows_of(const MxAttn& p, int b) {
 
 __device__ __forceinline__ int units_of(const MxAttn& p, int b) { return (rows_of(p, b) + kUnit - 1) / kUnit; }
 
-// U units over n = min(U, kWaves) waves: the first U % n take one more than the others.
+// U units over n waves: the first U % n take one more than the others. Up to 512 units
+// have a wave each; more units take more waves only while each has at least 8 units, as
+// every wave that shares a pair costs the merge a record (8 units against 1, in us: one
+// sequence of 1024 rows x 8 heads, 64 tokens 27.5 / 37.6; 8 sequences of 300 x 4, 16
+// tokens 20.6 / 25.6; 32 sequences of 8192 x 8, where all waves are full, 42.7 / 42.8).
+constexpr int kMinWaves = 512, kMinUnits = 8;
 struct Split {
   int n, q, r;
-  __device__ __forceinline__ explicit Split(int U) : n(min(U, kWaves)), q(U <= kWaves ? 1 : U / kWaves), r(U <= kWaves ? 0 : U % kWaves) {}
+  __device__ __forceinline__ explicit Split(int U) {
+    n = min(kWaves, max(U / kMinUnits, min(U, kMinWaves)));
+    q = n ? U / n : 0;
+    r = U - n * q;
+  }
   __device__ __forceinline__ int first(int w) const { return w * q + min(w, r); }
   __device__ __forceinline__ int wave_of(int u) const {
     const int big = r * (q + 1);
@@ -151,20 +160,25 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void mx_decode_kernel(const Mx
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int HS = p.Hkv * p.nset;
-  // Few units go one to a CU; waves that read the same rows (several column sets) share an XCD's L2.
-  const int w = ONCE ? wave * kBlocks + (int)blockIdx.x : xcd_remap(blockIdx.x, kBlocks) * kWavesPerBlock + wave;
 
   // The wave's units: every wave sums the sequences' unit counts by itself (64 a
   // round), so nothing waits at a barrier.
+  const bool first_wave = blockIdx.x == 0 && wave == 0;
   int total = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     const int incl = wave_scan(b0 + lane < p.B ? units_of(p, b0 + lane) : 0, lane);
-    if (w == 0 && b0 + lane < p.B) p.hdr[b0 + lane + 1] = total + incl;  // for the merge, which must not read the lengths
+    if (first_wave && b0 + lane < p.B) p.hdr[b0 + lane + 1] = total + incl;  // for the merge, which must not read the lengths
     total += __builtin_amdgcn_readlane(incl, 63);
   }
-  if (w == 0 && lane == 0) p.hdr[0] = 0;
+  if (first_wave && lane == 0) p.hdr[0] = 0;
   const Split split(total * HS);
-  if (w >= split.n) return;
+  // Blocks run round-robin on the 8 XCDs. Each XCD takes an eighth of the active waves,
+  // consecutive ones (which read the same rows where there are several column sets) on
+  // different CUs.
+  const int xcd = blockIdx.x & 7, j = wave * (kBlocks / 8) + ((int)blockIdx.x >> 3);
+  const int here = split.n / 8 + (xcd < split.n % 8);
+  if (j >= here) return;
+  const int w = xcd * (split.n / 8) + min(xcd, split.n % 8) + j;
   const int u0 = split.first(w), count = split.first(w + 1) - u0;
   Cursor cc{};
   for (int b0 = 0, before = 0; b0 < p.B; b0 += 64) {
@@ -254,6 +268,10 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void mx_decode_kernel(const Mx
       qf[t] = bf16x8{};
       if (valid) qf[t] = *reinterpret_cast<const bf16x8*>(q + g * (2 * LB) + 8 * t);
     }
+    // Waited for here: a use of loads that may still be under way makes the compiler wait
+    // for every load, the ring's included, before the first products of each unit.
+#pragma unroll
+    for (int t = 0; t < LW; ++t) asm volatile("" : "+v"(qf[t]));
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = floatx4{};
     m = -INFINITY;
@@ -487,16 +505,18 @@ int64_t header_bytes(int64_t B) { return (B + 1 + 63) / 64 * 256; }
 
 int64_t sets_of(int64_t groups, int64_t Sq) { return q3_cdiv(groups * Sq, kCols); }
 
-// The streaming kernel takes single tokens and chunks of up to 1024 pairs; a longer
-// chunk expands the cache to bf16 once and runs the chunk kernel of the bf16 cache, which
-// shares each row among 256 columns but does not split the rows. Microseconds, streaming
-// / expanding (8 KV heads of 4 query heads unless said otherwise): 8192 rows, 32 tokens
-// (64 pairs) 36 / 206, 128 (256) 60 / 210, 512 (1024) 166 / 211, 1024 (2048) 323 / 207;
-// 1024 rows, 256 tokens (512) 35 / 40, 512 (1024) 45 / 40; 8 sequences of 300 rows x 4 x
-// 8 heads, 100 tokens (1600) 37 / 26.
-constexpr int64_t kStreamPairs = 1024;
-bool streams(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq) {
-  return Sq == 1 || B * Hkv * sets_of(groups, Sq) <= kStreamPairs;
+// The streaming kernel takes single tokens, and chunks of few pairs: its time grows with
+// the pairs, 25 ns for each one's records and 16 ps for each of its rows. Otherwise the
+// cache is expanded to bf16 once and the chunk kernel of the bf16 cache runs, which
+// shares each row among 256 columns but does not split the rows: 9 us more for the
+// launches, and 23 ns a row for as long as the pairs do not fill the card. The rows are
+// the capacity, as the lengths are on the device. Microseconds, streaming / expanding, 8
+// KV heads of 4 query heads unless said otherwise: 8192 rows, 32 tokens (64 pairs) 38 /
+// 208, 128 (256) 62 / 212, 512 (1024) 179 / 213, 1000 (2000) 319 / 216; 4 x 2000 rows,
+// 64 tokens (512) 43 / 72, 128 (1024) 67 / 73, 200 (1600) 84 / 72; 1024 rows, 256 tokens
+// (512) 40 / 41, 512 (1024) 62 / 42; 8 x 300 rows of 4 x 8 heads, 60 tokens (960) 41 / 28.
+bool streams(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq, int64_t cap) {
+  return Sq == 1 || (double)(B * Hkv * sets_of(groups, Sq)) * (25e-3 + 16e-6 * cap) <= 9 + 23e-3 * cap;
 }
 
 int64_t stream_ws_bytes(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq, int64_t D) {
@@ -536,7 +556,7 @@ int check(const void* q, const void* kc, const void* ks, const void* vc, const v
   Q3_REQUIRE(B >= 0 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Sq >= 0 && D >= 1 && cap >= 0, Q3_ERR_SHAPE);
   Q3_REQUIRE(dtype == Q3_BF16, Q3_ERR_DTYPE);
   Q3_REQUIRE((D == 64 || D == 128) && B <= kMaxBatch && (cap + kUnit) * D / 2 < (1ll << 31) && Sq < (1ll << 31) &&
-                 Hq < (1ll << 16) && B * Hkv * sets_of(Hq / Hkv, streams(B, Hkv, Hq / Hkv, Sq) ? Sq : 1) * q3_cdiv(cap, kUnit) < (1ll << 31),
+                 Hq < (1ll << 16) && B * Hkv * sets_of(Hq / Hkv, streams(B, Hkv, Hq / Hkv, Sq, cap) ? Sq : 1) * q3_cdiv(cap, kUnit) < (1ll << 31),
              Q3_ERR_UNSUPPORTED);
   bool ok = q3_aligned(q, 16) && q3_aligned(kc, 16) && q3_aligned(vc, 16) && q3_aligned(o, 8);
   for (int i = 0; i < 6; ++i) ok = ok && strides[i] % 8 == 0;
@@ -636,7 +656,7 @@ int q3_decode_attention_mxfp4(const void* q, const void* k_codes, const void* k_
 int64_t q3_flash_attention_cache_mxfp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
                                                        int64_t max_len) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || D <= 0 || max_len < 0) return 0;
-  if (streams(B, Hkv, Hq / Hkv, Sq)) return stream_ws_bytes(B, Hkv, Hq / Hkv, Sq, D);
+  if (streams(B, Hkv, Hq / Hkv, Sq, max_len)) return stream_ws_bytes(B, Hkv, Hq / Hkv, Sq, D);
   return 2 * B * Hkv * max_len * D * 2;  // K and V in bf16
 }
 
@@ -653,7 +673,7 @@ int q3_flash_attention_cache_mxfp4(const void* q, const void* k_codes, const voi
              Q3_ERR_WORKSPACE);
   Q3_REQUIRE(q3_aligned(workspace, 16), Q3_ERR_ALIGN);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (streams(B, Hkv, Hq / Hkv, Sq)) {
+  if (streams(B, Hkv, Hq / Hkv, Sq, max_len)) {
     MxAttn p = arguments(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, Sq, max_len, strides, scale);
     p.len_add = 1;
     p.lens_inc = advance ? kv_lens : nullptr;

@@ -262,8 +262,8 @@ def test_decode_nan_row_reaches_its_block_of_the_output_only():
     assert torch.isnan(o[0]).all() and torch.isfinite(o[1]).all()
 
 
-# (KV heads, group, tokens): the last ones past the streaming kernel's 1024 pairs
-CHUNKS = [(1, 1, 2), (2, 4, 3), (1, 4, 4), (2, 4, 5), (2, 3, 40), (1, 8, 33), (2, 2, 100), (1, 1, 16), (1, 1, 17), (9, 5, 75),
+# (KV heads, group, tokens): the last ones over the expanded cache
+CHUNKS = [(1, 1, 2), (2, 4, 3), (1, 4, 4), (2, 4, 5), (2, 3, 40), (1, 8, 33), (2, 2, 100), (1, 1, 16), (1, 1, 17), (4, 8, 45), (9, 5, 75),
           (13, 4, 65)]
 
 
