@@ -533,10 +533,14 @@ int launch_stream(const MxAttn& p, hipStream_t st) {
   Q3_LAUNCH_CHECK();
   const int pairs = p.B * p.Hkv * p.nset;
   const dim3 merge((unsigned)pairs, (unsigned)std::min(kCols, p.groups * p.Sq));
-  // A pair has about kWaves / pairs records: with more than 16 of them all are in flight at once on 16 waves (8
-  // pairs of one sequence's 1500 rows: 4.9 us against 6.3 on 4; 256 pairs of 32 sequences 5.5 on 4, 8.5 on 16).
+  // The merge is bound by latency: all of a pair's records should be in flight at once and all blocks resident.
+  // A pair has up to kWaves / pairs records: 16 waves share more than 16 of them (8 pairs of one sequence's 1500
+  // rows: 4.4 us against 6.3 on 4), 4 waves fewer (256 pairs of 32 sequences: 5.6 us, 8.5 on 16 and on 1), one wave
+  // where 4 to each pair and column would not fit the card (320 pairs x 16 columns: 7.3 us against 10.2 on 4).
   if (kWaves / pairs > 16)
     hipLaunchKernelGGL((mx_decode_combine<D, 16>), merge, dim3(64 * 16), 0, st, p);
+  else if ((int64_t)pairs * merge.y > 256 * 8)
+    hipLaunchKernelGGL((mx_decode_combine<D, 1>), merge, dim3(64), 0, st, p);
   else
     hipLaunchKernelGGL((mx_decode_combine<D, 4>), merge, dim3(64 * 4), 0, st, p);
   Q3_LAUNCH_CHECK();
