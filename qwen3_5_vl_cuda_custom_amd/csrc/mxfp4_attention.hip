@@ -505,18 +505,18 @@ int64_t header_bytes(int64_t B) { return (B + 1 + 63) / 64 * 256; }
 
 int64_t sets_of(int64_t groups, int64_t Sq) { return q3_cdiv(groups * Sq, kCols); }
 
-// The streaming kernel takes single tokens, and chunks of few pairs: its time grows with
-// the pairs, 25 ns for each one's records and 16 ps for each of its rows. Otherwise the
-// cache is expanded to bf16 once and the chunk kernel of the bf16 cache runs, which
-// shares each row among 256 columns but does not split the rows: 9 us more for the
-// launches, and 23 ns a row for as long as the pairs do not fill the card. The rows are
-// the capacity, as the lengths are on the device. Microseconds, streaming / expanding, 8
-// KV heads of 4 query heads unless said otherwise: 8192 rows, 32 tokens (64 pairs) 38 /
-// 208, 128 (256) 62 / 212, 512 (1024) 179 / 213, 1000 (2000) 319 / 216; 4 x 2000 rows,
-// 64 tokens (512) 43 / 72, 128 (1024) 67 / 73, 200 (1600) 84 / 72; 1024 rows, 256 tokens
-// (512) 40 / 41, 512 (1024) 62 / 42; 8 x 300 rows of 4 x 8 heads, 60 tokens (960) 41 / 28.
+// The streaming kernel takes single tokens, and chunks of few pairs. Otherwise the cache
+// is expanded to bf16 once and the chunk kernel of the bf16 cache runs, which shares each
+// row among 256 columns but does not split the rows: its time grows with the rows until
+// the pairs fill the card, the streaming kernel's with pairs x rows. Microseconds,
+// streaming / expanding, 8 KV heads of 4 query heads unless said otherwise: 8192 rows, 32
+// tokens (64 pairs) 38 / 208, 128 (256) 60 / 213, 512 (1024) 168 / 214, 700 (1400) 216 /
+// 215, 1000 (2000) 294 / 215; 4 x 2000 rows, 64 tokens (512) 38 / 72, 128 (1024) 52 / 73,
+// 200 (1600) 63 / 72; 1024 rows, 256 tokens (512) 33 / 41, 512 (1024) 47 / 42; 8 x 300
+// rows of 4 x 8 heads, 40 tokens (640) 24 / 26, 100 (1600) 37 / 29. The rows of the rule
+// are the capacity: the lengths are on the device.
 bool streams(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq, int64_t cap) {
-  return Sq == 1 || (double)(B * Hkv * sets_of(groups, Sq)) * (25e-3 + 16e-6 * cap) <= 9 + 23e-3 * cap;
+  return Sq == 1 || B * Hkv * sets_of(groups, Sq) <= 1000 + cap / 20;
 }
 
 int64_t stream_ws_bytes(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq, int64_t D) {

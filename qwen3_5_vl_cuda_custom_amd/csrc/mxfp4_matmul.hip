@@ -179,7 +179,6 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(const MxGemm p) {
             at + kX + (group0 * WPT + i) * 1024);
 #pragma unroll
     for (int i = 0; i < PS; ++i) {
-      // a word's scales past the row's last are the next row's: their codes are not loaded (zeros)
       const uint32_t off = soff[i] != kOOB && sb[i] < left ? soff[i] + (uint32_t)t * CW : kOOB;
       if constexpr (ALIGNED) dma4(rs, off, at + kX + kW + wave * kS);
       else dma1(rs, off, at + kX + kW + wave * kS + 256 * i);

@@ -309,10 +309,15 @@ def qk_norm_rope_mxfp4(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torch.Tenso
     if (positions.dtype != torch.int32 or positions.get_device() != dev or positions.shape != (3, B, S)
             or not positions.is_contiguous()):
         raise ValueError(f"{op}: positions must be a contiguous int32 (3, {B}, {S}) device tensor")
-    if inv_freq.dtype != _F32 or inv_freq.get_device() != dev or inv_freq.numel() != D // 2:
-        raise ValueError(f"{op}: inv_freq must be a float32 ({D // 2},) device tensor")
+    if (inv_freq.dtype != _F32 or inv_freq.get_device() != dev or inv_freq.numel() != D // 2
+            or not inv_freq.is_contiguous()):
+        raise ValueError(f"{op}: inv_freq must be a contiguous float32 ({D // 2},) device tensor")
     if len(mrope_section) != 3 or sum(mrope_section) * 2 != D:
         raise ValueError(f"{op}: mrope_section {list(mrope_section)} must be three counts that sum to D/2 = {D // 2}")
+    if cap == 0:
+        raise ValueError(f"{op}: the cache has no rows")
+    if q_in.numel() == 0:
+        return
     _lib.call("q3_qk_norm_rope_mxfp4", q_in.data_ptr(), k_in.data_ptr(), v_in.data_ptr(), q_out.data_ptr(),
               k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), _lib.ptr(q_weight),
               _lib.ptr(k_weight), positions.data_ptr(), inv_freq.data_ptr(), kv_lens.data_ptr(), cap, B, S, Hq, Hkv, D,
@@ -356,7 +361,11 @@ def decode_attention_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: tor
     Hkv, cap, st = _check_cache(op, dev, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D)
     if Hkv == 0 or Hq % Hkv:
         raise ValueError(f"{op}: {Hq} query heads for {Hkv} KV heads")
+    if cap == 0:
+        raise ValueError(f"{op}: the cache has no rows")
     q, o = _query(op, q, out)
+    if B == 0:
+        return o
     nws = _decode_workspace(B, Hq, Hkv, D)
     ws = k_codes.new_empty(nws)
     qs, os = q.stride(), o.stride()
@@ -375,7 +384,8 @@ def flash_attention_cache_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales
 
     q (B, Hq, Sq, D) bf16, D 64 or 128; the chunk's rows [kv_lens[b], kv_lens[b] + Sq) are already in the cache.
     Query i of sequence b attends to cache rows [0, kv_lens[b] + i]; advance=True adds Sq to kv_lens afterwards.
-    `max_len` bounds every kv_lens[b] + Sq (default: cap) and sizes the workspace of a longer chunk.
+    `max_len` bounds every kv_lens[b] + Sq (default: cap): rows past it are not read. It sizes the workspace of a
+    longer chunk, 4 * B * Hkv * max_len * D bytes.
     """
     op = "flash_attention_cache_mxfp4"
     if q.dim() != 4:
@@ -386,9 +396,11 @@ def flash_attention_cache_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales
     if Hkv * num_kv_groups != Hq:
         raise ValueError(f"{op}: Hq={Hq} != Hkv={Hkv} * num_kv_groups={num_kv_groups}")
     ml = cap if max_len is None else int(max_len)
-    if not 0 <= ml <= cap:
-        raise ValueError(f"{op}: max_len {ml} must lie in [0, {cap}]")
+    if not Sq <= ml <= cap or cap == 0:
+        raise ValueError(f"{op}: max_len {ml} must lie in [Sq, cap] = [{Sq}, {cap}]")
     q, o = _query(op, q, out)
+    if q.numel() == 0:
+        return o
     nws = _lib.lib().q3_flash_attention_cache_mxfp4_workspace_bytes(B, Hq, Hkv, Sq, D, ml)
     ws = k_codes.new_empty(nws)
     qs, os = q.stride(), o.stride()

@@ -82,7 +82,9 @@ class MXFP4KVCache(StaticKVCache):
 
     k_codes, v_codes: (B, Hkv, capacity, D / 2), k_scales, v_scales: (B, Hkv, capacity, D / 32), uint8; `lens` and the
     host's lengths as in StaticKVCache. Rows are quantised from bf16 as they are written and read in place by the
-    attention kernels (bf16 queries, head_dim 64 or 128, up to 1024 sequences).
+    attention kernels (bf16 queries, head_dim 64 or 128, up to 1024 sequences). The attention module's first prefill, run
+    eagerly into an empty cache, attends to the rows before they are quantised; a captured one, and every later chunk
+    and step, to the cache.
     """
 
     def __init__(self, batch: int, num_kv_heads: int, capacity: int, head_dim: int, *,

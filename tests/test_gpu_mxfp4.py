@@ -444,7 +444,9 @@ def test_refusals():
         (lambda: K.flash_attention_cache_mxfp4(q.unsqueeze(2), *cache, lens, 1.0, 2), ValueError),
         (lambda: K.flash_attention_cache_mxfp4(q.unsqueeze(2), *cache, lens, 1.0, 4, max_len=33), ValueError),
         (lambda: K.flash_attention_cache_mxfp4(q.unsqueeze(2).expand(2, 8, 40, 128), *cache, lens, 1.0, 4),
-         RuntimeError),  # more tokens than the cache has rows
+         ValueError),  # more tokens than the cache has rows
+        (lambda: K.decode_attention_mxfp4(q, *(t[:, :, :0] for t in cache), lens, 1.0), ValueError),
+        (lambda: K.decode_attention_mxfp4(q, *cache, lens, 1.0, out=q.transpose(1, 2)), ValueError),
     ]:
         with pytest.raises(exc):
             bad()
@@ -453,3 +455,50 @@ def test_refusals():
         K.matmul_mxfp4(w, u(8, 32), u(8, 2))
     with pytest.raises(_lib.Q3Error):  # head dim 32: the cache can be written, not attended to
         K.decode_attention_mxfp4(q[..., :32], u(2, 2, 32, 16), u(2, 2, 32, 1), u(2, 2, 32, 16), u(2, 2, 32, 1), lens, 1.0)
+
+
+def test_no_sequences_and_no_tokens():
+    d = dict(device=DEV)
+    u = lambda *s: torch.zeros(*s, dtype=torch.uint8, **d)  # noqa: E731
+    for B in (0, 2):
+        cache = (u(B, 2, 32, 64), u(B, 2, 32, 4), u(B, 2, 32, 64), u(B, 2, 32, 4))
+        lens = torch.ones(B, dtype=torch.int32, **d)
+        kv = torch.ones(B, 0, 2, 128, dtype=torch.bfloat16, **d)
+        K.kv_append_mxfp4(kv, kv, *cache, lens)
+        q = torch.zeros(B, 8, 0, 128, dtype=torch.bfloat16, **d)
+        assert K.flash_attention_cache_mxfp4(q, *cache, lens, 1.0, 4, advance=True).shape == q.shape
+        if B == 0:
+            assert K.decode_attention_mxfp4(q.new_zeros(0, 8, 128), *cache, lens, 1.0, append=True).shape == (0, 8, 128)
+        assert not any(t.any() for t in cache) and lens.tolist() == [1] * B
+    x = torch.zeros(0, 64, dtype=torch.bfloat16, **d)
+    assert K.matmul_mxfp4(x, u(8, 32), u(8, 2)).shape == (0, 8)
+    assert [t.shape for t in K.mxfp4_quantize(x)] == [(0, 32), (0, 2)]
+
+
+def test_two_streams_at_once():
+    """Products, decode steps and chunks issued on two streams without waiting for each other: each call's workspace
+    is its own."""
+    g = torch.Generator().manual_seed(40)
+    codes, scales = (t.to(DEV) for t in M.quantize(torch.randn(4096, 2048, generator=g).to(torch.bfloat16)))
+    c = Cache([700, 40, 0], 2, 800, 128, seed=41, used=40)
+    dev, lens = c.device(), c.lens.to(DEV)
+    xs = [rnd(32, 2048, seed=42 + i).to(DEV) for i in range(2)]
+    qs = [rnd(3, 8, 40, 128, seed=44 + i).to(DEV) for i in range(2)]
+
+    def run(i):
+        return (K.matmul_mxfp4(xs[i], codes, scales), K.decode_attention_mxfp4(qs[i][:, :, 0], *dev, lens, 0.1),
+                K.flash_attention_cache_mxfp4(qs[i], *dev, lens, 0.1, 4))
+
+    want = [run(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            for a, b in zip(r, want[i]):
+                assert torch.equal(a, b)

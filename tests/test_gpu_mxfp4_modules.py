@@ -251,3 +251,32 @@ def test_moe_model_with_four_bit_attention():
     a = m.generate(ids, max_new_tokens=12, kv_format="mxfp4")
     b = m.generate(ids, max_new_tokens=12, kv_format="mxfp4", use_graph=False)
     assert torch.equal(a, b)
+
+
+def test_fused_append_refusals():
+    B, S, Hq, Hkv, d, cap = 2, 1, 4, 2, 128, 16
+    q, k = rnd(B, S, Hq, d), rnd(B, S, Hkv, d)
+    cache = MXFP4KVCache(B, Hkv, cap, d, device=DEV)
+    pos = torch.zeros(3, B, S, dtype=torch.int32, device=DEV)
+    inv = torch.ones(d // 2, device=DEV)
+    w = rnd(d)
+    good = dict(q=q, k=k, v=k, qo=torch.empty_like(q), t=cache.tensors, wq=w, wk=w, pos=pos, inv=inv,
+                sec=SECTIONS[d], lens=cache.lens)
+
+    def call(**change):
+        a = {**good, **change}
+        K.qk_norm_rope_mxfp4(a["q"], a["k"], a["v"], a["qo"], *a["t"], a["wq"], a["wk"], a["pos"], a["inv"], a["sec"],
+                             1e-6, a["lens"])
+    for change, exc in [
+        (dict(q=q.float()), TypeError), (dict(k=k[:, :, :1]), ValueError), (dict(v=k[:, :, :1]), ValueError),
+        (dict(qo=torch.empty_like(q)[:, :, :3]), ValueError), (dict(wk=None), ValueError), (dict(wq=w[:64]), ValueError),
+        (dict(pos=pos.long()), ValueError), (dict(pos=pos[:2]), ValueError), (dict(inv=inv.double()), ValueError),
+        (dict(inv=torch.ones(d, device=DEV)[::2]), ValueError), (dict(sec=(24, 20, 19)), ValueError),
+        (dict(lens=cache.lens.long()), ValueError), (dict(t=tuple(x[:, :, :0] for x in cache.tensors)), ValueError),
+        (dict(q=q.cpu()), RuntimeError),
+    ]:
+        with pytest.raises(exc):
+            call(**change)
+    assert not cache.k_codes.any() and not cache.v_codes.any()
+    call()
+    assert cache.k_codes[:, :, 0].any() and not cache.k_codes[:, :, 1:].any()
