@@ -590,6 +590,20 @@ int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, co
                     void* y, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t lds, int64_t ldr,
                     int64_t ldc, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Decode shapes, M <= 32 rows, in one launch (q3_matmul_segments / q3_matmul_swiglu and their rmsnorm_ forms with
+ * weights in MXFP4, packed):
+ * q3_matmul_segments_mxfp4: y (M, sum n_j) = x [w_0; w_1; ...]^T (+ [b_0; b_1; ...]), 1 to 4 weights of n[j] >= 1
+ * rows; codes, scales and bias are host arrays of device pointers (bias, or any of its entries, may be null).
+ * q3_matmul_swiglu_mxfp4: y (M, N) = silu(x g^T) * (x u^T).
+ * norm_weight (K), if not null: the rows of x are RMS-normalised first (eps; K <= 8192). bf16; K a multiple of 128
+ * (else Q3_ERR_UNSUPPORTED); x, its rows, the norm weight and the codes 16-byte aligned, the scales 4-byte. */
+int q3_matmul_segments_mxfp4(const void* x, const void* norm_weight, float eps, const void* const* codes,
+                             const void* const* scales, const void* const* bias, const int64_t* n, int64_t nseg,
+                             void* y, int64_t M, int64_t K, int64_t ldx, int64_t ldc, int dtype, void* stream);
+int q3_matmul_swiglu_mxfp4(const void* x, const void* norm_weight, float eps, const void* g_codes, const void* g_scales,
+                           const void* u_codes, const void* u_scales, void* y, int64_t M, int64_t N, int64_t K,
+                           int64_t ldx, int64_t ldc, int dtype, void* stream);
+
 /* Four-bit KV cache: codes (B, Hkv, cap, D / 2) and scales (B, Hkv, cap, D / 32) of keys and values, the rows of a
  * head packed, any batch and head strides (codes 16-byte aligned).
  * q3_kv_append_mxfp4: rows k, v (B, S, Hkv, D) quantised into cache rows kv_lens[b] + s; rows at or past cap (or

@@ -118,6 +118,8 @@ _SIGS: dict[str, tuple] = {
     "q3_mxfp4_dequantize": (c_int, [_V, _V, _V, _I, _I, _I, _V, c_int, _V]),
     "q3_matmul_mxfp4_workspace_bytes": (c_int64, [_I, _I, _I]),
     "q3_matmul_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, _I, _I, _I, c_int, _V, _I, _V]),
+    "q3_matmul_segments_mxfp4": (c_int, [_V, _V, c_float, _V, _V, _V, _i64p, _I, _V, _I, _I, _I, _I, c_int, _V]),
+    "q3_matmul_swiglu_mxfp4": (c_int, [_V, _V, c_float, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, c_int, _V]),
     "q3_kv_append_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, _V, c_int, _V]),
     "q3_qk_norm_rope_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, _I, _i64p,
                                       c_float, _V, c_int, _V]),

@@ -5,6 +5,7 @@
 
 #include "gemm_tile.h"
 #include "mxfp4.h"
+#include "mxfp4_rows.h"
 
 namespace {
 
@@ -46,12 +47,13 @@ __device__ __forceinline__ void store_y4(const MxGemm& p, int m, int n, floatx4 
   *reinterpret_cast<bf16x4*>(p.y + m * p.ldc + n) = o;
 }
 
-// ------------------------------------------------------------------ few rows (decode)
-// Bound by the weight stream (N=K=4096, one row: 6.1 us, 8.9 MB; an empty kernel takes
-// 2). A block takes 16 weight rows, a wave every eighth 128-value step of k: lane (r = l %
-// 16, g = l / 16) loads the 16 bytes of block 4 step + g of weight row r, its scale, and
-// the 32 values of x's row r at the same k, and forms 4 products of 16x16x32 (k permuted
-// alike in both). The eight waves' sums meet in LDS, in wave order.
+// ------------------------------------------------------------------ few rows, any K
+// Up to four rows whose K (or scales) the kernel of mxfp4_rows.hip does not take. Bound
+// by the weight stream (N=1000 K=1152, one row: 3.4 us; an empty kernel takes 2). A block
+// takes 16 weight rows, a wave every eighth 128-value step of k: lane (r = l % 16, g = l /
+// 16) loads the 16 bytes of block 4 step + g of weight row r, its scale, and the 32 values
+// of x's row r at the same k, and forms 4 products of 16x16x32 (k permuted alike in both).
+// The eight waves' sums meet in LDS, in wave order.
 constexpr int kGemvWaves = 8;
 
 __global__ __launch_bounds__(64 * kGemvWaves) void mx_gemv_kernel(const MxGemm p) {
@@ -114,8 +116,8 @@ __global__ __launch_bounds__(64 * kGemvWaves) void mx_gemv_kernel(const MxGemm p
 // the rows of scales start at multiples of four bytes), else byte by byte (a load of
 // one byte per lane costs as much as one of sixteen: M=32 N=151936 158 -> 113 us without).
 // 128 rows run at 1.1 PFLOP/s of the CUs they fill (M=512 N=12288 K=4096: 192 tiles, 67
-// us), 32 rows at the loads into LDS (N=4096 K=12288: 11 us for 26.7 MB of weights and
-// 98 KB of x per CU, and 4 for the sum over 8 ranges).
+// us), 32 rows at the loads into LDS (N=4096 K=12288: 10 us for 26.7 MB of weights and
+// 98 KB of x per CU, and 3 for the sum over 8 ranges).
 template <int RT, int BM, int WM, int BK, int NST, bool ALIGNED>
 __global__ __launch_bounds__(512) void mx_tile_kernel(const MxGemm p) {
   constexpr int NW = 8, WN = NW / WM, BN = 16 * RT * WN, MT = BM / 16 / WM;
@@ -277,8 +279,8 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const MxGemm p, int parts) 
   }
 }
 
-// How a product runs: one 16-row weight group per block (kRows), x through LDS in tiles
-// of 32, 64 or 128 rows, or the weights expanded to bf16 for the bf16 GEMM.
+// How a product runs: whole weight rows per block (kRows), x through LDS in tiles of 32,
+// 64 or 128 rows, or the weights expanded to bf16 for the bf16 GEMM.
 enum Form { kRows, kTile32, kTile64, kTile128, kExpand };
 
 struct Plan {
@@ -286,7 +288,10 @@ struct Plan {
   int bn, bm, parts;  // tile, and ranges of k whose sums are added by mx_sum_kernel
 };
 
-// kRows up to 4 rows, where x is next to nothing. Up to 64 rows always tiles. Above,
+// kRows up to 32 rows, but for 17 to 32 rows of K > 8192, where the reads of x by every CU
+// cost more than the sum over ranges of k: us, kRows / tiles, 32 rows: N=4096 K=4096 8.7 /
+// 9.6, K=12288 17.5 / 12.6, N=12288 K=4096 11.5 / 14.1, N=24576 16 / 22; 16 rows: 6.2 / 8.5,
+// 11.6 / 11.9, 9.2 / 13.3, 13.0 / 20.2. Up to 64 rows tiles. Above,
 // tiles unless the expansion is estimated faster: 128 x 256 tiles run in rounds of 256
 // at 1.1 PFLOP/s; expanding costs 2.53 bytes a weight at 5.5 TB/s, 16 us, and the
 // product at 1.3 PFLOP/s. Microseconds, tiles / expanded: N=12288 K=4096 M=64 21 / 69,
@@ -294,7 +299,7 @@ struct Plan {
 // / 144; N=K=4096 M=777 43 / 55, M=1500 66 / 77; N=K=1024 M=1500 19 / 18. With fewer tiles
 // than CUs, k is split until they fill them (ranges of at least 512 k).
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
-  if (M <= 4) return {kRows, 16, 16, 1};
+  if (M <= 4 || (M <= kMxRowsMax && K % 128 == 0 && (M <= 16 || K <= 8192))) return {kRows, 0, 0, 1};
   Plan g = M <= 32 ? Plan{kTile32, 128, 32, 1} : M <= 64 ? Plan{kTile64, 256, 64, 1} : Plan{kTile128, 256, 128, 1};
   const int64_t tiles = q3_cdiv(N, g.bn) * q3_cdiv(M, g.bm);
   if (g.form == kTile128) {
@@ -343,7 +348,22 @@ int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, co
   Q3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Q3_ERR_WORKSPACE);
   Q3_REQUIRE(need == 0 || q3_aligned(workspace, 16), Q3_ERR_ALIGN);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const Plan g = plan_of(M, N, K);
+  Plan g = plan_of(M, N, K);
+  if (g.form == kRows && mx_rows_ok(M, K, w_scales, lds)) {
+    MxRows p{};
+    p.x = static_cast<const bf16*>(x);
+    p.w[0] = static_cast<const uint8_t*>(w_codes);
+    p.s[0] = static_cast<const uint8_t*>(w_scales);
+    p.bias[0] = static_cast<const bf16*>(bias);
+    p.n[0] = (int)N;
+    p.nseg = 1;
+    p.res = static_cast<const bf16*>(residual);
+    p.y = static_cast<bf16*>(y);
+    p.M = (int)M, p.K = (int)K;
+    p.ldx = ldx, p.ldw = ldw, p.lds = lds, p.ldr = ldr, p.ldc = ldc;
+    return mx_rows(p, false, st);
+  }
+  if (g.form == kRows && M > 4) g = Plan{kTile32, 128, 32, 1};  // scales at odd addresses; no workspace
   if (g.form == kExpand) {
     Q3_REQUIRE(ldw == K / 2 && lds == K / kMxBlock, Q3_ERR_UNSUPPORTED);
     const int rc = mx_expand(w_codes, w_scales, static_cast<bf16*>(workspace), N * K, st);

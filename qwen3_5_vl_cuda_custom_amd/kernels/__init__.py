@@ -14,7 +14,7 @@ from .matmul import (RMSNORM_MATMUL_MAX_ROWS, matmul, matmul_gelu, matmul_segmen
 from .moe_routing import (cuda_batched_gemm, cuda_index_add, cuda_topk, moe_experts, moe_experts_train, moe_permute,
                           moe_route, moe_router, raise_device_errors)
 from .mxfp4 import (decode_attention_mxfp4, flash_attention_cache_mxfp4, kv_append_mxfp4, matmul_mxfp4,
-                    mxfp4_dequantize, mxfp4_quantize, qk_norm_rope_mxfp4)
+                    matmul_segments_mxfp4, matmul_swiglu_mxfp4, mxfp4_dequantize, mxfp4_quantize, qk_norm_rope_mxfp4)
 from .norms import layernorm, rmsnorm, softmax
 from .rotary import apply_mrope, apply_rope, qk_norm_rope, qk_norm_rope_paged
 from .vision import vision_pos_embed, vision_rope_tables
@@ -64,6 +64,8 @@ __all__ = [
     "mxfp4_quantize",
     "mxfp4_dequantize",
     "matmul_mxfp4",
+    "matmul_segments_mxfp4",
+    "matmul_swiglu_mxfp4",
     "kv_append_mxfp4",
     "qk_norm_rope_mxfp4",
     "decode_attention_mxfp4",

@@ -19,6 +19,8 @@ import torch
 
 from .. import _lib
 from ._common import mfma_operand, require_device, require_no_grad
+from .elementwise import swiglu
+from .norms import rmsnorm
 
 MX_BLOCK = 32
 _U8, _BF16, _F32 = torch.uint8, torch.bfloat16, torch.float32
@@ -187,6 +189,120 @@ def matmul_mxfp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bia
               y.data_ptr(), M, N, K, ldx, K // 2, K // MX_BLOCK, ldr, ldy, _lib.Q3_BF16, _lib.ptr(ws_), nws,
               _lib.raw_stream(dev))
     return y
+
+
+def _weight(op: str, K: int, codes: torch.Tensor, scales: torch.Tensor, dev: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """The codes and scales of a weight (N, K), packed and aligned as the kernels of few rows read them."""
+    if codes.get_device() != dev or scales.get_device() != dev:
+        _off_device(op, codes, scales)
+    if (codes.dtype != _U8 or scales.dtype != _U8 or codes.dim() != 2 or scales.dim() != 2
+            or codes.shape[0] != scales.shape[0] or codes.shape[1] != scales.shape[1] * (MX_BLOCK // 2)):
+        raise _pair_error(op, codes, scales)
+    if codes.shape[1] * 2 != K:
+        raise ValueError(f"{op}: codes {tuple(codes.shape)} do not match x (..., {K})")
+    if not codes.is_contiguous() or codes.data_ptr() % 16:
+        codes = codes.clone(memory_format=torch.contiguous_format)
+    if not scales.is_contiguous() or scales.data_ptr() % 4:
+        scales = scales.clone(memory_format=torch.contiguous_format)
+    return codes, scales
+
+
+def _few_rows(op: str, x: torch.Tensor, norm_weight: torch.Tensor | None, *others: torch.Tensor | None) -> tuple:
+    """Checks x (..., K), the norm weight and the biases; returns the device, K, M, x as rows, their stride, and
+    whether one launch takes the call."""
+    dev = x.get_device()
+    if dev < 0 or dev != _lib.current_device():
+        _off_device(op, x)
+    for t in (norm_weight, *others):
+        if t is not None and t.get_device() != dev:
+            _off_device(op, x, t)
+    require_no_grad(op, x, norm_weight, *others)
+    if x.dtype != _BF16:
+        raise TypeError(f"{op}: x must be bfloat16, got {x.dtype}")
+    for t in (norm_weight, *others):
+        if t is not None and t.dtype != _BF16:
+            raise TypeError(f"{op}: dtype mismatch ({t.dtype} vs {_BF16})")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"{op}: x {tuple(x.shape)} has no columns")
+    K = x.shape[-1]
+    if norm_weight is not None and norm_weight.shape != (K,):
+        raise ValueError(f"{op}: norm weight {tuple(norm_weight.shape)} != ({K},)")
+    M = x.numel() // K
+    x2, ldx = _rows(op, x, K)
+    if x2.data_ptr() % 16 or ldx % 8 or ldx >= 1 << 22:
+        x2, ldx = x2.clone(memory_format=torch.contiguous_format), K
+    fits = 0 < M <= 32 and K % 128 == 0 and K < 1 << 22 and (norm_weight is None or K <= 8192)
+    return dev, K, M, x2, ldx, fits
+
+
+def matmul_segments_mxfp4(x: torch.Tensor, weights, biases=None, *, norm_weight: torch.Tensor | None = None,
+                          eps: float = 0.0) -> torch.Tensor:
+    """matmul_segments with the weights held in MXFP4: x·[W_0; W_1; ...]ᵀ (+ [b_0; b_1; ...]) over 1 to 4 weights,
+    each a pair (codes, scales); returns (..., ΣN_i).
+
+    With norm_weight the rows of x are RMS-normalised first (rmsnorm_matmul_segments). Up to 32 rows of K a multiple of
+    128 (and at most 8192 with the norm) are one launch; more rows, or another K, a product per weight.
+    """
+    op = "matmul_segments_mxfp4"
+    weights = list(weights)
+    biases = list(biases) if biases is not None else [None] * len(weights)
+    if not 1 <= len(weights) <= 4 or len(biases) != len(weights):
+        raise ValueError(f"{op}: 1 to 4 weights, one bias (or None) each")
+    dev, K, M, x2, ldx, fits = _few_rows(op, x, norm_weight, *biases)
+    ws = [_weight(op, K, c, s, dev) for c, s in weights]
+    ns = [c.shape[0] for c, _ in ws]
+    for b, n in zip(biases, ns):
+        if b is not None and b.shape != (n,):
+            raise ValueError(f"{op}: bias {tuple(b.shape)} != ({n},)")
+    y = x.new_empty((*x.shape[:-1], sum(ns)))
+    if not fits or 0 in ns:
+        if M == 0:
+            return y
+        if norm_weight is not None:
+            x = rmsnorm(x, norm_weight, eps)
+        at = 0
+        for (c, s), b, n in zip(ws, biases, ns):
+            matmul_mxfp4(x, c, s, b, out=y[..., at:at + n])
+            at += n
+        return y
+    bs = [b.contiguous() if b is not None else None for b in biases]
+    nw = None if norm_weight is None else _aligned(norm_weight)
+    _lib.call("q3_matmul_segments_mxfp4", x2.data_ptr(), _lib.ptr(nw), eps, _lib.ptrs(*(c for c, _ in ws)),
+              _lib.ptrs(*(s for _, s in ws)), _lib.ptrs(*bs) if any(b is not None for b in bs) else None,
+              _lib.i64s(*ns), len(ns), y.data_ptr(), M, K, ldx, sum(ns), _lib.Q3_BF16, _lib.raw_stream(dev))
+    return y
+
+
+def matmul_swiglu_mxfp4(x: torch.Tensor, gate: tuple[torch.Tensor, torch.Tensor],
+                        up: tuple[torch.Tensor, torch.Tensor], *, norm_weight: torch.Tensor | None = None,
+                        eps: float = 0.0) -> torch.Tensor:
+    """matmul_swiglu with the weights held in MXFP4: silu(x·W_gateᵀ)·(x·W_upᵀ), `gate` and `up` pairs (codes, scales)
+    of (N, K).
+
+    With norm_weight the rows of x are RMS-normalised first (rmsnorm_matmul_swiglu). Up to 32 rows of K a multiple of
+    128 (and at most 8192 with the norm) are one launch; more rows, or another K, two products and swiglu.
+    """
+    op = "matmul_swiglu_mxfp4"
+    dev, K, M, x2, ldx, fits = _few_rows(op, x, norm_weight)
+    (gc, gs), (uc, us) = (_weight(op, K, c, s, dev) for c, s in (gate, up))
+    if gc.shape != uc.shape:
+        raise ValueError(f"{op}: gate {tuple(gc.shape)} and up {tuple(uc.shape)} codes must have one shape")
+    N = gc.shape[0]
+    if not fits or N == 0:
+        if M == 0 or N == 0:
+            return x.new_empty((*x.shape[:-1], N))
+        if norm_weight is not None:
+            x = rmsnorm(x, norm_weight, eps)
+        return swiglu(matmul_mxfp4(x, gc, gs), matmul_mxfp4(x, uc, us))
+    y = x.new_empty((*x.shape[:-1], N))
+    nw = None if norm_weight is None else _aligned(norm_weight)
+    _lib.call("q3_matmul_swiglu_mxfp4", x2.data_ptr(), _lib.ptr(nw), eps, gc.data_ptr(), gs.data_ptr(), uc.data_ptr(),
+              us.data_ptr(), y.data_ptr(), M, N, K, ldx, N, _lib.Q3_BF16, _lib.raw_stream(dev))
+    return y
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _check_cache(op: str, dev: int, k_codes, k_scales, v_codes, v_scales, kv_lens, B: int, D: int) -> tuple:

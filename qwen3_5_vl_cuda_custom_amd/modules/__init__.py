@@ -5,10 +5,11 @@ from .embedding import CudaEmbedding
 from .graph import StepGraph
 from .kv_cache import MXFP4KVCache, PagedKVCache, StaticKVCache
 from .linear import CudaLinear
+from .linear_mxfp4 import CudaLinearMXFP4
 from .mlp import CudaSwiGLUMLP, CudaVisionMLP
 from .moe import CudaSparseMoE
 from .norms import CudaLayerNorm, CudaRMSNorm
-from .quantized import CudaLinearMXFP4, quantize_text_linears
+from .quantized import quantize_text_linears
 from .rotary import MRoPEBinding, TextMRoPE, Vision2DRoPE
 from .text_decoder import CudaTextDecoderLayer
 from .vision_block import CudaVisionBlock

@@ -9,12 +9,13 @@ from ..kernels.backward import (FlashAttentionFunction, QKNormRopeFunction, Rope
                                 needs_grad)
 from ..kernels import (apply_rope, decode_attention, decode_attention_mxfp4, decode_attention_paged, flash_attention,
                        flash_attention_cache, flash_attention_cache_mxfp4, flash_attention_cache_paged,
-                       flash_attention_varlen, kv_append_mxfp4, matmul, matmul_segments, qk_norm_rope,
-                       qk_norm_rope_attention, qk_norm_rope_attention_ok, qk_norm_rope_mxfp4, qk_norm_rope_paged,
+                       flash_attention_varlen, kv_append_mxfp4, matmul, matmul_segments,
+                       matmul_segments_mxfp4, qk_norm_rope, qk_norm_rope_attention, qk_norm_rope_attention_ok, qk_norm_rope_mxfp4, qk_norm_rope_paged,
                        rmsnorm_matmul_segments)
 from .kv_cache import MXFP4KVCache, PagedKVCache, StaticKVCache
 from .linear import CudaLinear
-from .norms import CudaRMSNorm, fused_norm_ok
+from .linear_mxfp4 import CudaLinearMXFP4
+from .norms import CudaRMSNorm, fused_norm_ok, norm_operands
 from .rotary import MRoPEBinding, TextMRoPE
 
 
@@ -139,7 +140,10 @@ class CudaFullAttention(nn.Module):
         # q/k/v projections in one GEMM over the three weights (no concatenated
         # copy); q, k, v are column views of its output.
         projs = (self.q_proj, self.k_proj, self.v_proj)
-        if not all(isinstance(p, CudaLinear) for p in projs):
+        if all(isinstance(p, CudaLinearMXFP4) for p in projs):
+            nw, eps, x = (None, 0.0, x) if input_norm is None else norm_operands(x, input_norm)
+            qkv = matmul_segments_mxfp4(x, [p.pair for p in projs], [p.bias for p in projs], norm_weight=nw, eps=eps)
+        elif not all(isinstance(p, CudaLinear) for p in projs):
             qkv = self._project_apart(x if input_norm is None else input_norm(x), projs)
         else:
             weights = tuple(p.weight for p in projs)
@@ -216,8 +220,8 @@ class CudaFullAttention(nn.Module):
 
     @staticmethod
     def _project_apart(x, projs) -> torch.Tensor:
-        """The q/k/v rows side by side where some projections hold four-bit weights: one product each, into its
-        columns."""
+        """The q/k/v rows side by side where only some projections hold four-bit weights: one product each, into
+        its columns."""
         qkv = torch.empty((*x.shape[:-1], sum(p.out_features for p in projs)), dtype=x.dtype, device=x.device)
         at = 0
         for p in projs:

@@ -4,11 +4,12 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from ..kernels import gelu_tanh, matmul_gelu, matmul_swiglu, rmsnorm_matmul_swiglu, swiglu
+from ..kernels import gelu_tanh, matmul_gelu, matmul_swiglu, matmul_swiglu_mxfp4, rmsnorm_matmul_swiglu, swiglu
 from ..kernels.backward import needs_grad
 from ..kernels.matmul import line_padded_rows
 from .linear import CudaLinear
-from .norms import CudaRMSNorm, fused_norm_ok
+from .linear_mxfp4 import CudaLinearMXFP4
+from .norms import CudaRMSNorm, fused_norm_ok, norm_operands
 
 
 # Rows from which CudaVisionMLP pads its hidden rows to whole 128-byte lines (line_padded_rows). It makes fc2 about
@@ -35,8 +36,13 @@ class CudaSwiGLUMLP(nn.Module):
             if input_norm is not None:
                 x = input_norm(x)
             return self.down_proj(swiglu(self.gate_proj(x), self.up_proj(x)), residual=residual)
+        if (isinstance(self.gate_proj, CudaLinearMXFP4) and isinstance(self.up_proj, CudaLinearMXFP4)
+                and self.gate_proj.bias is None and self.up_proj.bias is None):
+            nw, eps, x = (None, 0.0, x) if input_norm is None else norm_operands(x, input_norm)
+            act = matmul_swiglu_mxfp4(x, self.gate_proj.pair, self.up_proj.pair, norm_weight=nw, eps=eps)
+            return self.down_proj(act, residual=residual)
         if not all(isinstance(p, CudaLinear) for p in (self.gate_proj, self.up_proj)):
-            # four-bit weights (CudaLinearMXFP4): each projection by its own forward
+            # four-bit weights in one of them, or with a bias: each projection by its own forward
             if input_norm is not None:
                 x = input_norm(x)
             return self.down_proj(swiglu(self.gate_proj(x), self.up_proj(x)), residual=residual)

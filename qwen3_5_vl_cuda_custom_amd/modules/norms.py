@@ -33,6 +33,11 @@ def fused_norm_ok(x: torch.Tensor, norm: CudaRMSNorm) -> bool:
             and 0 < x.numel() // K <= RMSNORM_MATMUL_MAX_ROWS)
 
 
+def norm_operands(x: torch.Tensor, norm: CudaRMSNorm) -> tuple[torch.Tensor | None, float, torch.Tensor]:
+    """(weight, eps, x) for a projection that can normalise the rows itself, (None, 0, norm(x)) where it can not."""
+    return (norm.weight, norm.eps, x) if fused_norm_ok(x, norm) else (None, 0.0, norm(x))
+
+
 class CudaLayerNorm(nn.Module):
     """nn.LayerNorm parameter layout: `weight` ones, `bias` zeros (or None)."""
 

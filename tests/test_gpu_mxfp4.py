@@ -134,6 +134,105 @@ def test_matmul_many_tiles_and_expanded_weights(m, n, k):
     check_matmul(y, x, codes, scales, b, r)
 
 
+# one to six 16-row groups per block, and more blocks than CUs
+@pytest.mark.parametrize("m", [3, 4, 12, 31])
+@pytest.mark.parametrize("n,k", [(4001, 128), (6000, 640), (12003, 640), (16000, 1152), (24000, 512), (30001, 128)])
+def test_matmul_few_rows_of_large_weights(m, n, k):
+    codes, scales = weight(n, k, seed=n)
+    x, b, r = rnd(m, k, seed=m), rnd(n, seed=1), rnd(m, n, seed=2)
+    y = K.matmul_mxfp4(x.to(DEV), codes.to(DEV), scales.to(DEV), b.to(DEV), r.to(DEV))
+    check_matmul(y, x, codes, scales, b, r)
+
+
+@pytest.mark.parametrize("m", [2, 16, 32])
+def test_matmul_scales_at_odd_addresses_and_long_rows(m):
+    n, k = 150, 9216
+    codes, scales = weight(n, k, seed=15)
+    odd = torch.empty(scales.numel() + 1, dtype=torch.uint8, device=DEV)[1:].view(scales.shape)
+    odd.copy_(scales)
+    x = rnd(m, k, seed=m)
+    for s in (odd, scales.to(DEV)):
+        check_matmul(K.matmul_mxfp4(x.to(DEV), codes.to(DEV), s), x, codes, scales)
+
+
+def normed(x, nw, eps):
+    """x * nw / rms(x) in float64, and the sum of the magnitudes' share of the rounding of x * nw to bf16."""
+    x = x.double()
+    return x * nw.double() * (x.square().mean(-1, keepdim=True) + eps).rsqrt()
+
+
+SEGMENTS = [((40,), 128), ((256, 64, 64), 512), ((1000, 96, 96), 1152), ((7, 9, 130, 33), 256), ((4096, 1024, 1024), 2048),
+            ((30, 50), 96)]
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("m", [1, 4, 7, 16, 32, 40])
+@pytest.mark.parametrize("ns,k", SEGMENTS)
+def test_matmul_segments_matches_float64(ns, k, m, norm):
+    ws = [weight(n, k, seed=n) for n in ns]
+    bs = [rnd(n, seed=n + 1) if i != 1 else None for i, n in enumerate(ns)]
+    x, nw, eps = rnd(m, k, seed=m), rnd(k, seed=3) * 0.2 + 1, 1e-5
+    kw = dict(norm_weight=nw.to(DEV), eps=eps) if norm else {}
+    y = K.matmul_segments_mxfp4(x.to(DEV).view(1, m, k), [(c.to(DEV), s.to(DEV)) for c, s in ws],
+                                [b if b is None else b.to(DEV) for b in bs], **kw)
+    assert y.shape == (1, m, sum(ns)) and y.dtype == torch.bfloat16
+    at = 0
+    xn = normed(x, nw, eps) if norm else x.double()
+    for (c, s), b, n in zip(ws, bs, ns):
+        w = M.values(c, s)
+        ref, mag = xn @ w.T, xn.abs() @ w.abs().T
+        # The norm adds one rounding to bf16 of each x, and fp32 errors of its own sum and square root.
+        err = (k + 2) * 2.0 ** -23 * mag + (mag * (HALF + (k + 4) * 2.0 ** -23) if norm else 0)
+        if b is not None:
+            ref, err = ref + b.double(), err + 2.0 ** -23 * b.double().abs()
+        tol = HALF * (ref.abs() + err) + err
+        d = (y[0, :, at:at + n].double().cpu() - ref).abs()
+        assert bool((d <= tol).all()), float((d / tol).max())
+        at += n
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("m", [1, 4, 7, 16, 32, 40])
+@pytest.mark.parametrize("n,k", [(40, 128), (1001, 640), (12288, 512), (15000, 128), (300, 4096), (64, 96)])
+def test_matmul_swiglu_matches_float64(n, k, m, norm):
+    (gc, gs), (uc, us) = weight(n, k, seed=n), weight(n, k, seed=n + 1)
+    x, nw, eps = rnd(m, k, seed=m), rnd(k, seed=3) * 0.2 + 1, 1e-5
+    kw = dict(norm_weight=nw.to(DEV), eps=eps) if norm else {}
+    y = K.matmul_swiglu_mxfp4(x.to(DEV), (gc.to(DEV), gs.to(DEV)), (uc.to(DEV), us.to(DEV)), **kw)
+    xn = normed(x, nw, eps) if norm else x.double()
+    wg, wu = M.values(gc, gs), M.values(uc, us)
+    g, u = xn @ wg.T, xn @ wu.T
+    share = (k + 2) * 2.0 ** -23 + (HALF + (k + 4) * 2.0 ** -23 if norm else 0)
+    if m > 32 or k % 128:  # two products, each rounded to bf16
+        eg, eu = ((1 + HALF) * share * (xn.abs() @ w.abs().T) + HALF * t.abs() for w, t in ((wg, g), (wu, u)))
+    else:
+        eg, eu = (share * (xn.abs() @ w.abs().T) for w in (wg, wu))
+    silu = torch.nn.functional.silu
+    # |silu'| <= 1.1; fp32's exponential, sum, reciprocal and product: 2^-20 of the result (|g| <= 16 here).
+    assert float(g.abs().max()) <= 16
+    err = 1.1 * eg * (u.abs() + eu) + silu(g).abs() * eu + 2.0 ** -20 * (silu(g) * u).abs()
+    ref = silu(g) * u
+    tol = HALF * (ref.abs() + err) + err
+    d = (y.double().cpu() - ref).abs()
+    assert y.shape == (m, n) and bool((d <= tol).all()), float((d / tol).max())
+
+
+def test_few_rows_keep_nan_and_infinity_to_their_row_and_weight():
+    k, m = 256, 7
+    ws = [weight(n, k, seed=n) for n in (40, 24)]
+    ws[1][1][3, 1] = 255
+    x = rnd(m, k, seed=1)
+    x[2, 5] = math.nan
+    x[4, 200] = math.inf
+    dev = [(c.to(DEV), s.to(DEV)) for c, s in ws]
+    nw = torch.ones(k, dtype=torch.bfloat16, device=DEV)
+    for kw in ({}, dict(norm_weight=nw, eps=1e-6)):
+        y = K.matmul_segments_mxfp4(x.to(DEV), dev, **kw).cpu()
+        assert torch.isnan(y[:, 43]).all() and torch.isnan(y[2]).all() and not torch.isfinite(y[4, :40]).any()
+        keep = [i for i in range(m) if i not in (2, 4)]
+        assert torch.isfinite(y[keep][:, [j for j in range(64) if j != 43]]).all()
+
+
 @pytest.mark.parametrize("m", [1, 3, 20, 70])
 def test_matmul_bias_residual_out_and_strides(m):
     n, k = 136, 320
@@ -432,6 +531,16 @@ def test_refusals():
         (lambda: K.matmul_mxfp4(x, u(8, 32), u(8, 2), bias=x[0, :7]), ValueError),
         (lambda: K.matmul_mxfp4(x, u(8, 32), u(8, 2), residual=x[:, :7]), ValueError),
         (lambda: K.matmul_mxfp4(x, u(8, 32), u(8, 2), out=x[:, :7]), ValueError),
+        (lambda: K.matmul_segments_mxfp4(x, []), ValueError),
+        (lambda: K.matmul_segments_mxfp4(x, [(u(8, 32), u(8, 2))] * 5), ValueError),
+        (lambda: K.matmul_segments_mxfp4(x, [(u(8, 16), u(8, 1))]), ValueError),
+        (lambda: K.matmul_segments_mxfp4(x, [(u(8, 32), u(8, 1))]), ValueError),
+        (lambda: K.matmul_segments_mxfp4(x, [(u(8, 32), u(8, 2))], [x[0, :7]]), ValueError),
+        (lambda: K.matmul_segments_mxfp4(x.float(), [(u(8, 32), u(8, 2))]), TypeError),
+        (lambda: K.matmul_segments_mxfp4(x, [(u(8, 32), u(8, 2))], norm_weight=x[0, :32], eps=1e-6), ValueError),
+        (lambda: K.matmul_segments_mxfp4(x, [(u(8, 32).cpu(), u(8, 2))]), RuntimeError),
+        (lambda: K.matmul_swiglu_mxfp4(x, (u(8, 32), u(8, 2)), (u(9, 32), u(9, 2))), ValueError),
+        (lambda: K.matmul_swiglu_mxfp4(x, (u(8, 32), u(8, 2)), (u(8, 32).int(), u(8, 2))), TypeError),
         (lambda: K.kv_append_mxfp4(kv, kv[:, :, :1], *cache, lens), ValueError),
         (lambda: K.kv_append_mxfp4(kv, kv, *cache, lens.long()), ValueError),
         (lambda: K.kv_append_mxfp4(kv, kv, *cache[:3], u(2, 2, 31, 4), lens), ValueError),
@@ -472,6 +581,10 @@ def test_no_sequences_and_no_tokens():
         assert not any(t.any() for t in cache) and lens.tolist() == [1] * B
     x = torch.zeros(0, 64, dtype=torch.bfloat16, **d)
     assert K.matmul_mxfp4(x, u(8, 32), u(8, 2)).shape == (0, 8)
+    assert K.matmul_segments_mxfp4(x, [(u(8, 32), u(8, 2))] * 2, norm_weight=x.new_ones(64)).shape == (0, 16)
+    assert K.matmul_swiglu_mxfp4(x, (u(8, 32), u(8, 2)), (u(8, 32), u(8, 2))).shape == (0, 8)
+    one = x.new_ones(1, 128)
+    assert K.matmul_segments_mxfp4(one, [(u(8, 64), u(8, 4)), (u(0, 64), u(0, 4))]).tolist() == [[0.0] * 8]
     assert [t.shape for t in K.mxfp4_quantize(x)] == [(0, 32), (0, 2)]
 
 

@@ -70,6 +70,27 @@ def test_matmul_refusals(L):
     assert mm(M_=0) == 0 and mm(N=0) == 0
 
 
+def test_few_rows_refusals(L):
+    def ptrs(*v):
+        return (ctypes.c_void_p * len(v))(*v)
+
+    def seg(x=FAKE, nw=None, c=ptrs(FAKE, FAKE), s=ptrs(FAKE, FAKE), n=i64(64, 32), nseg=2, M_=4, K=256, ldx=256,
+            ldc=96, dt=1):
+        return L.q3_matmul_segments_mxfp4(x, nw, 1e-6, c, s, None, n, nseg, FAKE, M_, K, ldx, ldc, dt, None)
+    assert seg(x=None) == -1 and seg(c=ptrs(FAKE, None)) == -1 and seg(s=None) == -1
+    assert seg(nseg=0) == -2 and seg(nseg=5) == -2 and seg(n=i64(64, 0)) == -2 and seg(ldc=95) == -2 and seg(ldx=128) == -2
+    assert seg(K=48, ldx=48) == -2 and seg(dt=0) == -3
+    assert seg(M_=33) == -5 and seg(K=96) == -5 and seg(nw=FAKE, K=8320, ldx=8320) == -5
+    assert seg(x=FAKE + 2) == -4 and seg(nw=FAKE + 8) == -4 and seg(ldx=260) == -4
+    assert seg(c=ptrs(FAKE, FAKE + 8)) == -4 and seg(s=ptrs(FAKE + 1, FAKE)) == -4
+    assert seg(M_=0) == 0
+
+    def sw(g=FAKE, u=FAKE, M_=4, N=64, K=256, ldc=64):
+        return L.q3_matmul_swiglu_mxfp4(FAKE, None, 0.0, g, FAKE, u, FAKE, FAKE, M_, N, K, K, ldc, 1, None)
+    assert sw(g=None) == -1 and sw(ldc=63) == -2 and sw(M_=33) == -5 and sw(K=160) == -5 and sw(u=FAKE + 8) == -4
+    assert sw(N=0) == 0 and sw(M_=0) == 0
+
+
 def test_cache_refusals(L):
     st = i64(*([128] * 14))
 
