@@ -6,12 +6,14 @@
 //   s_j = scale q . k_j,  o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  m = max_j s_j
 // over the sequence's rows, in one pass with a running m, sum and o in fp32.
 //
-//  * Work units are 32-row tiles of a (sequence, KV head) pair, listed pair-major;
-//    the waves take contiguous ranges of equal length, so ragged lengths cost
-//    nothing. A pair that one wave finishes is stored at once; a pair split
-//    between waves leaves a record (m, sum, o) per wave (record wave + pair, unique
-//    and increasing in both), merged by mx_decode_combine. Every wave finds its
-//    range by itself: no barrier, and no block waits for another.
+//  * Work units are 32-row tiles of a (sequence, KV head) pair. Where pairs are many or
+//    rows few (pair_waves), a block takes one pair, its waves equal ranges of the units,
+//    and their sums meet in LDS. Otherwise all units, listed pair-major, are split
+//    between all waves in ranges of equal length, so ragged lengths cost nothing: a pair
+//    that one wave finishes is stored at once, one split between waves leaves a record
+//    (m, sum, o) per wave (record wave + pair, unique and increasing in both), merged by
+//    mx_decode_combine. Every wave finds its range by itself: no barrier, and no block
+//    waits for another.
 //  * The up to 16 columns of a 16x16x32 MFMA are the query heads of the group
 //    (times the tokens of a short chunk); larger groups take several columns
 //    sets, each a pair of its own.
@@ -32,10 +34,10 @@
 //
 // Measured (us; the floor is the cache's bytes at 6.5 TB/s, what such a read reaches
 // here): 32 sequences of 8 KV heads x 4, lengths to 8192, 165 MB: 30 and 5.6 for the
-// merge (floor 25; the conversions and the transposition of V, 1000 of a unit's 1950
-// cycles in a wave, hide under the loads of the other two on its SIMD); one of 1500
-// rows, 1.6 MB: 5.5 and 4.4, all of it latency; 37 tokens on 4 x 2000 rows of 4 x 8
-// heads (304 column sets that read the same rows from the L2): 22 and 7.
+// merge (floor 25; with the arithmetic left out both take 40.5 in place of 42.8, so it
+// hides under the loads); one of 1500 rows, 1.6 MB: 5.5 and 4.4, all of it latency; a
+// block per pair, 32 sequences to 2000: 19 (split 23.5); 64 tokens on 4 x 2000 rows (512
+// pairs of 16 columns, which read the same rows from the L2): 27 (split 37).
 #include <algorithm>
 #include <type_traits>
 
@@ -155,8 +157,11 @@ struct WaveLds {
   static_assert(16 * D * 2 <= 2 * kCodes, "the rows of V being transposed");
 };
 
-template <int D, bool ONCE>
-__global__ __launch_bounds__(64 * kWavesPerBlock) void mx_decode_kernel(const MxAttn p) {
+// PW = 0: the units of all pairs split between all waves. PW > 0: a block of PW waves takes one pair, each wave an
+// equal range of its units; their sums meet in LDS and the block stores the pair's outputs. ONCE: the rows are read
+// once (non-temporal loads).
+template <int D, bool ONCE, int PW>
+__global__ __launch_bounds__(64 * (PW ? PW : kWavesPerBlock)) void mx_decode_kernel(const MxAttn p) {
   constexpr int LB = D / 8;         // bytes of codes a lane takes of a row
   constexpr int LW = LB / 4;        // the same in words: A fragments of 8 values
   constexpr int DT = D / 16;        // output tiles along the head dim
@@ -165,45 +170,55 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void mx_decode_kernel(const Mx
   constexpr int LOADS = 2 * PIECES + 1;
   typedef WaveLds<D> Lds;
   typedef uint32_t words __attribute__((ext_vector_type(LW)));
-  __shared__ __attribute__((aligned(1024))) char s_mem[kWavesPerBlock * Lds::kBytes];
+  __shared__ __attribute__((aligned(1024))) char s_mem[(PW ? PW : kWavesPerBlock) * Lds::kBytes];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int HS = p.Hkv * p.nset;
 
-  // The wave's units: every wave sums the sequences' unit counts by itself (64 a
-  // round), so nothing waits at a barrier.
-  const bool first_wave = blockIdx.x == 0 && wave == 0;
-  int total = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const int incl = wave_scan(b0 + lane < p.B ? units_of(p, b0 + lane) : 0, lane);
-    if (first_wave && b0 + lane < p.B) p.hdr[b0 + lane + 1] = total + incl;  // for the merge, which must not read the lengths
-    total += __builtin_amdgcn_readlane(incl, 63);
-  }
-  if (first_wave && lane == 0) p.hdr[0] = 0;
-  const Split split(total * HS);
-  // Blocks run round-robin on the 8 XCDs. Each XCD takes an eighth of the active waves,
-  // consecutive ones (which read the same rows where there are several column sets) on
-  // different CUs.
-  const int xcd = blockIdx.x & 7, j = wave * (kBlocks / 8) + ((int)blockIdx.x >> 3);
-  const int here = split.n / 8 + (xcd < split.n % 8);
-  if (j >= here) return;
-  const int w = xcd * (split.n / 8) + min(xcd, split.n % 8) + j;
-  const int u0 = split.first(w), count = split.first(w + 1) - u0;
+  int w = 0, count;  // the wave among all, and its units
   Cursor cc{};
-  for (int b0 = 0, before = 0; b0 < p.B; b0 += 64) {
-    const int n = b0 + lane < p.B ? units_of(p, b0 + lane) : 0;
-    const int incl = before + wave_scan(n, lane);
-    const int at = __popcll(__builtin_amdgcn_ballot_w64(incl * HS <= u0));  // sequences that end at or before u0
-    if (at < 64) {
-      cc.b = b0 + at;
-      cc.nb = __builtin_amdgcn_readlane(n, at);
-      const int r = u0 - (__builtin_amdgcn_readlane(incl, at) - cc.nb) * HS;
-      cc.hs = r / cc.nb;
-      cc.tile = r - cc.hs * cc.nb;
-      break;
+  if constexpr (PW > 0) {
+    cc.b = (int)blockIdx.x / HS;
+    cc.hs = (int)blockIdx.x - cc.b * HS;
+    cc.nb = units_of(p, cc.b);
+    cc.tile = cc.nb * wave / PW;
+    count = cc.nb * (wave + 1) / PW - cc.tile;
+  } else {
+    // The wave's units: every wave sums the sequences' unit counts by itself (64 a
+    // round), so nothing waits at a barrier.
+    const bool first_wave = blockIdx.x == 0 && wave == 0;
+    int total = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      const int incl = wave_scan(b0 + lane < p.B ? units_of(p, b0 + lane) : 0, lane);
+      if (first_wave && b0 + lane < p.B) p.hdr[b0 + lane + 1] = total + incl;  // for the merge, which must not read the lengths
+      total += __builtin_amdgcn_readlane(incl, 63);
     }
-    before = __builtin_amdgcn_readlane(incl, 63);
+    if (first_wave && lane == 0) p.hdr[0] = 0;
+    const Split split(total * HS);
+    // Blocks run round-robin on the 8 XCDs. Each XCD takes an eighth of the active waves,
+    // consecutive ones (which read the same rows where there are several column sets) on
+    // different CUs.
+    const int xcd = blockIdx.x & 7, j = wave * (kBlocks / 8) + ((int)blockIdx.x >> 3);
+    const int here = split.n / 8 + (xcd < split.n % 8);
+    if (j >= here) return;
+    w = xcd * (split.n / 8) + min(xcd, split.n % 8) + j;
+    const int u0 = split.first(w);
+    count = split.first(w + 1) - u0;
+    for (int b0 = 0, before = 0; b0 < p.B; b0 += 64) {
+      const int n = b0 + lane < p.B ? units_of(p, b0 + lane) : 0;
+      const int incl = before + wave_scan(n, lane);
+      const int at = __popcll(__builtin_amdgcn_ballot_w64(incl * HS <= u0));  // sequences that end at or before u0
+      if (at < 64) {
+        cc.b = b0 + at;
+        cc.nb = __builtin_amdgcn_readlane(n, at);
+        const int r = u0 - (__builtin_amdgcn_readlane(incl, at) - cc.nb) * HS;
+        cc.hs = r / cc.nb;
+        cc.tile = r - cc.hs * cc.nb;
+        break;
+      }
+      before = __builtin_amdgcn_readlane(incl, 63);
+    }
   }
   char* mem = s_mem + wave * Lds::kBytes;
   const uint32_t lmem = lds_addr(mem);
@@ -288,6 +303,7 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void mx_decode_kernel(const Mx
     lsum = 0.f;
   };
   auto flush = [&](const Cursor& x, bool whole) {
+    if constexpr (PW > 0) return;
     lsum += __shfl_xor(lsum, 16, 64);
     lsum += __shfl_xor(lsum, 32, 64);
     if (!valid) return;
@@ -312,6 +328,14 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void mx_decode_kernel(const Mx
   };
 
   start(cc);  // its loads before the ring's: loads retire in order
+  if constexpr (PW > 0) {
+    if (cc.nb == 0) {  // an empty sequence: zeros
+      if (valid && wave == 0)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) *reinterpret_cast<bf16x4*>(p.o + o_off + 16 * t + 4 * g) = bf16x4{};
+      return;
+    }
+  }
   open(ic);
   int issued = 0, islot = 0, slot_at = 0;
   auto issue_next = [&]() {
@@ -426,6 +450,50 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void mx_decode_kernel(const Mx
     }
   }
   vm_wait<0>();  // no load may still target this block's LDS when the wave retires
+  if constexpr (PW > 0) {  // this wave's statistics and sums over its slots: m[kCols], sum[kCols], o[kCols][D]
+    constexpr int N = D / 64;  // outputs per lane
+    typedef float outs __attribute__((ext_vector_type(N)));
+    static_assert(rec_floats(D) * 4 <= Lds::kBytes, "a wave's sums take the place of its slots");
+    lsum += __shfl_xor(lsum, 16, 64);
+    lsum += __shfl_xor(lsum, 32, 64);
+    asm volatile("" ::: "memory");
+    float* rec = reinterpret_cast<float*>(mem);
+    if (g == 0) {
+      rec[c] = m;
+      rec[kCols + c] = lsum;
+    }
+#pragma unroll
+    for (int t = 0; t < DT; ++t) *reinterpret_cast<floatx4*>(rec + 2 * kCols + c * D + 16 * t + 4 * g) = o[t];
+    __syncthreads();
+    const int kvh = cc.hs / p.nset, col0 = (cc.hs - kvh * p.nset) * kCols;
+    for (int col = wave; col < kCols; col += PW) {
+      const int tok = (col0 + col) / p.groups, hd = col0 + col - tok * p.groups;
+      if (tok >= p.Sq) break;
+      auto rec_of = [&](int k) { return reinterpret_cast<const float*>(s_mem + k * Lds::kBytes); };
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < PW; ++k) top = fmaxf(top, rec_of(k)[col]);
+      if (top == -INFINITY) top = 0.f;  // no row seen: weights 0, not NaN
+      float sum = 0.f;
+      outs v{};
+#pragma unroll
+      for (int k = 0; k < PW; ++k) {
+        const float r = exp2_(rec_of(k)[col] - top);
+        sum += rec_of(k)[kCols + col] * r;
+        v += *reinterpret_cast<const outs*>(rec_of(k) + 2 * kCols + col * D + N * lane) * r;
+      }
+      const float inv = sum != 0.f ? 1.0f / sum : 0.f;  // a NaN sum stays one
+      bf16* y = p.o + cc.b * p.ob + ((int64_t)kvh * p.groups + hd) * p.oh + tok * p.os + N * lane;
+#pragma unroll
+      for (int e = 0; e < N; ++e) y[e] = f2bf(v[e] * inv);
+    }
+  }
+}
+
+// Advances the lengths, behind a launch whose blocks all read them.
+__global__ void mx_advance_kernel(int* lens, int B, int inc) {
+  const int b = blockIdx.x * 64 + threadIdx.x;
+  if (b < B) lens[b] += inc;
 }
 
 // Merges the records of the pairs split between waves: a block per pair and column,
@@ -520,29 +588,63 @@ int64_t sets_of(int64_t groups, int64_t Sq) { return q3_cdiv(groups * Sq, kCols)
 // row among 256 columns but does not split the rows: its time grows with the rows until
 // the pairs fill the card, the streaming kernel's with pairs x rows. Microseconds,
 // streaming / expanding, 8 KV heads of 4 query heads unless said otherwise: 8192 rows, 32
-// tokens (64 pairs) 38 / 208, 128 (256) 60 / 213, 512 (1024) 168 / 214, 700 (1400) 216 /
-// 215, 1000 (2000) 294 / 215; 4 x 2000 rows, 64 tokens (512) 38 / 72, 128 (1024) 52 / 73,
-// 200 (1600) 63 / 72; 1024 rows, 256 tokens (512) 33 / 41, 512 (1024) 47 / 42; 8 x 300
-// rows of 4 x 8 heads, 40 tokens (640) 24 / 26, 100 (1600) 37 / 29. The rows of the rule
-// are the capacity: the lengths are on the device.
-bool streams(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq, int64_t cap) {
-  return Sq == 1 || B * Hkv * sets_of(groups, Sq) <= 1000 + cap / 20;
+// tokens (64 pairs) 38 / 209, 128 (256) 53 / 213, 512 (1024) 160 / 214, 700 (1400) 219 /
+// 215, 1000 (2000) 279 / 216; 4 x 2000 rows, 64 tokens (512) 27 / 72, 200 (1600) 54 / 73,
+// 300 (2432) 84 / 73; 1024 rows, 256 tokens (512) 20 / 41, 512 (1024) 34 / 42; 8 x 300
+// rows of 4 x 8 heads, 60 tokens (960) 21 / 28, 100 (1600) 28 / 29, 150 (2400) 37 / 30.
+constexpr int64_t kStreamPairs = 1400;
+bool streams(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq) {
+  return Sq == 1 || B * Hkv * sets_of(groups, Sq) <= kStreamPairs;
 }
 
 int64_t stream_ws_bytes(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq, int64_t D) {
   return header_bytes(B) + (kWaves + B * Hkv * sets_of(groups, Sq)) * (int64_t)rec_floats((int)D) * 4;
 }
 
+// Waves of a block that takes one pair, or 0 to split all units between all waves and merge records. Pairs per
+// block save the records and the merge, but each pair's rows go through few waves: right for few rows, for many pairs,
+// and the more columns a pair has (its records are that much larger). Rows are the capacity, as the lengths are on the
+// device. Both kernels, us, split / 8 waves / 4 waves: decode of 4 heads to a KV head, 8 pairs of 300 rows 11.0 / 10.3
+// / 9.7, 1000 11.3 / 13.0 / 13.1; 64 pairs, 500 12.9 / 10.8 / 10.5, 1500 15.1 / 15.5 / 18.0; 256 pairs, 300 15.8 /
+// 10.7 / 9.6, 2000 23.5 / 18.8 / 21.5; 512 pairs, 1000 24.6 / 22.3 / 18.5, 4000 42.7 / 48.9 / 44.0; 1024 pairs,
+// 1000 30.6 / 39.5 / 28.5, 4000 67 / 83 / 71; chunks of 16 columns, 128 pairs of 1024 rows 27.7 / 14.7 / 14.5, 304 of
+// 2000 31.9 / 24.8 / 25.0, 512 of 2000 37.6 / 32.5 / 26.1, 256 of 8192 58.7 / 49.9 / 65.6, 1024 of 8192 161 / 180 / 153.
+int pair_waves(int64_t pairs, int64_t cap, int64_t cols) {
+  if (cap > std::min<int64_t>(512 + 2 * cols * pairs, 640 * cols)) return 0;
+  return pairs <= 320 && cap > 1024 ? 8 : 4;
+}
+
+template <int D, int PW>
+void launch_pairs(const MxAttn& p, int pairs, hipStream_t st) {
+  if (p.nset == 1)  // every row is read once
+    hipLaunchKernelGGL((mx_decode_kernel<D, true, PW>), dim3((unsigned)pairs), dim3(64 * PW), 0, st, p);
+  else
+    hipLaunchKernelGGL((mx_decode_kernel<D, false, PW>), dim3((unsigned)pairs), dim3(64 * PW), 0, st, p);
+}
+
 template <int D>
 int launch_stream(const MxAttn& p, hipStream_t st) {
+  const int pairs = p.B * p.Hkv * p.nset;
+  const int cols = std::min(kCols, p.groups * p.Sq);
+  if (const int waves = pair_waves(pairs, p.cap, cols)) {
+    if (waves == 8)
+      launch_pairs<D, 8>(p, pairs, st);
+    else
+      launch_pairs<D, 4>(p, pairs, st);
+    Q3_LAUNCH_CHECK();
+    if (p.lens_inc) {
+      hipLaunchKernelGGL(mx_advance_kernel, dim3((unsigned)q3_cdiv(p.B, 64)), dim3(64), 0, st, p.lens_inc, p.B, p.inc);
+      Q3_LAUNCH_CHECK();
+    }
+    return Q3_OK;
+  }
   const dim3 grid(kBlocks), block(64 * kWavesPerBlock);
   if (p.nset == 1)  // every row is read once
-    hipLaunchKernelGGL((mx_decode_kernel<D, true>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((mx_decode_kernel<D, true, 0>), grid, block, 0, st, p);
   else
-    hipLaunchKernelGGL((mx_decode_kernel<D, false>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((mx_decode_kernel<D, false, 0>), grid, block, 0, st, p);
   Q3_LAUNCH_CHECK();
-  const int pairs = p.B * p.Hkv * p.nset;
-  const dim3 merge((unsigned)pairs, (unsigned)std::min(kCols, p.groups * p.Sq));
+  const dim3 merge((unsigned)pairs, (unsigned)cols);
   // The merge is bound by latency: all of a pair's records should be in flight at once and all blocks resident.
   // A pair has up to kWaves / pairs records: 16 waves share more than 16 of them (8 pairs of one sequence's 1500
   // rows: 4.4 us against 6.3 on 4), 4 waves fewer (256 pairs of 32 sequences: 5.6 us, 8.5 on 16 and on 1), one wave
@@ -570,7 +672,7 @@ int check(const void* q, const void* kc, const void* ks, const void* vc, const v
   Q3_REQUIRE(B >= 0 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Sq >= 0 && D >= 1 && cap >= 0, Q3_ERR_SHAPE);
   Q3_REQUIRE(dtype == Q3_BF16, Q3_ERR_DTYPE);
   Q3_REQUIRE((D == 64 || D == 128) && B <= kMaxBatch && (cap + kUnit) * D / 2 < (1ll << 31) && Sq < (1ll << 31) &&
-                 Hq < (1ll << 16) && B * Hkv * sets_of(Hq / Hkv, streams(B, Hkv, Hq / Hkv, Sq, cap) ? Sq : 1) * q3_cdiv(cap, kUnit) < (1ll << 31),
+                 Hq < (1ll << 16) && B * Hkv * sets_of(Hq / Hkv, streams(B, Hkv, Hq / Hkv, Sq) ? Sq : 1) * q3_cdiv(cap, kUnit) < (1ll << 31),
              Q3_ERR_UNSUPPORTED);
   bool ok = q3_aligned(q, 16) && q3_aligned(kc, 16) && q3_aligned(vc, 16) && q3_aligned(o, 8);
   for (int i = 0; i < 6; ++i) ok = ok && strides[i] % 8 == 0;
@@ -671,7 +773,7 @@ int q3_decode_attention_mxfp4(const void* q, const void* k_codes, const void* k_
 int64_t q3_flash_attention_cache_mxfp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
                                                        int64_t max_len) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || D <= 0 || max_len < 0) return 0;
-  if (streams(B, Hkv, Hq / Hkv, Sq, max_len)) return stream_ws_bytes(B, Hkv, Hq / Hkv, Sq, D);
+  if (streams(B, Hkv, Hq / Hkv, Sq)) return stream_ws_bytes(B, Hkv, Hq / Hkv, Sq, D);
   return 2 * B * Hkv * max_len * D * 2;  // K and V in bf16
 }
 
@@ -688,7 +790,7 @@ int q3_flash_attention_cache_mxfp4(const void* q, const void* k_codes, const voi
              Q3_ERR_WORKSPACE);
   Q3_REQUIRE(q3_aligned(workspace, 16), Q3_ERR_ALIGN);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (streams(B, Hkv, Hq / Hkv, Sq, max_len)) {
+  if (streams(B, Hkv, Hq / Hkv, Sq)) {
     MxAttn p = arguments(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, Sq, max_len, strides, scale);
     p.len_add = 1;
     p.lens_inc = advance ? kv_lens : nullptr;

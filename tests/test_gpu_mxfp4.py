@@ -321,6 +321,28 @@ def test_decode_matches_float64(hkv, groups, d):
     assert bool((o[0] == 0).all())
 
 
+# (lengths, KV heads, group, capacity): a block of four or of eight waves per pair, and units split between all waves
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens,hkv,groups,cap", [([0, 1, 33, 300, 512], 8, 4, 512), ([1100, 0, 1200, 31] * 4, 8, 4, 1200),
+                                                 ([1500, 700], 2, 4, 1500), ([5, 0, 600] * 10, 16, 1, 600),
+                                                 ([1300, 64, 0], 40, 2, 1300), ([700] * 3, 90, 1, 700)])
+def test_decode_by_pairs_and_split(lens, hkv, groups, cap, d):
+    c = Cache(lens, hkv, cap, d, seed=51, used=0)
+    q = rnd(len(lens), hkv * groups, d, seed=52)
+    o = K.decode_attention_mxfp4(q.to(DEV), *c.device(), c.lens.to(DEV), d ** -0.5)
+    check_attention(o.unsqueeze(2), q.unsqueeze(2), c, c.lens.view(-1, 1), d ** -0.5)
+
+
+@pytest.mark.parametrize("cap", [100, 1500])
+def test_steps_advance_past_the_capacity_alike(cap):
+    """Both forms attend to the rows up to the capacity and advance every length by one, the full ones too."""
+    c = Cache([cap - 1, cap, 3], 1, cap, 128, seed=53, used=1)
+    q, lens = rnd(3, 4, 128, seed=54), c.lens.to(DEV)
+    o = K.decode_attention_mxfp4(q.to(DEV), *c.device(), lens, 0.1, append=True)
+    assert lens.tolist() == [cap, cap + 1, 4]
+    check_attention(o.unsqueeze(2), q.unsqueeze(2), c, (c.lens + 1).clamp(max=cap).view(-1, 1), 0.1)
+
+
 def test_decode_one_long_sequence_and_large_scores():
     c = Cache([5003], 2, 5003, 128, seed=5)
     q = rnd(1, 8, 128, seed=6) * 6
@@ -363,7 +385,7 @@ def test_decode_nan_row_reaches_its_block_of_the_output_only():
 
 # (KV heads, group, tokens): the last ones over the expanded cache
 CHUNKS = [(1, 1, 2), (2, 4, 3), (1, 4, 4), (2, 4, 5), (2, 3, 40), (1, 8, 33), (2, 2, 100), (1, 1, 16), (1, 1, 17), (4, 8, 45), (9, 5, 75),
-          (13, 4, 65)]
+          (9, 5, 110), (13, 4, 92)]
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -405,14 +427,14 @@ def test_short_chunk_a_later_tokens_nan_is_masked(groups, sq):
 @pytest.mark.parametrize("advance", [False, True])
 def test_long_chunk_a_nan_row_reaches_the_tokens_that_see_it(d, advance):
     """Past the streaming kernel's pairs, over expanded rows."""
-    B, hkv, groups, sq = 2, 15, 8, 80
-    assert B * hkv * groups * sq / 16 > 1024
-    c = Cache([20, 31], hkv, 120, d, seed=26, used=sq)
+    B, hkv, groups, sq = 2, 15, 8, 100
+    assert B * hkv * groups * sq / 16 > 1400
+    c = Cache([20, 31], hkv, 140, d, seed=26, used=sq)
     q = rnd(B, hkv * groups, sq, d, seed=27)
     c.vs[0, 0, 20 + 50, 1] = 255  # token 50's value
     c.vs[1, 3, 31 + 7, 0] = 255
     c.ks[1, 4, 31 + 60, 0] = 255  # token 60's key
-    clean = Cache([20, 31], hkv, 120, d, seed=26, used=sq)
+    clean = Cache([20, 31], hkv, 140, d, seed=26, used=sq)
     lens = c.lens.to(DEV)
     o = K.flash_attention_cache_mxfp4(q.to(DEV), *c.device(), lens, 0.1, groups, advance=advance).cpu()
     ref = K.flash_attention_cache_mxfp4(q.to(DEV), *clean.device(), c.lens.to(DEV), 0.1, groups).cpu()
