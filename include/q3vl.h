@@ -627,8 +627,8 @@ int q3_qk_norm_rope_mxfp4(const void* q_in, const void* k_in, const void* v_in, 
  * step, whose row is already written; kv_lens[b] is then incremented in place), at most cap. q, o (B, Hq, D);
  * strides = [qb, qh, 0, ob, oh, 0] in elements, then [b, h] of k_codes, k_scales, v_codes, v_scales in bytes. An
  * empty sequence gives zeros; a NaN reaches only the queries that see its row. bf16, D = 64 or 128, B <= 1024 (else
- * Q3_ERR_UNSUPPORTED). */
-int64_t q3_decode_attention_mxfp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
+ * Q3_ERR_UNSUPPORTED). Small caches need no workspace: the query gives 0, and it may be null. */
+int64_t q3_decode_attention_mxfp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap);
 int q3_decode_attention_mxfp4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
                               const void* v_scales, int* kv_lens, int advance, void* o, int64_t B, int64_t Hq,
                               int64_t Hkv, int64_t D, int64_t cap, const int64_t* strides, float scale, int dtype,

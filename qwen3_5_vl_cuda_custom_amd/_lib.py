@@ -123,7 +123,7 @@ _SIGS: dict[str, tuple] = {
     "q3_kv_append_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, _V, c_int, _V]),
     "q3_qk_norm_rope_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, _I, _i64p,
                                       c_float, _V, c_int, _V]),
-    "q3_decode_attention_mxfp4_workspace_bytes": (c_int64, [_I, _I, _I, _I]),
+    "q3_decode_attention_mxfp4_workspace_bytes": (c_int64, [_I, _I, _I, _I, _I]),
     "q3_decode_attention_mxfp4": (c_int, [_V, _V, _V, _V, _V, _V, c_int, _V, _I, _I, _I, _I, _I, _V, c_float, c_int,
                                           _V, _I, _V]),
     "q3_flash_attention_cache_mxfp4_workspace_bytes": (c_int64, [_I, _I, _I, _I, _I, _I]),

@@ -597,10 +597,6 @@ bool streams(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq) {
   return Sq == 1 || B * Hkv * sets_of(groups, Sq) <= kStreamPairs;
 }
 
-int64_t stream_ws_bytes(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq, int64_t D) {
-  return header_bytes(B) + (kWaves + B * Hkv * sets_of(groups, Sq)) * (int64_t)rec_floats((int)D) * 4;
-}
-
 // Waves of a block that takes one pair, or 0 to split all units between all waves and merge records. Pairs per
 // block save the records and the merge, but each pair's rows go through few waves: right for few rows, for many pairs,
 // and the more columns a pair has (its records are that much larger). Rows are the capacity, as the lengths are on the
@@ -612,6 +608,12 @@ int64_t stream_ws_bytes(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq, int6
 int pair_waves(int64_t pairs, int64_t cap, int64_t cols) {
   if (cap > std::min<int64_t>(512 + 2 * cols * pairs, 640 * cols)) return 0;
   return pairs <= 320 && cap > 1024 ? 8 : 4;
+}
+
+int64_t stream_ws_bytes(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq, int64_t D, int64_t cap) {
+  const int64_t pairs = B * Hkv * sets_of(groups, Sq);
+  if (pair_waves(pairs, cap, std::min<int64_t>(kCols, groups * Sq))) return 0;
+  return header_bytes(B) + (kWaves + pairs) * (int64_t)rec_floats((int)D) * 4;
 }
 
 template <int D, int PW>
@@ -748,9 +750,9 @@ __global__ __launch_bounds__(256) void mx_chunk_nan_kernel(const MxAttn p, int o
 
 extern "C" {
 
-int64_t q3_decode_attention_mxfp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
-  if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return 0;
-  return stream_ws_bytes(B, Hkv, Hq / Hkv, 1, D);
+int64_t q3_decode_attention_mxfp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || cap < 0) return 0;
+  return stream_ws_bytes(B, Hkv, Hq / Hkv, 1, D, cap);
 }
 
 int q3_decode_attention_mxfp4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
@@ -759,9 +761,9 @@ int q3_decode_attention_mxfp4(const void* q, const void* k_codes, const void* k_
                               void* workspace, int64_t workspace_bytes, void* stream) {
   const int rc = check(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, 1, D, cap, strides, dtype);
   if (rc != Q3_OK || B == 0) return rc;
-  Q3_REQUIRE(workspace && workspace_bytes >= q3_decode_attention_mxfp4_workspace_bytes(B, Hq, Hkv, D),
-             Q3_ERR_WORKSPACE);
-  Q3_REQUIRE(q3_aligned(workspace, 16), Q3_ERR_ALIGN);
+  const int64_t need = q3_decode_attention_mxfp4_workspace_bytes(B, Hq, Hkv, D, cap);
+  Q3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Q3_ERR_WORKSPACE);
+  Q3_REQUIRE(need == 0 || q3_aligned(workspace, 16), Q3_ERR_ALIGN);
   MxAttn p = arguments(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, 1, cap, strides, scale);
   p.len_add = advance ? 1 : 0;
   p.lens_inc = advance ? kv_lens : nullptr;
@@ -773,7 +775,7 @@ int q3_decode_attention_mxfp4(const void* q, const void* k_codes, const void* k_
 int64_t q3_flash_attention_cache_mxfp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
                                                        int64_t max_len) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || D <= 0 || max_len < 0) return 0;
-  if (streams(B, Hkv, Hq / Hkv, Sq)) return stream_ws_bytes(B, Hkv, Hq / Hkv, Sq, D);
+  if (streams(B, Hkv, Hq / Hkv, Sq)) return stream_ws_bytes(B, Hkv, Hq / Hkv, Sq, D, max_len);
   return 2 * B * Hkv * max_len * D * 2;  // K and V in bf16
 }
 
@@ -785,10 +787,9 @@ int q3_flash_attention_cache_mxfp4(const void* q, const void* k_codes, const voi
       check(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, Sq, D, max_len, strides, dtype);
   if (rc != Q3_OK || B == 0 || Sq == 0) return rc;
   Q3_REQUIRE(Sq <= max_len, Q3_ERR_SHAPE);
-  Q3_REQUIRE(workspace &&
-                 workspace_bytes >= q3_flash_attention_cache_mxfp4_workspace_bytes(B, Hq, Hkv, Sq, D, max_len),
-             Q3_ERR_WORKSPACE);
-  Q3_REQUIRE(q3_aligned(workspace, 16), Q3_ERR_ALIGN);
+  const int64_t need = q3_flash_attention_cache_mxfp4_workspace_bytes(B, Hq, Hkv, Sq, D, max_len);
+  Q3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Q3_ERR_WORKSPACE);
+  Q3_REQUIRE(need == 0 || q3_aligned(workspace, 16), Q3_ERR_ALIGN);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (streams(B, Hkv, Hq / Hkv, Sq)) {
     MxAttn p = arguments(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, Sq, max_len, strides, scale);

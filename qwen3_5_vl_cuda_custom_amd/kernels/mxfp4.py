@@ -33,8 +33,8 @@ def _matmul_workspace(M: int, N: int, K: int) -> int:
 
 
 @lru_cache(maxsize=1024)
-def _decode_workspace(B: int, Hq: int, Hkv: int, D: int) -> int:
-    return _lib.lib().q3_decode_attention_mxfp4_workspace_bytes(B, Hq, Hkv, D)
+def _decode_workspace(B: int, Hq: int, Hkv: int, D: int, cap: int) -> int:
+    return _lib.lib().q3_decode_attention_mxfp4_workspace_bytes(B, Hq, Hkv, D, cap)
 
 
 def _off_device(op: str, *tensors: torch.Tensor | None) -> None:
@@ -482,12 +482,12 @@ def decode_attention_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: tor
     q, o = _query(op, q, out)
     if B == 0:
         return o
-    nws = _decode_workspace(B, Hq, Hkv, D)
-    ws = k_codes.new_empty(nws)
+    nws = _decode_workspace(B, Hq, Hkv, D, cap)
+    ws = k_codes.new_empty(nws) if nws else None
     qs, os = q.stride(), o.stride()
     _lib.call("q3_decode_attention_mxfp4", q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
               v_scales.data_ptr(), kv_lens.data_ptr(), 1 if append else 0, o.data_ptr(), B, Hq, Hkv, D, cap,
-              _i64x14(qs[0], qs[1], 0, os[0], os[1], 0, *st), scale, _lib.Q3_BF16, ws.data_ptr(), nws,
+              _i64x14(qs[0], qs[1], 0, os[0], os[1], 0, *st), scale, _lib.Q3_BF16, _lib.ptr(ws), nws,
               _lib.raw_stream(dev))
     return o
 
@@ -501,7 +501,7 @@ def flash_attention_cache_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales
     q (B, Hq, Sq, D) bf16, D 64 or 128; the chunk's rows [kv_lens[b], kv_lens[b] + Sq) are already in the cache.
     Query i of sequence b attends to cache rows [0, kv_lens[b] + i]; advance=True adds Sq to kv_lens afterwards.
     `max_len` bounds every kv_lens[b] + Sq (default: cap): rows past it are not read. It sizes the workspace of a
-    longer chunk, 4 * B * Hkv * max_len * D bytes.
+    chunk of more than 1400 (sequence, KV head, 16 columns), 4 * B * Hkv * max_len * D bytes.
     """
     op = "flash_attention_cache_mxfp4"
     if q.dim() != 4:
@@ -518,10 +518,10 @@ def flash_attention_cache_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales
     if q.numel() == 0:
         return o
     nws = _lib.lib().q3_flash_attention_cache_mxfp4_workspace_bytes(B, Hq, Hkv, Sq, D, ml)
-    ws = k_codes.new_empty(nws)
+    ws = k_codes.new_empty(nws) if nws else None
     qs, os = q.stride(), o.stride()
     _lib.call("q3_flash_attention_cache_mxfp4", q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(),
               v_codes.data_ptr(), v_scales.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), B, Hq, Hkv, Sq, D, ml,
-              _i64x14(*qs[:3], *os[:3], *st), scale, 1 if advance else 0, _lib.Q3_BF16, ws.data_ptr(), nws,
+              _i64x14(*qs[:3], *os[:3], *st), scale, 1 if advance else 0, _lib.Q3_BF16, _lib.ptr(ws), nws,
               _lib.raw_stream(dev))
     return o

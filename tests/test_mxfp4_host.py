@@ -111,13 +111,15 @@ def test_cache_refusals(L):
     assert decode(dt=0) == -3
     assert decode(kc=FAKE + 8) == -4 and decode(s=i64(4, *([128] * 13))) == -4
     assert decode(D=96) == -5 and decode(B=1025) == -5
-    assert decode(nws=100) == -6 and decode(ws=None) == -6
+    assert decode(cap=20000, nws=100) == -6 and decode(cap=20000, ws=None) == -6
+    assert decode(cap=20000, ws=FAKE + 8) == -4
+    assert L.q3_decode_attention_mxfp4_workspace_bytes(2, 8, 2, 128, 32) == 0  # a block per pair
     assert decode(B=0) == 0
 
     def chunk(Sq=64, ml=128, nws=1 << 30, ws=FAKE):
         return L.q3_flash_attention_cache_mxfp4(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 2, 8, 2, Sq, 128, ml, st,
                                                 1.0, 0, 1, ws, nws, None)
-    assert chunk(Sq=129) == -2 and chunk(nws=0) == -6 and chunk(ws=None) == -6
+    assert chunk(Sq=129) == -2 and chunk(ml=20000, nws=0) == -6 and chunk(ml=20000, ws=None) == -6
     assert chunk(Sq=0) == 0
 
 
