@@ -6,7 +6,7 @@
 //
 // Bound by the stream of weights. Every CU owns whole weight rows (all of k), so no
 // sums pass between blocks; codes, scales and x go global -> LDS past the registers in
-// stages of 512 k, a ring of up to four stages per block keeps the loads in flight, one
+// stages of 512 k, a ring of up to six stages per block keeps the loads in flight, one
 // barrier per stage. A wave takes a quarter of a stage: lane (i = l % 16, g = l /
 // 16) reads the 16 bytes of block g of that quarter of weight row i and its scale, and
 // the 32 values of x's row i at the same k, and forms four products of 16x16x32 (k
@@ -14,8 +14,8 @@
 // The norm: x becomes bf16(x * norm weight) on its way into the product, each lane keeps
 // the sum of x^2 over the k it sees, and the sums are scaled by rsqrt(sum / K + eps).
 //
-// Measured (us; an empty kernel takes 2): one row, N=K=4096 5.0, N=12288 K=4096 7.7 (3.5
-// TB/s), N=24576 12.7 (4.2 TB/s), N=4096 K=12288 9.2, N=151936 K=4096 62 (5.3 TB/s); 32
+// Measured (us; an empty kernel takes 2): one row, N=K=4096 5.1, N=12288 K=4096 7.4 (3.6
+// TB/s), N=24576 13.3 (4.0 TB/s), N=4096 K=12288 9.3, N=151936 K=4096 62 (5.3 TB/s); 32
 // rows, where each CU also reads all of x from the L2, 8.7, 11.5, 16, 17.5 and 93.
 #include <algorithm>
 
@@ -31,7 +31,6 @@ constexpr int kStageK = 512;
 constexpr int kWaves = 4;
 constexpr int kMaxGroups = 6;       // 16-row groups of a block (gate and up: 4 of each)
 constexpr int kNormMaxK = 8192;     // the norm weight is held in LDS
-constexpr int kRing = 4;            // stages in the ring
 
 template <int RG, int XR, bool SW, bool NORM>
 struct RowsShape {
@@ -41,11 +40,12 @@ struct RowsShape {
   static constexpr int PER = PW + PS + PX;
   static constexpr int kW = RGT * 4096, kS = PS * 1024, kX = XR * 1024, kSlot = kW + kS + kX;  // bytes
   static constexpr int kNorm = NORM ? kNormMaxK * 2 : 0;
-  // Stages of the ring: four, or what fits the LDS; where x takes little of it, what lets two blocks run on a CU,
-  // the next one's first loads under the last one's sums (one row, us, with 8 stages / 4 / 4 in half the LDS: N=12288
-  // K=4096 9.2 / 7.6 / 7.7, N=151936 75 / 69 / 62; 16 rows, 4 / 4 in half: N=12288 9.2 / 10.4).
+  // Stages of the ring. Where x takes little of the LDS, up to six, but no more than lets two blocks run on a CU, the
+  // next one's first loads under the last one's sums (one row, us, 4 stages / 6 / 8, half the LDS: N=4096 K=12288 10.5 /
+  // 9.3 / 9.4, N=6144 K=4096 6.3 / 6.0 / 6.0; N=12288 9.2 with 8 in the whole LDS, 7.4 in half, N=151936 75 / 62).
+  // Else up to four (16 rows, N=12288: 9.2 with 4, 10.4 in half the LDS).
   static constexpr int kLds = (XR < 16 ? 78 : 156) * 1024 - kNorm;
-  static constexpr int NS = std::max(2, std::min(kRing, kLds / kSlot));
+  static constexpr int NS = std::max(2, std::min(XR < 16 ? 6 : 4, kLds / kSlot));
   static_assert(NS * kSlot + kNorm <= 156 * 1024 && (NS - 2) * PER < 64, "the ring, and the count of its loads");
   static_assert(kWaves * RGT * MT * 1024 <= NS * kSlot, "the waves' sums");
 };
