@@ -590,7 +590,7 @@ int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, co
                     void* y, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int64_t lds, int64_t ldr,
                     int64_t ldc, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Decode shapes, M <= 32 rows, in one launch (q3_matmul_segments / q3_matmul_swiglu and their rmsnorm_ forms with
+/* Decode shapes, M <= 64 rows, in one launch (q3_matmul_segments / q3_matmul_swiglu and their rmsnorm_ forms with
  * weights in MXFP4, packed):
  * q3_matmul_segments_mxfp4: y (M, sum n_j) = x [w_0; w_1; ...]^T (+ [b_0; b_1; ...]), 1 to 4 weights of n[j] >= 1
  * rows; codes, scales and bias are host arrays of device pointers (bias, or any of its entries, may be null).

@@ -288,10 +288,13 @@ struct Plan {
   int bn, bm, parts;  // tile, and ranges of k whose sums are added by mx_sum_kernel
 };
 
-// kRows up to 32 rows, but for 17 to 32 rows of K > 8192, where the reads of x by every CU
+// kRows up to 32 rows (K a multiple of 128), but for 17 to 32 rows of K > 8192, where the reads of x by every CU
 // cost more than the sum over ranges of k: us, kRows / tiles, 32 rows: N=4096 K=4096 8.7 /
 // 9.6, K=12288 17.5 / 12.6, N=12288 K=4096 11.5 / 14.1, N=24576 16 / 22; 16 rows: 6.2 / 8.5,
-// 11.6 / 11.9, 9.2 / 13.3, 13.0 / 20.2. Up to 64 rows tiles. Above,
+// 11.6 / 11.9, 9.2 / 13.3, 13.0 / 20.2. 33 to 64 rows: kRows for K up to about 4096 where
+// every CU has one block and not too few rows: 64 rows, K=4096, N=1024 11.5 / 10.0, 4096
+// 12.3 / 14.5, 12288 16.0 / 18.5, 24576 23.2 / 26.0, 151936 143 / 110; N=2048 K=8192 19.5 /
+// 14.7; N=1000 K=1152 6.2 / 10.9. Otherwise tiles up to 64 rows. Above,
 // tiles unless the expansion is estimated faster: 128 x 256 tiles run in rounds of 256
 // at 1.1 PFLOP/s; expanding costs 2.53 bytes a weight at 5.5 TB/s, 16 us, and the
 // product at 1.3 PFLOP/s. Microseconds, tiles / expanded: N=12288 K=4096 M=64 21 / 69,
@@ -299,7 +302,9 @@ struct Plan {
 // / 144; N=K=4096 M=777 43 / 55, M=1500 66 / 77; N=K=1024 M=1500 19 / 18. With fewer tiles
 // than CUs, k is split until they fill them (ranges of at least 512 k).
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
-  if (M <= 4 || (M <= kMxRowsMax && K % 128 == 0 && (M <= 16 || K <= 8192))) return {kRows, 0, 0, 1};
+  if (M <= 4 || (M <= 32 && K % 128 == 0 && (M <= 16 || K <= 8192)) ||
+      (M <= kMxRowsMax && K % 128 == 0 && K <= 4608 && N >= K / 2 && N <= 24576))
+    return {kRows, 0, 0, 1};
   Plan g = M <= 32 ? Plan{kTile32, 128, 32, 1} : M <= 64 ? Plan{kTile64, 256, 64, 1} : Plan{kTile128, 256, 128, 1};
   const int64_t tiles = q3_cdiv(N, g.bn) * q3_cdiv(M, g.bm);
   if (g.form == kTile128) {
@@ -363,7 +368,8 @@ int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, co
     p.ldx = ldx, p.ldw = ldw, p.lds = lds, p.ldr = ldr, p.ldc = ldc;
     return mx_rows(p, false, st);
   }
-  if (g.form == kRows && M > 4) g = Plan{kTile32, 128, 32, 1};  // scales at odd addresses; no workspace
+  if (g.form == kRows && M > 4)  // scales at odd addresses; no workspace
+    g = M <= 32 ? Plan{kTile32, 128, 32, 1} : Plan{kTile64, 256, 64, 1};
   if (g.form == kExpand) {
     Q3_REQUIRE(ldw == K / 2 && lds == K / kMxBlock, Q3_ERR_UNSUPPORTED);
     const int rc = mx_expand(w_codes, w_scales, static_cast<bf16*>(workspace), N * K, st);

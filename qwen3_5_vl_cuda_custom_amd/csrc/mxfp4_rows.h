@@ -1,11 +1,11 @@
-// The product of up to 32 rows with MXFP4 weights (mxfp4_rows.hip).
+// The product of up to 64 rows with MXFP4 weights (mxfp4_rows.hip).
 #pragma once
 
 #include "q3_common.h"
 
 namespace q3 {
 
-constexpr int kMxRowsMax = 32;       // rows of x
+constexpr int kMxRowsMax = 64;       // rows of x
 constexpr int kMxRowsSegments = 4;   // weights side by side
 
 struct MxRows {

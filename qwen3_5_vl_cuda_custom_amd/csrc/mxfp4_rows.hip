@@ -1,4 +1,4 @@
-// Products of up to 32 rows (decode steps) with MXFP4 weights (format: mxfp4.h): one
+// Products of up to 64 rows (decode steps) with MXFP4 weights (format: mxfp4.h): one
 // launch for a single weight, for the weights of several projections side by side, or
 // for SwiGLU's gate and up, with the RMSNorm of the rows fused in if asked for.
 //   y = x w^T (+ bias) (+ residual),  y = silu(x g^T) * (x u^T),  x or norm(x)
@@ -10,13 +10,15 @@
 // barrier per stage. A wave takes a quarter of a stage: lane (i = l % 16, g = l /
 // 16) reads the 16 bytes of block g of that quarter of weight row i and its scale, and
 // the 32 values of x's row i at the same k, and forms four products of 16x16x32 (k
-// permuted alike in both). The 4 waves' sums meet in LDS, in wave order.
+// permuted alike in both). The 4 waves' sums meet in LDS, in wave order. Past 32 rows a
+// stage is 256 k, and two waves take a half of it each for one half of the rows.
 // The norm: x becomes bf16(x * norm weight) on its way into the product, each lane keeps
 // the sum of x^2 over the k it sees, and the sums are scaled by rsqrt(sum / K + eps).
 //
-// Measured (us; an empty kernel takes 2): one row, N=K=4096 5.1, N=12288 K=4096 7.4 (3.6
-// TB/s), N=24576 13.3 (4.0 TB/s), N=4096 K=12288 9.3, N=151936 K=4096 62 (5.3 TB/s); 32
-// rows, where each CU also reads all of x from the L2, 8.7, 11.5, 16, 17.5 and 93.
+// Measured (us; an empty kernel takes 2): one row, N=K=4096 5.1, N=12288 K=4096 7.6 (3.5
+// TB/s), N=24576 12.8 (4.2 TB/s), N=4096 K=12288 9.7, N=151936 K=4096 54 (6.1 TB/s); 32
+// rows, where each CU also reads all of x from the L2, 8.4, 11.2, 16.5, 17.4 and 97; 64
+// rows 12.3, 16.0, 23.2, 29.6 and 143.
 #include <algorithm>
 
 #include "gemm_tile.h"
@@ -27,110 +29,119 @@ namespace {
 
 using namespace q3;
 
-constexpr int kStageK = 512;
 constexpr int kWaves = 4;
 constexpr int kMaxGroups = 6;       // 16-row groups of a block (gate and up: 4 of each)
 constexpr int kNormMaxK = 8192;     // the norm weight is held in LDS
 
+// RG: 16-row groups of weights, XR: rows of x in LDS.
 template <int RG, int XR, bool SW, bool NORM>
 struct RowsShape {
+  static constexpr int KS = XR <= 32 ? 512 : 256;                    // k of a stage
+  static constexpr int WK = KS / 128, WM = kWaves / WK;              // waves along k, and along the tiles of x
   static constexpr int RGT = SW ? 2 * RG : RG;
-  static constexpr int MT = XR > 16 ? 2 : 1;                         // 16-row tiles of x
-  static constexpr int PW = RGT, PS = (RGT + 3) / 4, PX = XR / 4;    // loads per wave and stage: codes, scales, x
+  static constexpr int MT = XR > 16 ? XR / 16 : 1, MW = MT / WM;     // 16-row tiles of x, and those of a wave
+  static constexpr int CW = KS / 32, CX = KS / 8;                    // 16-byte chunks of a row's codes, of a row of x
+  // Loads per wave and stage: codes (GW per group), scales, x.
+  static constexpr int GW = 16 * CW / 64, PW = (RGT * GW + 3) / 4, PS = (RGT + 3) / 4, PX = XR * CX / 64 / kWaves;
   static constexpr int PER = PW + PS + PX;
-  static constexpr int kW = RGT * 4096, kS = PS * 1024, kX = XR * 1024, kSlot = kW + kS + kX;  // bytes
+  static constexpr int kW = PW * 4096, kS = PS * 1024, kX = XR * KS * 2, kSlot = kW + kS + kX;  // bytes
   static constexpr int kNorm = NORM ? kNormMaxK * 2 : 0;
   // Stages of the ring. Where x takes little of the LDS, up to six, but no more than lets two blocks run on a CU, the
   // next one's first loads under the last one's sums (one row, us, 4 stages / 6 / 8, half the LDS: N=4096 K=12288 10.5 /
   // 9.3 / 9.4, N=6144 K=4096 6.3 / 6.0 / 6.0; N=12288 9.2 with 8 in the whole LDS, 7.4 in half, N=151936 75 / 62).
-  // Else up to four (16 rows, N=12288: 9.2 with 4, 10.4 in half the LDS).
+  // Else up to four (16 rows, N=12288: 9.2 with 4, 10.4 in half the LDS). Three at least where x is small (N=24576, 13.9
+  // with 2).
   static constexpr int kLds = (XR < 16 ? 78 : 156) * 1024 - kNorm;
-  static constexpr int NS = std::max(2, std::min(XR < 16 ? 6 : 4, kLds / kSlot));
+  static constexpr int NS = std::max(XR < 16 ? 3 : 2, std::min(XR < 16 ? 6 : 4, kLds / kSlot));
   static_assert(NS * kSlot + kNorm <= 156 * 1024 && (NS - 2) * PER < 64, "the ring, and the count of its loads");
-  static_assert(kWaves * RGT * MT * 1024 <= NS * kSlot, "the waves' sums");
+  static_assert(XR * CX % (64 * kWaves) == 0 && MT % WM == 0, "whole loads and tiles per wave");
+  static_assert(WK * RGT * MT * 1024 <= NS * kSlot, "the waves' sums");
 };
 
 template <int RG, int XR, bool SW, bool NORM>
 __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
   typedef RowsShape<RG, XR, SW, NORM> S;
-  constexpr int RGT = S::RGT, MT = S::MT, NS = S::NS;
+  constexpr int RGT = S::RGT, MT = S::MT, MW = S::MW, NS = S::NS, KS = S::KS, CW = S::CW, CX = S::CX, WK = S::WK;
   __shared__ __attribute__((aligned(1024))) char smem[NS * S::kSlot + S::kNorm];
-  __shared__ float s_sq[NORM ? kWaves * 16 * MT : 1];
+  __shared__ float s_sq[NORM ? WK * 16 * MT : 1];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int i = lane & 15, g = lane >> 4;
+  const int i = lane & 15, g = lane >> 4, wk = wave % WK, wm = wave / WK;
   int seg = 0;
 #pragma unroll
   for (int j = 1; j < kMxRowsSegments; ++j)
     if (j < p.nseg && (int)blockIdx.x >= p.bstart[j]) seg = j;
   seg = __builtin_amdgcn_readfirstlane(seg);
   const int n0 = ((int)blockIdx.x - p.bstart[seg]) * p.r, rows = min(p.r, p.n[seg] - n0);
-  const int blocks = p.K / kMxBlock, steps = (p.K + kStageK - 1) / kStageK;
+  const int blocks = p.K / kMxBlock, steps = (p.K + KS - 1) / KS;
   const uint32_t lbase = lds_addr(smem);
 
   const int64_t wbytes = (int64_t)(rows - 1) * p.ldw + p.K / 2, sbytes = (int64_t)(rows - 1) * p.lds + blocks;
   const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, ((int64_t)(p.M - 1) * p.ldx + p.K) * 2);
-  const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w[seg] + (int64_t)n0 * p.ldw, wbytes);
-  const __amdgpu_buffer_rsrc_t ru = SW ? make_rsrc(p.w[1] + (int64_t)n0 * p.ldw, wbytes) : rw;
 
-  // This wave's loads, as byte offsets at k = 0, and their k. Row r of 16 keeps its 16-byte
-  // chunk c at slot c ^ r (x: c ^ (r & 15)), so the 16 rows of a fragment read use all banks.
-  // Codes: of group u rows 4 wave ... 4 wave + 3, 256 bytes each.
-  const int wr = 4 * wave + (lane >> 4), wc = (lane & 15) ^ wr;
-  uint32_t woff[RGT];
+  // This wave's loads, as byte offsets at k = 0, and their k. Row r of 16 keeps its 16-byte chunk c at slot c ^ wswz(r)
+  // (x: c ^ (r & 15)), so the 16 rows of a fragment read use all banks.
+  auto wswz = [](int r) { return r / (16 / CW) & (CW - 1); };
+  // Codes: load d of the stage is part d % GW of group d / GW.
+  uint32_t woff[S::PW];
+  int wc[S::PW];
+  __amdgpu_buffer_rsrc_t rw[S::PW];
 #pragma unroll
-  for (int u = 0; u < RGT; ++u) {
-    const int row = 16 * (u < RG ? u : u - RG) + wr;
-    woff[u] = row < rows ? (uint32_t)(row * p.ldw + 16 * wc) : kOOB;
+  for (int u = 0; u < S::PW; ++u) {
+    const int d = 4 * u + wave, q = d / S::GW, r = d % S::GW * (64 / CW) + lane / CW;
+    const int row = 16 * (q < RG ? q : q - RG) + r;
+    wc[u] = lane % CW ^ wswz(r);
+    woff[u] = q < RGT && row < rows ? (uint32_t)(row * p.ldw + 16 * wc[u]) : kOOB;
+    rw[u] = make_rsrc((SW && q >= RG ? p.w[1] : p.w[seg]) + (int64_t)n0 * p.ldw, wbytes);
   }
-  // Scales: all 16 rows of group 4 v + wave, a word (four blocks) per lane.
+  // Scales: the 16 rows of group 4 v + wave, a word (four blocks) per lane.
   uint32_t soff[S::PS];
+  const int sb = 4 * (lane % (CW / 4));
   __amdgpu_buffer_rsrc_t rs[S::PS];
 #pragma unroll
   for (int v = 0; v < S::PS; ++v) {
-    const int q = 4 * v + wave, row = 16 * (q < RG ? q : q - RG) + (lane >> 2);
-    soff[v] = q < RGT && row < rows ? (uint32_t)(row * p.lds + 4 * (lane & 3)) : kOOB;
+    const int q = 4 * v + wave, r = lane / (CW / 4), row = 16 * (q < RG ? q : q - RG) + r;
+    soff[v] = q < RGT && r < 16 && row < rows ? (uint32_t)(row * p.lds + sb) : kOOB;
     rs[v] = make_rsrc((SW && q >= RG ? p.s[1] : p.s[seg]) + (int64_t)n0 * p.lds, sbytes);
   }
-  // x: row 4 u + wave, 1024 bytes.
   uint32_t xoff[S::PX];
   int xc[S::PX];
 #pragma unroll
   for (int u = 0; u < S::PX; ++u) {
-    const int m = 4 * u + wave;
-    xc[u] = lane ^ (m & 15);
+    const int m = (4 * u + wave) * (64 / CX) + lane / CX;
+    xc[u] = lane % CX ^ (m & 15);
     xoff[u] = m < p.M ? (uint32_t)(m * p.ldx * 2 + 16 * xc[u]) : kOOB;
   }
   auto issue = [&](int t, int slot) {
     const uint32_t at = lbase + (uint32_t)slot;
-    const int left = blocks - 16 * t;  // blocks from this stage's first on (none past the last stage)
+    const int left = blocks - CW * t;  // blocks from this stage's first on (none past the last stage)
 #pragma unroll
     for (int u = 0; u < S::PX; ++u)
-      dma16(rx, xoff[u] != kOOB && xc[u] < 4 * left ? xoff[u] + (uint32_t)t * (kStageK * 2) : kOOB,
+      dma16(rx, xoff[u] != kOOB && xc[u] < 4 * left ? xoff[u] + (uint32_t)t * (KS * 2) : kOOB,
             at + S::kW + S::kS + (4 * u + wave) * 1024);
 #pragma unroll
     for (int v = 0; v < S::PS; ++v)
-      dma4(rs[v], soff[v] != kOOB && 4 * (lane & 3) < left ? soff[v] + (uint32_t)t * (kStageK / 32) : kOOB,
+      dma4(rs[v], soff[v] != kOOB && sb < left ? soff[v] + (uint32_t)t * (KS / 32) : kOOB,
            at + S::kW + (4 * v + wave) * 256);
 #pragma unroll
-    for (int u = 0; u < RGT; ++u)
-      dma16_nt(u < RG ? rw : ru, woff[u] != kOOB && wc < left ? woff[u] + (uint32_t)t * (kStageK / 2) : kOOB,
-               at + u * 4096 + wave * 1024);
+    for (int u = 0; u < S::PW; ++u)
+      dma16_nt(rw[u], woff[u] != kOOB && wc[u] < left ? woff[u] + (uint32_t)t * (KS / 2) : kOOB,
+               at + (4 * u + wave) * 1024);
   };
   if constexpr (NORM) {  // before the first stage: its wait covers these
     const __amdgpu_buffer_rsrc_t rn = make_rsrc(p.nw, (int64_t)p.K * 2);
-    for (int d = wave; d < steps; d += kWaves)
+    for (int d = wave; d < (p.K + 511) / 512; d += kWaves)
       dma16(rn, (uint32_t)(d * 1024 + 16 * lane), lbase + (uint32_t)(NS * S::kSlot + d * 1024));
   }
 
-  floatx4 acc[RGT][MT];
+  floatx4 acc[RGT][MW];
 #pragma unroll
   for (int q = 0; q < RGT; ++q)
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[q][t] = floatx4{};
-  float sq[MT];
+    for (int t = 0; t < MW; ++t) acc[q][t] = floatx4{};
+  float sq[MW];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) sq[t] = 0.f;
+  for (int t = 0; t < MW; ++t) sq[t] = 0.f;
 
 #pragma unroll 1
   for (int t = 0; t < NS - 1; ++t) issue(t, t * S::kSlot);
@@ -146,21 +157,22 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
     float s[RGT];
 #pragma unroll
     for (int q = 0; q < RGT; ++q) {
-      w[q] = *reinterpret_cast<const u32x4*>(st + q * 4096 + i * 256 + (((4 * wave + g) ^ i) << 4));
-      s[q] = mx_scale(*reinterpret_cast<const uint8_t*>(st + S::kW + q * 256 + i * 16 + 4 * wave + g));
+      w[q] = *reinterpret_cast<const u32x4*>(st + (16 * q + i) * (KS / 2) + (((4 * wk + g) ^ wswz(i)) << 4));
+      s[q] = mx_scale(*reinterpret_cast<const uint8_t*>(st + S::kW + q * 256 + i * CW + 4 * wk + g));
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      bf16x8 x[MT];
+      bf16x8 x[MW];
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const int m = 16 * j + (XR < 16 ? i % XR : i);  // fewer rows: repeated, the copies' sums are not used
-        x[j] = *reinterpret_cast<const bf16x8*>(st + S::kW + S::kS + m * 1024 + (((16 * wave + 4 * g + e) ^ (m & 15)) << 4));
+      for (int j = 0; j < MW; ++j) {
+        const int m = 16 * (MW * wm + j) + (XR < 16 ? i % XR : i);  // fewer rows: repeated, the copies' sums are not used
+        x[j] = *reinterpret_cast<const bf16x8*>(st + S::kW + S::kS + m * (KS * 2) +
+                                                (((16 * wk + 4 * g + e) ^ (m & 15)) << 4));
       }
       if constexpr (NORM) {
-        const bf16x8 nw = *reinterpret_cast<const bf16x8*>(smem + NS * S::kSlot + 2 * (t * kStageK + 128 * wave + 32 * g + 8 * e));
+        const bf16x8 nw = *reinterpret_cast<const bf16x8*>(smem + NS * S::kSlot + 2 * (t * KS + 128 * wk + 32 * g + 8 * e));
 #pragma unroll
-        for (int j = 0; j < MT; ++j)
+        for (int j = 0; j < MW; ++j)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const float f = bf2f(x[j][k]);
@@ -172,7 +184,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
       for (int q = 0; q < RGT; ++q) {
         const bf16x8 a = mx_bf16x8(w[q][e], s[q]);
 #pragma unroll
-        for (int j = 0; j < MT; ++j) acc[q][j] = mfma16x16x32(a, x[j], acc[q][j]);
+        for (int j = 0; j < MW; ++j) acc[q][j] = mfma16x16x32(a, x[j], acc[q][j]);
       }
     }
   }
@@ -182,14 +194,14 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
 #pragma unroll
   for (int q = 0; q < RGT; ++q)
 #pragma unroll
-    for (int j = 0; j < MT; ++j) sums[((wave * RGT + q) * MT + j) * 64 + lane] = acc[q][j];
+    for (int j = 0; j < MW; ++j) sums[((wk * RGT + q) * MT + MW * wm + j) * 64 + lane] = acc[q][j];
   if constexpr (NORM) {
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
+    for (int j = 0; j < MW; ++j) {
       float v = sq[j];
       v += __shfl_xor(v, 16);
       v += __shfl_xor(v, 32);
-      if (g == 0) s_sq[(wave * MT + j) * 16 + i] = v;
+      if (g == 0) s_sq[(wk * MT + MW * wm + j) * 16 + i] = v;
     }
   }
   __syncthreads();
@@ -201,7 +213,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
     auto total = [&](int group) {
       floatx4 v = sums[(group * MT + j) * 64 + l];
 #pragma unroll
-      for (int k = 1; k < kWaves; ++k) v += sums[((k * RGT + group) * MT + j) * 64 + l];
+      for (int k = 1; k < WK; ++k) v += sums[((k * RGT + group) * MT + j) * 64 + l];
       return v;
     };
     floatx4 v = total(q);
@@ -209,7 +221,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
     if constexpr (NORM) {
       float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k) sum += s_sq[k * MT * 16 + m];
+      for (int k = 0; k < WK; ++k) sum += s_sq[k * MT * 16 + m];
       norm = rsqrtf(sum / (float)p.K + p.eps);
       v *= norm;
     }
@@ -270,7 +282,8 @@ template <bool SW>
 void launch_rows(const MxRows& p, int grid, hipStream_t st) {
   if (p.M <= 4) launch_groups<4, SW>(p, grid, st);
   else if (p.M <= 16) launch_groups<16, SW>(p, grid, st);
-  else launch_groups<32, SW>(p, grid, st);
+  else if (p.M <= 32) launch_groups<32, SW>(p, grid, st);
+  else launch_groups<64, SW>(p, grid, st);
 }
 
 }  // namespace
@@ -294,8 +307,9 @@ int mx_rows(MxRows p, bool swiglu, hipStream_t st) {
     for (int j = 0; j < p.nseg; ++j) n += q3_cdiv(p.n[j], r);
     return n;
   };
-  const int most = 16 * (swiglu ? 4 : kMaxGroups);
-  int64_t rounds = q3_cdiv(total, 256 * most);
+  int most = 16 * (swiglu ? 4 : kMaxGroups);
+  if (p.M <= 4 && total > 256 * most) most = 64;  // then two blocks fit a CU: N=151936 K=4096 62 -> 54 us
+  const int64_t rounds = q3_cdiv(total, 256 * most);
   int r = 4;
   while (r < most && blocks(r) > 256 * rounds) r += 4;
   p.r = r;

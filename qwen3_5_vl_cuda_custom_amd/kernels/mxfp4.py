@@ -23,6 +23,7 @@ from .elementwise import swiglu
 from .norms import rmsnorm
 
 MX_BLOCK = 32
+MXFP4_FEW_ROWS = 64  # rows of the products over several weights, and with the norm, in one launch
 _U8, _BF16, _F32 = torch.uint8, torch.bfloat16, torch.float32
 _i64x4, _i64x14, _i64x20 = Struct("4q").pack, Struct("14q").pack, Struct("20q").pack
 
@@ -231,7 +232,7 @@ def _few_rows(op: str, x: torch.Tensor, norm_weight: torch.Tensor | None, *other
     x2, ldx = _rows(op, x, K)
     if x2.data_ptr() % 16 or ldx % 8 or ldx >= 1 << 22:
         x2, ldx = x2.clone(memory_format=torch.contiguous_format), K
-    fits = 0 < M <= 32 and K % 128 == 0 and K < 1 << 22 and (norm_weight is None or K <= 8192)
+    fits = 0 < M <= MXFP4_FEW_ROWS and K % 128 == 0 and K < 1 << 22 and (norm_weight is None or K <= 8192)
     return dev, K, M, x2, ldx, fits
 
 
@@ -240,7 +241,7 @@ def matmul_segments_mxfp4(x: torch.Tensor, weights, biases=None, *, norm_weight:
     """matmul_segments with the weights held in MXFP4: x·[W_0; W_1; ...]ᵀ (+ [b_0; b_1; ...]) over 1 to 4 weights,
     each a pair (codes, scales); returns (..., ΣN_i).
 
-    With norm_weight the rows of x are RMS-normalised first (rmsnorm_matmul_segments). Up to 32 rows of K a multiple of
+    With norm_weight the rows of x are RMS-normalised first (rmsnorm_matmul_segments). Up to 64 rows of K a multiple of
     128 (and at most 8192 with the norm) are one launch; more rows, or another K, a product per weight.
     """
     op = "matmul_segments_mxfp4"
@@ -279,7 +280,7 @@ def matmul_swiglu_mxfp4(x: torch.Tensor, gate: tuple[torch.Tensor, torch.Tensor]
     """matmul_swiglu with the weights held in MXFP4: silu(x·W_gateᵀ)·(x·W_upᵀ), `gate` and `up` pairs (codes, scales)
     of (N, K).
 
-    With norm_weight the rows of x are RMS-normalised first (rmsnorm_matmul_swiglu). Up to 32 rows of K a multiple of
+    With norm_weight the rows of x are RMS-normalised first (rmsnorm_matmul_swiglu). Up to 64 rows of K a multiple of
     128 (and at most 8192 with the norm) are one launch; more rows, or another K, two products and swiglu.
     """
     op = "matmul_swiglu_mxfp4"

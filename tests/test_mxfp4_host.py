@@ -80,14 +80,14 @@ def test_few_rows_refusals(L):
     assert seg(x=None) == -1 and seg(c=ptrs(FAKE, None)) == -1 and seg(s=None) == -1
     assert seg(nseg=0) == -2 and seg(nseg=5) == -2 and seg(n=i64(64, 0)) == -2 and seg(ldc=95) == -2 and seg(ldx=128) == -2
     assert seg(K=48, ldx=48) == -2 and seg(dt=0) == -3
-    assert seg(M_=33) == -5 and seg(K=96) == -5 and seg(nw=FAKE, K=8320, ldx=8320) == -5
+    assert seg(M_=65) == -5 and seg(K=96) == -5 and seg(nw=FAKE, K=8320, ldx=8320) == -5
     assert seg(x=FAKE + 2) == -4 and seg(nw=FAKE + 8) == -4 and seg(ldx=260) == -4
     assert seg(c=ptrs(FAKE, FAKE + 8)) == -4 and seg(s=ptrs(FAKE + 1, FAKE)) == -4
     assert seg(M_=0) == 0
 
     def sw(g=FAKE, u=FAKE, M_=4, N=64, K=256, ldc=64):
         return L.q3_matmul_swiglu_mxfp4(FAKE, None, 0.0, g, FAKE, u, FAKE, FAKE, M_, N, K, K, ldc, 1, None)
-    assert sw(g=None) == -1 and sw(ldc=63) == -2 and sw(M_=33) == -5 and sw(K=160) == -5 and sw(u=FAKE + 8) == -4
+    assert sw(g=None) == -1 and sw(ldc=63) == -2 and sw(M_=65) == -5 and sw(K=160) == -5 and sw(u=FAKE + 8) == -4
     assert sw(N=0) == 0 and sw(M_=0) == 0
 
 
