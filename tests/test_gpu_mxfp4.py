@@ -333,6 +333,34 @@ def test_decode_by_pairs_and_split(lens, hkv, groups, cap, d):
     check_attention(o.unsqueeze(2), q.unsqueeze(2), c, c.lens.view(-1, 1), d ** -0.5)
 
 
+@pytest.mark.parametrize("sq", [1, 3])
+def test_nan_rows_where_units_are_split_between_waves(sq):
+    """A value's NaN block reaches its block of the outputs that see it, a key's every output of its head, no other."""
+    cap, n = 3000, [2500, 1700]
+    c = Cache(n, 2, cap, 128, seed=55, used=sq)
+    clean = Cache(n, 2, cap, 128, seed=55, used=sq)
+    q = rnd(2, 8, sq, 128, seed=56)
+    c.vs[0, 0, 1234, 2] = 255
+    c.vs[1, 0, 1700 + sq - 1, 1] = 255  # the last token's own value
+    c.ks[1, 1, 7, 0] = 255
+    lens = c.lens.to(DEV)
+
+    def run(k):
+        if sq == 1:
+            return K.decode_attention_mxfp4(q.to(DEV)[:, :, 0], *k.device(), lens, 0.1, append=True).unsqueeze(2).cpu()
+        return K.flash_attention_cache_mxfp4(q.to(DEV), *k.device(), c.lens.to(DEV), 0.1, 4).cpu()
+
+    o = run(c)
+    lens.copy_(c.lens)
+    ref = run(clean)
+    bad = torch.zeros(o.shape, dtype=torch.bool)
+    bad[0, :4, :, 64:96] = True
+    bad[1, :4, -1:, 32:64] = True
+    bad[1, 4:] = True
+    assert torch.equal(torch.isnan(o), bad) and torch.isfinite(ref).all()
+    assert torch.equal(o[~bad], ref[~bad])
+
+
 @pytest.mark.parametrize("cap", [100, 1500])
 def test_steps_advance_past_the_capacity_alike(cap):
     """Both forms attend to the rows up to the capacity and advance every length by one, the full ones too."""
