@@ -47,65 +47,6 @@ __device__ __forceinline__ void store_y4(const MxGemm& p, int m, int n, floatx4 
   *reinterpret_cast<bf16x4*>(p.y + m * p.ldc + n) = o;
 }
 
-// ------------------------------------------------------------------ few rows, any K
-// Up to four rows whose K (or scales) the kernel of mxfp4_rows.hip does not take. Bound
-// by the weight stream (N=1000 K=1152, one row: 3.4 us; an empty kernel takes 2). A block
-// takes 16 weight rows, a wave every eighth 128-value step of k: lane (r = l % 16, g = l /
-// 16) loads the 16 bytes of block 4 step + g of weight row r, its scale, and the 32 values
-// of x's row r at the same k, and forms 4 products of 16x16x32 (k permuted alike in both).
-// The eight waves' sums meet in LDS, in wave order.
-constexpr int kGemvWaves = 8;
-
-__global__ __launch_bounds__(64 * kGemvWaves) void mx_gemv_kernel(const MxGemm p) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const int blocks = p.K / kMxBlock, steps = (blocks + 3) / 4;
-
-  struct Step {
-    u32x4 w;
-    uint32_t s;
-    bf16x8 x[4];
-  };
-  const int64_t row = min(n0 + r, p.N - 1);
-  auto load = [&](int t, Step& d) {
-    const int kb = 4 * t + g;
-    const bool in = kb < blocks;
-    d.w = u32x4{};
-    d.s = 0;
-    if (in) {
-      d.w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p.w + row * p.ldw + kb * 16));
-      d.s = p.s[row * p.lds + kb];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      d.x[e] = bf16x8{};
-      if (in && r < p.M) d.x[e] = *reinterpret_cast<const bf16x8*>(p.x + r * p.ldx + kb * 32 + 8 * e);
-    }
-  };
-  floatx4 acc{};
-  Step cur, nxt;
-  load(wave, cur);
-  for (int t = wave; t < steps; t += kGemvWaves) {
-    load(t + kGemvWaves, nxt);
-    const float s = mx_scale(cur.s);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc = mfma16x16x32(mx_bf16x8(cur.w[e], s), cur.x[e], acc);
-    cur = nxt;
-  }
-
-  __shared__ floatx4 s_acc[kGemvWaves][64];
-  s_acc[wave][lane] = acc;
-  __syncthreads();
-  if (wave != 0 || r >= p.M) return;
-#pragma unroll
-  for (int k = 1; k < kGemvWaves; ++k) acc += s_acc[k][lane];
-  const int n = n0 + 4 * g;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (n + e < p.N) store_y(p, r, n + e, acc[e]);
-}
-
 // ------------------------------------------------------------------ more rows
 // x through LDS. A block of eight waves, WM along m and 8 / WM along n, forms a tile
 // of BN = 16 RT (8 / WM) columns and BM rows over its k range, in stages of BK: every
@@ -279,8 +220,8 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const MxGemm p, int parts) 
   }
 }
 
-// How a product runs: whole weight rows per block (kRows), x through LDS in tiles of 32,
-// 64 or 128 rows, or the weights expanded to bf16 for the bf16 GEMM.
+// How a product runs: whole weight rows per block and 64 rows of x (kRows, mxfp4_rows.hip), x through LDS in tiles of
+// 32, 64 or 128 rows, or the weights expanded to bf16 for the bf16 GEMM.
 enum Form { kRows, kTile32, kTile64, kTile128, kExpand };
 
 struct Plan {
@@ -288,33 +229,48 @@ struct Plan {
   int bn, bm, parts;  // tile, and ranges of k whose sums are added by mx_sum_kernel
 };
 
-// kRows up to 32 rows (K a multiple of 128), but for 17 to 32 rows of K > 8192, where the reads of x by every CU
-// cost more than the sum over ranges of k: us, kRows / tiles, 32 rows: N=4096 K=4096 8.7 /
-// 9.6, K=12288 17.5 / 12.6, N=12288 K=4096 11.5 / 14.1, N=24576 16 / 22; 16 rows: 6.2 / 8.5,
-// 11.6 / 11.9, 9.2 / 13.3, 13.0 / 20.2. 33 to 64 rows: kRows for K up to about 4096 where
-// every CU has one block and not too few rows: 64 rows, K=4096, N=1024 11.5 / 10.0, 4096
-// 12.3 / 14.5, 12288 16.0 / 18.5, 24576 23.2 / 26.0, 151936 143 / 110; N=2048 K=8192 19.5 /
-// 14.7; N=1000 K=1152 6.2 / 10.9. Otherwise tiles up to 64 rows. Above,
-// tiles unless the expansion is estimated faster: 128 x 256 tiles run in rounds of 256
-// at 1.1 PFLOP/s; expanding costs 2.53 bytes a weight at 5.5 TB/s, 16 us, and the
-// product at 1.3 PFLOP/s. Microseconds, tiles / expanded: N=12288 K=4096 M=64 21 / 69,
-// M=256 45 / 77, M=512 (192 tiles) 67 / 98, M=777 (336) 126 / 115; N=4096 K=12288 M=777 95
-// / 144; N=K=4096 M=777 43 / 55, M=1500 66 / 77; N=K=1024 M=1500 19 / 18. With fewer tiles
-// than CUs, k is split until they fill them (ranges of at least 512 k).
+// Estimates, us. kRows: every block streams all of its rows of x from the L2 (75 KB a us and CU; fewer where x does
+// not stay in it and many blocks read) and then its weights (18 KB), and stores: N=4096 K=4096, 64 rows 13 (measured
+// 12.3), N=24576 25 (23.2), N=4096 K=12288 31 (29.6); 616 rows, N=393 K=7232 28 (27.8).
+double rows_us(int64_t M, int64_t N, int64_t K) {
+  const int64_t r = mx_rows_per_block(M, N, false), blocks = q3_cdiv(N, r) * q3_cdiv(M, kMxRowsMax);
+  const double x = 2.0 * (double)M * (double)K;
+  const double rate = blocks <= 64 || x <= 2e6 ? 75e3 : x <= 16e6 ? 45e3 : 30e3;
+  return 1.5 + (double)q3_cdiv(blocks, 256) *
+                   (2 + 0.03 * (double)r + (double)K * ((M <= 32 ? 64 : 128) / rate + 0.53 * (double)r / 18e3));
+}
+// Tiles: a fixed part (more where N is no multiple of four: single stores), each stage of k, and the sum over ranges:
+// 32 rows, N=4096 K=12288 14 (12.8); 64 rows, N=12288 K=4096 18 (18.5); 512 rows, N=12288 K=4096 67 (67).
+double tile_us(const Plan& g, int64_t M, int64_t N, int64_t K) {
+  const int64_t blocks = q3_cdiv(N, g.bn) * q3_cdiv(M, g.bm) * g.parts;
+  const bool big = g.form == kTile128;
+  const double stage = big ? (blocks > 128 ? 1.85 : 1.4) : g.form == kTile64 ? 2.3 : 0.8;
+  return (big ? 8 : 5) + (N % 4 == 0 ? 0 : big ? 10 : 3) + (g.parts > 1 ? 4 : 0) +
+         (double)q3_cdiv(blocks, 256) * (double)q3_cdiv(q3_cdiv(K, big ? 128 : 256), g.parts) * stage;
+}
+// The expansion moves 2.53 bytes a weight at 5.5 TB/s, the product runs at 1.3 PFLOP/s.
+double expand_us(int64_t M, int64_t N, int64_t K) {
+  const double nk = (double)N * (double)K;
+  return 16 + nk * 2.53 / 5.5e6 + 2 * (double)M * nk / 1.3e9;
+}
+
+// kRows up to 16 rows, where x is little. Above, the least estimate; the expansion only from 65 rows and one round of
+// tiles on. Measured (us), rows / tiles / expanded: 32 rows, N=4096 K=4096 8.4 / 9.6 / -, K=12288 17.4 / 12.8 / -,
+// N=12288 K=4096 11.2 / 14.1 / -; 64 rows, N=1024 K=4096 11.5 / 10.0 / -, N=4096 12.3 / 14.5 / -, N=12288 16.0 / 18.5 / -;
+// 136 rows, N=1114 K=416 6.5 / 31.5 / 22; 616, N=393 K=7232 27.8 / 26.6 / 59; 3018, N=78 K=512 6.3 / 21.7 / 13.8; 3102,
+// N=667 K=9024 108 / 65 / 82; 469, N=9936 K=224 30 / 19 / 23; N=12288 K=4096, 256 rows - / 45 / 77, 512 - / 67 / 98, 777 - / 126 / 115.
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
-  if (M <= 4 || (M <= 32 && K % 128 == 0 && (M <= 16 || K <= 8192)) ||
-      (M <= kMxRowsMax && K % 128 == 0 && K <= 4608 && N >= K / 2 && N <= 24576))
-    return {kRows, 0, 0, 1};
+  const Plan rows{kRows, 0, 0, 1};
+  if (M <= 16) return rows;
   Plan g = M <= 32 ? Plan{kTile32, 128, 32, 1} : M <= 64 ? Plan{kTile64, 256, 64, 1} : Plan{kTile128, 256, 128, 1};
   const int64_t tiles = q3_cdiv(N, g.bn) * q3_cdiv(M, g.bm);
-  if (g.form == kTile128) {
-    const double nk = (double)N * (double)K;
-    const double tile_us = (double)q3_cdiv(tiles, 256) * 256 * 128 * 256 * 2 * (double)K / 1.1e9;
-    const double expand_us = 2 * (double)M * nk / 1.3e9 + nk * 2.53 / 5.5e6 + 16;
-    if (tiles > 256 && expand_us < tile_us) return {kExpand, 0, 0, 1};
-  }
   g.parts = (int)std::max<int64_t>(1, std::min<int64_t>(256 / tiles, q3_cdiv(K, 256) / 2));
-  return g;
+  double us = tile_us(g, M, N, K);
+  if (M > 64 && tiles > 256 && expand_us(M, N, K) < us) {
+    g = {kExpand, 0, 0, 1};
+    us = expand_us(M, N, K);
+  }
+  return q3_cdiv(M, kMxRowsMax) <= 65535 && rows_us(M, N, K) < us ? rows : g;
 }
 
 template <int RT, int BM, int WM, int BK, int NST>
@@ -353,8 +309,8 @@ int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, co
   Q3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Q3_ERR_WORKSPACE);
   Q3_REQUIRE(need == 0 || q3_aligned(workspace, 16), Q3_ERR_ALIGN);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  Plan g = plan_of(M, N, K);
-  if (g.form == kRows && mx_rows_ok(M, K, w_scales, lds)) {
+  const Plan g = plan_of(M, N, K);
+  if (g.form == kRows) {
     MxRows p{};
     p.x = static_cast<const bf16*>(x);
     p.w[0] = static_cast<const uint8_t*>(w_codes);
@@ -368,8 +324,6 @@ int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, co
     p.ldx = ldx, p.ldw = ldw, p.lds = lds, p.ldr = ldr, p.ldc = ldc;
     return mx_rows(p, false, st);
   }
-  if (g.form == kRows && M > 4)  // scales at odd addresses; no workspace
-    g = M <= 32 ? Plan{kTile32, 128, 32, 1} : Plan{kTile64, 256, 64, 1};
   if (g.form == kExpand) {
     Q3_REQUIRE(ldw == K / 2 && lds == K / kMxBlock, Q3_ERR_UNSUPPORTED);
     const int rc = mx_expand(w_codes, w_scales, static_cast<bf16*>(workspace), N * K, st);
@@ -381,9 +335,7 @@ int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, co
            g.parts > 1 ? static_cast<float*>(workspace) : nullptr, (int)M, (int)N, (int)K, ldx, ldw, lds, ldr, ldc, 0};
   p.vec = N % 4 == 0 && q3_aligned(y, 8) && ldc % 4 == 0 && (!bias || q3_aligned(bias, 8)) &&
           (!residual || (q3_aligned(residual, 8) && ldr % 4 == 0));
-  if (g.form == kRows)
-    hipLaunchKernelGGL(mx_gemv_kernel, dim3((unsigned)q3_cdiv(N, 16)), dim3(64 * kGemvWaves), 0, st, p);
-  else if (g.form == kTile32)
+  if (g.form == kTile32)
     launch_tile<1, 32, 1, 256, 2>(p, g, st);
   else if (g.form == kTile64)
     launch_tile<2, 64, 1, 256, 2>(p, g, st);

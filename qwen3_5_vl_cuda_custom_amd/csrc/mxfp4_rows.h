@@ -1,11 +1,11 @@
-// The product of up to 64 rows with MXFP4 weights (mxfp4_rows.hip).
+// Products by whole MXFP4 weight rows (mxfp4_rows.hip).
 #pragma once
 
 #include "q3_common.h"
 
 namespace q3 {
 
-constexpr int kMxRowsMax = 64;       // rows of x
+constexpr int kMxRowsMax = 64;       // rows of x per block
 constexpr int kMxRowsSegments = 4;   // weights side by side
 
 struct MxRows {
@@ -25,8 +25,10 @@ struct MxRows {
   int r, vec;                                         // weight rows of a block; whether y, bias, residual go in 8-byte pieces
 };
 
-// Whether the kernel takes a product (K a multiple of 128, whole words of scales).
-bool mx_rows_ok(int64_t M, int64_t K, const void* scales, int64_t lds);
+// Any M (64 rows per block), K a multiple of 32 below 2^23; of 128 with whole words of scales for several weights,
+// SwiGLU and the norm.
 int mx_rows(MxRows p, bool swiglu, hipStream_t st);
+// Weight rows a block takes.
+int64_t mx_rows_per_block(int64_t M, int64_t N, bool swiglu);
 
 }  // namespace q3

@@ -1,4 +1,5 @@
-// Products of up to 64 rows (decode steps) with MXFP4 weights (format: mxfp4.h): one
+// Products by whole weight rows, 64 rows of x at a time (decode steps, and small weights)
+// with MXFP4 weights (format: mxfp4.h): one
 // launch for a single weight, for the weights of several projections side by side, or
 // for SwiGLU's gate and up, with the RMSNorm of the rows fused in if asked for.
 //   y = x w^T (+ bias) (+ residual),  y = silu(x g^T) * (x u^T),  x or norm(x)
@@ -33,8 +34,9 @@ constexpr int kWaves = 4;
 constexpr int kMaxGroups = 6;       // 16-row groups of a block (gate and up: 4 of each)
 constexpr int kNormMaxK = 8192;     // the norm weight is held in LDS
 
-// RG: 16-row groups of weights, XR: rows of x in LDS.
-template <int RG, int XR, bool SW, bool NORM>
+// RG: 16-row groups of weights, XR: rows of x in LDS. AL: the rows of scales start at multiples of four bytes and are
+// whole words (K a multiple of 128), so a lane loads four scales; else one, into a word of its own.
+template <int RG, int XR, bool SW, bool NORM, bool AL>
 struct RowsShape {
   static constexpr int KS = XR <= 32 ? 512 : 256;                    // k of a stage
   static constexpr int WK = KS / 128, WM = kWaves / WK;              // waves along k, and along the tiles of x
@@ -42,7 +44,8 @@ struct RowsShape {
   static constexpr int MT = XR > 16 ? XR / 16 : 1, MW = MT / WM;     // 16-row tiles of x, and those of a wave
   static constexpr int CW = KS / 32, CX = KS / 8;                    // 16-byte chunks of a row's codes, of a row of x
   // Loads per wave and stage: codes (GW per group), scales, x.
-  static constexpr int GW = 16 * CW / 64, PW = (RGT * GW + 3) / 4, PS = (RGT + 3) / 4, PX = XR * CX / 64 / kWaves;
+  static constexpr int GW = 16 * CW / 64, PW = (RGT * GW + 3) / 4;
+  static constexpr int GS = AL ? 1 : GW, PS = (RGT * GS + 3) / 4, PX = XR * CX / 64 / kWaves;
   static constexpr int PER = PW + PS + PX;
   static constexpr int kW = PW * 4096, kS = PS * 1024, kX = XR * KS * 2, kSlot = kW + kS + kX;  // bytes
   static constexpr int kNorm = NORM ? kNormMaxK * 2 : 0;
@@ -58,9 +61,9 @@ struct RowsShape {
   static_assert(WK * RGT * MT * 1024 <= NS * kSlot, "the waves' sums");
 };
 
-template <int RG, int XR, bool SW, bool NORM>
+template <int RG, int XR, bool SW, bool NORM, bool AL>
 __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
-  typedef RowsShape<RG, XR, SW, NORM> S;
+  typedef RowsShape<RG, XR, SW, NORM, AL> S;
   constexpr int RGT = S::RGT, MT = S::MT, MW = S::MW, NS = S::NS, KS = S::KS, CW = S::CW, CX = S::CX, WK = S::WK;
   __shared__ __attribute__((aligned(1024))) char smem[NS * S::kSlot + S::kNorm];
   __shared__ float s_sq[NORM ? WK * 16 * MT : 1];
@@ -77,7 +80,8 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
   const uint32_t lbase = lds_addr(smem);
 
   const int64_t wbytes = (int64_t)(rows - 1) * p.ldw + p.K / 2, sbytes = (int64_t)(rows - 1) * p.lds + blocks;
-  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, ((int64_t)(p.M - 1) * p.ldx + p.K) * 2);
+  const int m0 = blockIdx.y * XR, M = min(p.M - m0, XR);  // this block's rows of x
+  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x + m0 * p.ldx, ((int64_t)(M - 1) * p.ldx + p.K) * 2);
 
   // This wave's loads, as byte offsets at k = 0, and their k. Row r of 16 keeps its 16-byte chunk c at slot c ^ wswz(r)
   // (x: c ^ (r & 15)), so the 16 rows of a fragment read use all banks.
@@ -94,13 +98,15 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
     woff[u] = q < RGT && row < rows ? (uint32_t)(row * p.ldw + 16 * wc[u]) : kOOB;
     rw[u] = make_rsrc((SW && q >= RG ? p.w[1] : p.w[seg]) + (int64_t)n0 * p.ldw, wbytes);
   }
-  // Scales: the 16 rows of group 4 v + wave, a word (four blocks) per lane.
+  // Scales: load d is the 16 rows of group d, a word (four blocks) per lane; or, one block per lane, part d % GS of
+  // group d / GS.
   uint32_t soff[S::PS];
-  const int sb = 4 * (lane % (CW / 4));
+  const int sb = AL ? 4 * (lane % (CW / 4)) : lane % CW;
   __amdgpu_buffer_rsrc_t rs[S::PS];
 #pragma unroll
   for (int v = 0; v < S::PS; ++v) {
-    const int q = 4 * v + wave, r = lane / (CW / 4), row = 16 * (q < RG ? q : q - RG) + r;
+    const int d = 4 * v + wave, q = d / S::GS, r = AL ? lane / (CW / 4) : d % S::GS * (64 / CW) + lane / CW;
+    const int row = 16 * (q < RG ? q : q - RG) + r;
     soff[v] = q < RGT && r < 16 && row < rows ? (uint32_t)(row * p.lds + sb) : kOOB;
     rs[v] = make_rsrc((SW && q >= RG ? p.s[1] : p.s[seg]) + (int64_t)n0 * p.lds, sbytes);
   }
@@ -110,7 +116,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
   for (int u = 0; u < S::PX; ++u) {
     const int m = (4 * u + wave) * (64 / CX) + lane / CX;
     xc[u] = lane % CX ^ (m & 15);
-    xoff[u] = m < p.M ? (uint32_t)(m * p.ldx * 2 + 16 * xc[u]) : kOOB;
+    xoff[u] = m < M ? (uint32_t)(m * p.ldx * 2 + 16 * xc[u]) : kOOB;
   }
   auto issue = [&](int t, int slot) {
     const uint32_t at = lbase + (uint32_t)slot;
@@ -121,8 +127,12 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
             at + S::kW + S::kS + (4 * u + wave) * 1024);
 #pragma unroll
     for (int v = 0; v < S::PS; ++v)
-      dma4(rs[v], soff[v] != kOOB && sb < left ? soff[v] + (uint32_t)t * (KS / 32) : kOOB,
-           at + S::kW + (4 * v + wave) * 256);
+      if constexpr (AL)
+        dma4(rs[v], soff[v] != kOOB && sb < left ? soff[v] + (uint32_t)t * (KS / 32) : kOOB,
+             at + S::kW + (4 * v + wave) * 256);
+      else
+        dma1(rs[v], soff[v] != kOOB && sb < left ? soff[v] + (uint32_t)t * (KS / 32) : kOOB,
+             at + S::kW + (4 * v + wave) * 256);
 #pragma unroll
     for (int u = 0; u < S::PW; ++u)
       dma16_nt(rw[u], woff[u] != kOOB && wc[u] < left ? woff[u] + (uint32_t)t * (KS / 2) : kOOB,
@@ -158,7 +168,9 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
 #pragma unroll
     for (int q = 0; q < RGT; ++q) {
       w[q] = *reinterpret_cast<const u32x4*>(st + (16 * q + i) * (KS / 2) + (((4 * wk + g) ^ wswz(i)) << 4));
-      s[q] = mx_scale(*reinterpret_cast<const uint8_t*>(st + S::kW + q * 256 + i * CW + 4 * wk + g));
+      const int at = i * CW + 4 * wk + g;
+      s[q] = mx_scale(AL ? *reinterpret_cast<const uint8_t*>(st + S::kW + q * 256 + at)
+                         : *reinterpret_cast<const uint32_t*>(st + S::kW + (q * 16 * CW + at) * 4));
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -209,7 +221,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
   for (int it = tid; it < RG * MT * 64; it += 64 * kWaves) {
     const int l = it & 63, j = it / 64 % MT, q = it / (64 * MT);
     const int m = 16 * j + (l & 15), row = 16 * q + 4 * (l >> 4);
-    if (m >= p.M || row >= rows) continue;
+    if (m >= M || row >= rows) continue;
     auto total = [&](int group) {
       floatx4 v = sums[(group * MT + j) * 64 + l];
 #pragma unroll
@@ -233,8 +245,8 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
     }
     const int col = p.col[seg] + n0 + row;
     const bf16* bias = p.bias[seg] ? p.bias[seg] + n0 + row : nullptr;
-    const bf16* res = p.res ? p.res + (int64_t)m * p.ldr + col : nullptr;
-    bf16* y = p.y + (int64_t)m * p.ldc + col;
+    const bf16* res = p.res ? p.res + (int64_t)(m0 + m) * p.ldr + col : nullptr;
+    bf16* y = p.y + (int64_t)(m0 + m) * p.ldc + col;
     if (p.vec && row + 3 < rows) {  // 8-byte pieces: n0, the columns and the strides are multiples of four
       if (bias) {
         const bf16x4 b = *reinterpret_cast<const bf16x4*>(bias);
@@ -261,37 +273,57 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const MxRows p) {
 }
 
 template <int RG, int XR, bool SW>
-void launch_norm(const MxRows& p, int grid, hipStream_t st) {
+void launch_form(const MxRows& p, dim3 grid, bool words, hipStream_t st) {
+  const dim3 block(64 * kWaves);
+  if constexpr (!SW)
+    if (!words) {  // a single weight without the norm
+      hipLaunchKernelGGL((mx_rows_kernel<RG, XR, false, false, false>), grid, block, 0, st, p);
+      return;
+    }
   if (p.nw)
-    hipLaunchKernelGGL((mx_rows_kernel<RG, XR, SW, true>), dim3(grid), dim3(64 * kWaves), 0, st, p);
+    hipLaunchKernelGGL((mx_rows_kernel<RG, XR, SW, true, true>), grid, block, 0, st, p);
   else
-    hipLaunchKernelGGL((mx_rows_kernel<RG, XR, SW, false>), dim3(grid), dim3(64 * kWaves), 0, st, p);
+    hipLaunchKernelGGL((mx_rows_kernel<RG, XR, SW, false, true>), grid, block, 0, st, p);
 }
 template <int XR, bool SW>
-void launch_groups(const MxRows& p, int grid, hipStream_t st) {
+void launch_groups(const MxRows& p, int blocks, bool words, hipStream_t st) {
+  const dim3 grid((unsigned)blocks, (unsigned)q3_cdiv(p.M, XR));
   switch ((p.r + 15) / 16) {
-    case 1: launch_norm<1, XR, SW>(p, grid, st); break;
-    case 2: launch_norm<2, XR, SW>(p, grid, st); break;
-    case 3: launch_norm<3, XR, SW>(p, grid, st); break;
-    case 4: launch_norm<4, XR, SW>(p, grid, st); break;
+    case 1: launch_form<1, XR, SW>(p, grid, words, st); break;
+    case 2: launch_form<2, XR, SW>(p, grid, words, st); break;
+    case 3: launch_form<3, XR, SW>(p, grid, words, st); break;
+    case 4: launch_form<4, XR, SW>(p, grid, words, st); break;
     default:
-      if constexpr (!SW) launch_norm<6, XR, SW>(p, grid, st);
+      if constexpr (!SW) launch_form<6, XR, SW>(p, grid, words, st);
   }
 }
 template <bool SW>
-void launch_rows(const MxRows& p, int grid, hipStream_t st) {
-  if (p.M <= 4) launch_groups<4, SW>(p, grid, st);
-  else if (p.M <= 16) launch_groups<16, SW>(p, grid, st);
-  else if (p.M <= 32) launch_groups<32, SW>(p, grid, st);
-  else launch_groups<64, SW>(p, grid, st);
+void launch_rows(const MxRows& p, int blocks, bool words, hipStream_t st) {
+  if (p.M <= 4) launch_groups<4, SW>(p, blocks, words, st);
+  else if (p.M <= 16) launch_groups<16, SW>(p, blocks, words, st);
+  else if (p.M <= 32) launch_groups<32, SW>(p, blocks, words, st);
+  else launch_groups<64, SW>(p, blocks, words, st);
+}
+
+// Whether the scales are whole words.
+bool words_of(const MxRows& p) {
+  bool ok = p.K % 128 == 0 && p.lds % 4 == 0;
+  for (int j = 0; j < p.nseg; ++j) ok = ok && q3_aligned(p.s[j], 4);
+  return ok;
 }
 
 }  // namespace
 
 namespace q3 {
 
-bool mx_rows_ok(int64_t M, int64_t K, const void* scales, int64_t lds) {
-  return M <= kMxRowsMax && K % 128 == 0 && K < (1 << 24) && lds % 4 == 0 && q3_aligned(scales, 4);
+int64_t mx_rows_per_block(int64_t M, int64_t N, bool swiglu) {
+  const int64_t chunks = q3_cdiv(M, kMxRowsMax);
+  int64_t most = 16 * (swiglu ? 4 : kMaxGroups);
+  if (M <= 4 && N > 256 * most) most = 64;  // then two blocks fit a CU: N=151936 K=4096 62 -> 54 us
+  const int64_t rounds = q3_cdiv(N * chunks, 256 * most);
+  int64_t r = 4;
+  while (r < most && q3_cdiv(N, r) * chunks > 256 * rounds) r += 4;
+  return r;
 }
 
 int mx_rows(MxRows p, bool swiglu, hipStream_t st) {
@@ -302,16 +334,14 @@ int mx_rows(MxRows p, bool swiglu, hipStream_t st) {
   }
   // The fewest rows per block (whole 8-byte pieces of y) that give every CU one block, or an equal number of them
   // where even the largest block does not cover N.
-  auto blocks = [&](int r) {
+  int r = (int)mx_rows_per_block(p.M, total, swiglu);
+  auto blocks = [&](int rows) {
     int64_t n = 0;
-    for (int j = 0; j < p.nseg; ++j) n += q3_cdiv(p.n[j], r);
+    for (int j = 0; j < p.nseg; ++j) n += q3_cdiv(p.n[j], rows);
     return n;
   };
-  int most = 16 * (swiglu ? 4 : kMaxGroups);
-  if (p.M <= 4 && total > 256 * most) most = 64;  // then two blocks fit a CU: N=151936 K=4096 62 -> 54 us
-  const int64_t rounds = q3_cdiv(total, 256 * most);
-  int r = 4;
-  while (r < most && blocks(r) > 256 * rounds) r += 4;
+  const int64_t rounds = q3_cdiv(q3_cdiv(total, r), 256);
+  while (p.nseg > 1 && r < 64 && blocks(r) > 256 * rounds) r += 4;
   p.r = r;
   int64_t grid = 0;
   for (int j = 0; j < p.nseg; ++j) {
@@ -321,9 +351,9 @@ int mx_rows(MxRows p, bool swiglu, hipStream_t st) {
   p.vec = q3_aligned(p.y, 8) && p.ldc % 4 == 0 && (!p.res || (q3_aligned(p.res, 8) && p.ldr % 4 == 0));
   for (int j = 0; j < p.nseg; ++j) p.vec = p.vec && p.col[j] % 4 == 0 && (!p.bias[j] || q3_aligned(p.bias[j], 8));
   if (swiglu)
-    launch_rows<true>(p, (int)grid, st);
+    launch_rows<true>(p, (int)grid, true, st);
   else
-    launch_rows<false>(p, (int)grid, st);
+    launch_rows<false>(p, (int)grid, words_of(p), st);
   Q3_LAUNCH_CHECK();
   return Q3_OK;
 }

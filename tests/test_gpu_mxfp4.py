@@ -144,6 +144,29 @@ def test_matmul_few_rows_of_large_weights(m, n, k):
     check_matmul(y, x, codes, scales, b, r)
 
 
+# tiles of 32, 64 and 128 rows, their scales by words and by bytes, odd N, split k and not; expanded weights
+@pytest.mark.parametrize("m,n,k", [(20, 4096, 12288), (20, 1001, 12320), (50, 1024, 8192), (50, 1003, 8224), (300, 4096, 8192),
+                                   (300, 4001, 8224), (200, 40000, 640), (1500, 8192, 2048)])
+def test_matmul_tiles_and_expansion(m, n, k):
+    codes, scales = weight(n, k, seed=n)
+    x, b, r = rnd(m, k, seed=m), rnd(n, seed=1), rnd(m, n, seed=2)
+    dc, ds = codes.to(DEV), scales.to(DEV)
+    check_matmul(K.matmul_mxfp4(x.to(DEV), dc, ds, b.to(DEV), r.to(DEV)), x, codes, scales, b, r)
+    x[1, 7] = math.nan
+    y = K.matmul_mxfp4(x.to(DEV), dc, ds).cpu()
+    assert torch.isnan(y[1]).all() and torch.isfinite(y[[i for i in range(m) if i != 1]]).all()
+
+
+@pytest.mark.parametrize("m", [65, 130, 300])
+@pytest.mark.parametrize("n,k", [(1, 64), (37, 480), (300, 640), (4000, 96)])
+def test_matmul_many_rows_of_small_weights(m, n, k):
+    codes, scales = weight(n, k, seed=n)
+    wide = rnd(m, k + 32, seed=m)
+    x, b, r = wide[:, :k], rnd(n, seed=1), rnd(m, n, seed=2)
+    y = K.matmul_mxfp4(wide.to(DEV)[:, :k], codes.to(DEV), scales.to(DEV), b.to(DEV), r.to(DEV))
+    check_matmul(y, x, codes, scales, b, r)
+
+
 @pytest.mark.parametrize("m", [2, 16, 32, 50])
 def test_matmul_scales_at_odd_addresses_and_long_rows(m):
     n, k = 150, 9216 if m < 50 else 256
