@@ -160,7 +160,8 @@ def matmul_mxfp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bia
     if residual is not None and residual.shape != shape:
         raise ValueError(f"{op}: residual {tuple(residual.shape)} != output {shape}")
     if out is None:
-        y, ldy = x.new_empty(shape), N
+        same = residual is not None and residual.is_contiguous()
+        y, ldy = torch.empty_like(residual) if same else x.new_empty(shape), N  # empty_like: 0.4 us less
     else:
         if out.shape != shape or (N > 1 and out.stride(-1) != 1):
             raise ValueError(f"{op}: out {tuple(out.shape)} must be {shape} with contiguous elements")
@@ -447,10 +448,11 @@ def _query(op: str, q: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Te
         require_no_grad(op, q, out)
     if q.dtype != _BF16:
         raise TypeError(f"{op}: q must be bfloat16, got {q.dtype}")
-    if not q.is_contiguous() or q.data_ptr() % 16:
+    packed = q.is_contiguous()
+    if not packed or q.data_ptr() % 16:
         q = mfma_operand(op, q if q.stride(-1) == 1 else q.contiguous())
     if out is None:
-        return q, q.new_empty(q.shape)
+        return q, torch.empty_like(q) if packed else q.new_empty(q.shape)
     if (out.get_device() != q.get_device() or out.shape != q.shape or out.dtype != _BF16 or out.data_ptr() % 16
             or out.stride(-1) != 1 or any(out.stride(i) % 8 for i in range(out.dim() - 1))):
         raise ValueError(f"{op}: out must be {tuple(q.shape)} {_BF16} on q's device with a contiguous head dim, 16-byte "
