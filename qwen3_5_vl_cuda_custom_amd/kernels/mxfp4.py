@@ -20,6 +20,7 @@ import torch
 from .. import _lib
 from ._common import mfma_operand, require_device, require_no_grad
 from .elementwise import swiglu
+from .matmul import matmul_segments, matmul_swiglu
 from .norms import rmsnorm
 
 MX_BLOCK = 32
@@ -31,6 +32,12 @@ _i64x4, _i64x14, _i64x20 = Struct("4q").pack, Struct("14q").pack, Struct("20q").
 @lru_cache(maxsize=4096)
 def _matmul_workspace(M: int, N: int, K: int) -> int:
     return _lib.lib().q3_matmul_mxfp4_workspace_bytes(M, N, K)
+
+
+def _expands(M: int, N: int, K: int) -> bool:
+    """Whether q3_matmul_mxfp4 would expand the weight to bf16: its workspace is then the weight (and not sums over
+    ranges of k, which only fewer than 256 tiles of 128 x 256 need)."""
+    return -(-M // 128) * -(-N // 256) > 256 and _matmul_workspace(M, N, K) == 2 * N * K
 
 
 @lru_cache(maxsize=1024)
@@ -243,7 +250,8 @@ def matmul_segments_mxfp4(x: torch.Tensor, weights, biases=None, *, norm_weight:
     each a pair (codes, scales); returns (..., ΣN_i).
 
     With norm_weight the rows of x are RMS-normalised first (rmsnorm_matmul_segments). Up to 64 rows of K a multiple of
-    128 (and at most 8192 with the norm) are one launch; more rows, or another K, a product per weight.
+    128 (and at most 8192 with the norm) are one launch; more rows, or another K, a product per weight, or where its
+    weight would be expanded to bf16 (many rows), matmul_segments over the expanded weights.
     """
     op = "matmul_segments_mxfp4"
     weights = list(weights)
@@ -262,6 +270,8 @@ def matmul_segments_mxfp4(x: torch.Tensor, weights, biases=None, *, norm_weight:
             return y
         if norm_weight is not None:
             x = rmsnorm(x, norm_weight, eps)
+        if 0 not in ns and _expands(M, sum(ns), K):
+            return matmul_segments(x, [mxfp4_dequantize(c, s) for c, s in ws], biases)
         at = 0
         for (c, s), b, n in zip(ws, biases, ns):
             matmul_mxfp4(x, c, s, b, out=y[..., at:at + n])
@@ -282,7 +292,8 @@ def matmul_swiglu_mxfp4(x: torch.Tensor, gate: tuple[torch.Tensor, torch.Tensor]
     of (N, K).
 
     With norm_weight the rows of x are RMS-normalised first (rmsnorm_matmul_swiglu). Up to 64 rows of K a multiple of
-    128 (and at most 8192 with the norm) are one launch; more rows, or another K, two products and swiglu.
+    128 (and at most 8192 with the norm) are one launch; more rows, or another K, two products and swiglu, or where their
+    weights would be expanded to bf16 (many rows), matmul_swiglu over the expanded weights.
     """
     op = "matmul_swiglu_mxfp4"
     dev, K, M, x2, ldx, fits = _few_rows(op, x, norm_weight)
@@ -295,6 +306,8 @@ def matmul_swiglu_mxfp4(x: torch.Tensor, gate: tuple[torch.Tensor, torch.Tensor]
             return x.new_empty((*x.shape[:-1], N))
         if norm_weight is not None:
             x = rmsnorm(x, norm_weight, eps)
+        if _expands(M, N, K):
+            return matmul_swiglu(x, mxfp4_dequantize(gc, gs), mxfp4_dequantize(uc, us))
         return swiglu(matmul_mxfp4(x, gc, gs), matmul_mxfp4(x, uc, us))
     y = x.new_empty((*x.shape[:-1], N))
     nw = None if norm_weight is None else _aligned(norm_weight)

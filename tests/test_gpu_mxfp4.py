@@ -240,6 +240,27 @@ def test_matmul_swiglu_matches_float64(n, k, m, norm):
     assert y.shape == (m, n) and bool((d <= tol).all()), float((d / tol).max())
 
 
+def test_segments_and_swiglu_of_many_rows_over_expanded_weights():
+    m, k, ns = 2100, 1024, (4096, 1024, 2048)
+    ws = [weight(n, k, seed=n) for n in ns]
+    dev = [(c.to(DEV), s.to(DEV)) for c, s in ws]
+    x = rnd(m, k, seed=61)
+    b = rnd(1024, seed=62)
+    y = K.matmul_segments_mxfp4(x.to(DEV), dev, [None, b.to(DEV), None]).cpu()
+    for i, at in enumerate((0, 4096, 5120)):
+        check_matmul(y[:, at:at + ns[i]], x, *ws[i], b if i == 1 else None)
+    gate, up = weight(8192, k, seed=63), weight(8192, k, seed=64)
+    y = K.matmul_swiglu_mxfp4(x.to(DEV), *(tuple(t.to(DEV) for t in w) for w in (gate, up)))
+    w = [M.values(*t) for t in (gate, up)]
+    g, u = (x.double() @ t.T for t in w)
+    eg, eu = ((k + 2) * 2.0 ** -23 * (x.double().abs() @ t.abs().T) for t in w)
+    ref = torch.nn.functional.silu(g) * u
+    # as in test_matmul_swiglu_matches_float64, in one epilogue
+    err = 1.1 * eg * (u.abs() + eu) + torch.nn.functional.silu(g).abs() * eu + 2.0 ** -20 * ref.abs()
+    assert float(g.abs().max()) <= 16
+    assert bool(((y.double().cpu() - ref).abs() <= HALF * (ref.abs() + err) + err).all())
+
+
 def test_few_rows_keep_nan_and_infinity_to_their_row_and_weight():
     k, m = 256, 7
     ws = [weight(n, k, seed=n) for n in (40, 24)]
