@@ -595,7 +595,7 @@ int q3_matmul_mxfp4(const void* x, const void* w_codes, const void* w_scales, co
  * q3_matmul_segments_mxfp4: y (M, sum n_j) = x [w_0; w_1; ...]^T (+ [b_0; b_1; ...]), 1 to 4 weights of n[j] >= 1
  * rows; codes, scales and bias are host arrays of device pointers (bias, or any of its entries, may be null).
  * q3_matmul_swiglu_mxfp4: y (M, N) = silu(x g^T) * (x u^T).
- * norm_weight (K), if not null: the rows of x are RMS-normalised first (eps; K <= 8192). bf16; K a multiple of 128
+ * norm_weight (K), if not null: the rows of x are RMS-normalised first (eps; M <= 32, K <= 8192). bf16; K a multiple of 128
  * (else Q3_ERR_UNSUPPORTED); x, its rows, the norm weight and the codes 16-byte aligned, the scales 4-byte. */
 int q3_matmul_segments_mxfp4(const void* x, const void* norm_weight, float eps, const void* const* codes,
                              const void* const* scales, const void* const* bias, const int64_t* n, int64_t nseg,

@@ -33,6 +33,9 @@ using namespace q3;
 constexpr int kWaves = 4;
 constexpr int kMaxGroups = 6;       // 16-row groups of a block (gate and up: 4 of each)
 constexpr int kNormMaxK = 8192;     // the norm weight is held in LDS
+// Every block normalises all rows, which costs as much as a launch of its own for 32 (gate and up, N=12288 K=4096: 16.5 us
+// without, 20 with; 64 rows 23 and 31).
+constexpr int kNormMaxRows = 32;
 
 // RG: 16-row groups of weights, XR: rows of x in LDS. AL: the rows of scales start at multiples of four bytes and are
 // whole words (K a multiple of 128), so a lane loads four scales; else one, into a word of its own.
@@ -280,10 +283,12 @@ void launch_form(const MxRows& p, dim3 grid, bool words, hipStream_t st) {
       hipLaunchKernelGGL((mx_rows_kernel<RG, XR, false, false, false>), grid, block, 0, st, p);
       return;
     }
-  if (p.nw)
-    hipLaunchKernelGGL((mx_rows_kernel<RG, XR, SW, true, true>), grid, block, 0, st, p);
-  else
-    hipLaunchKernelGGL((mx_rows_kernel<RG, XR, SW, false, true>), grid, block, 0, st, p);
+  if constexpr (XR <= kNormMaxRows)
+    if (p.nw) {
+      hipLaunchKernelGGL((mx_rows_kernel<RG, XR, SW, true, true>), grid, block, 0, st, p);
+      return;
+    }
+  hipLaunchKernelGGL((mx_rows_kernel<RG, XR, SW, false, true>), grid, block, 0, st, p);
 }
 template <int XR, bool SW>
 void launch_groups(const MxRows& p, int blocks, bool words, hipStream_t st) {
@@ -369,7 +374,7 @@ int check_rows(const void* x, const void* norm_weight, const void* y, int64_t M,
   Q3_REQUIRE(M >= 0 && K >= kMxBlock && K % kMxBlock == 0 && N >= 0 && ldx >= K && ldc >= N, Q3_ERR_SHAPE);
   Q3_REQUIRE(dtype == Q3_BF16, Q3_ERR_DTYPE);
   Q3_REQUIRE(M <= kMxRowsMax && K % 128 == 0 && K < (1 << 23) && ldx < (1 << 22) && N < (1ll << 31) - 256 &&
-                 (!norm_weight || K <= kNormMaxK),
+                 (!norm_weight || (K <= kNormMaxK && M <= kNormMaxRows)),
              Q3_ERR_UNSUPPORTED);
   return q3_aligned(x, 16) && ldx % 8 == 0 && q3_aligned(norm_weight, 16) ? Q3_OK : Q3_ERR_ALIGN;
 }

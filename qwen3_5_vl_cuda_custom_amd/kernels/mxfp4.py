@@ -24,7 +24,7 @@ from .matmul import matmul_segments, matmul_swiglu
 from .norms import rmsnorm
 
 MX_BLOCK = 32
-MXFP4_FEW_ROWS = 64  # rows of the products over several weights, and with the norm, in one launch
+MXFP4_FEW_ROWS, MXFP4_NORM_ROWS = 64, 32  # rows of the products over several weights in one launch, with the norm
 _U8, _BF16, _F32 = torch.uint8, torch.bfloat16, torch.float32
 _i64x4, _i64x14, _i64x20 = Struct("4q").pack, Struct("14q").pack, Struct("20q").pack
 
@@ -240,7 +240,7 @@ def _few_rows(op: str, x: torch.Tensor, norm_weight: torch.Tensor | None, *other
     x2, ldx = _rows(op, x, K)
     if x2.data_ptr() % 16 or ldx % 8 or ldx >= 1 << 22:
         x2, ldx = x2.clone(memory_format=torch.contiguous_format), K
-    fits = 0 < M <= MXFP4_FEW_ROWS and K % 128 == 0 and K < 1 << 22 and (norm_weight is None or K <= 8192)
+    fits = 0 < M <= MXFP4_FEW_ROWS and K % 128 == 0 and K < 1 << 22
     return dev, K, M, x2, ldx, fits
 
 
@@ -250,8 +250,9 @@ def matmul_segments_mxfp4(x: torch.Tensor, weights, biases=None, *, norm_weight:
     each a pair (codes, scales); returns (..., ΣN_i).
 
     With norm_weight the rows of x are RMS-normalised first (rmsnorm_matmul_segments). Up to 64 rows of K a multiple of
-    128 (and at most 8192 with the norm) are one launch; more rows, or another K, a product per weight, or where its
-    weight would be expanded to bf16 (many rows), matmul_segments over the expanded weights.
+    128 are one launch (with the norm up to 32 of K at most 8192, else the norm is another); more rows, or another K, a
+    product per weight, or where its weight would be expanded to bf16 (many rows), matmul_segments over the expanded
+    weights.
     """
     op = "matmul_segments_mxfp4"
     weights = list(weights)
@@ -261,15 +262,17 @@ def matmul_segments_mxfp4(x: torch.Tensor, weights, biases=None, *, norm_weight:
     dev, K, M, x2, ldx, fits = _few_rows(op, x, norm_weight, *biases)
     ws = [_weight(op, K, c, s, dev) for c, s in weights]
     ns = [c.shape[0] for c, _ in ws]
+    fits = fits and 0 not in ns
+    if norm_weight is not None and M > 0 and (not fits or M > MXFP4_NORM_ROWS or K > 8192):
+        x = x2 = rmsnorm(x, norm_weight, eps)
+        norm_weight, ldx = None, K
     for b, n in zip(biases, ns):
         if b is not None and b.shape != (n,):
             raise ValueError(f"{op}: bias {tuple(b.shape)} != ({n},)")
     y = x.new_empty((*x.shape[:-1], sum(ns)))
-    if not fits or 0 in ns:
+    if not fits:
         if M == 0:
             return y
-        if norm_weight is not None:
-            x = rmsnorm(x, norm_weight, eps)
         if 0 not in ns and _expands(M, sum(ns), K):
             return matmul_segments(x, [mxfp4_dequantize(c, s) for c, s in ws], biases)
         at = 0
@@ -292,11 +295,15 @@ def matmul_swiglu_mxfp4(x: torch.Tensor, gate: tuple[torch.Tensor, torch.Tensor]
     of (N, K).
 
     With norm_weight the rows of x are RMS-normalised first (rmsnorm_matmul_swiglu). Up to 64 rows of K a multiple of
-    128 (and at most 8192 with the norm) are one launch; more rows, or another K, two products and swiglu, or where their
-    weights would be expanded to bf16 (many rows), matmul_swiglu over the expanded weights.
+    128 are one launch (with the norm up to 32 of K at most 8192, else the norm is another); more rows, or another K, two
+    products and swiglu, or where their weights would be expanded to bf16 (many rows), matmul_swiglu over the expanded
+    weights.
     """
     op = "matmul_swiglu_mxfp4"
     dev, K, M, x2, ldx, fits = _few_rows(op, x, norm_weight)
+    if norm_weight is not None and M > 0 and (not fits or M > MXFP4_NORM_ROWS or K > 8192):
+        x = x2 = rmsnorm(x, norm_weight, eps)
+        norm_weight, ldx = None, K
     (gc, gs), (uc, us) = (_weight(op, K, c, s, dev) for c, s in (gate, up))
     if gc.shape != uc.shape:
         raise ValueError(f"{op}: gate {tuple(gc.shape)} and up {tuple(uc.shape)} codes must have one shape")
@@ -304,8 +311,6 @@ def matmul_swiglu_mxfp4(x: torch.Tensor, gate: tuple[torch.Tensor, torch.Tensor]
     if not fits or N == 0:
         if M == 0 or N == 0:
             return x.new_empty((*x.shape[:-1], N))
-        if norm_weight is not None:
-            x = rmsnorm(x, norm_weight, eps)
         if _expands(M, N, K):
             return matmul_swiglu(x, mxfp4_dequantize(gc, gs), mxfp4_dequantize(uc, us))
         return swiglu(matmul_mxfp4(x, gc, gs), matmul_mxfp4(x, uc, us))

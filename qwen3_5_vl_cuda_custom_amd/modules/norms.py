@@ -5,7 +5,6 @@ import torch
 from torch import nn
 
 from ..kernels import RMSNORM_MATMUL_MAX_ROWS, layernorm, rmsnorm
-from ..kernels.mxfp4 import MXFP4_FEW_ROWS
 
 
 class CudaRMSNorm(nn.Module):
@@ -24,20 +23,20 @@ class CudaRMSNorm(nn.Module):
         return f"{self.dim}, eps={self.eps}"
 
 
-def fused_norm_ok(x: torch.Tensor, norm: CudaRMSNorm, rows: int = RMSNORM_MATMUL_MAX_ROWS) -> bool:
+def fused_norm_ok(x: torch.Tensor, norm: CudaRMSNorm) -> bool:
     """Whether `norm` can run inside the projection that consumes x
     (rmsnorm_matmul_segments / rmsnorm_matmul_swiglu): decode shapes of at most
-    32 (`rows`) bf16 rows, 16-byte aligned rows of a multiple of 8 elements."""
+    32 bf16 rows, 16-byte aligned rows of a multiple of 8 elements."""
     K = x.shape[-1]
     return (x.is_cuda and x.dtype == torch.bfloat16 and norm.weight.dtype == torch.bfloat16 and K == norm.dim
             and K % 8 == 0 and x.is_contiguous() and x.data_ptr() % 16 == 0
-            and 0 < x.numel() // K <= rows)
+            and 0 < x.numel() // K <= RMSNORM_MATMUL_MAX_ROWS)
 
 
 def norm_operands(x: torch.Tensor, norm: CudaRMSNorm) -> tuple[torch.Tensor | None, float, torch.Tensor]:
-    """(weight, eps, x) where a projection of four-bit weights can normalise the rows itself, (None, 0, norm(x)) where it
-    can not."""
-    return (norm.weight, norm.eps, x) if fused_norm_ok(x, norm, MXFP4_FEW_ROWS) else (None, 0.0, norm(x))
+    """(weight, eps, x) for a projection of four-bit weights that can normalise the rows itself, (None, 0, norm(x)) for
+    one that can not."""
+    return (norm.weight, norm.eps, x) if fused_norm_ok(x, norm) else (None, 0.0, norm(x))
 
 
 class CudaLayerNorm(nn.Module):

@@ -679,6 +679,10 @@ def test_no_sequences_and_no_tokens():
     assert K.matmul_swiglu_mxfp4(x, (u(8, 32), u(8, 2)), (u(8, 32), u(8, 2))).shape == (0, 8)
     one = x.new_ones(1, 128)
     assert K.matmul_segments_mxfp4(one, [(u(8, 64), u(8, 4)), (u(0, 64), u(0, 4))]).tolist() == [[0.0] * 8]
+    w = tuple(t.to(DEV) for t in weight(8, 128, seed=1))
+    a = K.matmul_segments_mxfp4(2 * one, [w, (u(0, 64), u(0, 4))], norm_weight=one[0], eps=0.0)
+    b = K.matmul_mxfp4(one, *w)  # rows of a constant normalise to ones
+    assert torch.equal(a, b)
     assert [t.shape for t in K.mxfp4_quantize(x)] == [(0, 32), (0, 2)]
 
 

@@ -80,7 +80,7 @@ def test_few_rows_refusals(L):
     assert seg(x=None) == -1 and seg(c=ptrs(FAKE, None)) == -1 and seg(s=None) == -1
     assert seg(nseg=0) == -2 and seg(nseg=5) == -2 and seg(n=i64(64, 0)) == -2 and seg(ldc=95) == -2 and seg(ldx=128) == -2
     assert seg(K=48, ldx=48) == -2 and seg(dt=0) == -3
-    assert seg(M_=65) == -5 and seg(K=96) == -5 and seg(nw=FAKE, K=8320, ldx=8320) == -5
+    assert seg(M_=65) == -5 and seg(K=96) == -5 and seg(nw=FAKE, K=8320, ldx=8320) == -5 and seg(nw=FAKE, M_=33) == -5
     assert seg(x=FAKE + 2) == -4 and seg(nw=FAKE + 8) == -4 and seg(ldx=260) == -4
     assert seg(c=ptrs(FAKE, FAKE + 8)) == -4 and seg(s=ptrs(FAKE + 1, FAKE)) == -4
     assert seg(M_=0) == 0
