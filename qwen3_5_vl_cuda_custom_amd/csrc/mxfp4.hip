@@ -4,9 +4,9 @@
 // All three are bound by memory: eight values (a 16-byte load or store of bf16,
 // 4 bytes of codes) per lane and piece, so the four lanes of a block exchange
 // their largest magnitude with two lane shuffles and nothing goes through LDS. A lane has
-// four pieces in flight where rows are long. Measured: quantising 12288 x 4096 fp32 46 us
-// (228 MB, 5.0 TB/s), back to bf16 21 us (127 MB, 6.1 TB/s); 256 x 128 bf16 2.6 and 2.4 us;
-// writing 4 x 512 new rows of 8 heads x 128 (K and V) 5.9 us, one row 1.8 us.
+// four pieces in flight where rows are long. Measured: quantising 12288 x 4096 fp32 39 us
+// (228 MB, 5.8 TB/s), back to bf16 20 us (127 MB, 6.4 TB/s); 256 x 128 bf16 2.6 and 2.4 us;
+// writing 4 x 512 new rows of 8 heads x 128 (K and V) 5.7 us, one row 1.8 us.
 #include "mxfp4.h"
 
 namespace {
@@ -90,7 +90,8 @@ __global__ __launch_bounds__(256) void mx_expand_kernel(const ExpandArgs a) {
     if (i >= pieces) return;
     const bf16x8 v = mx_bf16x8(w[u], mx_scale(b[u]));
     if constexpr (sizeof(T) == 2) {
-      reinterpret_cast<bf16x8*>(o)[i] = v;
+      // past the L2 (12288 x 4096 there and back 68 -> 61 us; the same for codes or loads was slower)
+      __builtin_nontemporal_store(v, reinterpret_cast<bf16x8*>(o) + i);
     } else {
       floatx4 lo, hi;
 #pragma unroll
