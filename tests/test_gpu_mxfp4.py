@@ -377,6 +377,28 @@ def test_decode_by_pairs_and_split(lens, hkv, groups, cap, d):
     check_attention(o.unsqueeze(2), q.unsqueeze(2), c, c.lens.view(-1, 1), d ** -0.5)
 
 
+def test_decode_of_many_pairs_split_between_waves():
+    """2160 pairs of one column: their records are merged by one wave each. Against float64 on the GPU: the weights'
+    rounding to bf16 (2^-8 of each), an fp32 score's error (64 2^-24 sum |q k| scale < 2^-12 of a weight, as the sum stays
+    below 64), the fp32 sums (700 2^-23) and the output's rounding."""
+    B, H, cap, d = 24, 90, 700, 64
+    g = torch.Generator().manual_seed(57)
+    kc, vc = (torch.randint(0, 256, (B, H, cap, d // 2), generator=g, dtype=torch.uint8).to(DEV) for _ in range(2))
+    ks, vs = (torch.randint(122, 127, (B, H, cap, d // 32), generator=g, dtype=torch.uint8).to(DEV) for _ in range(2))
+    lens = torch.randint(0, cap + 1, (B,), generator=g, dtype=torch.int32).to(DEV)
+    lens[0], lens[1] = 0, cap
+    q = rnd(B, H, d, seed=58).to(DEV)
+    o = K.decode_attention_mxfp4(q, kc, ks, vc, vs, lens, 0.1).double()
+    k, v = K.mxfp4_dequantize(kc, ks).double(), K.mxfp4_dequantize(vc, vs).double()
+    assert float((q.double().abs()[:, :, None] * k.abs()).sum(-1).max()) * 0.1 < 64
+    sc = (q.double()[:, :, None] * k).sum(-1) * 0.1
+    sc.masked_fill_(torch.arange(cap, device=DEV) >= lens[:, None, None], -math.inf)
+    w = torch.softmax(sc, -1).nan_to_num(0.0)  # an empty sequence: zeros
+    ref, spread = (w[..., None] * v).sum(2), (w[..., None] * v.abs()).sum(2)
+    tol = (HALF + 2.0 ** -11 + 700 * 2.0 ** -23) * spread * (1 + HALF) + HALF * ref.abs()
+    assert bool(((o - ref).abs() <= tol).all()) and not o[0].any()
+
+
 @pytest.mark.parametrize("sq", [1, 3])
 def test_nan_rows_where_units_are_split_between_waves(sq):
     """A value's NaN block reaches its block of the outputs that see it, a key's every output of its head, no other."""
