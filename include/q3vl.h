@@ -626,8 +626,9 @@ int q3_qk_norm_rope_mxfp4(const void* q_in, const void* k_in, const void* v_in, 
 /* q3_decode_attention over a four-bit cache: sequence b attends to rows [0, kv_lens[b] + advance) (advance = 1: the
  * step, whose row is already written; kv_lens[b] is then incremented in place), at most cap. q, o (B, Hq, D);
  * strides = [qb, qh, 0, ob, oh, 0] in elements, then [b, h] of k_codes, k_scales, v_codes, v_scales in bytes. An
- * empty sequence gives zeros; a NaN reaches only the queries that see its row. bf16, D = 64 or 128, B <= 1024 (else
- * Q3_ERR_UNSUPPORTED). Small caches need no workspace: the query gives 0, and it may be null. */
+ * empty sequence gives zeros; a NaN reaches only the queries that see its row. scale must be positive and finite (else
+ * Q3_ERR_SHAPE). bf16, D = 64 or 128, B <= 1024 (else Q3_ERR_UNSUPPORTED). Small caches need no workspace: the query
+ * gives 0, and it may be null. */
 int64_t q3_decode_attention_mxfp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap);
 int q3_decode_attention_mxfp4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
                               const void* v_scales, int* kv_lens, int advance, void* o, int64_t B, int64_t Hq,
@@ -636,7 +637,8 @@ int q3_decode_attention_mxfp4(const void* q, const void* k_codes, const void* k_
 
 /* q3_flash_attention_cache over a four-bit cache: query i of sequence b attends to rows [0, kv_lens[b] + i], whose
  * last Sq are already written; kv_lens[b] += Sq afterwards with `advance`. max_len >= every kv_lens[b] + Sq bounds
- * the rows (and the workspace). strides = [qb, qh, qs, ob, oh, os], then as q3_decode_attention_mxfp4. */
+ * the rows (and the workspace). scale must be positive and finite. strides = [qb, qh, qs, ob, oh, os], then as
+ * q3_decode_attention_mxfp4. */
 int64_t q3_flash_attention_cache_mxfp4_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
                                                        int64_t max_len);
 int q3_flash_attention_cache_mxfp4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,

@@ -669,9 +669,12 @@ int launch_stream(const MxAttn& p, int64_t D, hipStream_t st) {
 // elements, then [b, h] of k_codes, k_scales, v_codes, v_scales in bytes.
 int check(const void* q, const void* kc, const void* ks, const void* vc, const void* vs, const int* lens,
           const void* o, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D, int64_t cap,
-          const int64_t* strides, int dtype) {
+          const int64_t* strides, float scale, int dtype) {
   Q3_REQUIRE(q && kc && ks && vc && vs && lens && o && strides, Q3_ERR_NULL);
   Q3_REQUIRE(B >= 0 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Sq >= 0 && D >= 1 && cap >= 0, Q3_ERR_SHAPE);
+  // The kernels mask unscaled scores with -inf and take the running maximum of these: 0 would make a NaN of a masked
+  // row, a negative scale an infinity.
+  Q3_REQUIRE(scale > 0.f && scale < INFINITY, Q3_ERR_SHAPE);
   Q3_REQUIRE(dtype == Q3_BF16, Q3_ERR_DTYPE);
   Q3_REQUIRE((D == 64 || D == 128) && B <= kMaxBatch && (cap + kUnit) * D / 2 < (1ll << 31) && Sq < (1ll << 31) &&
                  Hq < (1ll << 16) && B * Hkv * sets_of(Hq / Hkv, streams(B, Hkv, Hq / Hkv, Sq) ? Sq : 1) * q3_cdiv(cap, kUnit) < (1ll << 31),
@@ -759,7 +762,8 @@ int q3_decode_attention_mxfp4(const void* q, const void* k_codes, const void* k_
                               const void* v_scales, int* kv_lens, int advance, void* o, int64_t B, int64_t Hq,
                               int64_t Hkv, int64_t D, int64_t cap, const int64_t* strides, float scale, int dtype,
                               void* workspace, int64_t workspace_bytes, void* stream) {
-  const int rc = check(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, 1, D, cap, strides, dtype);
+  const int rc = check(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, 1, D, cap, strides, scale,
+                       dtype);
   if (rc != Q3_OK || B == 0) return rc;
   const int64_t need = q3_decode_attention_mxfp4_workspace_bytes(B, Hq, Hkv, D, cap);
   Q3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Q3_ERR_WORKSPACE);
@@ -784,7 +788,7 @@ int q3_flash_attention_cache_mxfp4(const void* q, const void* k_codes, const voi
                                    int64_t Sq, int64_t D, int64_t max_len, const int64_t* strides, float scale,
                                    int advance, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   int rc =
-      check(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, Sq, D, max_len, strides, dtype);
+      check(q, k_codes, k_scales, v_codes, v_scales, kv_lens, o, B, Hq, Hkv, Sq, D, max_len, strides, scale, dtype);
   if (rc != Q3_OK || B == 0 || Sq == 0) return rc;
   Q3_REQUIRE(Sq <= max_len, Q3_ERR_SHAPE);
   const int64_t need = q3_flash_attention_cache_mxfp4_workspace_bytes(B, Hq, Hkv, Sq, D, max_len);

@@ -12,6 +12,7 @@ decode step take a few microseconds each, so the checks here are written for the
 """
 from __future__ import annotations
 
+import math
 from functools import lru_cache
 from struct import Struct
 
@@ -478,6 +479,13 @@ def _query(op: str, q: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Te
     return q, out
 
 
+def _scale(op: str, scale: float) -> float:
+    scale = float(scale)
+    if not 0 < scale < math.inf:
+        raise ValueError(f"{op}: scale must be positive and finite, got {scale}")
+    return scale
+
+
 def decode_attention_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
                            v_scales: torch.Tensor, kv_lens: torch.Tensor, scale: float, *,
                            out: torch.Tensor | None = None, append: bool = False) -> torch.Tensor:
@@ -485,14 +493,15 @@ def decode_attention_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: tor
 
     q (B, Hq, D) (or (B, Hq, 1, D)) bf16, D 64 or 128; codes (B, Hkv, cap, D / 2), scales (B, Hkv, cap, D / 32);
     sequence b attends to cache rows [0, kv_lens[b]). append=True is the decode step with the new token's row
-    already written at kv_lens[b]: it is attended to as well, and kv_lens is then incremented in place. Returns (B,
-    Hq, D); an empty sequence gives zeros.
+    already written at kv_lens[b]: it is attended to as well, and kv_lens is then incremented in place. scale must be
+    positive. Returns (B, Hq, D); an empty sequence gives zeros.
     """
     op = "decode_attention_mxfp4"
     if q.dim() == 4 and q.shape[2] == 1:
         q = q[:, :, 0]
     if q.dim() != 3:
         raise ValueError(f"{op}: q must be (B, Hq, D), got {tuple(q.shape)}")
+    scale = _scale(op, scale)
     dev = q.get_device()
     B, Hq, D = q.shape
     Hkv, cap, st = _check_cache(op, dev, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D)
@@ -520,13 +529,14 @@ def flash_attention_cache_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales
     """flash_attention_cache over a four-bit cache: causal attention of a prefill chunk.
 
     q (B, Hq, Sq, D) bf16, D 64 or 128; the chunk's rows [kv_lens[b], kv_lens[b] + Sq) are already in the cache.
-    Query i of sequence b attends to cache rows [0, kv_lens[b] + i]; advance=True adds Sq to kv_lens afterwards.
-    `max_len` bounds every kv_lens[b] + Sq (default: cap): rows past it are not read. It sizes the workspace of a
+    Query i of sequence b attends to cache rows [0, kv_lens[b] + i]; advance=True adds Sq to kv_lens afterwards. scale
+    must be positive. `max_len` bounds every kv_lens[b] + Sq (default: cap): rows past it are not read. It sizes the workspace of a
     chunk of more than 1400 (sequence, KV head, 16 columns), 4 * B * Hkv * max_len * D bytes.
     """
     op = "flash_attention_cache_mxfp4"
     if q.dim() != 4:
         raise ValueError(f"{op}: q must be (B, Hq, Sq, D), got {tuple(q.shape)}")
+    scale = _scale(op, scale)
     dev = q.get_device()
     B, Hq, Sq, D = q.shape
     Hkv, cap, st = _check_cache(op, dev, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D)

@@ -735,3 +735,15 @@ def test_two_streams_at_once():
         for r in got[i]:
             for a, b in zip(r, want[i]):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, math.inf, math.nan])
+def test_attention_refuses_a_scale_that_is_not_positive(scale):
+    """Masked scores are -inf before they are scaled, and the running maximum is that of the unscaled scores."""
+    c = Cache([40, 7], 1, 64, 128, seed=60, used=3)
+    q, lens = rnd(2, 4, 3, 128, seed=61).to(DEV), c.lens.to(DEV)
+    for run in (lambda: K.decode_attention_mxfp4(q[:, :, 0], *c.device(), lens, scale, append=True),
+                lambda: K.flash_attention_cache_mxfp4(q, *c.device(), lens, scale, 4, advance=True)):
+        with pytest.raises(ValueError, match="scale"):
+            run()
+    assert torch.equal(lens.cpu(), c.lens)

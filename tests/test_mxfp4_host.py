@@ -154,3 +154,13 @@ def test_cache_lengths_on_the_host():
         with pytest.raises(ValueError):
             bad()
     c.check_kernels(torch.bfloat16, 2, 64)
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, float("inf"), float("nan")])
+def test_attention_refuses_a_scale_that_is_not_positive(L, scale):
+    st = i64(*([128] * 14))
+    assert L.q3_decode_attention_mxfp4(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 0, FAKE, 2, 8, 2, 128, 32, st, scale, 1, None,
+                                       0, None) == -2
+    for Sq in (4, 1000):  # streamed, and over expanded rows
+        assert L.q3_flash_attention_cache_mxfp4(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 2, 64, 8, Sq, 128, 1000, st, scale,
+                                                0, 1, FAKE, 1 << 40, None) == -2
