@@ -16,8 +16,8 @@ from torch import nn
 
 from ..configs import Qwen3VLConfig
 from ..kernels import cuda_index_add
-from ..modules import (CudaEmbedding, CudaLinear, CudaRMSNorm, CudaTextDecoderLayer, MXFP4KVCache, PagedKVCache,
-                       StaticKVCache, StepGraph, TextMRoPE)
+from ..modules import (CudaEmbedding, CudaLinear, CudaLinearMXFP4, CudaRMSNorm, CudaTextDecoderLayer, MXFP4KVCache,
+                       PagedKVCache, StaticKVCache, StepGraph, TextMRoPE)
 from .common import CudaVisionTower
 
 
@@ -88,7 +88,7 @@ class _TextLM(nn.Module):
     def _head_weight(self) -> torch.Tensor:
         """The tensor whose device and type the serving path goes by: lm_head's weight, or where that is in four bits
         the final norm's."""
-        return self.lm_head.weight if isinstance(self.lm_head, CudaLinear) else self.norm.weight
+        return self.norm.weight if isinstance(self.lm_head, CudaLinearMXFP4) else self.lm_head.weight
 
     # ------------------------------------------------------------ KV-cache serving path
     def new_caches(self, batch: int, capacity: int, device=None, dtype=None, *, page_rows: int = 0,

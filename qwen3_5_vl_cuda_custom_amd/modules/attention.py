@@ -140,12 +140,13 @@ class CudaFullAttention(nn.Module):
         # q/k/v projections in one GEMM over the three weights (no concatenated
         # copy); q, k, v are column views of its output.
         projs = (self.q_proj, self.k_proj, self.v_proj)
-        if all(isinstance(p, CudaLinearMXFP4) for p in projs):
+        four_bit = [isinstance(p, CudaLinearMXFP4) for p in projs]
+        if all(four_bit):
             nw, eps, x = (None, 0.0, x) if input_norm is None else norm_operands(x, input_norm)
             qkv = matmul_segments_mxfp4(x, [p.pair for p in projs], [p.bias for p in projs], norm_weight=nw, eps=eps)
-        elif not all(isinstance(p, CudaLinear) for p in projs):
+        elif any(four_bit):
             qkv = self._project_apart(x if input_norm is None else input_norm(x), projs)
-        else:
+        else:  # any modules with a weight and a bias
             weights = tuple(p.weight for p in projs)
             biases = tuple(p.bias for p in projs)
             if input_norm is not None and fused_norm_ok(x, input_norm):
@@ -222,15 +223,13 @@ class CudaFullAttention(nn.Module):
     def _project_apart(x, projs) -> torch.Tensor:
         """The q/k/v rows side by side where only some projections hold four-bit weights: one product each, into
         its columns."""
-        qkv = torch.empty((*x.shape[:-1], sum(p.out_features for p in projs)), dtype=x.dtype, device=x.device)
-        at = 0
-        for p in projs:
-            out = qkv[..., at:at + p.out_features]
-            if isinstance(p, CudaLinear):
-                matmul(x, p.weight, p.bias, out=out)
-            else:
+        ns = [p.out_features if isinstance(p, CudaLinearMXFP4) else p.weight.shape[0] for p in projs]
+        qkv = torch.empty((*x.shape[:-1], sum(ns)), dtype=x.dtype, device=x.device)
+        for p, out in zip(projs, qkv.split(ns, -1)):
+            if isinstance(p, CudaLinearMXFP4):
                 p(x, out=out)
-            at += p.out_features
+            else:
+                matmul(x, p.weight, p.bias, out=out)
         return qkv
 
     def _forward_autograd(self, x, mrope_apply, past_kv, kv_cache, residual, input_norm):

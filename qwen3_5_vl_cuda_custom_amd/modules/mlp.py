@@ -36,13 +36,12 @@ class CudaSwiGLUMLP(nn.Module):
             if input_norm is not None:
                 x = input_norm(x)
             return self.down_proj(swiglu(self.gate_proj(x), self.up_proj(x)), residual=residual)
-        if (isinstance(self.gate_proj, CudaLinearMXFP4) and isinstance(self.up_proj, CudaLinearMXFP4)
-                and self.gate_proj.bias is None and self.up_proj.bias is None):
+        four_bit = [isinstance(p, CudaLinearMXFP4) for p in (self.gate_proj, self.up_proj)]
+        if all(four_bit) and self.gate_proj.bias is None and self.up_proj.bias is None:
             nw, eps, x = (None, 0.0, x) if input_norm is None else norm_operands(x, input_norm)
             act = matmul_swiglu_mxfp4(x, self.gate_proj.pair, self.up_proj.pair, norm_weight=nw, eps=eps)
             return self.down_proj(act, residual=residual)
-        if not all(isinstance(p, CudaLinear) for p in (self.gate_proj, self.up_proj)):
-            # four-bit weights in one of them, or with a bias: each projection by its own forward
+        if any(four_bit):  # in one of them, or with a bias: each projection by its own forward
             if input_norm is not None:
                 x = input_norm(x)
             return self.down_proj(swiglu(self.gate_proj(x), self.up_proj(x)), residual=residual)

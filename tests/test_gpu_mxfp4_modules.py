@@ -280,3 +280,51 @@ def test_fused_append_refusals():
     assert not cache.k_codes.any() and not cache.v_codes.any()
     call()
     assert cache.k_codes[:, :, 0].any() and not cache.k_codes[:, :, 1:].any()
+
+
+def _plain(linear):
+    """nn.Linear of the same weight (and bias)."""
+    p = torch.nn.Linear(linear.in_features, linear.out_features, bias=linear.bias is not None, device=DEV,
+                        dtype=linear.weight.dtype).requires_grad_(False)
+    p.load_state_dict(linear.state_dict())
+    return p
+
+
+@pytest.mark.parametrize("S", [1, 40])
+def test_projections_of_another_class_run_as_before(S):
+    """q/k/v and gate/up as nn.Linear take the same fused products as CudaLinear, with and without the fused norm."""
+    cfg = _cfg()
+    x, pos = rnd(2, S, cfg.hidden, seed=80), _pos([0, 0], S)
+    for names in (("q_proj",), ("q_proj", "k_proj", "v_proj")):
+        layer = W.make_text_layer(cfg, torch.bfloat16, DEV, seed=81).requires_grad_(False)
+        bound = W.make_rope(cfg, DEV).bind(pos)
+        want = layer(x, bound)[0]
+        for n in names:
+            setattr(layer.self_attn, n, _plain(getattr(layer.self_attn, n)))
+        layer.mlp.gate_proj = _plain(layer.mlp.gate_proj)
+        if len(names) > 1:
+            layer.mlp.up_proj = _plain(layer.mlp.up_proj)
+        assert torch.equal(layer(x, bound)[0], want)
+        cache = StaticKVCache(2, cfg.kv_heads, S, cfg.head_dim, device=DEV)
+        layer(x, bound, kv_cache=cache)
+        assert cache.max_len == S
+
+
+@pytest.mark.parametrize("S", [1, 40])
+def test_projections_of_another_class_beside_four_bit_ones(S):
+    cfg = _cfg()
+    x, pos = rnd(2, S, cfg.hidden, seed=82), _pos([0, 0], S)
+    layer, bound = W.make_text_layer(cfg, torch.bfloat16, DEV, seed=83).requires_grad_(False), W.make_rope(cfg, DEV).bind(pos)
+    for m, n in ((layer.self_attn, "k_proj"), (layer.mlp, "up_proj")):
+        setattr(m, n, CudaLinearMXFP4.from_linear(getattr(m, n)))
+    want = layer(x, bound)[0]
+    layer.self_attn.q_proj = _plain(layer.self_attn.q_proj)
+    assert torch.equal(layer(x, bound)[0], want)
+
+
+def test_caches_go_by_the_type_of_a_head_of_another_class():
+    m = _dense()
+    m.lm_head = _plain(m.lm_head)
+    m.norm.float()
+    assert m.new_caches(1, 8)[0].k.dtype == torch.bfloat16
+    assert len(m.new_caches(1, 8, kv_format="mxfp4")) == 2
