@@ -326,9 +326,10 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _check_cache(op: str, dev: int, k_codes, k_scales, v_codes, v_scales, kv_lens, B: int, D: int) -> tuple:
+def _check_cache(op: str, dev: int, k_codes, k_scales, v_codes, v_scales, kv_lens, B: int, D: int,
+                 align: int = 1) -> tuple:
     """Checks a (B, Hkv, cap, D) cache in MXFP4 and its lengths; returns Hkv, cap and the strides [b, h] of the four
-    tensors."""
+    tensors. align: bytes to which the kernel needs every row of scales aligned."""
     if dev < 0 or dev != _lib.current_device() or kv_lens.get_device() != dev:
         _off_device(op, kv_lens, k_codes)
     if kv_lens.dtype != torch.int32 or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
@@ -343,7 +344,7 @@ def _check_cache(op: str, dev: int, k_codes, k_scales, v_codes, v_scales, kv_len
                 and k_codes.get_device() == k_scales.get_device() == v_codes.get_device() == v_scales.get_device() == dev
                 and k_codes.is_contiguous() and k_scales.is_contiguous() and v_codes.is_contiguous()
                 and v_scales.is_contiguous() and (k_codes.data_ptr() | v_codes.data_ptr()) % 16 == 0
-                and (k_scales.data_ptr() | v_scales.data_ptr()) % n == 0):
+                and (k_scales.data_ptr() | v_scales.data_ptr()) % align == 0):
             c, s = (Hkv * cap * W, cap * W), (Hkv * cap * n, cap * n)  # whole caches: the usual call
             return Hkv, cap, (*c, *s, *c, *s)
     st = []
@@ -362,8 +363,8 @@ def _check_cache(op: str, dev: int, k_codes, k_scales, v_codes, v_scales, kv_len
             raise ValueError(f"{op}: the rows of a cache head must be packed")
         if c.data_ptr() % 16 or ct[0] % 16 or ct[1] % 16:
             raise ValueError(f"{op}: the cache codes must be 16-byte aligned")
-        if ss[3] and (s.data_ptr() % ss[3] or s_t[0] % ss[3] or s_t[1] % ss[3]):
-            raise ValueError(f"{op}: the cache scales must be whole rows apart and aligned to one")
+        if s.data_ptr() % align or s_t[0] % align or s_t[1] % align:
+            raise ValueError(f"{op}: the cache scales must be aligned to a row of them ({align} bytes)")
         st += (ct[0], ct[1], s_t[0], s_t[1])
     return shape[1], shape[2], st
 
@@ -373,8 +374,9 @@ def kv_append_mxfp4(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_s
     """Quantise new key / value rows into a four-bit cache.
 
     k, v (B, S, Hkv, D) bf16 or fp32, any strides with D contiguous; codes (B, Hkv, cap, D / 2) and scales (B, Hkv,
-    cap, D / 32) of keys and values; kv_lens (B,) int32: row s of sequence b goes to cache row kv_lens[b] + s, and is
-    dropped at or past cap. kv_lens is left as it is (the attention that follows advances it).
+    cap, D / 32) of keys and values, D a multiple of 32 up to 256; kv_lens (B,) int32: row s of sequence b goes to
+    cache row kv_lens[b] + s, and is dropped at or past cap. kv_lens is left as it is (the attention that follows
+    advances it).
     """
     op = "kv_append_mxfp4"
     dev, shape = k.get_device(), k.shape
@@ -479,6 +481,11 @@ def _query(op: str, q: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Te
     return q, out
 
 
+# Bytes of a row of scales, which the attention kernels load at once, by the head dims they take (the entry points refuse
+# the others).
+_SCALE_ROW = {64: 2, 128: 4}
+
+
 def _scale(op: str, scale: float) -> float:
     scale = float(scale)
     if not 0 < scale < math.inf:
@@ -504,7 +511,7 @@ def decode_attention_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: tor
     scale = _scale(op, scale)
     dev = q.get_device()
     B, Hq, D = q.shape
-    Hkv, cap, st = _check_cache(op, dev, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D)
+    Hkv, cap, st = _check_cache(op, dev, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D, _SCALE_ROW.get(D, 1))
     if Hkv == 0 or Hq % Hkv:
         raise ValueError(f"{op}: {Hq} query heads for {Hkv} KV heads")
     if cap == 0:
@@ -539,7 +546,7 @@ def flash_attention_cache_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales
     scale = _scale(op, scale)
     dev = q.get_device()
     B, Hq, Sq, D = q.shape
-    Hkv, cap, st = _check_cache(op, dev, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D)
+    Hkv, cap, st = _check_cache(op, dev, k_codes, k_scales, v_codes, v_scales, kv_lens, B, D, _SCALE_ROW.get(D, 1))
     if Hkv * num_kv_groups != Hq:
         raise ValueError(f"{op}: Hq={Hq} != Hkv={Hkv} * num_kv_groups={num_kv_groups}")
     ml = cap if max_len is None else int(max_len)

@@ -747,3 +747,65 @@ def test_attention_refuses_a_scale_that_is_not_positive(scale):
         with pytest.raises(ValueError, match="scale"):
             run()
     assert torch.equal(lens.cpu(), c.lens)
+
+
+@pytest.mark.parametrize("d", [96, 160, 192, 224])
+def test_append_of_head_dims_with_an_odd_count_of_blocks(d):
+    """Rows of 3, 5, 6 and 7 scales: no address of an allocation is a multiple of those, and none need be."""
+    B, S, H, cap = 3, 4, 2, 20
+    lens = torch.tensor([0, 7, 18], dtype=torch.int32)  # the last sequence runs past the cap
+    k, v = rnd(B, S, H, d, seed=62), rnd(B, S, H, d, seed=63)
+    for shift in (0, 1, 2, 3):
+        cache = [torch.full((B, H, cap, w), 0xA5, dtype=torch.uint8) for w in (d // 2, d // 32, d // 2, d // 32)]
+        dev = [t.to(DEV) for t in cache]
+        for i in (1, 3):  # the scales at any byte
+            dev[i] = torch.full((cache[i].numel() + shift,), 0xA5, dtype=torch.uint8, device=DEV)[shift:].view(cache[i].shape)
+        K.kv_append_mxfp4(k.to(DEV), v.to(DEV), *dev, lens.to(DEV))
+        for x, c, s in ((k, 0, 1), (v, 2, 3)):
+            qc, qs = M.quantize(x)
+            for b in range(B):
+                for i in range(S):
+                    if int(lens[b]) + i < cap:
+                        cache[c][b, :, int(lens[b]) + i] = qc[b, i]
+                        cache[s][b, :, int(lens[b]) + i] = qs[b, i]
+        for got, want in zip(dev, cache):
+            assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_append_writes_scales_at_any_byte_and_attention_refuses_them(d):
+    B, H, cap = 2, 2, 16
+    k, q = rnd(B, 1, H, d, seed=64).to(DEV), rnd(B, 4, d, seed=65).to(DEV)
+    lens = torch.tensor([0, 3], dtype=torch.int32, device=DEV)
+    even = [torch.zeros(B, H, cap, w, dtype=torch.uint8, device=DEV) for w in (d // 2, d // 32, d // 2, d // 32)]
+    odd = [t if i % 2 == 0 else torch.zeros(t.numel() + 1, dtype=torch.uint8, device=DEV)[1:].view(t.shape)
+           for i, t in enumerate(t.clone() for t in even)]
+    for cache in (even, odd):
+        K.kv_append_mxfp4(k, k, *cache, lens)
+    for a, b in zip(even, odd):
+        assert torch.equal(a, b)
+    pos = torch.zeros(3, B, 1, dtype=torch.int32, device=DEV)
+    for cache in (even, odd):
+        K.qk_norm_rope_mxfp4(q.unsqueeze(1), k, k, torch.empty_like(q.unsqueeze(1)), *cache, None, None, pos,
+                             torch.ones(d // 2, device=DEV), (d // 2, 0, 0), 1e-6, lens + 1)
+    for a, b in zip(even, odd):
+        assert torch.equal(a, b)
+    K.decode_attention_mxfp4(q, *even, lens, 0.1)
+    for bad in (lambda: K.decode_attention_mxfp4(q, *odd, lens, 0.1),
+                lambda: K.flash_attention_cache_mxfp4(q.unsqueeze(2), *odd, lens, 0.1, 2)):
+        with pytest.raises(ValueError, match="scales"):
+            bad()
+
+
+@pytest.mark.parametrize("d", [32, 96, 160, 256])
+def test_attention_refuses_head_dims_by_the_dim_alone(d):
+    u = lambda w: torch.zeros(2, 1, 40, w, dtype=torch.uint8, device=DEV)  # noqa: E731
+    q, lens = rnd(2, 2, 1, d).to(DEV), torch.ones(2, dtype=torch.int32, device=DEV)
+    cache = (u(d // 2), u(d // 32), u(d // 2), u(d // 32))
+    for shift in (0, 1):
+        cache = (cache[0], torch.zeros(80 * (d // 32) + shift, dtype=torch.uint8, device=DEV)[shift:].view(2, 1, 40, d // 32),
+                 *cache[2:])
+        for bad in (lambda: K.decode_attention_mxfp4(q[:, :, 0], *cache, lens, 0.1),
+                    lambda: K.flash_attention_cache_mxfp4(q, *cache, lens, 0.1, 2)):
+            with pytest.raises(_lib.Q3Error, match="outside what"):
+                bad()
