@@ -583,18 +583,31 @@ int64_t header_bytes(int64_t B) { return (B + 1 + 63) / 64 * 256; }
 
 int64_t sets_of(int64_t groups, int64_t Sq) { return q3_cdiv(groups * Sq, kCols); }
 
-// The streaming kernel takes single tokens, and chunks of few pairs. Otherwise the cache
-// is expanded to bf16 once and the chunk kernel of the bf16 cache runs, which shares each
-// row among 256 columns but does not split the rows: its time grows with the rows until
-// the pairs fill the card, the streaming kernel's with pairs x rows. Microseconds,
-// streaming / expanding, 8 KV heads of 4 query heads unless said otherwise: 8192 rows, 32
-// tokens (64 pairs) 38 / 209, 128 (256) 53 / 213, 512 (1024) 160 / 214, 700 (1400) 219 /
-// 215, 1000 (2000) 279 / 216; 4 x 2000 rows, 64 tokens (512) 27 / 72, 200 (1600) 54 / 73,
-// 300 (2432) 84 / 73; 1024 rows, 256 tokens (512) 20 / 41, 512 (1024) 34 / 42; 8 x 300
-// rows of 4 x 8 heads, 60 tokens (960) 21 / 28, 100 (1600) 28 / 29, 150 (2400) 37 / 30.
-constexpr int64_t kStreamPairs = 1400;
+// The streaming kernel takes single tokens, chunks of few pairs, and chunks of few column
+// sets per KV head. Otherwise the cache is expanded to bf16 once and the chunk kernel of
+// the bf16 cache runs.
+//
+// Few pairs: the chunk kernel shares each row among 256 columns but does not split the
+// rows, so its time grows with the rows until the pairs fill the card, the streaming
+// kernel's with pairs x rows. Microseconds, streaming / expanding, 8 KV heads of 4 query
+// heads unless said otherwise: 8192 rows, 32 tokens (64 pairs) 38 / 209, 128 (256) 53 /
+// 213, 512 (1024) 160 / 214, 700 (1400) 219 / 215, 1000 (2000) 279 / 216; 4 x 2000 rows,
+// 64 tokens (512) 27 / 72, 200 (1600) 54 / 73, 300 (2432) 84 / 73; 1024 rows, 256 tokens
+// (512) 20 / 41, 512 (1024) 34 / 42; 8 x 300 rows of 4 x 8 heads, 60 tokens (960) 21 / 28,
+// 100 (1600) 28 / 29, 150 (2400) 37 / 30.
+//
+// Few sets: the streaming kernel reads and converts a row once per 16 columns of its KV
+// head, while the expansion moves 4.8 times the bytes of the rows to make them bf16 and
+// the chunk kernel reads those, however few columns there are. The same, by sets per KV
+// head, 1 / 4 / 8 / 12 / 16: 256 sequences x 8 KV heads of 8192 rows 389 / 1258 / 2440 /
+// 3403 / 4374 against 3776 / 3904 / 3921 / 4100 / 4121 (and 8.6 GB), of 300 rows 35 / 103 /
+// 194 / 288 / 385 against 193 / 212 / 229 / 256 / 276; 32 x 8 of 2000, from 4 on: 57 / 95 /
+// 127 / 163 against 124 / 126 / 141 / 154; D = 64, 256 x 8 of 2000: 59 / 186 / 363 / 539 /
+// 684 against 596 / 573 / 591 / 624 / 632.
+constexpr int64_t kStreamPairs = 1400, kStreamSets = 12;
 bool streams(int64_t B, int64_t Hkv, int64_t groups, int64_t Sq) {
-  return Sq == 1 || B * Hkv * sets_of(groups, Sq) <= kStreamPairs;
+  const int64_t sets = sets_of(groups, Sq);
+  return Sq == 1 || sets <= kStreamSets || B * Hkv * sets <= kStreamPairs;
 }
 
 // Waves of a block that takes one pair, or 0 to split all units between all waves and merge records. Pairs per

@@ -537,8 +537,9 @@ def flash_attention_cache_mxfp4(q: torch.Tensor, k_codes: torch.Tensor, k_scales
 
     q (B, Hq, Sq, D) bf16, D 64 or 128; the chunk's rows [kv_lens[b], kv_lens[b] + Sq) are already in the cache.
     Query i of sequence b attends to cache rows [0, kv_lens[b] + i]; advance=True adds Sq to kv_lens afterwards. scale
-    must be positive. `max_len` bounds every kv_lens[b] + Sq (default: cap): rows past it are not read. It sizes the workspace of a
-    chunk of more than 1400 (sequence, KV head, 16 columns), 4 * B * Hkv * max_len * D bytes.
+    must be positive. `max_len` bounds every kv_lens[b] + Sq (default: cap): rows past it are not read. It sizes the
+    workspace of a chunk over expanded rows, 4 * B * Hkv * max_len * D bytes: one of more than 192 columns (tokens x
+    query heads of a KV head) and of more than 1400 (sequence, KV head, 16 columns).
     """
     op = "flash_attention_cache_mxfp4"
     if q.dim() != 4:

@@ -809,3 +809,31 @@ def test_attention_refuses_head_dims_by_the_dim_alone(d):
                     lambda: K.flash_attention_cache_mxfp4(q, *cache, lens, 0.1, 2)):
             with pytest.raises(_lib.Q3Error, match="outside what"):
                 bad()
+
+
+# more than 1400 pairs of a KV head and 16 columns, with one to twelve column sets to a head: streamed all the same
+@pytest.mark.parametrize("B,hkv,groups,sq,cap,d", [(180, 8, 4, 2, 90, 128), (40, 40, 1, 5, 200, 64), (90, 16, 8, 2, 60, 128),
+                                                   (45, 16, 4, 8, 120, 128), (16, 8, 4, 48, 130, 64), (2, 720, 1, 3, 2100, 64)])
+def test_chunks_of_few_columns_and_many_sequences(B, hkv, groups, sq, cap, d):
+    """Against float64 on the GPU, at the bound of the module's docstring."""
+    assert B * hkv * -(-groups * sq // 16) > 1400
+    g = torch.Generator().manual_seed(66)
+    kc, vc = (torch.randint(0, 256, (B, hkv, cap, d // 2), generator=g, dtype=torch.uint8).to(DEV) for _ in range(2))
+    ks, vs = (torch.randint(122, 127, (B, hkv, cap, d // 32), generator=g, dtype=torch.uint8).to(DEV) for _ in range(2))
+    lens = torch.randint(0, cap - sq + 1, (B,), generator=g, dtype=torch.int32).to(DEV)
+    lens[0], lens[1] = 0, cap - sq
+    row = torch.arange(cap, device=DEV)
+    for t in (ks, vs):  # rows behind the chunk's: NaN
+        t.masked_fill_((row >= (lens + sq)[:, None])[:, None, :, None], 255)
+    q, scale, dl = rnd(B, hkv * groups, sq, d, seed=68).to(DEV), 0.1, lens.clone()
+    o = K.flash_attention_cache_mxfp4(q, kc, ks, vc, vs, dl, scale, groups, advance=True)
+    assert torch.equal(dl, lens + sq)
+    k, v = (K.mxfp4_dequantize(*t).double().nan_to_num(0.0) for t in ((kc, ks), (vc, vs)))
+    k, q2 = k.transpose(-1, -2).contiguous(), q.double().reshape(B, hkv, groups * sq, d)
+    seen = (lens[:, None] + 1 + torch.arange(sq, device=DEV)).repeat(1, groups)[:, None, :, None]
+    w = torch.softmax((q2 @ k * scale).masked_fill(row >= seen, -math.inf), -1)
+    ref, spread = (w @ t for t in (v, v.abs()))
+    mag = float((q2.abs() @ k.abs()).max()) * scale
+    err = HALF + 2 * (d * 2.0 ** -24 * mag + 2.0 ** -22 * (1 + mag)) + cap * 2.0 ** -23
+    tol = err * spread * (1 + HALF) + HALF * ref.abs()
+    assert bool(((o.double().reshape(ref.shape) - ref).abs() <= tol).all())

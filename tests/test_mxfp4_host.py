@@ -164,3 +164,14 @@ def test_attention_refuses_a_scale_that_is_not_positive(L, scale):
     for Sq in (4, 1000):  # streamed, and over expanded rows
         assert L.q3_flash_attention_cache_mxfp4(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 2, 64, 8, Sq, 128, 1000, st, scale,
                                                 0, 1, FAKE, 1 << 40, None) == -2
+
+
+def test_chunks_of_few_columns_keep_to_the_four_bit_rows(L):
+    """A chunk whose columns (tokens x query heads of a KV head) read a row only a few times streams the cache, however
+    many sequences it has: its workspace is records, not the rows in bf16."""
+    ws = L.q3_flash_attention_cache_mxfp4_workspace_bytes
+    for B, Hq, Hkv, Sq in ((256, 32, 8, 2), (256, 32, 8, 4), (64, 128, 32, 3), (1024, 8, 8, 16), (256, 32, 8, 48)):
+        sets = -(-Sq * (Hq // Hkv) // 16)
+        for max_len in (300, 8192):
+            assert ws(B, Hq, Hkv, Sq, 128, max_len) <= 8192 + (3072 + B * Hkv * sets) * 16 * 130 * 4
+    assert ws(256, 32, 8, 64, 128, 8192) == 4 * 256 * 8 * 8192 * 128  # 16 times: expanded
