@@ -128,18 +128,20 @@ struct AppendArgs {
 };
 
 // One piece per lane, ordered (token, k | v, head, piece of the row): a row is
-// D / 8 lanes, a multiple of four, so a block's lanes are neighbours.
-template <typename T>
+// D / 8 lanes, a multiple of four, so a block's lanes are neighbours. I: the type
+// that the pieces are counted in; 64 bits where 32 do not hold them (a whole cache
+// of 34 GB quantised at once), as their divisions cost several times as much.
+template <typename T, typename I>
 __global__ __launch_bounds__(256) void mx_append_kernel(const AppendArgs a) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const uint32_t i = (uint32_t)min(t, a.pieces - 4 + (threadIdx.x & 3));
-  uint32_t r = i / a.D8;
-  const uint32_t j = i % a.D8;
-  const uint32_t h = r % a.Hkv;
-  r /= a.Hkv;
-  const int kv = r & 1;
+  const int64_t t = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
+  const I i = (I)min(t, a.pieces - 4 + (threadIdx.x & 3));
+  I r = i / (uint32_t)a.D8;
+  const uint32_t j = (uint32_t)(i % (uint32_t)a.D8);
+  const uint32_t h = (uint32_t)(r % (uint32_t)a.Hkv);
+  r /= (uint32_t)a.Hkv;
+  const int kv = (int)(r & 1);
   r >>= 1;
-  const uint32_t s = r % a.S, b = r / a.S;
+  const uint32_t s = (uint32_t)(r % (uint32_t)a.S), b = (uint32_t)(r / (uint32_t)a.S);
   const T* x = static_cast<const T*>(kv ? a.x[1] : a.x[0]);
   float v[8];
   mx_load8<T>(x + b * (kv ? a.xs[1][0] : a.xs[0][0]) + s * (kv ? a.xs[1][1] : a.xs[0][1]) +
@@ -262,7 +264,7 @@ int q3_kv_append_mxfp4(const void* k, const void* v, void* k_codes, void* k_scal
   if (B == 0 || S == 0) return Q3_OK;
   Q3_REQUIRE(B < (1ll << 31) && S < (1ll << 31) && Hkv < (1ll << 20) && cap < (1ll << 31), Q3_ERR_SHAPE);
   const int64_t per_token = 2 * Hkv * (D / 8);
-  Q3_REQUIRE(B * S < (1ll << 31) / per_token, Q3_ERR_SHAPE);  // 32-bit piece index
+  Q3_REQUIRE(B * S < (1ll << 38) / per_token, Q3_ERR_SHAPE);  // the grid: 2^30 blocks
   const int64_t es = dtype == Q3_BF16 ? 2 : 4;
   bool ok = q3_aligned(k, 16) && q3_aligned(v, 16) && q3_aligned(k_codes, 4) && q3_aligned(v_codes, 4);
   for (int i = 0; i < 6; ++i) ok = ok && strides[i] * es % 16 == 0;
@@ -288,12 +290,18 @@ int q3_kv_append_mxfp4(const void* k, const void* v, void* k_codes, void* k_scal
   a.D8 = (int)(D / 8);
   a.cap = cap;
   a.pieces = B * S * per_token;
-  const dim3 grid((unsigned)q3_cdiv(a.pieces, 256));
+  const bool wide = a.pieces >= (1ll << 31);
+  const int64_t blocks = q3_cdiv(a.pieces, 256);  // a launch has less than 2^32 threads along x
+  const dim3 grid((unsigned)(wide ? 1 << 23 : blocks), (unsigned)(wide ? q3_cdiv(blocks, 1 << 23) : 1));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == Q3_BF16)
-    hipLaunchKernelGGL((mx_append_kernel<bf16>), grid, dim3(256), 0, st, a);
+  if (dtype == Q3_BF16 && !wide)
+    hipLaunchKernelGGL((mx_append_kernel<bf16, uint32_t>), grid, dim3(256), 0, st, a);
+  else if (dtype == Q3_BF16)
+    hipLaunchKernelGGL((mx_append_kernel<bf16, uint64_t>), grid, dim3(256), 0, st, a);
+  else if (!wide)
+    hipLaunchKernelGGL((mx_append_kernel<float, uint32_t>), grid, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((mx_append_kernel<float>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((mx_append_kernel<float, uint64_t>), grid, dim3(256), 0, st, a);
   Q3_LAUNCH_CHECK();
   return Q3_OK;
 }

@@ -328,3 +328,23 @@ def test_caches_go_by_the_type_of_a_head_of_another_class():
     m.norm.float()
     assert m.new_caches(1, 8)[0].k.dtype == torch.bfloat16
     assert len(m.new_caches(1, 8, kv_format="mxfp4")) == 2
+
+
+def test_a_large_cache_is_quantised_whatever_its_size():
+    """More values than 32 bits count in pieces of eight. The bf16 rows are views that repeat one sequence's or one
+    row's values, so only the four-bit rows take memory (9 GB)."""
+    B, H, cap, d = 1024, 8, 8200, 128
+    assert B * cap * 2 * H * (d // 8) > 2 ** 31
+    k, v = rnd(B, H, 1, d, seed=90), rnd(1, H, cap, d, seed=91)
+    plain = StaticKVCache(1, 1, 1, d, device=DEV)
+    plain.k, plain.v, plain.capacity = k.expand(B, H, cap, d), v.expand(B, H, cap, d), cap
+    plain.lens = torch.full((B,), 5, dtype=torch.int32, device=DEV)
+    plain.set_host_state((5, 5))
+    c = MXFP4KVCache.from_static(plain)
+    assert c.lens.tolist() == [5] * B and c.max_len == 5 and c.capacity == cap
+    for x, codes, scales in ((k, c.k_codes, c.k_scales), (v, c.v_codes, c.v_scales)):
+        qc, qs = K.mxfp4_quantize(x)
+        for b in range(0, B, 128):
+            s = slice(b, b + 128)
+            assert bool((codes[s] == (qc[s] if qc.shape[0] > 1 else qc)).all())
+            assert bool((scales[s] == (qs[s] if qs.shape[0] > 1 else qs)).all())
