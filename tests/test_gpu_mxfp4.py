@@ -837,3 +837,51 @@ def test_chunks_of_few_columns_and_many_sequences(B, hkv, groups, sq, cap, d):
     err = HALF + 2 * (d * 2.0 ** -24 * mag + 2.0 ** -22 * (1 + mag)) + cap * 2.0 ** -23
     tol = err * spread * (1 + HALF) + HALF * ref.abs()
     assert bool(((o.double().reshape(ref.shape) - ref).abs() <= tol).all())
+
+
+def test_heads_that_start_past_32_bits():
+    """The last head's codes start at 4.3e9 bytes, past 2^32. Everything but the written rows holds codes of 0x77 and
+    scales of 255, so an offset cut to 32 bits, signed or not, would read those; the append must have written there."""
+    B, H, G, D, cap, n = 2, 4, 4, 128, 9_600_000, 40
+    assert (B * H - 1) * cap * (D // 2) > 2 ** 32
+    cache = [torch.full((B, H, cap, w), 255 if w == 4 else 0x77, dtype=torch.uint8, device=DEV) for w in (64, 4, 64, 4)]
+    assert cache[0][-1, -1].data_ptr() - cache[0].data_ptr() > 2 ** 32
+    k, v = rnd(B, n, H, D, seed=69), rnd(B, n, H, D, seed=70)
+    K.kv_append_mxfp4(k.to(DEV), v.to(DEV), *cache, torch.zeros(B, dtype=torch.int32, device=DEV))
+    small = Cache([n] * B, H, n, D, seed=0)
+    small.kc, small.ks = (t.transpose(1, 2).contiguous() for t in M.quantize(k))
+    small.vc, small.vs = (t.transpose(1, 2).contiguous() for t in M.quantize(v))
+    for big, want in zip(cache, (small.kc, small.ks, small.vc, small.vs)):
+        assert torch.equal(big[:, :, :n].cpu(), want)
+    assert int((cache[1] != 255).sum()) <= B * H * n * 4  # and nothing else was written
+    lens = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    q = rnd(B, H * G, D, seed=71)
+    o = K.decode_attention_mxfp4(q.to(DEV), *cache, lens, 0.1)
+    check_attention(o.unsqueeze(2), q.unsqueeze(2), small, torch.full((B, 1), n), 0.1)
+    for sq in (5, 32):
+        q = rnd(B, H * G, sq, D, seed=72)
+        o = K.flash_attention_cache_mxfp4(q.to(DEV), *cache, lens - sq, 0.1, G)
+        check_attention(o, q, small, n - sq + 1 + torch.arange(sq).expand(B, sq), 0.1)
+    y = K.mxfp4_dequantize(cache[0][:, :, :n], cache[1][:, :, :n])
+    assert same_bits(y.double(), M.values(small.kc, small.ks))
+    # the fused form's own addresses; at position 0 the rotation leaves the rows as they are
+    rows = k.to(DEV)[:, :1]
+    K.qk_norm_rope_mxfp4(rows, rows, v.to(DEV)[:, :1], torch.empty_like(rows), *cache, None, None,
+                         torch.zeros(3, B, 1, dtype=torch.int32, device=DEV), torch.ones(D // 2, device=DEV),
+                         (D // 2, 0, 0), 1e-6, lens)
+    for i, want in enumerate((small.kc, small.ks, small.vc, small.vs)):
+        assert torch.equal(cache[i][:, :, n].cpu(), want[:, :, 0])
+
+
+
+def test_long_chunk_over_heads_that_start_past_32_bits():
+    """Over expanded rows: to the bit what the same rows give in a cache that ends after them."""
+    B, H, G, D, cap, sq, n = 2, 4, 16, 128, 9_600_000, 200, 230
+    assert B * H * G * sq // 16 > 1400 and (B * H - 1) * cap * (D // 2) > 2 ** 32
+    cache = [torch.full((B, H, cap, w), 255 if w == 4 else 0x77, dtype=torch.uint8, device=DEV) for w in (64, 4, 64, 4)]
+    k, v, zero = rnd(B, n, H, D, seed=73).to(DEV), rnd(B, n, H, D, seed=74).to(DEV), torch.zeros(B, dtype=torch.int32, device=DEV)
+    K.kv_append_mxfp4(k, v, *cache, zero)
+    q, lens = rnd(B, H * G, sq, D, seed=75).to(DEV), torch.tensor([n - sq, 3], dtype=torch.int32, device=DEV)
+    o = K.flash_attention_cache_mxfp4(q, *cache, lens, 0.1, G, max_len=n)
+    ref = K.flash_attention_cache_mxfp4(q, *(t[:, :, :n].contiguous() for t in cache), lens, 0.1, G)
+    assert torch.isfinite(o).all() and torch.equal(o, ref)
