@@ -885,3 +885,43 @@ def test_long_chunk_over_heads_that_start_past_32_bits():
     o = K.flash_attention_cache_mxfp4(q, *cache, lens, 0.1, G, max_len=n)
     ref = K.flash_attention_cache_mxfp4(q, *(t[:, :, :n].contiguous() for t in cache), lens, 0.1, G)
     assert torch.isfinite(o).all() and torch.equal(o, ref)
+
+
+# Several weights and one, with the norm, whose rows come to three, four and six 16-row groups a block
+@pytest.mark.parametrize("m", [1, 3, 7, 16, 20, 32])
+@pytest.mark.parametrize("ns,k", [((8192, 1024, 1024), 256), ((9000, 3000, 1), 384), ((14000, 2384), 128), ((24000,), 128),
+                                  ((12003,), 640)])
+def test_matmul_segments_with_the_norm_of_many_output_rows(ns, k, m):
+    ws = [weight(n, k, seed=n) for n in ns]
+    x, nw, eps = rnd(m, k, seed=m), rnd(k, seed=3) * 0.2 + 1, 1e-5
+    y = K.matmul_segments_mxfp4(x.to(DEV), [(c.to(DEV), s.to(DEV)) for c, s in ws], norm_weight=nw.to(DEV), eps=eps).cpu()
+    xn, at = normed(x, nw, eps), 0
+    for (c, s), n in zip(ws, ns):
+        w = M.values(c, s)
+        ref, mag = xn @ w.T, xn.abs() @ w.abs().T
+        # as in test_matmul_segments_matches_float64: x * norm weight rounds to bf16, fp32 sums and square root
+        err = (k + 2) * 2.0 ** -23 * mag + mag * (HALF + (k + 4) * 2.0 ** -23)
+        tol = HALF * (ref.abs() + err) + err
+        d = (y[:, at:at + n].double() - ref).abs()
+        assert bool((d <= tol).all()), float((d / tol).max())
+        at += n
+
+
+# scales by bytes (K no multiple of 128, or their first byte at an odd address) with one to six 16-row groups a block
+@pytest.mark.parametrize("m", [1, 4, 12, 16, 20, 32, 50])
+@pytest.mark.parametrize("n,k", [(4001, 96), (6000, 160), (12003, 544), (16000, 96), (24000, 288), (30001, 32)])
+def test_matmul_scales_by_bytes_of_many_weight_rows(n, k, m):
+    codes, scales = weight(n, k, seed=n)
+    x, b, r = rnd(m, k, seed=m), rnd(n, seed=1), rnd(m, n, seed=2)
+    y = K.matmul_mxfp4(x.to(DEV), codes.to(DEV), scales.to(DEV), b.to(DEV), r.to(DEV))
+    check_matmul(y, x, codes, scales, b, r)
+
+
+@pytest.mark.parametrize("m", [2, 14, 30])
+@pytest.mark.parametrize("n,k", [(6000, 256), (12003, 1024), (24000, 128)])
+def test_matmul_scales_at_odd_addresses_of_many_weight_rows(n, k, m):
+    codes, scales = weight(n, k, seed=n)
+    odd = torch.empty(scales.numel() + 1, dtype=torch.uint8, device=DEV)[1:].view(scales.shape)
+    odd.copy_(scales)
+    x = rnd(m, k, seed=m)
+    check_matmul(K.matmul_mxfp4(x.to(DEV), codes.to(DEV), odd), x, codes, scales)
