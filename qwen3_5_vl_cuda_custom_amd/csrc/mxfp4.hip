@@ -4,9 +4,9 @@
 // All three are bound by memory: eight values (a 16-byte load or store of bf16,
 // 4 bytes of codes) per lane and piece, so the four lanes of a block exchange
 // their largest magnitude with two lane shuffles and nothing goes through LDS. A lane has
-// four pieces in flight where rows are long. Measured: quantising 12288 x 4096 fp32 39 us
-// (228 MB, 5.8 TB/s), back to bf16 20 us (127 MB, 6.4 TB/s); 256 x 128 bf16 2.6 and 2.4 us;
-// writing 4 x 512 new rows of 8 heads x 128 (K and V) 5.7 us, one row 1.8 us.
+// four pieces in flight where rows are long. Measured: quantising 12288 x 4096 fp32 40 us
+// (228 MB, 5.7 TB/s), back to bf16 20 us (127 MB, 6.4 TB/s); 256 x 128 bf16 2.6 and 2.4 us;
+// writing 4 x 512 new rows of 8 heads x 128 (K and V) 5.9 us, one row 1.9 us.
 #include "mxfp4.h"
 
 namespace {

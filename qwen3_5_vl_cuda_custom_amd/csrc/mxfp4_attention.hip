@@ -28,16 +28,20 @@
 //    time, and read with ds_read_b64_tr_b16. P^T comes straight from the S^T
 //    accumulators (lane (c, g) holds rows 4 g + i and 16 + 4 g + i of column c; V's
 //    fragment reads follow that order).
-//  * P is rounded to bf16 for the second product (relative 2^-9 each, averaged
-//    over the rows: the output's own rounding to bf16 is larger); q, K and V enter
-//    exactly; m, the sum and o are fp32.
+//  * P is rounded to bf16 for the second product (at most 2^-8 of each weight), as in the
+//    kernels of the bf16 cache; q, K and V enter exactly; m, the sum and o are fp32. The
+//    roundings of a row's weights are independent, so numerator and error shrink alike and
+//    the share stays: the outputs are 0.0023 of their norm from float64, 0.0017 of which
+//    their own rounding to bf16 makes. P in two bf16 terms would leave those 0.0017 alone
+//    and takes a second product per tile of V: the 32 sequences below 43.9 -> 46.1 us
+//    with the merge, 37 tokens on 4 x 2000 rows 23.3 -> 25.0.
 //
 // Measured (us; the floor is the cache's bytes at 6.5 TB/s, what such a read reaches
-// here): 32 sequences of 8 KV heads x 4, lengths to 8192, 165 MB: 30 and 5.6 for the
-// merge (floor 25; with the arithmetic left out both take 40.5 in place of 42.8, so it
-// hides under the loads); one of 1500 rows, 1.6 MB: 5.5 and 4.4, all of it latency; a
-// block per pair, 32 sequences to 2000: 19 (split 23.5); 64 tokens on 4 x 2000 rows (512
-// pairs of 16 columns, which read the same rows from the L2): 27 (split 37).
+// here): 32 sequences of 8 KV heads x 4, lengths to 8192, 138 MB of rows in use 31 and 6
+// for the merge (floor 21), 178 MB 36.5 and 5.7 (27); one of 1500 rows, 1.6 MB: 5.6 and
+// 4.5, all of it latency; a block per pair, 32 sequences to 2000: 19 (split 23.5); 64
+// tokens on 4 x 2000 rows (512 pairs of 16 columns, which read the same rows from the
+// L2): 27 (split 37).
 #include <algorithm>
 #include <type_traits>
 
@@ -92,9 +96,10 @@ __device__ __forceinline__ int units_of(const MxAttn& p, int b) { return (rows_o
 
 // U units over n waves: the first U % n take one more than the others. Up to 512 units
 // have a wave each; more units take more waves only while each has at least 8 units, as
-// every wave that shares a pair costs the merge a record (8 units against 1, in us: one
-// sequence of 1024 rows x 8 heads, 64 tokens 27.5 / 37.6; 8 sequences of 300 x 4, 16
-// tokens 20.6 / 25.6; 32 sequences of 8192 x 8, where all waves are full, 42.7 / 42.8).
+// every wave that shares a pair costs the merge a record (8 units against 1, in us with the
+// merge, 8 KV heads of 4: one sequence of 8192 rows 12.2 / 14.0, of 16 tokens 22.5 / 26.5,
+// of 64 46.4 / 46.0; 8 of 8192 24.2 / 25.4; 16 of 3000 x 4 heads of 8 19.4 / 23.7; 32 of
+// 8192, where all waves are full, 57.9 / 58.1).
 constexpr int kMinWaves = 512, kMinUnits = 8;
 struct Split {
   int n, q, r;

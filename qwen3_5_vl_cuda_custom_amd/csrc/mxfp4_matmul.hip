@@ -57,8 +57,8 @@ __device__ __forceinline__ void store_y4(const MxGemm& p, int m, int n, floatx4 
 // the rows of scales start at multiples of four bytes), else byte by byte (a load of
 // one byte per lane costs as much as one of sixteen: M=32 N=151936 158 -> 113 us without).
 // 128 rows run at 1.1 PFLOP/s of the CUs they fill (M=512 N=12288 K=4096: 192 tiles, 67
-// us), 32 rows at the loads into LDS (N=4096 K=12288: 10 us for 26.7 MB of weights and
-// 98 KB of x per CU, and 3 for the sum over 8 ranges).
+// us), 32 rows at the loads into LDS (N=4096 K=12288: 11 us for 26.7 MB of weights and
+// 98 KB of x per CU, and 3.8 for the sum over 8 ranges).
 template <int RT, int BM, int WM, int BK, int NST, bool ALIGNED>
 __global__ __launch_bounds__(512) void mx_tile_kernel(const MxGemm p) {
   constexpr int NW = 8, WN = NW / WM, BN = 16 * RT * WN, MT = BM / 16 / WM;
@@ -259,6 +259,7 @@ double expand_us(int64_t M, int64_t N, int64_t K) {
 // N=12288 K=4096 11.2 / 14.1 / -; 64 rows, N=1024 K=4096 11.5 / 10.0 / -, N=4096 12.3 / 14.5 / -, N=12288 16.0 / 18.5 / -;
 // 136 rows, N=1114 K=416 6.5 / 31.5 / 22; 616, N=393 K=7232 27.8 / 26.6 / 59; 3018, N=78 K=512 6.3 / 21.7 / 13.8; 3102,
 // N=667 K=9024 108 / 65 / 82; 469, N=9936 K=224 30 / 19 / 23; N=12288 K=4096, 256 rows - / 45 / 77, 512 - / 67 / 98, 777 - / 126 / 115.
+// (kernels/mxfp4.py, _expands, tells from the tiles and the workspace whether a product expands.)
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
   const Plan rows{kRows, 0, 0, 1};
   if (M <= 16) return rows;

@@ -37,7 +37,7 @@ def _matmul_workspace(M: int, N: int, K: int) -> int:
 
 def _expands(M: int, N: int, K: int) -> bool:
     """Whether q3_matmul_mxfp4 would expand the weight to bf16: its workspace is then the weight (and not sums over
-    ranges of k, which only fewer than 256 tiles of 128 x 256 need)."""
+    ranges of k, which only fewer than 256 tiles of 128 x 256 need). Follows plan_of in csrc/mxfp4_matmul.hip."""
     return -(-M // 128) * -(-N // 256) > 256 and _matmul_workspace(M, N, K) == 2 * N * K
 
 
@@ -136,7 +136,8 @@ def matmul_mxfp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bia
                  residual: torch.Tensor | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """matmul with the weight (N, K) held in MXFP4: x·Wᵀ (+ bias) (+ residual), x (..., K) bf16, one rounding.
 
-    `out`, when given: (..., N) whose rows have one stride and contiguous elements, written in place (a column
+    Many rows run over the weight expanded to bf16, 2 * N * K bytes of workspace for the time of the call. `out`, when
+    given: (..., N) whose rows have one stride and contiguous elements, written in place (a column
     slice of a wider buffer).
     """
     op = "matmul_mxfp4"
@@ -253,7 +254,7 @@ def matmul_segments_mxfp4(x: torch.Tensor, weights, biases=None, *, norm_weight:
     With norm_weight the rows of x are RMS-normalised first (rmsnorm_matmul_segments). Up to 64 rows of K a multiple of
     128 are one launch (with the norm up to 32 of K at most 8192, else the norm is another); more rows, or another K, a
     product per weight, or where its weight would be expanded to bf16 (many rows), matmul_segments over the expanded
-    weights.
+    weights, all of them at once: 2 * ΣN_i * K bytes for the time of the call.
     """
     op = "matmul_segments_mxfp4"
     weights = list(weights)
@@ -298,7 +299,7 @@ def matmul_swiglu_mxfp4(x: torch.Tensor, gate: tuple[torch.Tensor, torch.Tensor]
     With norm_weight the rows of x are RMS-normalised first (rmsnorm_matmul_swiglu). Up to 64 rows of K a multiple of
     128 are one launch (with the norm up to 32 of K at most 8192, else the norm is another); more rows, or another K, two
     products and swiglu, or where their weights would be expanded to bf16 (many rows), matmul_swiglu over the expanded
-    weights.
+    weights, both at once: 4 * N * K bytes for the time of the call (200 MB at N 12288, K 4096).
     """
     op = "matmul_swiglu_mxfp4"
     dev, K, M, x2, ldx, fits = _few_rows(op, x, norm_weight)
@@ -481,8 +482,8 @@ def _query(op: str, q: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Te
     return q, out
 
 
-# Bytes of a row of scales, which the attention kernels load at once, by the head dims they take (the entry points refuse
-# the others).
+# Bytes of a row of scales, which the attention kernels load at once, by the head dims they take (the entry points
+# refuse the others).
 _SCALE_ROW = {64: 2, 128: 4}
 
 

@@ -77,8 +77,8 @@ class StaticKVCache:
 
 
 class MXFP4KVCache(StaticKVCache):
-    """StaticKVCache held in four bits (MXFP4, blocks of 32 along the head dim): 4.25 bits a value, an eighth more
-    than a quarter of a bf16 cache (no reference counterpart).
+    """StaticKVCache held in four bits (MXFP4, blocks of 32 along the head dim): 4.25 bits a value, a sixteenth
+    more than a quarter of a bf16 cache (no reference counterpart).
 
     k_codes, v_codes: (B, Hkv, capacity, D / 2), k_scales, v_scales: (B, Hkv, capacity, D / 32), uint8; `lens` and the
     host's lengths as in StaticKVCache. Rows are quantised from bf16 as they are written and read in place by the
