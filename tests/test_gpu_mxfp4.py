@@ -925,3 +925,42 @@ def test_matmul_scales_at_odd_addresses_of_many_weight_rows(n, k, m):
     odd.copy_(scales)
     x = rnd(m, k, seed=m)
     check_matmul(K.matmul_mxfp4(x.to(DEV), codes.to(DEV), odd), x, codes, scales)
+
+
+@pytest.mark.parametrize("m", [1, 20, 64, 200, 700])
+def test_products_of_weights_below_the_normal_range(m):
+    """Scale bytes 0 to 4: the smallest magnitudes are subnormal in bf16, and enter the products as they are."""
+    n, k = (66000, 64) if m == 200 else (600, 1024)  # 200 rows: over the expanded weight
+    g = torch.Generator().manual_seed(76)
+    codes = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
+    scales = torch.randint(0, 5, (n, k // 32), generator=g, dtype=torch.uint8)
+    x = rnd(m, k, seed=77, dtype=torch.float32).mul(2.0 ** 110).to(torch.bfloat16)
+    y = K.matmul_mxfp4(x.to(DEV), codes.to(DEV), scales.to(DEV))
+    check_matmul(y, x, codes, scales)
+    if m <= 64:
+        w = (codes[:64].to(DEV), scales[:64].to(DEV))
+        check_matmul(K.matmul_segments_mxfp4(x.to(DEV), [w])[:, :64], x, codes[:64], scales[:64])
+
+
+@pytest.mark.parametrize("sq,cap,groups", [(1, 90, 4), (1, 3000, 4), (5, 90, 4), (400, 420, 8)])
+def test_attention_over_rows_below_the_normal_range(sq, cap, groups):
+    """Keys and values of scale bytes 0 to 4, and queries large enough for scores of ordinary size."""
+    B, hkv, d = 2, 16 if sq == 400 else 2, 128
+    g = torch.Generator().manual_seed(78)
+    kc, vc = (torch.randint(0, 256, (B, hkv, cap, d // 2), generator=g, dtype=torch.uint8).to(DEV) for _ in range(2))
+    ks, vs = (torch.randint(0, 5, (B, hkv, cap, d // 32), generator=g, dtype=torch.uint8).to(DEV) for _ in range(2))
+    lens = torch.full((B,), cap - sq, dtype=torch.int32, device=DEV)
+    q, scale = rnd(B, hkv * groups, sq, d, seed=79, dtype=torch.float32).mul(2.0 ** 120).to(torch.bfloat16).to(DEV), 0.02
+    o = K.flash_attention_cache_mxfp4(q, kc, ks, vc, vs, lens, scale, groups)
+    k, v = (K.mxfp4_dequantize(*t).double() for t in ((kc, ks), (vc, vs)))
+    k, q2 = k.transpose(-1, -2).contiguous(), q.double().reshape(B, hkv, groups * sq, d)
+    seen = (lens[:, None] + 1 + torch.arange(sq, device=DEV)).repeat(1, groups)[:, None, :, None]
+    w = torch.softmax((q2 @ k * scale).masked_fill(torch.arange(cap, device=DEV) >= seen, -math.inf), -1)
+    ref, spread = (w @ t for t in (v, v.abs()))
+    mag = float((q2.abs() @ k.abs()).max()) * scale
+    assert 0.5 < mag < 64
+    err = HALF + 2 * (d * 2.0 ** -24 * mag + 2.0 ** -22 * (1 + mag)) + cap * 2.0 ** -23
+    # below 2^-126 bf16 has the step 2^-133, and fp32 (the sums) 2^-149
+    tol = err * spread * (1 + HALF) + HALF * ref.abs() + 2.0 ** -134 + cap * 2.0 ** -149
+    assert bool(((o.double().reshape(ref.shape) - ref).abs() <= tol).all())
+    assert float(spread.max()) > 2.0 ** -128

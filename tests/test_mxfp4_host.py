@@ -173,5 +173,5 @@ def test_chunks_of_few_columns_keep_to_the_four_bit_rows(L):
     for B, Hq, Hkv, Sq in ((256, 32, 8, 2), (256, 32, 8, 4), (64, 128, 32, 3), (1024, 8, 8, 16), (256, 32, 8, 48)):
         sets = -(-Sq * (Hq // Hkv) // 16)
         for max_len in (300, 8192):
-            assert ws(B, Hq, Hkv, Sq, 128, max_len) <= 8192 + (3072 + B * Hkv * sets) * 16 * 130 * 4
+            assert ws(B, Hq, Hkv, Sq, 128, max_len) <= 8192 + (256 * 12 + B * Hkv * sets) * 16 * 130 * 4
     assert ws(256, 32, 8, 64, 128, 8192) == 4 * 256 * 8 * 8192 * 128  # 16 times: expanded
