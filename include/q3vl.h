@@ -646,6 +646,54 @@ int q3_flash_attention_cache_mxfp4(const void* q, const void* k_codes, const voi
                                    int64_t Sq, int64_t D, int64_t max_len, const int64_t* strides, float scale,
                                    int advance, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- eight-bit activations and weights (MXFP8)
+ * No counterpart in the reference (bf16 and fp32 only); for inference with products on the card's 8-bit matrix
+ * instructions. A row is cut into blocks of 32 consecutive values; a value is an 8-bit float (E4M3: up to 448, no
+ * infinities, NaN as 0x7f), a block has one power-of-two scale held as its exponent (E8M0: byte s stands for
+ * 2^(s - 127), 255 for NaN). Rows of codes (cols bytes) and of scales (cols / 32 bytes) are packed.
+ * Quantisation: the smallest scale, 2^-127 at least, that keeps the block's largest magnitude within 448; values over
+ * the scale round to the nearest, ties to even (sign kept, also of zeros); a block of zeros has s = 0, one with an
+ * infinity or a NaN s = 255 and codes 0 and reads as NaN.
+ *
+ * q3_mxfp8_quantize: x (rows, cols) with row stride ldx. cols a multiple of 32 (else Q3_ERR_SHAPE); x 16-byte aligned,
+ * ldx whole 16-byte pieces, codes 8-byte aligned.
+ * q3_mxfp8_dequantize: n values (a multiple of 32) of packed rows to y, of type dtype, rounded to it (exact in fp32; in
+ * bf16 for every value of 2^-133 or more, its smallest). codes 8-byte, y 16-byte aligned. */
+int q3_mxfp8_quantize(const void* x, void* codes, void* scales, int64_t rows, int64_t cols, int64_t ldx, int dtype,
+                      void* stream);
+int q3_mxfp8_dequantize(const void* codes, const void* scales, void* y, int64_t n, int dtype, void* stream);
+
+/* q3_residual_add, q3_rmsnorm and q3_mxfp8_quantize in one launch: sum = x + residual, rounded to dtype; y = rmsnorm(sum;
+ * weight, eps) in fp32, quantised from there (not rounded to dtype in between). x, residual, sum (rows, cols) with row
+ * strides ldx, ldr and cols; residual and sum may both be null: the norm of x. sum must not overlap x or residual.
+ * cols a multiple of 32 below 2^24; x, residual, weight, sum and their rows 16-byte aligned, codes 8-byte. */
+int q3_add_rmsnorm_mxfp8(const void* x, const void* residual, const void* weight, void* sum, void* codes, void* scales,
+                         int64_t rows, int64_t cols, int64_t ldx, int64_t ldr, float eps, int dtype, void* stream);
+
+/* y = act(x w^T (+ bias)) (+ residual), x (M, K) and w (N, K) in MXFP8, packed; fp32 accumulators, one rounding. act: 0
+ * none, 1 gelu_tanh, 2 silu. bias (N), residual (M, N; row stride ldr) bf16 or null. The output is y (M, N) bf16 with
+ * row stride ldc, or with y null, y_codes and y_scales: the fp32 values in MXFP8, packed (N a multiple of 32). K a
+ * multiple of 32 below 2^23; codes 16-byte aligned (y_codes 8-byte). The matrix instruction cuts the products of eight
+ * consecutive k 13 bits below the largest of them: a result is within 7 * 2^-13 of the sum of those largest ones.
+ * q3_matmul_segments_mxfp8: y (M, sum n_j) = x [w_0; w_1; ...]^T (+ [b_0; b_1; ...]), 1 to 4 weights of n[j] >= 1 rows;
+ * w_codes, w_scales and bias are host arrays of device pointers (bias, or any of its entries, may be null).
+ * q3_matmul_swiglu_mxfp8: silu(x g^T) * (x u^T), into y or y_codes and y_scales.
+ * Workspace: q3_matmul_mxfp8_workspace_bytes (n: the rows of each weight, one for SwiGLU); 16-byte aligned, needs no
+ * clearing, calls that may run at the same time must not share it. */
+int64_t q3_matmul_mxfp8_workspace_bytes(int64_t M, const int64_t* n, int64_t nseg, int64_t K, int swiglu);
+int q3_matmul_mxfp8(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales,
+                    const void* bias, const void* residual, void* y, void* y_codes, void* y_scales, int64_t M,
+                    int64_t N, int64_t K, int64_t ldr, int64_t ldc, int act, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+int q3_matmul_segments_mxfp8(const void* x_codes, const void* x_scales, const void* const* w_codes,
+                             const void* const* w_scales, const void* const* bias, const int64_t* n, int64_t nseg,
+                             void* y, int64_t M, int64_t K, int64_t ldc, void* workspace, int64_t workspace_bytes,
+                             void* stream);
+int q3_matmul_swiglu_mxfp8(const void* x_codes, const void* x_scales, const void* g_codes, const void* g_scales,
+                           const void* u_codes, const void* u_scales, void* y, void* y_codes, void* y_scales,
+                           int64_t M, int64_t N, int64_t K, int64_t ldc, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

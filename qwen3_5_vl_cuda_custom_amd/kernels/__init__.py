@@ -15,6 +15,8 @@ from .moe_routing import (cuda_batched_gemm, cuda_index_add, cuda_topk, moe_expe
                           moe_route, moe_router, raise_device_errors)
 from .mxfp4 import (decode_attention_mxfp4, flash_attention_cache_mxfp4, kv_append_mxfp4, matmul_mxfp4,
                     matmul_segments_mxfp4, matmul_swiglu_mxfp4, mxfp4_dequantize, mxfp4_quantize, qk_norm_rope_mxfp4)
+from .mxfp8 import (add_rmsnorm_mxfp8, matmul_mxfp8, matmul_segments_mxfp8, matmul_swiglu_mxfp8, mxfp8_dequantize,
+                    mxfp8_quantize)
 from .norms import layernorm, rmsnorm, softmax
 from .rotary import apply_mrope, apply_rope, qk_norm_rope, qk_norm_rope_paged
 from .vision import vision_pos_embed, vision_rope_tables
@@ -70,6 +72,12 @@ __all__ = [
     "qk_norm_rope_mxfp4",
     "decode_attention_mxfp4",
     "flash_attention_cache_mxfp4",
+    "mxfp8_quantize",
+    "mxfp8_dequantize",
+    "add_rmsnorm_mxfp8",
+    "matmul_mxfp8",
+    "matmul_segments_mxfp8",
+    "matmul_swiglu_mxfp8",
     "qk_norm_rope",
     "qk_norm_rope_paged",
     "qk_norm_rope_attention",
