@@ -1,5 +1,6 @@
 // Products of MXFP8 rows with MXFP8 weights: the entry points.
 #include "mxfp8.h"
+#include "mxfp8_tile.h"
 
 namespace {
 
@@ -21,7 +22,7 @@ int check(Call& c, const void* x_codes, const void* x_scales, const void* residu
   Q3_REQUIRE(!residual || ldr >= c.N, Q3_ERR_SHAPE);
   Q3_REQUIRE(act >= kMx8None && act <= kMx8Silu, Q3_ERR_UNSUPPORTED);
   Q3_REQUIRE(K < (1 << 23) && c.N < (1ll << 31) - 256 && M < (1ll << 31) - 256, Q3_ERR_UNSUPPORTED);
-  Q3_REQUIRE(q3_aligned(x_codes, 16) && (y || q3_aligned(y_codes, 8)), Q3_ERR_ALIGN);
+  Q3_REQUIRE(q3_aligned(x_codes, 16) && q3_aligned(x_scales, 4) && (y || q3_aligned(y_codes, 8)), Q3_ERR_ALIGN);
   a.x = static_cast<const uint8_t*>(x_codes);
   a.xs = static_cast<const uint8_t*>(x_scales);
   a.res = static_cast<const bf16*>(residual);
@@ -39,7 +40,7 @@ int check(Call& c, const void* x_codes, const void* x_scales, const void* residu
 int weight(Mx8Args& a, int j, const void* codes, const void* scales, const void* bias, int64_t n) {
   Q3_REQUIRE(codes && scales, Q3_ERR_NULL);
   Q3_REQUIRE(n >= 0 && n < (1ll << 31) - 256, Q3_ERR_SHAPE);
-  Q3_REQUIRE(q3_aligned(codes, 16), Q3_ERR_ALIGN);
+  Q3_REQUIRE(q3_aligned(codes, 16) && q3_aligned(scales, 4), Q3_ERR_ALIGN);
   a.w[j] = static_cast<const uint8_t*>(codes);
   a.ws[j] = static_cast<const uint8_t*>(scales);
   a.bias[j] = static_cast<const bf16*>(bias);
@@ -47,13 +48,18 @@ int weight(Mx8Args& a, int j, const void* codes, const void* scales, const void*
   return Q3_OK;
 }
 
-int64_t workspace_of(const Mx8Args& a, int64_t N, bool swiglu) { return 0; }
+// Rows of x up to which whole weight rows are taken (mxfp8_rows.hip).
+constexpr int kFewRows = 64;
+
+int64_t workspace_of(const Mx8Args& a, bool swiglu) { return a.M <= kFewRows ? 0 : mx8_tile_workspace(a, swiglu); }
 
 int launch(const Call& c, bool swiglu, void* workspace, int64_t workspace_bytes, void* stream) {
   if (c.a.M == 0 || c.N == 0) return Q3_OK;
-  const int64_t need = workspace_of(c.a, c.N, swiglu);
+  const int64_t need = workspace_of(c.a, swiglu);
   Q3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Q3_ERR_WORKSPACE);
-  return mx8_rows(c.a, swiglu, static_cast<hipStream_t>(stream));
+  Q3_REQUIRE(q3_aligned(workspace, 16), Q3_ERR_ALIGN);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return c.a.M <= kFewRows ? mx8_rows(c.a, swiglu, st) : mx8_tile(c.a, c.N, swiglu, workspace, st);
 }
 
 }  // namespace
@@ -73,7 +79,7 @@ int64_t q3_matmul_mxfp8_workspace_bytes(int64_t M, const int64_t* n, int64_t nse
   a.nseg = (int)nseg;
   a.M = (int)M;
   a.K = (int)K;
-  return workspace_of(a, N, swiglu != 0);
+  return workspace_of(a, swiglu != 0);
 }
 
 int q3_matmul_mxfp8(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales,

@@ -146,7 +146,6 @@ void launch_tiles(const Mx8Args& p, unsigned blocks, hipStream_t st) {
 namespace q3 {
 
 int mx8_rows(const Mx8Args& p, bool swiglu, hipStream_t st) {
-  Q3_REQUIRE(q3_cdiv(p.M, 64) <= 65535, Q3_ERR_UNSUPPORTED);
   auto blocks = [&](int rows) {
     int64_t n = 0;
     for (int j = 0; j < p.nseg; ++j) n += q3_cdiv(p.n[j], rows);

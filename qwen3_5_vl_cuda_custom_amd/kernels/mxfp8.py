@@ -47,8 +47,8 @@ def _packed(op: str, codes: torch.Tensor, scales: torch.Tensor, dev: int) -> Pai
         raise ValueError(f"{op}: codes {tuple(cs)} and scales {tuple(ss)} must be (..., K) and (..., K / 32)")
     if not codes.is_contiguous() or codes.data_ptr() % 16:
         codes = codes.clone(memory_format=torch.contiguous_format)
-    if not scales.is_contiguous():
-        scales = scales.contiguous()
+    if not scales.is_contiguous() or scales.data_ptr() % 4:
+        scales = scales.clone(memory_format=torch.contiguous_format)
     return codes, scales
 
 
