@@ -2,8 +2,7 @@
 // (format and matrix instruction: mxfp8.h).
 //
 // Codes go global -> LDS past the registers (buffer loads with the lds flag), a stage of
-// 128 k (one matrix instruction's) at a time, 128 bytes a row; scales, a word a row and
-// stage, the same way. Row r keeps its 16-byte chunk c at slot c ^ (r & 7) ^ (r >> 3 & 1),
+// 128 k (one matrix instruction's) at a time, 128 bytes a row. Row r keeps its 16-byte chunk c at slot c ^ (r & 7) ^ (r >> 3 & 1),
 // so the 16 rows of a fragment read use all banks. A wave holds the stage's TN weight
 // fragments and takes the TM fragments of x (columns, below) one after the other, each
 // read three columns ahead, TN products to a column. Before the last two columns every
@@ -14,6 +13,12 @@
 // With two slots (256 x 256 tiles fill the LDS) a stage's weight slot is free once every
 // wave has the fragments, after the first column: a second barrier there lets the weights
 // after next, which come from further away than x, set out most of a stage earlier.
+//
+// Scales are laid out anew first, by a kernel of their own: the scales of 64 rows and four
+// stages are 1 KB as the instruction's lanes take them, word l of a stage lane l's block
+// of rows l % 16, + 16, + 32, + 48 (the instruction picks the byte). A load brings a stage
+// of them, and three words a stage are all that a wave reads. As rows of bytes their loads
+// cost a line per row and the reads twelve bytes a stage.
 #include <algorithm>
 
 #include "gemm_tile.h"
@@ -26,7 +31,8 @@ using namespace q3;
 
 struct TileArgs {
   Mx8Args a;
-  int64_t slx, slw;  // bytes between rows of scales: whole words
+  const uint8_t* xs;                // scales of x, and of each weight (SwiGLU: of both), laid out as above
+  const uint8_t* ws[kMx8Segments];
   int N;             // columns of y
   int tiles_m, tiles_n;
   int kt;            // stages of a block
@@ -94,16 +100,27 @@ __device__ __forceinline__ bool vec_of(const Mx8Args& p, int col0) {
          (!p.res || (p.ldr % 8 == 0 && (reinterpret_cast<uintptr_t>(p.res) & 15) == 0));
 }
 
+// The product with byte bi and bj of the scale words.
+__device__ __forceinline__ floatx4 mfma_of(i32x8 a, i32x8 b, floatx4 c, int sa, int sb, int bi, int bj) {
+#define Q3_MX8_MFMA(I, J) \
+  if (bi == I && bj == J) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, I, sa, J, sb);
+#define Q3_MX8_ROW(I) Q3_MX8_MFMA(I, 0) Q3_MX8_MFMA(I, 1) Q3_MX8_MFMA(I, 2) Q3_MX8_MFMA(I, 3)
+  Q3_MX8_ROW(0) Q3_MX8_ROW(1) Q3_MX8_ROW(2) Q3_MX8_ROW(3)
+#undef Q3_MX8_ROW
+#undef Q3_MX8_MFMA
+  return c;
+}
+
 template <int BM, int BN, int WM, int WN, int NS, bool SW>
 __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t) {
   constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
   constexpr int BN_OUT = SW ? BN / 2 : BN;
-  constexpr int PX = BM / 8 / NW, PW = BN / 8 / NW, PS = ((BM + BN) / 64 + NW - 1) / NW;  // loads per wave and stage
+  constexpr int GX = BM / 64, GS = (BM + BN) / 64, PS = (GS + NW - 1) / NW;  // groups of 64 rows; loads of scales
+  constexpr int PX = BM / 8 / NW, PW = BN / 8 / NW;                          // loads of codes per wave and stage
   constexpr bool EARLY = NS == 2;  // the weights' slot is released by a barrier of its own
-  constexpr int NSS = NS + 2;      // slots of scales
-  constexpr int kX = BM * 128, kW = BN * 128, kS = PS * NW * 256, kLds = NS * (kX + kW) + NSS * kS;
+  constexpr int kX = BM * 128, kW = BN * 128, kS = PS * NW * 256, kLds = NS * (kX + kW) + 4 * kS;
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NW % 2 == 0, "whole loads per wave, one swizzle per lane");
-  static_assert(TM % 4 == 0 && WTN % (SW ? 64 : 16) == 0 && kLds <= 160 * 1024, "wave tiles");
+  static_assert(TM % 4 == 0 && TN == 4 && kLds <= 160 * 1024, "wave tiles");
   __shared__ __attribute__((aligned(1024))) char smem[kLds];
 
   const Mx8Args& p = t.a;
@@ -125,12 +142,11 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
   seg = pin(seg), tn = pin(tn), col0 = pin(col0);
   const int n0 = tn * BN_OUT, rows_n = pin(min(BN_OUT, p.n[seg] - n0)), rows_m = pin(min(BM, p.M - m0));
   const int k_first = blockIdx.z * t.kt, nk = min(t.kt, (K + 127) / 128 - k_first);  // stages
+  const int groups_k = (K + 511) / 512;  // of four stages
 
   const __amdgpu_buffer_rsrc_t rx = make_rsrc(pin(p.x + (int64_t)m0 * K), rows_m * K);
   const uint8_t* const wa = pin(p.w[SW ? 0 : seg] + (int64_t)n0 * K);  // SwiGLU: gate's, and up's
   const uint8_t* const wb = SW ? pin(p.w[1] + (int64_t)n0 * K) : wa;
-  const uint8_t* const sa = pin(p.ws[SW ? 0 : seg] + n0 * t.slw);
-  const uint8_t* const sb = SW ? pin(p.ws[1] + n0 * t.slw) : sa;
   auto swz = [](int r) { return (r & 7) ^ ((r >> 3) & 1); };
   // Load i of this wave fills rows 8 (wave + NW i) .. + 7 of the tile.
   const int lrow = lane >> 3, dc = (lane & 7) ^ swz(wave * 8 + lrow);
@@ -142,18 +158,18 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
     const int r = (wave + NW * i) * 8 + lrow;
     woff[i] = (uint32_t)((SW ? (r >> 6) * 32 + (r & 31) : r) * K);  // SwiGLU: 32 gate rows, the same 32 up rows, ...
   }
-  // Scales: load s of this wave is the rows 64 (wave + NW s) .. + 63 of x, then of the weights (SwiGLU: of gate, of up).
-  uint32_t soff[PS];
+  // Scales: load s of this wave is a stage of 64 rows, x's and then the weights'.
   const uint8_t* sp[PS];
   int sbytes[PS];
 #pragma unroll
   for (int s = 0; s < PS; ++s) {
-    const int e = (wave + NW * s) * 64;
-    const bool of_x = e < BM, up = SW && e - BM >= BN_OUT;
-    const int row = (of_x ? e : up ? e - BM - BN_OUT : e - BM) + lane;
-    sp[s] = pin(of_x ? p.xs + m0 * t.slx : up ? sb : sa);
-    sbytes[s] = pin(of_x ? rows_m * (int)t.slx : rows_n * (int)t.slw);
-    soff[s] = e < BM + BN ? (uint32_t)(row * (int)(of_x ? t.slx : t.slw)) : kOOB;
+    const int e = wave + NW * s;
+    const bool of_x = e < GX;
+    const int g = of_x ? m0 / 64 + e : (SW ? 2 * n0 : n0) / 64 + e - GX;
+    // 64-row groups that exist: of all rows, SwiGLU 32 of each weight to a group
+    const int all = of_x ? (p.M + 63) / 64 : SW ? (p.n[0] + 31) / 32 : (p.n[seg] + 63) / 64;
+    sp[s] = pin((of_x ? t.xs : t.ws[seg]) + (int64_t)g * groups_k * 1024);
+    sbytes[s] = pin(e < GS && g < all ? groups_k * 1024 : 0);
   }
   const uint32_t lbase = lds_addr(smem);
   constexpr int kW0 = NS * kX, kS0 = kW0 + NS * kW;
@@ -168,13 +184,14 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
   };
   auto dma_w = [&](int kt, int i) {
     const bool up = SW && ((wave + NW * i) & 4);
-    dma16(make_rsrc(SW ? pin(up ? wb : wa) : wa, rows_n * K), woff[i] + kofs(kt), lbase + (uint32_t)(kW0 + kt % NS * kW + (wave + NW * i) * 1024));
+    dma16(make_rsrc(SW ? pin(up ? wb : wa) : wa, rows_n * K), woff[i] + kofs(kt),
+          lbase + (uint32_t)(kW0 + kt % NS * kW + (wave + NW * i) * 1024));
   };
   auto dma_s = [&](int kt, int s) {
-    dma4(make_rsrc(sp[s], sbytes[s]), kt < nk && soff[s] != kOOB ? soff[s] + (uint32_t)(k_first + kt) * 4 : kOOB,
-         lbase + (uint32_t)(kS0 + kt % NSS * kS + (wave + NW * s) * 256));
+    dma4(make_rsrc(sp[s], sbytes[s]), kt < nk ? (uint32_t)((k_first + kt) * 256 + lane * 4) : kOOB,
+         lbase + (uint32_t)(kS0 + (kt & 3) * kS + (wave + NW * s) * 256));
   };
-  // d-th load of what is issued in the columns before the stage barrier: scales, weights (and with more slots x)
+  // d-th load of what is issued in the columns before the stage barrier: scales, weights (and with more slots x).
   constexpr int ND = PS + PW + (EARLY ? 0 : PX);
   auto dma = [&](int kt, int d) {
     if (d < PS) dma_s(kt, d);
@@ -188,7 +205,7 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
 #pragma unroll
     for (int j = 0; j < TM; ++j) acc[i][j] = floatx4{};
   i32x8 fw[TN], fx[4];
-  int sw[TN], sx[4];
+  int sw, sx[TM / 4], sw_next, sx_next[TM / 4];  // a stage's words of scales
   const int rn = wn * WTN, rm = wm * WTM;
   auto frag = [&](const char* slot, int r) {
     const char* row = slot + r * 128;
@@ -196,19 +213,23 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
     const i32x4 hi = *reinterpret_cast<const i32x4*>(row + (((4 + q4) ^ swz(r)) << 4));
     return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
-  auto rd_w = [&](int kt, int i) {
-    const int r = rn + 16 * i + l16, e = SW ? (r >> 5 & 1) * BN_OUT + (r >> 6) * 32 + (r & 31) : r;
-    fw[i] = frag(smem + kW0 + kt % NS * kW, r);
-    sw[i] = *reinterpret_cast<const uint8_t*>(smem + kS0 + kt % NSS * kS + (BM + e) * 4 + q4);
+  auto rd_w = [&](int kt, int i) { fw[i] = frag(smem + kW0 + kt % NS * kW, rn + 16 * i + l16); };
+  auto rd_x = [&](int kt, int j) { fx[j & 3] = frag(smem + kt % NS * kX, rm + 16 * j + l16); };
+  auto rd_s = [&](int kt) {
+    const char* s = smem + kS0 + (kt & 3) * kS + lane * 4;
+    sw_next = *reinterpret_cast<const int*>(s + (GX + rn / 64) * 256);
+#pragma unroll
+    for (int g = 0; g < TM / 4; ++g) sx_next[g] = *reinterpret_cast<const int*>(s + (rm / 64 + g) * 256);
   };
-  auto rd_x = [&](int kt, int j) {
-    const int r = rm + 16 * j + l16;
-    fx[j & 3] = frag(smem + kt % NS * kX, r);
-    sx[j & 3] = *reinterpret_cast<const uint8_t*>(smem + kS0 + kt % NSS * kS + r * 4 + q4);
+  auto take_s = [&]() {
+    sw = sw_next;
+#pragma unroll
+    for (int g = 0; g < TM / 4; ++g) sx[g] = sx_next[g];
   };
-  auto mf = [&](int i, int j) { acc[i][j] = mfma_mx8(fw[i], fx[j & 3], acc[i][j], sw[i], sx[j & 3]); };
+  auto mf = [&](int i, int j) { acc[i][j] = mfma_of(fw[i], fx[j & 3], acc[i][j], sw, sx[j / 4], i, j & 3); };
 
   constexpr int kAhead = EARLY ? 2 : NS - 1;  // stages issued before the loop
+  constexpr int kAll = PX + PW + PS;
 #pragma unroll
   for (int s = 0; s < kAhead; ++s) {
 #pragma unroll
@@ -218,12 +239,14 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
       for (int i = 0; i < PX; ++i) dma_x(s, i);
     }
   }
-  vm_wait<(kAhead - 1) * (PX + PW + PS)>();  // stage 0 has landed
+  vm_wait<(kAhead - 1) * kAll>();  // stage 0 has landed
   __syncthreads();
 
   auto main = [&](auto active_c) {
     constexpr bool A = decltype(active_c)::value;  // a wave without rows loads and waits only
     if constexpr (A) {
+      rd_s(0);
+      take_s();
 #pragma unroll
       for (int i = 0; i < TN; ++i) rd_w(0, i);
 #pragma unroll
@@ -246,15 +269,19 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
           if (at >= 0 && at % gap == gap - 1 && d < ND) dma(next, d++);
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (EARLY && j == 0) asm volatile("s_barrier" ::: "memory");  // every wave holds the weights' fragments
+        if (EARLY && j == 0) {  // every wave holds the weights' fragments (read before the last one of x)
+          asm volatile("s_waitcnt lgkmcnt(2)\n\ts_barrier" ::: "memory");
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
 #pragma unroll
       for (; d < ND; ++d) dma(next, d);
-      // Stage kt + 1 has landed and every fragment of stage kt is in registers, in every wave.
-      vm_wait<EARLY ? PS + PW : (NS - 2) * (PX + PW + PS)>();
+      // Stage kt + 1 has landed (later ones may not have) and every fragment of stage kt is in registers, in every wave.
+      vm_wait<EARLY ? PS + PW : (NS - 2) * kAll>();
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (A) {
+        rd_s(kt + 1);
         rd_x(kt + 1, 0);
         rd_x(kt + 1, 1);
         __builtin_amdgcn_sched_barrier(0);
@@ -267,6 +294,7 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
           __builtin_amdgcn_sched_barrier(0);
         }
         rd_x(kt + 1, 2);
+        take_s();
       }
       if constexpr (EARLY) {
 #pragma unroll
@@ -329,25 +357,51 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
   }
 }
 
-// Rows of scales copied to whole words, zeros behind: x's, then each weight's.
-struct PadArgs {
-  const uint8_t* s[1 + kMx8Segments];
-  int64_t rows[1 + kMx8Segments];
-  uint8_t* out;
-  int kb, ld;
+// Scales of 64 rows and four stages as the kernel above takes them (the file's head), zeros past the last row and block;
+// SwiGLU: 32 rows of gate, then the same of up. A block lays out 64 rows of 16 stages.
+struct LayArgs {
+  const uint8_t *s[1 + kMx8Segments], *s2;  // x's, each weight's (rows, kb); up's
+  int rows[1 + kMx8Segments], first[1 + kMx8Segments];  // of each; the first block of each
+  uint8_t* out[1 + kMx8Segments];
+  int kb, groups_k, nb, mats;  // blocks of 32 k, groups of four stages, blocks along k, matrices
 };
-__global__ __launch_bounds__(256) void mx8_pad_scales_kernel(const PadArgs a) {
-  const int j = blockIdx.y;
-  uint8_t* out = a.out;
-  const uint8_t* s = a.s[0];
-  int64_t rows = a.rows[0];
+__global__ __launch_bounds__(256) void mx8_lay_scales_kernel(const LayArgs a) {
+  __shared__ uint8_t tile[64][64 + 4];
+  int j = 0;
 #pragma unroll
   for (int u = 1; u <= kMx8Segments; ++u)
-    if (j >= u) out += rows * a.ld, s = a.s[u], rows = a.rows[u];
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * a.ld; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / a.ld;
-    const int b = (int)(i - r * a.ld);
-    out[i] = b < a.kb ? s[r * a.kb + b] : 0;
+    if (u < a.mats && (int)blockIdx.x >= a.first[u]) j = u;
+  const int at = blockIdx.x - a.first[j], g = at / a.nb, b0 = at % a.nb * 64;  // 64-row group, first block of k
+  const bool pair = j == 1 && a.s2;
+  const int tid = threadIdx.x, r = tid >> 2, b = tid & 3;
+  const int row = pair ? g * 32 + (r & 31) : g * 64 + r;
+  const uint8_t* src = (pair && r >= 32 ? a.s2 : a.s[j]) + (int64_t)row * a.kb;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {  // four bytes at 4 (b + 4 i)
+    const int c = 4 * (b + 4 * i);
+    uint32_t v = 0;
+    if (row < a.rows[j]) {
+      if (a.kb % 4 == 0) {
+        if (b0 + c < a.kb) v = *reinterpret_cast<const uint32_t*>(src + b0 + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (b0 + c + e < a.kb) v |= (uint32_t)src[b0 + c + e] << (8 * e);
+      }
+    }
+    *reinterpret_cast<uint32_t*>(&tile[r][c]) = v;
+  }
+  __syncthreads();
+  // Word (stage, lane): blocks 4 stage + lane / 16 of rows lane % 16 + 16 e.
+  uint32_t* out = reinterpret_cast<uint32_t*>(a.out[j]) + ((int64_t)g * a.groups_k + b0 / 16) * 256;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int w = tid + 256 * i, stage = w >> 6, lane = w & 63;
+    if (b0 / 16 + stage / 4 >= a.groups_k) break;
+    uint32_t v = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v |= (uint32_t)tile[(lane & 15) + 16 * e][4 * stage + (lane >> 4)] << (8 * e);
+    out[w] = v;
   }
 }
 
@@ -372,57 +426,55 @@ void launch_form(const TileArgs& t, int form, int splits, hipStream_t st) {
   else launch_tile<128, 128, 2, 2, 2, SW>(t, splits, st);
 }
 
-struct Plan {
-  int form;
-  bool pad;
-};
-Plan plan_of(const Mx8Args& a, bool swiglu) {
-  Plan p;
-  p.pad = a.K % 128 != 0;
+int form_of(const Mx8Args& a, bool swiglu) {
   const int out = swiglu ? 2 : 1;
-  p.form = q3_cdiv(a.M, 256) * tiles_of(a, 256 / out) >= 200 ? 0 : q3_cdiv(a.M, 128) * tiles_of(a, 256 / out) >= 200 ? 1 : 2;
-  return p;
+  return q3_cdiv(a.M, 256) * tiles_of(a, 256 / out) >= 200 ? 0 : q3_cdiv(a.M, 128) * tiles_of(a, 256 / out) >= 200 ? 1 : 2;
 }
+
+// Bytes of laid out scales of n rows.
+int64_t laid_bytes(int64_t n, int64_t K) { return q3_cdiv(n, 64) * q3_cdiv(K, 512) * 1024; }
 
 }  // namespace
 
 namespace q3 {
 
 int64_t mx8_tile_workspace(const Mx8Args& a, bool swiglu) {
-  const Plan plan = plan_of(a, swiglu);
-  if (!plan.pad) return 0;
-  int64_t rows = a.M;
-  for (int j = 0; j < (swiglu ? 2 : a.nseg); ++j) rows += a.n[swiglu ? 0 : j];
-  return rows * (q3_cdiv(a.K, 128) * 4);
+  int64_t bytes = laid_bytes(a.M, a.K);
+  if (swiglu) return bytes + laid_bytes(2 * q3_cdiv(a.n[0], 32) * 32, a.K);
+  for (int j = 0; j < a.nseg; ++j) bytes += laid_bytes(a.n[j], a.K);
+  return bytes;
 }
 
 int mx8_tile(const Mx8Args& a, int64_t N, bool swiglu, void* workspace, hipStream_t st) {
-  const Plan plan = plan_of(a, swiglu);
   TileArgs t{};
   t.a = a;
   t.N = (int)N;
   t.kt = (int)q3_cdiv(a.K, 128);
-  t.slx = t.slw = a.K / kMx8Block;
-  if (plan.pad) {
-    PadArgs p{};
-    p.kb = a.K / kMx8Block;
-    p.ld = 4 * t.kt;
-    p.out = static_cast<uint8_t*>(workspace);
-    uint8_t* out = p.out;
-    const int weights = swiglu ? 2 : a.nseg;
-    for (int j = -1; j < weights; ++j) {
-      const int64_t rows = j < 0 ? a.M : a.n[swiglu ? 0 : j];
-      p.s[j + 1] = j < 0 ? a.xs : a.ws[j];
-      p.rows[j + 1] = rows;
-      (j < 0 ? t.a.xs : t.a.ws[j]) = out;
-      out += rows * p.ld;
-    }
-    hipLaunchKernelGGL(mx8_pad_scales_kernel, dim3(256, 1 + weights), dim3(256), 0, st, p);
-    Q3_LAUNCH_CHECK();
-    t.slx = t.slw = p.ld;
+
+  LayArgs l{};
+  l.kb = a.K / kMx8Block;
+  l.groups_k = (int)q3_cdiv(a.K, 512);
+  l.nb = (int)q3_cdiv(l.kb, 64);
+  l.mats = 1 + a.nseg;
+  l.s2 = swiglu ? a.ws[1] : nullptr;
+  uint8_t* out = static_cast<uint8_t*>(workspace);
+  int64_t blocks = 0;
+  for (int j = 0; j < l.mats; ++j) {
+    l.s[j] = j ? a.ws[j - 1] : a.xs;
+    l.rows[j] = j ? a.n[j - 1] : a.M;
+    l.first[j] = (int)blocks;
+    l.out[j] = out;
+    (j ? t.ws[j - 1] : t.xs) = out;
+    const int64_t groups = j && swiglu ? q3_cdiv(l.rows[j], 32) : q3_cdiv(l.rows[j], 64);
+    blocks += groups * l.nb;
+    out += groups * l.groups_k * 1024;
   }
-  if (swiglu) launch_form<true>(t, plan.form, 1, st);
-  else launch_form<false>(t, plan.form, 1, st);
+  Q3_REQUIRE(blocks < (1ll << 31), Q3_ERR_UNSUPPORTED);
+  hipLaunchKernelGGL(mx8_lay_scales_kernel, dim3((unsigned)blocks), dim3(256), 0, st, l);
+  Q3_LAUNCH_CHECK();
+  const int form = form_of(a, swiglu);
+  if (swiglu) launch_form<true>(t, form, 1, st);
+  else launch_form<false>(t, form, 1, st);
   Q3_LAUNCH_CHECK();
   return Q3_OK;
 }
