@@ -2,13 +2,15 @@
 // (format and matrix instruction: mxfp8.h).
 //
 // Codes go global -> LDS past the registers (buffer loads with the lds flag), a stage of
-// 128 k (one matrix instruction's) at a time, 128 bytes a row. Row r keeps its 16-byte chunk c at slot c ^ (r & 7) ^ (r >> 3 & 1),
-// so the 16 rows of a fragment read use all banks. A wave holds the stage's TN weight
-// fragments and takes the TM fragments of x (columns, below) one after the other, each
-// read three columns ahead, TN products to a column. Before the last two columns every
-// fragment of the stage has been read: there the stage barrier stands, the next stage's
-// fragments are read between the products after it, each weight fragment once its last
-// product has issued.
+// 128 k (one matrix instruction's) at a time, 128 bytes a row. Row r keeps its 16-byte
+// chunk c at slot c ^ (r & 7), which leaves the fragments' reads without bank conflicts
+// (with r >> 3 in the exclusive or as well, 3.5 cycles each were counted). A wave holds the
+// stage's TN weight fragments and takes the TM fragments of x (columns, below) one after
+// the other, each read three columns ahead, TN products to a column. Before the last two
+// columns every fragment of the stage has been read: there the stage barrier stands, the
+// next stage's fragments are read between the products after it, each weight fragment once
+// its last product has issued. No branch stands in the loop: the compiler moves products
+// past one.
 //
 // With two slots (256 x 256 tiles fill the LDS) a stage's weight slot is free once every
 // wave has the fragments, after the first column: a second barrier there lets the weights
@@ -147,7 +149,7 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
   const __amdgpu_buffer_rsrc_t rx = make_rsrc(pin(p.x + (int64_t)m0 * K), rows_m * K);
   const uint8_t* const wa = pin(p.w[SW ? 0 : seg] + (int64_t)n0 * K);  // SwiGLU: gate's, and up's
   const uint8_t* const wb = SW ? pin(p.w[1] + (int64_t)n0 * K) : wa;
-  auto swz = [](int r) { return (r & 7) ^ ((r >> 3) & 1); };
+  auto swz = [](int r) { return r & 7; };
   // Load i of this wave fills rows 8 (wave + NW i) .. + 7 of the tile.
   const int lrow = lane >> 3, dc = (lane & 7) ^ swz(wave * 8 + lrow);
   uint32_t xoff[PX], woff[PW];
@@ -251,6 +253,8 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
       for (int i = 0; i < TN; ++i) rd_w(0, i);
 #pragma unroll
       for (int j = 0; j < 3; ++j) rd_x(0, j);
+      // Nothing is left under way here, so that the loop's waits are counted from its own loads (lgkmcnt 0).
+      __builtin_amdgcn_s_waitcnt(0xc07f);
     }
     for (int kt = 0; kt < nk; ++kt) {
       const int next = kt + kAhead;  // the stage whose loads go out
@@ -358,50 +362,80 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
 }
 
 // Scales of 64 rows and four stages as the kernel above takes them (the file's head), zeros past the last row and block;
-// SwiGLU: 32 rows of gate, then the same of up. A block lays out 64 rows of 16 stages.
+// SwiGLU: 32 rows of gate, then the same of up. A wave lays out 64 rows of 16 stages: lane l holds 16 bytes of row l at a
+// time, and the words of four stages are a transposition between the lanes l % 16 + 16 e and the bytes.
 struct LayArgs {
   const uint8_t *s[1 + kMx8Segments], *s2;  // x's, each weight's (rows, kb); up's
-  int rows[1 + kMx8Segments], first[1 + kMx8Segments];  // of each; the first block of each
+  int rows[1 + kMx8Segments], first[1 + kMx8Segments];  // of each; the first wave of each
   uint8_t* out[1 + kMx8Segments];
-  int kb, groups_k, nb, mats;  // blocks of 32 k, groups of four stages, blocks along k, matrices
+  int kb, groups_k, nb, mats, waves;  // blocks of 32 k, groups of four stages, waves along k, matrices
 };
+
+// Words s of lane l, row l's four stages, to words s: byte e that of block l / 16 of row 16 e + l % 16.
+__device__ __forceinline__ void mx8_turn(uint32_t (&w)[4]) {
+  // 4 x 4 bytes: words s, bytes q to words q, bytes s; and back
+  auto bytes = [](uint32_t (&v)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u), b = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);
+    const uint32_t c = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u), d = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
+    v[0] = __builtin_amdgcn_perm(c, a, 0x05040100u), v[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    v[2] = __builtin_amdgcn_perm(d, b, 0x05040100u), v[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+  };
+  bytes(w);
+  // words q of the lanes 16 e + .. to words e of the lanes 16 q + ..
+  const auto p = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), q = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+  const auto u = __builtin_amdgcn_permlane16_swap(p[0], q[0], false, false), v = __builtin_amdgcn_permlane16_swap(p[1], q[1], false, false);
+  w[0] = u[0], w[1] = u[1], w[2] = v[0], w[3] = v[1];
+  bytes(w);
+}
+
 __global__ __launch_bounds__(256) void mx8_lay_scales_kernel(const LayArgs a) {
-  __shared__ uint8_t tile[64][64 + 4];
+  const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6))), lane = threadIdx.x & 63;
+  if (wave >= a.waves) return;
   int j = 0;
 #pragma unroll
   for (int u = 1; u <= kMx8Segments; ++u)
-    if (u < a.mats && (int)blockIdx.x >= a.first[u]) j = u;
-  const int at = blockIdx.x - a.first[j], g = at / a.nb, b0 = at % a.nb * 64;  // 64-row group, first block of k
+    if (u < a.mats && wave >= a.first[u]) j = u;
+  const int at = wave - a.first[j], g = at / a.nb, g0 = at % a.nb * 4;  // 64 rows, first group of four stages
   const bool pair = j == 1 && a.s2;
-  const int tid = threadIdx.x, r = tid >> 2, b = tid & 3;
-  const int row = pair ? g * 32 + (r & 31) : g * 64 + r;
-  const uint8_t* src = (pair && r >= 32 ? a.s2 : a.s[j]) + (int64_t)row * a.kb;
+  const int row = pair ? g * 32 + (lane & 31) : g * 64 + lane;
+  // Every address lies in the matrix; what is past its rows or a row's end becomes zero after the loads.
+  const uint8_t* src = (pair && lane >= 32 ? a.s2 : a.s[j]) + (int64_t)min(row, a.rows[j] - 1) * a.kb;
+  const int end = row < a.rows[j] ? a.kb : 0, c0 = g0 * 16;
+  uint32_t w[4][4];
+  if (a.kb % 16 == 0) {
+    typedef uint32_t words __attribute__((ext_vector_type(4), aligned(4)));
+    words v[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {  // four bytes at 4 (b + 4 i)
-    const int c = 4 * (b + 4 * i);
-    uint32_t v = 0;
-    if (row < a.rows[j]) {
-      if (a.kb % 4 == 0) {
-        if (b0 + c < a.kb) v = *reinterpret_cast<const uint32_t*>(src + b0 + c);
-      } else {
+    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const words*>(src + min(c0 + 16 * i, a.kb - 16));
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (b0 + c + e < a.kb) v |= (uint32_t)src[b0 + c + e] << (8 * e);
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) w[i][s] = c0 + 16 * i < end ? v[i][s] : 0;
+  } else if (a.kb % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i / 4][i % 4] = *reinterpret_cast<const uint32_t*>(src + min(c0 + 4 * i, a.kb - 4));
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (c0 + 4 * i >= end) w[i / 4][i % 4] = 0;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      w[i / 4][i % 4] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = c0 + 4 * i + e;
+        const uint32_t v = src[min(c, a.kb - 1)];
+        w[i / 4][i % 4] |= c < end ? v << (8 * e) : 0;
       }
     }
-    *reinterpret_cast<uint32_t*>(&tile[r][c]) = v;
   }
-  __syncthreads();
-  // Word (stage, lane): blocks 4 stage + lane / 16 of rows lane % 16 + 16 e.
-  uint32_t* out = reinterpret_cast<uint32_t*>(a.out[j]) + ((int64_t)g * a.groups_k + b0 / 16) * 256;
+  uint32_t* out = reinterpret_cast<uint32_t*>(a.out[j]) + ((int64_t)g * a.groups_k + g0) * 256 + lane;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int w = tid + 256 * i, stage = w >> 6, lane = w & 63;
-    if (b0 / 16 + stage / 4 >= a.groups_k) break;
-    uint32_t v = 0;
+    if (g0 + i >= a.groups_k) break;
+    mx8_turn(w[i]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v |= (uint32_t)tile[(lane & 15) + 16 * e][4 * stage + (lane >> 4)] << (8 * e);
-    out[w] = v;
+    for (int s = 0; s < 4; ++s) out[i * 256 + s * 64] = w[i][s];
   }
 }
 
@@ -454,23 +488,24 @@ int mx8_tile(const Mx8Args& a, int64_t N, bool swiglu, void* workspace, hipStrea
   LayArgs l{};
   l.kb = a.K / kMx8Block;
   l.groups_k = (int)q3_cdiv(a.K, 512);
-  l.nb = (int)q3_cdiv(l.kb, 64);
+  l.nb = (int)q3_cdiv(l.groups_k, 4);
   l.mats = 1 + a.nseg;
   l.s2 = swiglu ? a.ws[1] : nullptr;
   uint8_t* out = static_cast<uint8_t*>(workspace);
-  int64_t blocks = 0;
+  int64_t waves = 0;
   for (int j = 0; j < l.mats; ++j) {
     l.s[j] = j ? a.ws[j - 1] : a.xs;
     l.rows[j] = j ? a.n[j - 1] : a.M;
-    l.first[j] = (int)blocks;
+    l.first[j] = (int)waves;
     l.out[j] = out;
     (j ? t.ws[j - 1] : t.xs) = out;
     const int64_t groups = j && swiglu ? q3_cdiv(l.rows[j], 32) : q3_cdiv(l.rows[j], 64);
-    blocks += groups * l.nb;
+    waves += groups * l.nb;
     out += groups * l.groups_k * 1024;
   }
-  Q3_REQUIRE(blocks < (1ll << 31), Q3_ERR_UNSUPPORTED);
-  hipLaunchKernelGGL(mx8_lay_scales_kernel, dim3((unsigned)blocks), dim3(256), 0, st, l);
+  Q3_REQUIRE(waves < (1ll << 31) - 4, Q3_ERR_UNSUPPORTED);
+  l.waves = (int)waves;
+  hipLaunchKernelGGL(mx8_lay_scales_kernel, dim3((unsigned)q3_cdiv(waves, 4)), dim3(256), 0, st, l);
   Q3_LAUNCH_CHECK();
   const int form = form_of(a, swiglu);
   if (swiglu) launch_form<true>(t, form, 1, st);
