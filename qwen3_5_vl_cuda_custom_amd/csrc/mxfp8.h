@@ -123,6 +123,8 @@ struct Mx8Args {
   uint8_t *yc, *ys;                          // the output in eight bits, packed
   int M, K, act;
   int64_t ldr, ldc;
+  // set by mx8_rows
+  int r, vec;  // weight rows of a block; whether y and the residual go in 8-byte pieces
 };
 
 // The epilogue of an output value: activation of product + bias.

@@ -4,10 +4,9 @@
 // over one weight, or the weights of several projections side by side; y in bf16 or in
 // eight bits again.
 //
-// A block owns 16 or 32 weight rows and all of k, so no sums pass between blocks: its
-// four waves take every fourth 128 k each and their sums meet in LDS, in wave order. The
-// weight is the instruction's first operand, so lane l holds columns 4 (l / 16) .. + 3 of
-// y's row l % 16.
+// A block owns whole weight rows, all of k, so no sums pass between blocks: its four waves
+// take a quarter of the k each and their sums meet in LDS, in wave order. The weight is the
+// instruction's first operand, so lane l holds columns 4 (l / 16) .. + 3 of y's row l % 16.
 #include "gemm_tile.h"
 #include "mxfp8.h"
 
@@ -17,6 +16,90 @@ using namespace q3;
 
 constexpr int kWaves = 4;
 
+// The block's sums (wave, group, tile of x; lane l: columns 4 (l / 16) .. + 3 of y's row l % 16), joined in wave order,
+// finished and stored: rows [m0, m0 + M) of y, `rows` columns from n0 of weight seg, which starts at column col0. Four
+// columns of a row per lane; the eight lanes of 32 columns are neighbours.
+template <int RG, int MT, bool SW>
+__device__ __forceinline__ void finish_block(const Mx8Args& p, const floatx4* sums, int seg, int m0, int M, int n0, int rows,
+                                             int col0) {
+  constexpr int RGT = SW ? 2 * RG : RG;
+  for (int it = threadIdx.x; it < RG * MT * 64; it += 64 * kWaves) {
+    const int m = it / (4 * RG), c = it % (4 * RG), at = (m & 15) + 16 * (c & 3);
+    if (m >= M || 4 * c >= rows) continue;
+    auto total = [&](int g) {
+      floatx4 v = sums[(g * MT + m / 16) * 64 + at];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) v += sums[((w * RGT + g) * MT + m / 16) * 64 + at];
+      return v;
+    };
+    floatx4 v = total(c / 4);
+    if constexpr (SW) {
+      const floatx4 u = total(RG + c / 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = silu_mul(v[e], u[e]);
+    }
+    const int left = rows - 4 * c, n = n0 + 4 * c, col = col0 + n;
+    const int64_t row = m0 + m;
+    const bool vec = p.vec && left >= 4;  // whole 8-byte pieces
+    if (!SW) {
+      if (const bf16* b = p.bias[seg]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < left) v[e] += bf2f(b[n + e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = mx8_act(v[e], p.act);
+    }
+    if (p.res) {
+      const bf16* r = p.res + row * p.ldr + col;
+      if (vec) {
+        const bf16x4 b = *reinterpret_cast<const bf16x4*>(r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += bf2f(b[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < left) v[e] += bf2f(r[e]);
+      }
+    }
+    if (p.yc) {  // the columns are whole blocks
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, mx8_magnitude(v[e]));
+#pragma unroll
+      for (int o = 1; o < 8; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+      const uint32_t byte = mx8_scale_byte(top);
+      const uint32_t codes = byte == 255 ? 0 : mx8_pack4(v[0], v[1], v[2], v[3], mx8_scale(byte));
+      *reinterpret_cast<uint32_t*>(p.yc + row * p.ldc + col) = codes;
+      if ((c & 7) == 0) p.ys[row * (p.ldc / kMx8Block) + col / kMx8Block] = (uint8_t)byte;
+    } else {
+      bf16* y = p.y + row * p.ldc + col;
+      if (vec) {
+        *reinterpret_cast<bf16x4*>(y) = bf16x4{f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < left) y[e] = f2bf(v[e]);
+      }
+    }
+  }
+}
+
+// Weight and block of it that block b of the grid takes, and y's column at which the weight starts.
+__device__ __forceinline__ int segment_of_block(const Mx8Args& p, int rows, int& b, int& col0) {
+  int seg = 0;
+  col0 = 0;
+#pragma unroll
+  for (int j = 0; j + 1 < kMx8Segments; ++j) {
+    const int nb = (p.n[j] + rows - 1) / rows;
+    if (seg == j && j + 1 < p.nseg && b >= nb) b -= nb, col0 += p.n[j], seg = j + 1;
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  col0 = __builtin_amdgcn_readfirstlane(col0);
+  return __builtin_amdgcn_readfirstlane(seg);
+}
+
+// Any K and any alignment of the rows of scales: fragments and scales straight into registers.
 // RG: 16-row groups of weights (SwiGLU: of each of the two), MT: 16-row tiles of x.
 template <int RG, int MT, bool SW>
 __global__ __launch_bounds__(64 * kWaves) void mx8_rows_kernel(const Mx8Args p) {
@@ -24,13 +107,8 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_rows_kernel(const Mx8Args p) 
   __shared__ floatx4 sums[kWaves * RGT * MT * 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, q = lane >> 4;
-  int seg = 0, b = blockIdx.x, col0 = 0;  // weight, its block, the column of y at which it starts
-#pragma unroll
-  for (int j = 0; j + 1 < kMx8Segments; ++j) {
-    const int nb = (p.n[j] + 16 * RG - 1) / (16 * RG);
-    if (seg == j && j + 1 < p.nseg && b >= nb) b -= nb, col0 += p.n[j], seg = j + 1;
-  }
-  seg = __builtin_amdgcn_readfirstlane(seg);
+  int b = blockIdx.x, col0;
+  const int seg = segment_of_block(p, 16 * RG, b, col0);
   const int n0 = b * 16 * RG, rows = min(16 * RG, p.n[seg] - n0), K = p.K, kb = K / kMx8Block;
   const int m0 = blockIdx.y * 16 * MT, M = min(p.M - m0, 16 * MT);
 
@@ -85,49 +163,133 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_rows_kernel(const Mx8Args p) 
     for (int j = 0; j < MT; ++j) sums[((wave * RGT + g) * MT + j) * 64 + lane] = acc[g][j];
   __syncthreads();
 
-  // Four columns of a row per lane; the eight lanes of 32 columns are neighbours.
-  for (int it = tid; it < RG * MT * 64; it += 64 * kWaves) {
-    const int m = it / (4 * RG), c = it % (4 * RG), at = (m & 15) + 16 * (c & 3);
-    if (m >= M || 4 * c >= rows) continue;
-    auto total = [&](int g) {
-      floatx4 v = sums[(g * MT + m / 16) * 64 + at];
+  finish_block<RG, MT, SW>(p, sums, seg, m0, M, n0, rows, col0);
+}
+
+// The same with K a multiple of 128, fed by a ring of stages of 512 k: codes (whole row pieces) and scales go global -> LDS
+// past the registers, up to five stages ahead, one barrier a stage. Row r keeps its 16-byte chunk c at slot c ^ (r & 15). A
+// wave takes a quarter of a stage, one matrix instruction for each group and tile. XR: rows of x in LDS.
+template <int RG, int XR, bool SW>
+struct RingShape {
+  static constexpr int RGT = SW ? 2 * RG : RG, MT = XR > 16 ? XR / 16 : 1;
+  static constexpr int PW = 2 * RGT, PX = XR / 8, PER = PW + PX + 1;  // loads of a wave and stage: weights, x, scales
+  static constexpr int kW = RGT * 8192, kX = XR * 512, kSlot = kW + kX + kWaves * 1024;
+  // As many stages as leave room for two blocks on a CU where x is small, the next one's first loads under the last one's
+  // sums; else as the LDS holds.
+  static constexpr int kLds = (XR <= 8 && 3 * kSlot <= 78 * 1024 ? 78 : 156) * 1024;
+  static constexpr int NS = kLds / kSlot >= 6 ? 6 : kLds / kSlot;
+  static_assert(NS >= 2 && (NS - 2) * PER < 64 && kWaves * RGT * MT * 1024 <= NS * kSlot, "the ring, and the waves' sums");
+  static_assert(SW ? RG <= 4 : RG <= 12, "a wave's load holds the scales of gate, of up; three waves' those of the weights");
+};
+
+template <int RG, int XR, bool SW>
+__global__ __launch_bounds__(64 * kWaves) void mx8_ring_kernel(const Mx8Args p) {
+  typedef RingShape<RG, XR, SW> S;
+  constexpr int RGT = S::RGT, MT = S::MT, NS = S::NS, kS = S::kW + S::kX;
+  __shared__ __attribute__((aligned(1024))) char smem[NS * S::kSlot];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, q = lane >> 4;
+  int b = blockIdx.x, col0;
+  const int seg = segment_of_block(p, p.r, b, col0);
+  const int n0 = b * p.r, rows = __builtin_amdgcn_readfirstlane(min(p.r, p.n[seg] - n0)), M = p.M;
+  const int K = p.K, kb = K / kMx8Block, steps = (K + 511) / 512;
+  const uint32_t lbase = lds_addr(smem);
+
+  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, (int64_t)M * K);
+  const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.w[SW ? 0 : seg] + (int64_t)n0 * K, (int64_t)rows * K);
+  const __amdgpu_buffer_rsrc_t rb = SW ? make_rsrc(p.w[1] + (int64_t)n0 * K, (int64_t)rows * K) : ra;
+  // Scales, a row's 16 bytes a lane: wave 3 x's, waves 0 and 1 gate's and up's, or waves 0 to 2 64 weight rows each.
+  const bool of_x = wave == kWaves - 1;
+  const uint8_t* const sp = of_x ? p.xs : p.ws[SW ? (wave == 0 ? 0 : 1) : seg] + (int64_t)n0 * kb;
+  const int srows = of_x ? M : SW ? (wave < 2 ? rows : 0) : max(0, rows - 64 * wave);
+  const __amdgpu_buffer_rsrc_t rs = make_rsrc(SW || of_x ? sp : sp + (int64_t)(64 * wave) * kb, (int64_t)srows * kb);
+  // A load of codes is two rows: load u of this wave rows 8 u + lr of x or of the groups. Its chunk, and offset at k = 0,
+  // for even and odd u.
+  const int lr = 2 * wave + (lane >> 5);
+  int kof[2];
+  uint32_t off0[2];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) v += sums[((w * RGT + g) * MT + m / 16) * 64 + at];
-      return v;
+  for (int h = 0; h < 2; ++h) {
+    kof[h] = 16 * ((lane & 31) ^ (8 * h + lr));
+    off0[h] = (uint32_t)((8 * h + lr) * K + kof[h]);
+  }
+  auto issue = [&](int t, int at0) {
+    const uint32_t at = lbase + (uint32_t)at0, k = (uint32_t)t * 512;
+    const bool in[2] = {(int)k + kof[0] < K, (int)k + kof[1] < K};
+#pragma unroll
+    for (int u = 0; u < S::PX; ++u)
+      dma16(rx, in[u & 1] ? off0[u & 1] + (uint32_t)(u / 2 * 16 * K) + k : kOOB, at + S::kW + (4 * u + wave) * 1024);
+    dma16(rs, (uint32_t)(lane * kb + t * 16), at + kS + wave * 1024);  // past a row's end: not used
+#pragma unroll
+    for (int u = 0; u < S::PW; ++u) {
+      const int g = u / 2;
+      dma16_nt(SW && g >= RG ? rb : ra, in[u & 1] ? off0[u & 1] + (uint32_t)((g < RG ? g : g - RG) * 16 * K) + k : kOOB,
+               at + (4 * u + wave) * 1024);
+    }
+  };
+
+  floatx4 acc[RGT][MT];
+#pragma unroll
+  for (int g = 0; g < RGT; ++g)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[g][j] = floatx4{};
+#pragma unroll 1
+  for (int t = 0; t < NS - 1; ++t) issue(t, t * S::kSlot);
+  int cur = 0, next = (NS - 1) * S::kSlot;  // slots of stage t and of stage t + NS - 1
+  for (int t = 0; t < steps; ++t) {
+    vm_wait<(NS - 2) * S::PER>();                                    // this wave's part of stage t has landed
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // every wave's; nobody reads stage t - 1 any more
+    issue(t + NS - 1, next);
+    const char* st = smem + cur;
+    next = cur;
+    cur = cur == (NS - 1) * S::kSlot ? 0 : cur + S::kSlot;
+    const bool in = t * 16 + 4 * wave + q < kb;  // past the row's end codes are 0, scales may be anything
+    auto frag = [&](const char* row, int r) {
+      const i32x4 lo = *reinterpret_cast<const i32x4*>(row + (((8 * wave + q) ^ r) << 4));
+      const i32x4 hi = *reinterpret_cast<const i32x4*>(row + (((8 * wave + 4 + q) ^ r) << 4));
+      return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
-    floatx4 v = total(c / 4);
-    if constexpr (SW) {
-      const floatx4 u = total(RG + c / 4);
+    auto scale = [&](int row) {
+      const int v = *reinterpret_cast<const uint8_t*>(st + kS + row * 16 + 4 * wave + q);
+      return in ? v : 0;
+    };
+    i32x8 x[MT];
+    int sx[MT];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = silu_mul(v[e], u[e]);
+    for (int j = 0; j < MT; ++j) {
+      const int r = XR < 16 ? i % XR : i;  // fewer rows: repeated, the copies' sums are not used
+      x[j] = frag(st + S::kW + (16 * j + r) * 512, r);
+      sx[j] = scale(64 * (kWaves - 1) + 16 * j + r);
     }
-    const int left = rows - 4 * c, n = n0 + 4 * c, col = col0 + n;
-    const int64_t row = m0 + m;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (e >= left) break;
-      if (!SW) {
-        if (p.bias[seg]) v[e] += bf2f(p.bias[seg][n + e]);
-        v[e] = mx8_act(v[e], p.act);
-      }
-      if (p.res) v[e] += bf2f(p.res[row * p.ldr + col + e]);
-    }
-    if (p.yc) {  // the columns are whole blocks
-      uint32_t top = 0;
+    for (int g = 0; g < RGT; ++g) {
+      const i32x8 w = frag(st + (16 * g + i) * 512, i);
+      const int sw = scale(SW ? (g < RG ? 16 * g : 64 + 16 * (g - RG)) + i : 16 * g + i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top = max(top, mx8_magnitude(v[e]));
-#pragma unroll
-      for (int o = 1; o < 8; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-      const uint32_t byte = mx8_scale_byte(top);
-      const uint32_t codes = byte == 255 ? 0 : mx8_pack4(v[0], v[1], v[2], v[3], mx8_scale(byte));
-      *reinterpret_cast<uint32_t*>(p.yc + row * p.ldc + col) = codes;
-      if ((c & 7) == 0) p.ys[row * (p.ldc / kMx8Block) + col / kMx8Block] = (uint8_t)byte;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < left) p.y[row * p.ldc + col + e] = f2bf(v[e]);
+      for (int j = 0; j < MT; ++j) acc[g][j] = mfma_mx8(w, x[j], acc[g][j], sw, sx[j]);
     }
   }
+  vm_wait<0>();  // the ring's last loads (zeros) have landed, and every wave has read its last stage
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  floatx4* sums = reinterpret_cast<floatx4*>(smem);
+#pragma unroll
+  for (int g = 0; g < RGT; ++g)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sums[((wave * RGT + g) * MT + j) * 64 + lane] = acc[g][j];
+  __syncthreads();
+  finish_block<RG, MT, SW>(p, sums, seg, 0, M, n0, rows, col0);
+}
+
+template <int XR, bool SW>
+void launch_ring(const Mx8Args& p, unsigned blocks, hipStream_t st) {
+  const dim3 grid(blocks), block(64 * kWaves);
+  constexpr int most = (XR <= 16 ? 8 : XR == 32 ? 6 : 4) / (SW ? 2 : 1);  // groups
+  const int rg = (p.r + 15) / 16;
+  if (rg == 1) hipLaunchKernelGGL((mx8_ring_kernel<1, XR, SW>), grid, block, 0, st, p);
+  else if (rg == 2) hipLaunchKernelGGL((mx8_ring_kernel<2, XR, SW>), grid, block, 0, st, p);
+  else if (rg == 3 && most >= 3) hipLaunchKernelGGL((mx8_ring_kernel<most >= 3 ? 3 : 2, XR, SW>), grid, block, 0, st, p);
+  else if (rg == 4 && most >= 4) hipLaunchKernelGGL((mx8_ring_kernel<most >= 4 ? 4 : 2, XR, SW>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((mx8_ring_kernel<most >= 6 ? 6 : 2, XR, SW>), grid, block, 0, st, p);
 }
 
 template <int RG, bool SW>
@@ -145,20 +307,53 @@ void launch_tiles(const Mx8Args& p, unsigned blocks, hipStream_t st) {
 
 namespace q3 {
 
-int mx8_rows(const Mx8Args& p, bool swiglu, hipStream_t st) {
+int mx8_rows(const Mx8Args& args, bool swiglu, hipStream_t st) {
+  Mx8Args p = args;
+  int64_t N = 0;
+  p.vec = q3_aligned(p.y, 8) && p.ldc % 4 == 0 && (!p.res || (q3_aligned(p.res, 8) && p.ldr % 4 == 0));
+  for (int j = 0; j < p.nseg; ++j) {
+    p.vec = p.vec && (j == 0 || N % 4 == 0);
+    N += p.n[j];
+  }
   auto blocks = [&](int rows) {
     int64_t n = 0;
     for (int j = 0; j < p.nseg; ++j) n += q3_cdiv(p.n[j], rows);
-    return (unsigned)n;
+    return n;
   };
+  if (p.K % 128 == 0 && p.M <= 64) {
+    // The fewest rows a block (whole 8-byte pieces of y, or whole blocks of 32 in eight bits) that give every CU one block,
+    // or an equal number of them where even the largest block does not cover N.
+    const int unit = p.yc ? 32 : 4;
+    int most = 16 * (p.M <= 16 ? (swiglu ? 4 : 6) : p.M <= 32 ? (swiglu ? 3 : 6) : swiglu ? 2 : 4);
+    most = most / unit * unit;
+    const int64_t rounds = q3_cdiv(N, 256 * most);
+    int r = unit;
+    while (r < most && blocks(r) > 256 * rounds) r += unit;
+    p.r = r;
+    const unsigned n = (unsigned)blocks(r);
+    if (swiglu) {
+      if (p.M <= 8) launch_ring<8, true>(p, n, st);
+      else if (p.M <= 16) launch_ring<16, true>(p, n, st);
+      else if (p.M <= 32) launch_ring<32, true>(p, n, st);
+      else launch_ring<64, true>(p, n, st);
+    } else {
+      if (p.M <= 8) launch_ring<8, false>(p, n, st);
+      else if (p.M <= 16) launch_ring<16, false>(p, n, st);
+      else if (p.M <= 32) launch_ring<32, false>(p, n, st);
+      else launch_ring<64, false>(p, n, st);
+    }
+    Q3_LAUNCH_CHECK();
+    return Q3_OK;
+  }
   // 32 weight rows a block where the output's blocks of 32 ask for it, or where that still gives every CU two blocks.
   const bool wide = p.yc || blocks(32) >= 512;
+  const unsigned n = (unsigned)blocks(wide ? 32 : 16);
   if (swiglu) {
-    if (wide) launch_tiles<2, true>(p, blocks(32), st);
-    else launch_tiles<1, true>(p, blocks(16), st);
+    if (wide) launch_tiles<2, true>(p, n, st);
+    else launch_tiles<1, true>(p, n, st);
   } else {
-    if (wide) launch_tiles<2, false>(p, blocks(32), st);
-    else launch_tiles<1, false>(p, blocks(16), st);
+    if (wide) launch_tiles<2, false>(p, n, st);
+    else launch_tiles<1, false>(p, n, st);
   }
   Q3_LAUNCH_CHECK();
   return Q3_OK;
