@@ -108,6 +108,14 @@ __device__ __forceinline__ void mx8_store8(T* p, const float (&v)[8]) {
   }
 }
 
+// A uniform pointer or number in scalar registers (a select can leave it in vector ones).
+__device__ __forceinline__ int mx8_pin(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ const uint8_t* mx8_pin(const uint8_t* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
+}
+
 // Products in eight bits: the arguments of every form.
 constexpr int kMx8Segments = 4;  // weights side by side
 enum Mx8Act : int { kMx8None = 0, kMx8GeluTanh = 1, kMx8Silu = 2 };

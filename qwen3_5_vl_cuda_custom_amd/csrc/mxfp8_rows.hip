@@ -166,27 +166,29 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_rows_kernel(const Mx8Args p) 
   finish_block<RG, MT, SW>(p, sums, seg, m0, M, n0, rows, col0);
 }
 
-// The same with K a multiple of 128, fed by a ring of stages of 512 k: codes (whole row pieces) and scales go global -> LDS
-// past the registers, up to five stages ahead, one barrier a stage. Row r keeps its 16-byte chunk c at slot c ^ (r & 15). A
-// wave takes a quarter of a stage, one matrix instruction for each group and tile. XR: rows of x in LDS.
+// The same with K a multiple of 128, fed by a ring of stages of 512 k: codes (whole row pieces) go global -> LDS past the
+// registers, up to four stages ahead, one barrier a stage. Row r keeps its 16-byte chunk c at slot c ^ (r & 15). A wave takes
+// a quarter of a stage, one matrix instruction for each group and tile. Scales come 64 bytes of a row at a time, four
+// stages' (as 16 bytes with every stage, a line each for the same lines again, they cost 3 of 21 us at 32 rows of K 12288).
+// XR: rows of x in LDS.
 template <int RG, int XR, bool SW>
 struct RingShape {
   static constexpr int RGT = SW ? 2 * RG : RG, MT = XR > 16 ? XR / 16 : 1;
-  static constexpr int PW = 2 * RGT, PX = XR / 8, PER = PW + PX + 1;  // loads of a wave and stage: weights, x, scales
-  static constexpr int kW = RGT * 8192, kX = XR * 512, kSlot = kW + kX + kWaves * 1024;
+  static constexpr int PW = 2 * RGT, PX = XR / 8, PER = PW + PX;  // loads of a wave and stage: weights, x
+  static constexpr int kW = RGT * 8192, kX = XR * 512, kSlot = kW + kX;
+  static constexpr int kS = (RGT + MT) * 1024;  // four stages' scales, two slots
   // As many stages as leave room for two blocks on a CU where x is small, the next one's first loads under the last one's
   // sums; else as the LDS holds.
-  static constexpr int kLds = (XR <= 8 && 3 * kSlot <= 78 * 1024 ? 78 : 156) * 1024;
-  static constexpr int NS = kLds / kSlot >= 6 ? 6 : kLds / kSlot;
+  static constexpr int kLds = (XR <= 8 && 3 * kSlot + 2 * kS <= 80 * 1024 ? 80 : 160) * 1024 - 2 * kS;
+  static constexpr int NS = kLds / kSlot >= 5 ? 5 : kLds / kSlot;  // the loads run at most one slot of scales ahead
   static_assert(NS >= 2 && (NS - 2) * PER < 64 && kWaves * RGT * MT * 1024 <= NS * kSlot, "the ring, and the waves' sums");
-  static_assert(SW ? RG <= 4 : RG <= 12, "a wave's load holds the scales of gate, of up; three waves' those of the weights");
 };
 
 template <int RG, int XR, bool SW>
 __global__ __launch_bounds__(64 * kWaves) void mx8_ring_kernel(const Mx8Args p) {
   typedef RingShape<RG, XR, SW> S;
-  constexpr int RGT = S::RGT, MT = S::MT, NS = S::NS, kS = S::kW + S::kX;
-  __shared__ __attribute__((aligned(1024))) char smem[NS * S::kSlot];
+  constexpr int RGT = S::RGT, MT = S::MT, NS = S::NS, kS0 = NS * S::kSlot;
+  __shared__ __attribute__((aligned(1024))) char smem[kS0 + 2 * S::kS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, q = lane >> 4;
   int b = blockIdx.x, col0;
@@ -198,11 +200,9 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_ring_kernel(const Mx8Args p) 
   const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, (int64_t)M * K);
   const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.w[SW ? 0 : seg] + (int64_t)n0 * K, (int64_t)rows * K);
   const __amdgpu_buffer_rsrc_t rb = SW ? make_rsrc(p.w[1] + (int64_t)n0 * K, (int64_t)rows * K) : ra;
-  // Scales, a row's 16 bytes a lane: wave 3 x's, waves 0 and 1 gate's and up's, or waves 0 to 2 64 weight rows each.
-  const bool of_x = wave == kWaves - 1;
-  const uint8_t* const sp = of_x ? p.xs : p.ws[SW ? (wave == 0 ? 0 : 1) : seg] + (int64_t)n0 * kb;
-  const int srows = of_x ? M : SW ? (wave < 2 ? rows : 0) : max(0, rows - 64 * wave);
-  const __amdgpu_buffer_rsrc_t rs = make_rsrc(SW || of_x ? sp : sp + (int64_t)(64 * wave) * kb, (int64_t)srows * kb);
+  const uint8_t* const sa = mx8_pin(p.ws[SW ? 0 : seg] + (int64_t)n0 * kb);  // SwiGLU: gate's, and up's
+  const uint8_t* const sb = SW ? mx8_pin(p.ws[1] + (int64_t)n0 * kb) : sa;
+  const uint32_t soff = (uint32_t)((lane >> 2) * kb + (lane & 3) * 16);
   // A load of codes is two rows: load u of this wave rows 8 u + lr of x or of the groups. Its chunk, and offset at k = 0,
   // for even and odd u.
   const int lr = 2 * wave + (lane >> 5);
@@ -215,11 +215,21 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_ring_kernel(const Mx8Args p) 
   }
   auto issue = [&](int t, int at0) {
     const uint32_t at = lbase + (uint32_t)at0, k = (uint32_t)t * 512;
+    if (t % 4 == 0) {  // scales of 16 rows a load: the groups', x's tiles'. What lies past a row's end is not used.
+#pragma unroll
+      for (int u = 0; u < (RGT + MT + kWaves - 1) / kWaves; ++u) {
+        const int d = u * kWaves + wave;
+        if (d >= RGT + MT) break;
+        const bool of_x = d >= RGT, up = SW && d >= RG;
+        const int row = 16 * (of_x ? d - RGT : up ? d - RG : d);
+        dma16(make_rsrc(mx8_pin(of_x ? p.xs : up ? sb : sa), mx8_pin((of_x ? M : rows) * kb)), soff + (uint32_t)(row * kb) + (uint32_t)t * 16,
+              lbase + (uint32_t)(kS0 + (t / 4 & 1) * S::kS + d * 1024));
+      }
+    }
     const bool in[2] = {(int)k + kof[0] < K, (int)k + kof[1] < K};
 #pragma unroll
     for (int u = 0; u < S::PX; ++u)
       dma16(rx, in[u & 1] ? off0[u & 1] + (uint32_t)(u / 2 * 16 * K) + k : kOOB, at + S::kW + (4 * u + wave) * 1024);
-    dma16(rs, (uint32_t)(lane * kb + t * 16), at + kS + wave * 1024);  // past a row's end: not used
 #pragma unroll
     for (int u = 0; u < S::PW; ++u) {
       const int g = u / 2;
@@ -249,8 +259,9 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_ring_kernel(const Mx8Args p) 
       const i32x4 hi = *reinterpret_cast<const i32x4*>(row + (((8 * wave + 4 + q) ^ r) << 4));
       return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
+    const char* const ss = smem + kS0 + (t / 4 & 1) * S::kS + (t & 3) * 16 + 4 * wave + q;
     auto scale = [&](int row) {
-      const int v = *reinterpret_cast<const uint8_t*>(st + kS + row * 16 + 4 * wave + q);
+      const int v = *reinterpret_cast<const uint8_t*>(ss + row * 64);
       return in ? v : 0;
     };
     i32x8 x[MT];
@@ -259,12 +270,12 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_ring_kernel(const Mx8Args p) 
     for (int j = 0; j < MT; ++j) {
       const int r = XR < 16 ? i % XR : i;  // fewer rows: repeated, the copies' sums are not used
       x[j] = frag(st + S::kW + (16 * j + r) * 512, r);
-      sx[j] = scale(64 * (kWaves - 1) + 16 * j + r);
+      sx[j] = scale(16 * (RGT + j) + r);
     }
 #pragma unroll
     for (int g = 0; g < RGT; ++g) {
       const i32x8 w = frag(st + (16 * g + i) * 512, i);
-      const int sw = scale(SW ? (g < RG ? 16 * g : 64 + 16 * (g - RG)) + i : 16 * g + i);
+      const int sw = scale(16 * g + i);
 #pragma unroll
       for (int j = 0; j < MT; ++j) acc[g][j] = mfma_mx8(w, x[j], acc[g][j], sw, sx[j]);
     }
@@ -283,7 +294,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_ring_kernel(const Mx8Args p) 
 template <int XR, bool SW>
 void launch_ring(const Mx8Args& p, unsigned blocks, hipStream_t st) {
   const dim3 grid(blocks), block(64 * kWaves);
-  constexpr int most = (XR <= 16 ? 8 : XR == 32 ? 6 : 4) / (SW ? 2 : 1);  // groups
+  constexpr int most = (XR <= 8 ? 8 : XR <= 32 ? 6 : 4) / (SW ? 2 : 1);  // groups
   const int rg = (p.r + 15) / 16;
   if (rg == 1) hipLaunchKernelGGL((mx8_ring_kernel<1, XR, SW>), grid, block, 0, st, p);
   else if (rg == 2) hipLaunchKernelGGL((mx8_ring_kernel<2, XR, SW>), grid, block, 0, st, p);
@@ -324,7 +335,7 @@ int mx8_rows(const Mx8Args& args, bool swiglu, hipStream_t st) {
     // The fewest rows a block (whole 8-byte pieces of y, or whole blocks of 32 in eight bits) that give every CU one block,
     // or an equal number of them where even the largest block does not cover N.
     const int unit = p.yc ? 32 : 4;
-    int most = 16 * (p.M <= 16 ? (swiglu ? 4 : 6) : p.M <= 32 ? (swiglu ? 3 : 6) : swiglu ? 2 : 4);
+    int most = 16 * (p.M <= 8 ? (swiglu ? 4 : 6) : p.M <= 32 ? (swiglu ? 3 : 6) : swiglu ? 2 : 4);
     most = most / unit * unit;
     const int64_t rounds = q3_cdiv(N, 256 * most);
     int r = unit;

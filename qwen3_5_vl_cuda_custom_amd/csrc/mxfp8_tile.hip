@@ -41,14 +41,6 @@ struct TileArgs {
   float* part;       // fp32 partial sums (splits, M, N), or null
 };
 
-// A uniform pointer or number in scalar registers (a select can leave it in vector ones).
-__device__ __forceinline__ int pin(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ const uint8_t* pin(const uint8_t* p) {
-  const uint64_t v = reinterpret_cast<uint64_t>(p);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-  return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
-}
-
 // Eight columns of y from n on (of its segment; `left` of them exist), the row's m.
 __device__ __forceinline__ void finish8(const Mx8Args& p, int seg, int64_t m, int n, int col, int left, bool vec,
                                         bool plain, float (&v)[8]) {
@@ -141,14 +133,14 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
     const int nt = (p.n[j] + BN_OUT - 1) / BN_OUT;
     if (seg == j && j + 1 < p.nseg && tn >= nt) tn -= nt, col0 += p.n[j], seg = j + 1;
   }
-  seg = pin(seg), tn = pin(tn), col0 = pin(col0);
-  const int n0 = tn * BN_OUT, rows_n = pin(min(BN_OUT, p.n[seg] - n0)), rows_m = pin(min(BM, p.M - m0));
+  seg = mx8_pin(seg), tn = mx8_pin(tn), col0 = mx8_pin(col0);
+  const int n0 = tn * BN_OUT, rows_n = mx8_pin(min(BN_OUT, p.n[seg] - n0)), rows_m = mx8_pin(min(BM, p.M - m0));
   const int k_first = blockIdx.z * t.kt, nk = min(t.kt, (K + 127) / 128 - k_first);  // stages
   const int groups_k = (K + 511) / 512;  // of four stages
 
-  const __amdgpu_buffer_rsrc_t rx = make_rsrc(pin(p.x + (int64_t)m0 * K), rows_m * K);
-  const uint8_t* const wa = pin(p.w[SW ? 0 : seg] + (int64_t)n0 * K);  // SwiGLU: gate's, and up's
-  const uint8_t* const wb = SW ? pin(p.w[1] + (int64_t)n0 * K) : wa;
+  const __amdgpu_buffer_rsrc_t rx = make_rsrc(mx8_pin(p.x + (int64_t)m0 * K), rows_m * K);
+  const uint8_t* const wa = mx8_pin(p.w[SW ? 0 : seg] + (int64_t)n0 * K);  // SwiGLU: gate's, and up's
+  const uint8_t* const wb = SW ? mx8_pin(p.w[1] + (int64_t)n0 * K) : wa;
   auto swz = [](int r) { return r & 7; };
   // Load i of this wave fills rows 8 (wave + NW i) .. + 7 of the tile.
   const int lrow = lane >> 3, dc = (lane & 7) ^ swz(wave * 8 + lrow);
@@ -170,8 +162,8 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
     const int g = of_x ? m0 / 64 + e : (SW ? 2 * n0 : n0) / 64 + e - GX;
     // 64-row groups that exist: of all rows, SwiGLU 32 of each weight to a group
     const int all = of_x ? (p.M + 63) / 64 : SW ? (p.n[0] + 31) / 32 : (p.n[seg] + 63) / 64;
-    sp[s] = pin((of_x ? t.xs : t.ws[seg]) + (int64_t)g * groups_k * 1024);
-    sbytes[s] = pin(e < GS && g < all ? groups_k * 1024 : 0);
+    sp[s] = mx8_pin((of_x ? t.xs : t.ws[seg]) + (int64_t)g * groups_k * 1024);
+    sbytes[s] = mx8_pin(e < GS && g < all ? groups_k * 1024 : 0);
   }
   const uint32_t lbase = lds_addr(smem);
   constexpr int kW0 = NS * kX, kS0 = kW0 + NS * kW;
@@ -186,7 +178,7 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
   };
   auto dma_w = [&](int kt, int i) {
     const bool up = SW && ((wave + NW * i) & 4);
-    dma16(make_rsrc(SW ? pin(up ? wb : wa) : wa, rows_n * K), woff[i] + kofs(kt),
+    dma16(make_rsrc(SW ? mx8_pin(up ? wb : wa) : wa, rows_n * K), woff[i] + kofs(kt),
           lbase + (uint32_t)(kW0 + kt % NS * kW + (wave + NW * i) * 1024));
   };
   auto dma_s = [&](int kt, int s) {
