@@ -12,6 +12,7 @@ stream it uses. The kernels of a decode step take a few microseconds each, so th
 from __future__ import annotations
 
 from functools import lru_cache
+from struct import Struct
 
 import torch
 
@@ -19,7 +20,9 @@ from .. import _lib
 from ._common import require_device, require_no_grad
 
 MX8_BLOCK = 32
+_FEW_ROWS = 64  # up to which the products need no workspace (csrc/mxfp8_matmul.hip)
 _U8, _F8, _BF16 = torch.uint8, torch.float8_e4m3fn, torch.bfloat16
+_i64s = [Struct(f"{n}q").pack for n in range(5)]  # C arrays of up to four numbers or addresses
 _ACTS = {None: 0, "gelu_tanh": 1, "silu": 2}
 
 Pair = tuple[torch.Tensor, torch.Tensor]
@@ -27,7 +30,7 @@ Pair = tuple[torch.Tensor, torch.Tensor]
 
 @lru_cache(maxsize=4096)
 def _workspace(M: int, K: int, swiglu: int, *ns: int) -> int:
-    return _lib.lib().q3_matmul_mxfp8_workspace_bytes(M, _lib.i64s(*ns), len(ns), K, swiglu)
+    return _lib.lib().q3_matmul_mxfp8_workspace_bytes(M, _i64s[len(ns)](*ns), len(ns), K, swiglu)
 
 
 def _off_device(op: str, *tensors: torch.Tensor | None) -> None:
@@ -38,9 +41,13 @@ def _off_device(op: str, *tensors: torch.Tensor | None) -> None:
 
 def _packed(op: str, codes: torch.Tensor, scales: torch.Tensor, dev: int) -> Pair:
     """The pair checked, packed and aligned as the kernels read it."""
+    cs, ss = codes.shape, scales.shape
+    if (codes.dtype is _F8 and scales.dtype is _U8 and codes.get_device() == dev and scales.get_device() == dev
+            and codes.is_contiguous() and scales.is_contiguous() and cs and cs[:-1] == ss[:-1]
+            and cs[-1] == ss[-1] * MX8_BLOCK and not (codes.data_ptr() % 16 or scales.data_ptr() % 4)):
+        return codes, scales  # the usual call
     if codes.get_device() != dev or scales.get_device() != dev:
         _off_device(op, codes, scales)
-    cs, ss = codes.shape, scales.shape
     if codes.dtype != _F8 or scales.dtype != _U8:
         raise TypeError(f"{op}: codes must be float8_e4m3fn and scales uint8, got {codes.dtype} and {scales.dtype}")
     if not cs or len(cs) != len(ss) or cs[:-1] != ss[:-1] or cs[-1] != ss[-1] * MX8_BLOCK:
@@ -85,12 +92,15 @@ def mxfp8_quantize(x: torch.Tensor) -> Pair:
     if not shape or shape[-1] % MX8_BLOCK:
         raise ValueError(f"{op}: the last dim of {tuple(shape)} must be a multiple of {MX8_BLOCK}")
     K = shape[-1]
-    codes = x.new_empty(shape, dtype=_F8)
-    scales = x.new_empty((*shape[:-1], K // MX8_BLOCK), dtype=_U8)
+    packed = x.is_contiguous()
+    codes = torch.empty_like(x, dtype=_F8) if packed else x.new_empty(shape, dtype=_F8)  # empty_like: 0.3 us less
+    scales = codes.new_empty((*shape[:-1], K // MX8_BLOCK), dtype=_U8)
     n = x.numel()
     if n == 0:
         return codes, scales
-    x, ld = _strided(x, K)
+    ld = K
+    if not packed or x.data_ptr() % 16:
+        x, ld = _strided(x, K)
     _lib.call("q3_mxfp8_quantize", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), n // K, K, ld, dt,
               _lib.raw_stream(dev))
     return codes, scales
@@ -103,7 +113,7 @@ def mxfp8_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dty
     dev = _device(op, codes)
     codes, scales = _packed(op, codes, scales, dev)
     dt = _lib.dtype_code(dtype)
-    y = codes.new_empty(codes.shape, dtype=dtype)
+    y = torch.empty_like(codes, dtype=dtype)
     n = y.numel()
     if n:
         _lib.call("q3_mxfp8_dequantize", codes.data_ptr(), scales.data_ptr(), y.data_ptr(), n, dt,
@@ -137,14 +147,18 @@ def add_rmsnorm_mxfp8(x: torch.Tensor, residual: torch.Tensor | None, weight: to
         raise ValueError(f"{op}: weight {tuple(weight.shape)} != ({K},)")
     if residual is not None and residual.shape != shape:
         raise ValueError(f"{op}: residual {tuple(residual.shape)} != x {tuple(shape)}")
-    codes = x.new_empty(shape, dtype=_F8)
-    scales = x.new_empty((*shape[:-1], K // MX8_BLOCK), dtype=_U8)
-    h = x if residual is None else x.new_empty(shape)
+    packed = x.is_contiguous()
+    codes = torch.empty_like(x, dtype=_F8) if packed else x.new_empty(shape, dtype=_F8)
+    scales = codes.new_empty((*shape[:-1], K // MX8_BLOCK), dtype=_U8)
+    h = x if residual is None else torch.empty_like(x) if packed else x.new_empty(shape)
     n = x.numel()
     if n == 0:
         return h, codes, scales
-    x2, ldx = _strided(x, K)
-    r2, ldr = _strided(residual, K) if residual is not None else (None, 0)
+    x2, ldx, r2, ldr = x, K, residual, K
+    if not packed or x.data_ptr() % 16:
+        x2, ldx = _strided(x, K)
+    if residual is not None and (not residual.is_contiguous() or residual.data_ptr() % 16):
+        r2, ldr = _strided(residual, K)
     if not weight.is_contiguous() or weight.data_ptr() % 16:
         weight = weight.clone(memory_format=torch.contiguous_format)
     _lib.call("q3_add_rmsnorm_mxfp8", x2.data_ptr(), _lib.ptr(r2), weight.data_ptr(),
@@ -164,7 +178,9 @@ def _operand(op: str, x: torch.Tensor | Pair) -> tuple[int, torch.Tensor, torch.
         codes, scales = mxfp8_quantize(x)
     else:
         codes, scales = x
-        dev = _device(op, codes)
+        dev = codes.get_device()
+        if dev < 0 or dev != _lib.current_device():
+            _off_device(op, codes)
         codes, scales = _packed(op, codes, scales, dev)
     if codes.shape[-1] == 0:
         raise ValueError(f"{op}: x {tuple(codes.shape)} has no columns")
@@ -190,16 +206,15 @@ def _vector(op: str, bias: torch.Tensor, n: int, dev: int) -> torch.Tensor:
     return bias if bias.is_contiguous() else bias.contiguous()
 
 
-def _outputs(op: str, codes: torch.Tensor, N: int, quantize: bool) -> tuple:
+def _outputs(op: str, codes: torch.Tensor, shape: tuple, quantize: bool) -> tuple:
     """The output, and the pointers to it, its codes and its scales."""
-    shape = (*codes.shape[:-1], N)
     if not quantize:
         y = codes.new_empty(shape, dtype=_BF16)
-        return y, (y.data_ptr(), None, None)
-    if N % MX8_BLOCK:
-        raise ValueError(f"{op}: quantize=True needs outputs of a multiple of {MX8_BLOCK} columns, got {N}")
-    pair = codes.new_empty(shape), codes.new_empty((*shape[:-1], N // MX8_BLOCK), dtype=_U8)
-    return pair, (None, pair[0].data_ptr(), pair[1].data_ptr())
+        return y, y.data_ptr(), None, None
+    if shape[-1] % MX8_BLOCK:
+        raise ValueError(f"{op}: quantize=True needs outputs of a multiple of {MX8_BLOCK} columns, got {shape[-1]}")
+    pair = codes.new_empty(shape), codes.new_empty((*shape[:-1], shape[-1] // MX8_BLOCK), dtype=_U8)
+    return pair, None, pair[0].data_ptr(), pair[1].data_ptr()
 
 
 def matmul_mxfp8(x: torch.Tensor | Pair, weight: Pair, bias: torch.Tensor | None = None,
@@ -217,13 +232,14 @@ def matmul_mxfp8(x: torch.Tensor | Pair, weight: Pair, bias: torch.Tensor | None
     if act < 0:
         raise ValueError(f"{op}: activation must be None, 'gelu_tanh' or 'silu', got {activation!r}")
     dev, xc, xs = _operand(op, x)
-    K = xc.shape[-1]
+    lead = xc.shape
+    K = lead[-1]
     wc, ws = _weight(op, weight, K, dev)
     N = wc.shape[0]
-    shape = (*xc.shape[:-1], N)
+    shape = (*lead[:-1], N)
     if bias is not None:
         bias = _vector(op, bias, N, dev)
-    ldr, ldc = 0, N
+    ldr, ldc, same = N, N, False
     if residual is not None:
         if residual.get_device() != dev:
             _off_device(op, residual)
@@ -233,14 +249,19 @@ def matmul_mxfp8(x: torch.Tensor | Pair, weight: Pair, bias: torch.Tensor | None
             require_no_grad(op, residual)
         if residual.shape != shape:
             raise ValueError(f"{op}: residual {tuple(residual.shape)} != output {shape}")
-        ldr = N
-        if not residual.is_contiguous():
+        same = residual.is_contiguous()
+        if not same:
             residual = residual.reshape(-1, N)
             if N > 1 and residual.stride(1) != 1 or residual.shape[0] > 1 and residual.stride(0) < N:
                 residual = residual.contiguous()
             ldr = residual.stride(0) if residual.shape[0] > 1 else N
+    yc = ys = None
     if out is None:
-        y, ptrs = _outputs(op, xc, N, quantize)
+        if same and not quantize:
+            y = torch.empty_like(residual)
+            yp = y.data_ptr()
+        else:
+            y, yp, yc, ys = _outputs(op, xc, shape, quantize)
     else:
         if quantize:
             raise ValueError(f"{op}: give either out or quantize=True")
@@ -252,7 +273,7 @@ def matmul_mxfp8(x: torch.Tensor | Pair, weight: Pair, bias: torch.Tensor | None
             require_no_grad(op, out)
         if out.shape != shape or (N > 1 and out.stride(-1) != 1):
             raise ValueError(f"{op}: out {tuple(out.shape)} must be {shape} with contiguous elements")
-        y, ptrs = out, (out.data_ptr(), None, None)
+        y, yp = out, out.data_ptr()
         if not out.is_contiguous() and out.numel() > N:
             ldc = out.view(-1, N).stride(0)
             if ldc < N:
@@ -260,10 +281,10 @@ def matmul_mxfp8(x: torch.Tensor | Pair, weight: Pair, bias: torch.Tensor | None
     M = xc.numel() // K
     if M == 0 or N == 0:
         return y
-    nws = _workspace(M, K, 0, N)
+    nws = 0 if M <= _FEW_ROWS else _workspace(M, K, 0, N)
     buf = xs.new_empty(nws) if nws else None
     _lib.call("q3_matmul_mxfp8", xc.data_ptr(), xs.data_ptr(), wc.data_ptr(), ws.data_ptr(), _lib.ptr(bias),
-              _lib.ptr(residual), *ptrs, M, N, K, ldr, ldc, act, _lib.ptr(buf), nws, _lib.raw_stream(dev))
+              _lib.ptr(residual), yp, yc, ys, M, N, K, ldr, ldc, act, _lib.ptr(buf), nws, _lib.raw_stream(dev))
     return y
 
 
@@ -272,25 +293,28 @@ def matmul_segments_mxfp8(x: torch.Tensor | Pair, weights, biases=None) -> torch
     x as in matmul_mxfp8. Returns (..., ΣN_i) bf16."""
     op = "matmul_segments_mxfp8"
     weights = list(weights)
-    biases = list(biases) if biases is not None else [None] * len(weights)
-    if not 1 <= len(weights) <= 4 or len(biases) != len(weights):
+    given = [None] * len(weights) if biases is None else list(biases)
+    if not 1 <= len(weights) <= 4 or len(given) != len(weights):
         raise ValueError(f"{op}: 1 to 4 weights, one bias (or None) each")
     dev, xc, xs = _operand(op, x)
     K = xc.shape[-1]
     ws = [_weight(op, w, K, dev) for w in weights]
     ns = [c.shape[0] for c, _ in ws]
-    bs = [None if b is None else _vector(op, b, n, dev) for b, n in zip(biases, ns)]
-    y, N = xc.new_empty((*xc.shape[:-1], sum(ns)), dtype=_BF16), sum(ns)
+    bs = [None if b is None else _vector(op, b, n, dev) for b, n in zip(given, ns)]
+    N = sum(ns)
+    y = xc.new_empty((*xc.shape[:-1], N), dtype=_BF16)
     M = xc.numel() // K
     if M == 0 or N == 0:
         return y
     if 0 in ns:
         ws, bs, ns = zip(*((w, b, n) for w, b, n in zip(ws, bs, ns) if n))
-    nws = _workspace(M, K, 0, *ns)
+    array = _i64s[len(ns)]
+    some = array(*(b.data_ptr() if b is not None else 0 for b in bs)) if biases is not None else None
+    nws = 0 if M <= _FEW_ROWS else _workspace(M, K, 0, *ns)
     buf = xs.new_empty(nws) if nws else None
-    _lib.call("q3_matmul_segments_mxfp8", xc.data_ptr(), xs.data_ptr(), _lib.ptrs(*(c for c, _ in ws)),
-              _lib.ptrs(*(s for _, s in ws)), _lib.ptrs(*bs) if any(b is not None for b in bs) else None,
-              _lib.i64s(*ns), len(ns), y.data_ptr(), M, K, N, _lib.ptr(buf), nws, _lib.raw_stream(dev))
+    _lib.call("q3_matmul_segments_mxfp8", xc.data_ptr(), xs.data_ptr(), array(*[c.data_ptr() for c, _ in ws]),
+              array(*[t.data_ptr() for _, t in ws]), some, array(*ns), len(ns), y.data_ptr(), M, K, N, _lib.ptr(buf), nws,
+              _lib.raw_stream(dev))
     return y
 
 
@@ -305,12 +329,12 @@ def matmul_swiglu_mxfp8(x: torch.Tensor | Pair, gate: Pair, up: Pair, *, quantiz
     if gc.shape != uc.shape:
         raise ValueError(f"{op}: gate {tuple(gc.shape)} and up {tuple(uc.shape)} must have one shape")
     N = gc.shape[0]
-    y, ptrs = _outputs(op, xc, N, quantize)
+    y, yp, yc, ys = _outputs(op, xc, (*xc.shape[:-1], N), quantize)
     M = xc.numel() // K
     if M == 0 or N == 0:
         return y
-    nws = _workspace(M, K, 1, N)
+    nws = 0 if M <= _FEW_ROWS else _workspace(M, K, 1, N)
     buf = xs.new_empty(nws) if nws else None
     _lib.call("q3_matmul_swiglu_mxfp8", xc.data_ptr(), xs.data_ptr(), gc.data_ptr(), gs.data_ptr(), uc.data_ptr(),
-              us.data_ptr(), *ptrs, M, N, K, N, _lib.ptr(buf), nws, _lib.raw_stream(dev))
+              us.data_ptr(), yp, yc, ys, M, N, K, N, _lib.ptr(buf), nws, _lib.raw_stream(dev))
     return y
