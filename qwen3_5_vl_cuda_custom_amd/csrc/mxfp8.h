@@ -142,6 +142,8 @@ __device__ __forceinline__ float mx8_act(float v, int act) {
   return v;
 }
 
+// Whether mx8_rows takes the product: it needs no workspace.
+bool mx8_rows_takes(const Mx8Args& a, bool swiglu);
 int mx8_rows(const Mx8Args& a, bool swiglu, hipStream_t st);
 
 }  // namespace q3

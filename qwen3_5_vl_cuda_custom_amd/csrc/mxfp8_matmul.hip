@@ -48,10 +48,7 @@ int weight(Mx8Args& a, int j, const void* codes, const void* scales, const void*
   return Q3_OK;
 }
 
-// Rows of x up to which whole weight rows are taken (mxfp8_rows.hip).
-constexpr int kFewRows = 64;
-
-int64_t workspace_of(const Mx8Args& a, bool swiglu) { return a.M <= kFewRows ? 0 : mx8_tile_workspace(a, swiglu); }
+int64_t workspace_of(const Mx8Args& a, bool swiglu) { return mx8_rows_takes(a, swiglu) ? 0 : mx8_tile_workspace(a, swiglu); }
 
 int launch(const Call& c, bool swiglu, void* workspace, int64_t workspace_bytes, void* stream) {
   if (c.a.M == 0 || c.N == 0) return Q3_OK;
@@ -59,7 +56,7 @@ int launch(const Call& c, bool swiglu, void* workspace, int64_t workspace_bytes,
   Q3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), Q3_ERR_WORKSPACE);
   Q3_REQUIRE(q3_aligned(workspace, 16), Q3_ERR_ALIGN);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return c.a.M <= kFewRows ? mx8_rows(c.a, swiglu, st) : mx8_tile(c.a, c.N, swiglu, workspace, st);
+  return mx8_rows_takes(c.a, swiglu) ? mx8_rows(c.a, swiglu, st) : mx8_tile(c.a, swiglu, workspace, st);
 }
 
 }  // namespace

@@ -1,5 +1,5 @@
-// Products of MXFP8 rows with MXFP8 weights by whole weight rows, 64 rows of x at a
-// time (format and matrix instruction: mxfp8.h):
+// Products of MXFP8 rows with MXFP8 weights by whole weight rows, up to 64 rows of x to
+// a block (format and matrix instruction: mxfp8.h):
 //   y = act(x w^T (+ bias)) (+ residual),  y = silu(x g^T) * (x u^T)
 // over one weight, or the weights of several projections side by side; y in bf16 or in
 // eight bits again.
@@ -99,7 +99,7 @@ __device__ __forceinline__ int segment_of_block(const Mx8Args& p, int rows, int&
   return __builtin_amdgcn_readfirstlane(seg);
 }
 
-// Any K and any alignment of the rows of scales: fragments and scales straight into registers.
+// Any K and any alignment of the rows of scales, up to 64 rows: fragments and scales straight into registers.
 // RG: 16-row groups of weights (SwiGLU: of each of the two), MT: 16-row tiles of x.
 template <int RG, int MT, bool SW>
 __global__ __launch_bounds__(64 * kWaves) void mx8_rows_kernel(const Mx8Args p) {
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_rows_kernel(const Mx8Args p) 
   int b = blockIdx.x, col0;
   const int seg = segment_of_block(p, 16 * RG, b, col0);
   const int n0 = b * 16 * RG, rows = min(16 * RG, p.n[seg] - n0), K = p.K, kb = K / kMx8Block;
-  const int m0 = blockIdx.y * 16 * MT, M = min(p.M - m0, 16 * MT);
+  const int M = p.M;
 
   __amdgpu_buffer_rsrc_t rw[2], rs[2];
 #pragma unroll
@@ -118,8 +118,8 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_rows_kernel(const Mx8Args p) 
     rw[u] = make_rsrc(p.w[SW ? u : seg] + (int64_t)n0 * K, (int64_t)rows * K);
     rs[u] = make_rsrc(p.ws[SW ? u : seg] + (int64_t)n0 * kb, (int64_t)rows * kb);
   }
-  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x + (int64_t)m0 * K, (int64_t)M * K);
-  const __amdgpu_buffer_rsrc_t rxs = make_rsrc(p.xs + (int64_t)m0 * kb, (int64_t)M * kb);
+  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, (int64_t)M * K);
+  const __amdgpu_buffer_rsrc_t rxs = make_rsrc(p.xs, (int64_t)M * kb);
 
   // Row `row`'s 16 bytes at k and at k + 64, and the scale of block s: zeros past the row's end and the last row.
   auto frag = [&](__amdgpu_buffer_rsrc_t r, int row, int k) {
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_rows_kernel(const Mx8Args p) 
     for (int j = 0; j < MT; ++j) sums[((wave * RGT + g) * MT + j) * 64 + lane] = acc[g][j];
   __syncthreads();
 
-  finish_block<RG, MT, SW>(p, sums, seg, m0, M, n0, rows, col0);
+  finish_block<RG, MT, SW>(p, sums, seg, 0, M, n0, rows, col0);
 }
 
 // The same with K a multiple of 128, fed by a ring of stages of 512 k: codes (whole row pieces) go global -> LDS past the
@@ -191,17 +191,38 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_ring_kernel(const Mx8Args p) 
   __shared__ __attribute__((aligned(1024))) char smem[kS0 + 2 * S::kS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, q = lane >> 4;
-  int b = blockIdx.x, col0;
+  int b = blockIdx.x, col0, part = 0;
+  if constexpr (XR == 64) {
+    const int parts = (p.M + 63) / 64;
+    if (parts > 1) {  // blocks of the same weight rows are neighbours on one XCD
+      const int pid = xcd_remap(b, gridDim.x);
+      b = pid / parts;
+      part = pid - b * parts;
+    }
+  }
   const int seg = segment_of_block(p, p.r, b, col0);
-  const int n0 = b * p.r, rows = __builtin_amdgcn_readfirstlane(min(p.r, p.n[seg] - n0)), M = p.M;
+  const int n0 = b * p.r, rows = __builtin_amdgcn_readfirstlane(min(p.r, p.n[seg] - n0));
+  const int m0 = XR == 64 ? mx8_pin(64 * part) : 0, M = XR == 64 ? mx8_pin(min(p.M - m0, 64)) : p.M;
   const int K = p.K, kb = K / kMx8Block, steps = (K + 511) / 512;
   const uint32_t lbase = lds_addr(smem);
 
-  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, (int64_t)M * K);
+  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x + (int64_t)m0 * K, (int64_t)M * K);
   const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.w[SW ? 0 : seg] + (int64_t)n0 * K, (int64_t)rows * K);
   const __amdgpu_buffer_rsrc_t rb = SW ? make_rsrc(p.w[1] + (int64_t)n0 * K, (int64_t)rows * K) : ra;
-  const uint8_t* const sa = mx8_pin(p.ws[SW ? 0 : seg] + (int64_t)n0 * kb);  // SwiGLU: gate's, and up's
-  const uint8_t* const sb = SW ? mx8_pin(p.ws[1] + (int64_t)n0 * kb) : sa;
+  // Scales, four stages of 16 rows a load: the groups' (SwiGLU: gate's, then up's), x's tiles'. What lies past a row's end
+  // is not used.
+  constexpr int kSL = (RGT + MT + kWaves - 1) / kWaves;
+  const uint8_t* sp[kSL];
+  int sbytes[kSL];
+#pragma unroll
+  for (int u = 0; u < kSL; ++u) {
+    const int d = u * kWaves + wave, g = SW && d >= RG ? d - RG : d, left = 16 * (d >= RGT ? d - RGT : g);
+    const uint8_t* of = p.ws[SW ? 0 : seg] + (int64_t)n0 * kb;
+    if (SW && d >= RG) of = p.ws[1] + (int64_t)n0 * kb;
+    if (d >= RGT) of = p.xs + (int64_t)m0 * kb;
+    sp[u] = mx8_pin(of + (int64_t)left * kb);
+    sbytes[u] = mx8_pin(max(((d >= RGT ? M : rows) - left) * kb, 0));
+  }
   const uint32_t soff = (uint32_t)((lane >> 2) * kb + (lane & 3) * 16);
   // A load of codes is two rows: load u of this wave rows 8 u + lr of x or of the groups. Its chunk, and offset at k = 0,
   // for even and odd u.
@@ -215,16 +236,12 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_ring_kernel(const Mx8Args p) 
   }
   auto issue = [&](int t, int at0) {
     const uint32_t at = lbase + (uint32_t)at0, k = (uint32_t)t * 512;
-    if (t % 4 == 0) {  // scales of 16 rows a load: the groups', x's tiles'. What lies past a row's end is not used.
+    if (t % 4 == 0) {
 #pragma unroll
-      for (int u = 0; u < (RGT + MT + kWaves - 1) / kWaves; ++u) {
-        const int d = u * kWaves + wave;
-        if (d >= RGT + MT) break;
-        const bool of_x = d >= RGT, up = SW && d >= RG;
-        const int row = 16 * (of_x ? d - RGT : up ? d - RG : d);
-        dma16(make_rsrc(mx8_pin(of_x ? p.xs : up ? sb : sa), mx8_pin((of_x ? M : rows) * kb)), soff + (uint32_t)(row * kb) + (uint32_t)t * 16,
-              lbase + (uint32_t)(kS0 + (t / 4 & 1) * S::kS + d * 1024));
-      }
+      for (int u = 0; u < kSL; ++u)
+        if (u * kWaves + wave < RGT + MT)
+          dma16(make_rsrc(sp[u], sbytes[u]), soff + (uint32_t)t * 16,
+                lbase + (uint32_t)(kS0 + (t / 4 & 1) * S::kS + (u * kWaves + wave) * 1024));
     }
     const bool in[2] = {(int)k + kof[0] < K, (int)k + kof[1] < K};
 #pragma unroll
@@ -288,7 +305,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_ring_kernel(const Mx8Args p) 
 #pragma unroll
     for (int j = 0; j < MT; ++j) sums[((wave * RGT + g) * MT + j) * 64 + lane] = acc[g][j];
   __syncthreads();
-  finish_block<RG, MT, SW>(p, sums, seg, 0, M, n0, rows, col0);
+  finish_block<RG, MT, SW>(p, sums, seg, m0, M, n0, rows, col0);
 }
 
 template <int XR, bool SW>
@@ -311,12 +328,24 @@ void launch_tiles(const Mx8Args& p, unsigned blocks, hipStream_t st) {
   else if (p.M <= 32)
     hipLaunchKernelGGL((mx8_rows_kernel<RG, 2, SW>), dim3(blocks), block, 0, st, p);
   else
-    hipLaunchKernelGGL((mx8_rows_kernel<RG, 4, SW>), dim3(blocks, (unsigned)q3_cdiv(p.M, 64)), block, 0, st, p);
+    hipLaunchKernelGGL((mx8_rows_kernel<RG, 4, SW>), dim3(blocks), block, 0, st, p);
 }
 
 }  // namespace
 
 namespace q3 {
+
+// Few rows, or rows of which every 64 with up to 64 weight rows (SwiGLU: 32 of each) a block give each CU two blocks at
+// most. What the blocks read is what bounds them, and tiles share more of it, but start slower and find their scales laid
+// out only after another launch. Tiles against this, one block a CU: 100 rows, N 4096, K 4096 29.7 and 12.6 us, K 12288
+// 69.4 and 24.5; two: 128 rows, N 12288, K 4096 32.8 and 27.8, 512 rows, N 4096 32.6 and 31.7; three: SwiGLU of 128 rows,
+// N 12288 36.1 and 42.3; four: 1000 rows, N 4096 34.6 and 63.2.
+bool mx8_rows_takes(const Mx8Args& p, bool swiglu) {
+  if (p.M <= 64) return true;
+  int64_t blocks = 0;
+  for (int j = 0; j < p.nseg; ++j) blocks += q3_cdiv(p.n[j], swiglu ? 32 : 64);
+  return p.K % 128 == 0 && blocks * q3_cdiv(p.M, 64) <= 512;
+}
 
 int mx8_rows(const Mx8Args& args, bool swiglu, hipStream_t st) {
   Mx8Args p = args;
@@ -331,17 +360,17 @@ int mx8_rows(const Mx8Args& args, bool swiglu, hipStream_t st) {
     for (int j = 0; j < p.nseg; ++j) n += q3_cdiv(p.n[j], rows);
     return n;
   };
-  if (p.K % 128 == 0 && p.M <= 64) {
+  if (p.K % 128 == 0) {
     // The fewest rows a block (whole 8-byte pieces of y, or whole blocks of 32 in eight bits) that give every CU one block,
     // or an equal number of them where even the largest block does not cover N.
     const int unit = p.yc ? 32 : 4;
     int most = 16 * (p.M <= 8 ? (swiglu ? 4 : 6) : p.M <= 32 ? (swiglu ? 3 : 6) : swiglu ? 2 : 4);
     most = most / unit * unit;
-    const int64_t rounds = q3_cdiv(N, 256 * most);
+    const int64_t parts = q3_cdiv(p.M, 64), rounds = q3_cdiv(N * parts, 256 * most);
     int r = unit;
-    while (r < most && blocks(r) > 256 * rounds) r += unit;
+    while (r < most && blocks(r) * parts > 256 * rounds) r += unit;
     p.r = r;
-    const unsigned n = (unsigned)blocks(r);
+    const unsigned n = (unsigned)(blocks(r) * parts);
     if (swiglu) {
       if (p.M <= 8) launch_ring<8, true>(p, n, st);
       else if (p.M <= 16) launch_ring<16, true>(p, n, st);

@@ -7,6 +7,6 @@ namespace q3 {
 
 int64_t mx8_tile_workspace(const Mx8Args& a, bool swiglu);
 // N: columns of y. workspace: mx8_tile_workspace bytes, 16-byte aligned.
-int mx8_tile(const Mx8Args& a, int64_t N, bool swiglu, void* workspace, hipStream_t st);
+int mx8_tile(const Mx8Args& a, bool swiglu, void* workspace, hipStream_t st);
 
 }  // namespace q3

@@ -21,8 +21,6 @@
 // of rows l % 16, + 16, + 32, + 48 (the instruction picks the byte). A load brings a stage
 // of them, and three words a stage are all that a wave reads. As rows of bytes their loads
 // cost a line per row and the reads twelve bytes a stage.
-#include <algorithm>
-
 #include "gemm_tile.h"
 #include "mxfp8.h"
 #include "mxfp8_tile.h"
@@ -35,10 +33,7 @@ struct TileArgs {
   Mx8Args a;
   const uint8_t* xs;                // scales of x, and of each weight (SwiGLU: of both), laid out as above
   const uint8_t* ws[kMx8Segments];
-  int N;             // columns of y
   int tiles_m, tiles_n;
-  int kt;            // stages of a block
-  float* part;       // fp32 partial sums (splits, M, N), or null
 };
 
 // Eight columns of y from n on (of its segment; `left` of them exist), the row's m.
@@ -135,8 +130,7 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
   }
   seg = mx8_pin(seg), tn = mx8_pin(tn), col0 = mx8_pin(col0);
   const int n0 = tn * BN_OUT, rows_n = mx8_pin(min(BN_OUT, p.n[seg] - n0)), rows_m = mx8_pin(min(BM, p.M - m0));
-  const int k_first = blockIdx.z * t.kt, nk = min(t.kt, (K + 127) / 128 - k_first);  // stages
-  const int groups_k = (K + 511) / 512;  // of four stages
+  const int nk = (K + 127) / 128, groups_k = (K + 511) / 512;  // stages, and groups of four
 
   const __amdgpu_buffer_rsrc_t rx = make_rsrc(mx8_pin(p.x + (int64_t)m0 * K), rows_m * K);
   const uint8_t* const wa = mx8_pin(p.w[SW ? 0 : seg] + (int64_t)n0 * K);  // SwiGLU: gate's, and up's
@@ -167,11 +161,10 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
   }
   const uint32_t lbase = lds_addr(smem);
   constexpr int kW0 = NS * kX, kS0 = kW0 + NS * kW;
-  // Byte of a row at which the lane's chunk of stage kt lies; past the row's end, and past the block's stages, past
-  // every resource too.
+  // Byte of a row at which the lane's chunk of stage kt lies; past the row's end past every resource too.
   auto kofs = [&](int kt) {
-    const int k = (k_first + kt) * 128 + dc * 16;
-    return kt < nk && k < K ? (uint32_t)k : kOOB;
+    const int k = kt * 128 + dc * 16;
+    return k < K ? (uint32_t)k : kOOB;
   };
   auto dma_x = [&](int kt, int i) {
     dma16(rx, xoff[i] + kofs(kt), lbase + (uint32_t)(kt % NS * kX + (wave + NW * i) * 1024));
@@ -182,7 +175,7 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
           lbase + (uint32_t)(kW0 + kt % NS * kW + (wave + NW * i) * 1024));
   };
   auto dma_s = [&](int kt, int s) {
-    dma4(make_rsrc(sp[s], sbytes[s]), kt < nk ? (uint32_t)((k_first + kt) * 256 + lane * 4) : kOOB,
+    dma4(make_rsrc(sp[s], sbytes[s]), kt < nk ? (uint32_t)(kt * 256 + lane * 4) : kOOB,
          lbase + (uint32_t)(kS0 + (kt & 3) * kS + (wave + NW * s) * 256));
   };
   // d-th load of what is issued in the columns before the stage barrier: scales, weights (and with more slots x).
@@ -341,14 +334,7 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
       float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
       const int64_t m = m0 + r0 + r;
       const int n = n0 + 8 * c;
-      if (t.part) {
-        float* o = t.part + ((int64_t)blockIdx.z * p.M + m) * t.N + col0 + n;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < left) o[e] = v[e];
-      } else {
-        finish8(p, seg, m, n, col0 + n, left, vec, !SW, v);
-      }
+      finish8(p, seg, m, n, col0 + n, left, vec, !SW, v);
     }
   }
 }
@@ -438,18 +424,18 @@ int tiles_of(const Mx8Args& a, int bn) {
 }
 
 template <int BM, int BN, int WM, int WN, int NS, bool SW>
-void launch_tile(TileArgs t, int splits, hipStream_t st) {
+void launch_tile(TileArgs t, hipStream_t st) {
   t.tiles_m = (int)q3_cdiv(t.a.M, BM);
   t.tiles_n = tiles_of(t.a, SW ? BN / 2 : BN);
-  hipLaunchKernelGGL((mx8_tile_kernel<BM, BN, WM, WN, NS, SW>), dim3((unsigned)(t.tiles_m * t.tiles_n), 1, (unsigned)splits),
+  hipLaunchKernelGGL((mx8_tile_kernel<BM, BN, WM, WN, NS, SW>), dim3((unsigned)(t.tiles_m * t.tiles_n)),
                      dim3(WM * WN * 64), 0, st, t);
 }
 
 template <bool SW>
-void launch_form(const TileArgs& t, int form, int splits, hipStream_t st) {
-  if (form == 0) launch_tile<256, 256, 2, 4, 2, SW>(t, splits, st);
-  else if (form == 1) launch_tile<128, 256, 2, 4, 3, SW>(t, splits, st);
-  else launch_tile<128, 128, 2, 2, 2, SW>(t, splits, st);
+void launch_form(const TileArgs& t, int form, hipStream_t st) {
+  if (form == 0) launch_tile<256, 256, 2, 4, 2, SW>(t, st);
+  else if (form == 1) launch_tile<128, 256, 2, 4, 3, SW>(t, st);
+  else launch_tile<128, 128, 2, 2, 2, SW>(t, st);
 }
 
 int form_of(const Mx8Args& a, bool swiglu) {
@@ -471,11 +457,9 @@ int64_t mx8_tile_workspace(const Mx8Args& a, bool swiglu) {
   return bytes;
 }
 
-int mx8_tile(const Mx8Args& a, int64_t N, bool swiglu, void* workspace, hipStream_t st) {
+int mx8_tile(const Mx8Args& a, bool swiglu, void* workspace, hipStream_t st) {
   TileArgs t{};
   t.a = a;
-  t.N = (int)N;
-  t.kt = (int)q3_cdiv(a.K, 128);
 
   LayArgs l{};
   l.kb = a.K / kMx8Block;
@@ -500,8 +484,8 @@ int mx8_tile(const Mx8Args& a, int64_t N, bool swiglu, void* workspace, hipStrea
   hipLaunchKernelGGL(mx8_lay_scales_kernel, dim3((unsigned)q3_cdiv(waves, 4)), dim3(256), 0, st, l);
   Q3_LAUNCH_CHECK();
   const int form = form_of(a, swiglu);
-  if (swiglu) launch_form<true>(t, form, 1, st);
-  else launch_form<false>(t, form, 1, st);
+  if (swiglu) launch_form<true>(t, form, st);
+  else launch_form<false>(t, form, st);
   Q3_LAUNCH_CHECK();
   return Q3_OK;
 }

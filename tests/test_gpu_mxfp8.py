@@ -326,6 +326,37 @@ def test_segments_of_exact_values(m, ns, k):
     assert torch.equal(y, torch.cat(parts, -1))
 
 
+@pytest.mark.parametrize("m,n,k", [(1030, 2100, 384), (1600, 4400, 256), (3300, 4100, 384), (2600, 6500, 160)])
+def test_tiles_of_every_size(m, n, k):
+    """More rows and columns than 512 blocks of 64 by 64 cover: exact sums, one weight, two, and of SwiGLU."""
+    x, g, u = ((c, s - 5) for c, s in (exact_pair(r, k, i) for i, r in enumerate((m, n, n))))
+    xd, gd, ud = dev(x), dev(g), dev(u)
+    a, b = (M.values(*x).float() @ M.values(*w).float().T for w in (g, u))  # exact in 24 bits
+    r = rnd(m, n, seed=2)
+    assert torch.equal(K.matmul_mxfp8(xd, gd).cpu(), a.to(torch.bfloat16))
+    want, tol = a.double() + r.double(), 2.0 ** -22 * (a.double().abs() + r.double().abs())
+    check(K.matmul_mxfp8(xd, gd, residual=r.to(DEV)), want, tol)
+    cut = n // 2 + 3
+    y = K.matmul_segments_mxfp8(xd, [(gd[0][:cut], gd[1][:cut]), (ud[0][cut:], ud[1][cut:])])
+    assert torch.equal(y.cpu(), torch.cat([a[:, :cut], b[:, cut:]], -1).to(torch.bfloat16))
+    s = a.double() * torch.sigmoid(a.double())
+    want, err = s * b.double(), (2.0 ** -20 + 2.0 ** -22) * (s * b.double()).abs() + 2.0 ** -30
+    check(K.matmul_swiglu_mxfp8(xd, gd, ud), want, err)
+    n -= n % 32
+    pair = K.matmul_swiglu_mxfp8(xd, (gd[0][:n], gd[1][:n]), (ud[0][:n], ud[1][:n]), quantize=True)
+    check_eight_bits(pair, want[:, :n], err[:, :n])
+
+
+@pytest.mark.parametrize("m", [65, 127, 129, 200])
+@pytest.mark.parametrize("n,k", [(4, 128), (100, 640), (2000, 1152), (4096, 4224)])
+def test_rows_in_parts_of_64(m, n, k):
+    x, w, r = exact_pair(m, k, m), exact_pair(n, k, n), rnd(m, n, seed=3)
+    want = M.values(*x).float() @ M.values(*w).float().T
+    assert torch.equal(K.matmul_mxfp8(dev(x), dev(w)).cpu(), want.to(torch.bfloat16))
+    want = want.double() + r.double()
+    check(K.matmul_mxfp8(dev(x), dev(w), residual=r.to(DEV)), want, 2.0 ** -22 * ((want - r.double()).abs() + r.double().abs()))
+
+
 def test_bf16_rows_are_quantised_first():
     x, w = rnd(2, 40, 256, seed=1).to(DEV), dev(normal_pair(64, 256, 2))
     pair = K.mxfp8_quantize(x)
