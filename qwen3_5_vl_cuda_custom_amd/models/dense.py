@@ -16,8 +16,8 @@ from torch import nn
 
 from ..configs import Qwen3VLConfig
 from ..kernels import cuda_index_add
-from ..modules import (CudaEmbedding, CudaLinear, CudaLinearMXFP4, CudaRMSNorm, CudaTextDecoderLayer, MXFP4KVCache,
-                       PagedKVCache, StaticKVCache, StepGraph, TextMRoPE)
+from ..modules import (CudaEmbedding, CudaLinear, CudaLinearMXFP4, CudaLinearMXFP8, CudaRMSNorm, CudaTextDecoderLayer,
+                       MXFP4KVCache, PagedKVCache, StaticKVCache, StepGraph, TextMRoPE)
 from .common import CudaVisionTower
 
 
@@ -86,9 +86,9 @@ class _TextLM(nn.Module):
         return self.norm(x), new_kvs
 
     def _head_weight(self) -> torch.Tensor:
-        """The tensor whose device and type the serving path goes by: lm_head's weight, or where that is in four bits
-        the final norm's."""
-        return self.norm.weight if isinstance(self.lm_head, CudaLinearMXFP4) else self.lm_head.weight
+        """The tensor whose device and type the serving path goes by: lm_head's weight, or where that is in four or
+        eight bits the final norm's."""
+        return self.norm.weight if isinstance(self.lm_head, (CudaLinearMXFP4, CudaLinearMXFP8)) else self.lm_head.weight
 
     # ------------------------------------------------------------ KV-cache serving path
     def new_caches(self, batch: int, capacity: int, device=None, dtype=None, *, page_rows: int = 0,

@@ -6,6 +6,7 @@ from .graph import StepGraph
 from .kv_cache import MXFP4KVCache, PagedKVCache, StaticKVCache
 from .linear import CudaLinear
 from .linear_mxfp4 import CudaLinearMXFP4
+from .linear_mxfp8 import CudaLinearMXFP8
 from .mlp import CudaSwiGLUMLP, CudaVisionMLP
 from .moe import CudaSparseMoE
 from .norms import CudaLayerNorm, CudaRMSNorm
@@ -36,6 +37,7 @@ __all__ = [
     "StaticKVCache",
     "MXFP4KVCache",
     "CudaLinearMXFP4",
+    "CudaLinearMXFP8",
     "quantize_text_linears",
     "StepGraph",
 ]

@@ -10,11 +10,12 @@ from ..kernels.backward import (FlashAttentionFunction, QKNormRopeFunction, Rope
 from ..kernels import (apply_rope, decode_attention, decode_attention_mxfp4, decode_attention_paged, flash_attention,
                        flash_attention_cache, flash_attention_cache_mxfp4, flash_attention_cache_paged,
                        flash_attention_varlen, kv_append_mxfp4, matmul, matmul_segments,
-                       matmul_segments_mxfp4, qk_norm_rope, qk_norm_rope_attention, qk_norm_rope_attention_ok, qk_norm_rope_mxfp4, qk_norm_rope_paged,
+                       matmul_segments_mxfp4, matmul_segments_mxfp8, qk_norm_rope, qk_norm_rope_attention, qk_norm_rope_attention_ok, qk_norm_rope_mxfp4, qk_norm_rope_paged,
                        rmsnorm_matmul_segments)
 from .kv_cache import MXFP4KVCache, PagedKVCache, StaticKVCache
 from .linear import CudaLinear
 from .linear_mxfp4 import CudaLinearMXFP4
+from .linear_mxfp8 import CudaLinearMXFP8, norm_to_eight_bits
 from .norms import CudaRMSNorm, fused_norm_ok, norm_operands
 from .rotary import MRoPEBinding, TextMRoPE
 
@@ -104,7 +105,8 @@ class CudaFullAttention(nn.Module):
       residual=tensor         added to o_proj's output in the GEMM epilogue
       input_norm=CudaRMSNorm  x is the layer input before this RMSNorm; for
                               decode shapes (at most 32 tokens, bf16) the norm
-                              runs inside the q/k/v projection, else first
+                              runs inside the q/k/v projection, else first (for
+                              weights in eight bits first, with x's quantisation)
     When `mrope_apply` is a TextMRoPE.bind(...) binding, q/k normalisation and
     rotation run as one fused kernel on the projection outputs; for a prefill
     without past_kv (bf16, GQA groups a multiple of 4), k's runs alone and q's
@@ -140,11 +142,14 @@ class CudaFullAttention(nn.Module):
         # q/k/v projections in one GEMM over the three weights (no concatenated
         # copy); q, k, v are column views of its output.
         projs = (self.q_proj, self.k_proj, self.v_proj)
-        four_bit = [isinstance(p, CudaLinearMXFP4) for p in projs]
-        if all(four_bit):
+        four_bit, eight_bit = ([isinstance(p, kind) for p in projs] for kind in (CudaLinearMXFP4, CudaLinearMXFP8))
+        if all(eight_bit):
+            qkv = matmul_segments_mxfp8(norm_to_eight_bits(x, input_norm), [p.pair for p in projs],
+                                        [p.bias for p in projs])
+        elif all(four_bit):
             nw, eps, x = (None, 0.0, x) if input_norm is None else norm_operands(x, input_norm)
             qkv = matmul_segments_mxfp4(x, [p.pair for p in projs], [p.bias for p in projs], norm_weight=nw, eps=eps)
-        elif any(four_bit):
+        elif any(four_bit) or any(eight_bit):
             qkv = self._project_apart(x if input_norm is None else input_norm(x), projs)
         else:  # any modules with a weight and a bias
             weights = tuple(p.weight for p in projs)
@@ -221,12 +226,13 @@ class CudaFullAttention(nn.Module):
 
     @staticmethod
     def _project_apart(x, projs) -> torch.Tensor:
-        """The q/k/v rows side by side where only some projections hold four-bit weights: one product each, into
-        its columns."""
-        ns = [p.out_features if isinstance(p, CudaLinearMXFP4) else p.weight.shape[0] for p in projs]
+        """The q/k/v rows side by side where only some projections hold weights in four or eight bits: one product
+        each, into its columns."""
+        quantized = (CudaLinearMXFP4, CudaLinearMXFP8)
+        ns = [p.out_features if isinstance(p, quantized) else p.weight.shape[0] for p in projs]
         qkv = torch.empty((*x.shape[:-1], sum(ns)), dtype=x.dtype, device=x.device)
         for p, out in zip(projs, qkv.split(ns, -1)):
-            if isinstance(p, CudaLinearMXFP4):
+            if isinstance(p, quantized):
                 p(x, out=out)
             else:
                 matmul(x, p.weight, p.bias, out=out)

@@ -4,11 +4,12 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from ..kernels import gelu_tanh, matmul_gelu, matmul_swiglu, matmul_swiglu_mxfp4, rmsnorm_matmul_swiglu, swiglu
+from ..kernels import gelu_tanh, matmul_gelu, matmul_swiglu, matmul_swiglu_mxfp4, matmul_swiglu_mxfp8, rmsnorm_matmul_swiglu, swiglu
 from ..kernels.backward import needs_grad
 from ..kernels.matmul import line_padded_rows
 from .linear import CudaLinear
 from .linear_mxfp4 import CudaLinearMXFP4
+from .linear_mxfp8 import CudaLinearMXFP8, norm_to_eight_bits
 from .norms import CudaRMSNorm, fused_norm_ok, norm_operands
 
 
@@ -31,21 +32,28 @@ class CudaSwiGLUMLP(nn.Module):
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, *,
                 input_norm: CudaRMSNorm | None = None) -> torch.Tensor:
         """`input_norm`: x is taken before this RMSNorm; for decode shapes (at
-        most 32 bf16 tokens) it runs inside the gate/up GEMM, else first."""
+        most 32 bf16 tokens) it runs inside the gate/up GEMM, else first. With
+        weights in eight bits it runs first, in the launch that quantises x,
+        and the activation stays in eight bits for down_proj."""
         if needs_grad(x, residual, *self.parameters()):  # training: modules/mlp.py:19-22 on differentiable ops
             if input_norm is not None:
                 x = input_norm(x)
             return self.down_proj(swiglu(self.gate_proj(x), self.up_proj(x)), residual=residual)
-        four_bit = [isinstance(p, CudaLinearMXFP4) for p in (self.gate_proj, self.up_proj)]
-        if all(four_bit) and self.gate_proj.bias is None and self.up_proj.bias is None:
+        no_bias = self.gate_proj.bias is None and self.up_proj.bias is None
+        four_bit, eight_bit = ([isinstance(p, kind) for p in (self.gate_proj, self.up_proj)]
+                               for kind in (CudaLinearMXFP4, CudaLinearMXFP8))
+        if all(eight_bit) and no_bias:
+            act = matmul_swiglu_mxfp8(norm_to_eight_bits(x, input_norm), self.gate_proj.pair, self.up_proj.pair,
+                                      quantize=isinstance(self.down_proj, CudaLinearMXFP8))
+            return self.down_proj(act, residual=residual)
+        if all(four_bit) and no_bias:
             nw, eps, x = (None, 0.0, x) if input_norm is None else norm_operands(x, input_norm)
             act = matmul_swiglu_mxfp4(x, self.gate_proj.pair, self.up_proj.pair, norm_weight=nw, eps=eps)
             return self.down_proj(act, residual=residual)
-        if any(four_bit):  # in one of them, or with a bias: each projection by its own forward
+        if any(four_bit) or any(eight_bit):  # in one of them, or with a bias: each projection by its own forward
             if input_norm is not None:
                 x = input_norm(x)
             return self.down_proj(swiglu(self.gate_proj(x), self.up_proj(x)), residual=residual)
-        no_bias = self.gate_proj.bias is None and self.up_proj.bias is None
         if input_norm is not None and no_bias and fused_norm_ok(x, input_norm):
             act = rmsnorm_matmul_swiglu(x, input_norm.weight, input_norm.eps, self.gate_proj.weight,
                                         self.up_proj.weight)
