@@ -4,23 +4,36 @@
 // Codes go global -> LDS past the registers (buffer loads with the lds flag), a stage of
 // 128 k (one matrix instruction's) at a time, 128 bytes a row. Row r keeps its 16-byte
 // chunk c at slot c ^ (r & 7), which leaves the fragments' reads without bank conflicts
-// (with r >> 3 in the exclusive or as well, 3.5 cycles each were counted). A wave holds the
-// stage's TN weight fragments and takes the TM fragments of x (columns, below) one after
-// the other, each read three columns ahead, TN products to a column. Before the last two
-// columns every fragment of the stage has been read: there the stage barrier stands, the
-// next stage's fragments are read between the products after it, each weight fragment once
-// its last product has issued. No branch stands in the loop: the compiler moves products
-// past one.
+// (with r >> 3 in the exclusive or as well, 3.5 cycles each were counted). The instructions
+// of a full chip run at 3.5 to 3.75 PFLOP/s with nothing else to do (the clock falls to
+// 2.0 GHz), and no branch stands in the loops: the compiler moves products past one.
 //
-// With two slots (256 x 256 tiles fill the LDS) a stage's weight slot is free once every
-// wave has the fragments, after the first column: a second barrier there lets the weights
-// after next, which come from further away than x, set out most of a stage earlier.
+// 256 x 256 tiles, eight waves of 128 x 64: a wave holds the stage's TN weight fragments and
+// takes the TM fragments of x (columns, below) one after the other, each read three columns
+// ahead, TN products to a column. Before the last two columns every fragment of the stage
+// has been read: there the stage barrier stands, the next stage's fragments are read between
+// the products after it, each weight fragment once its last product has issued. The two slots
+// fill the LDS; a stage's weight slot is free once every wave has the fragments, after the
+// first column: a second barrier there lets the weights after next, which come from further
+// away than x, set out most of a stage earlier. Gate and up of 4096 rows, N 12288, K 4096:
+// 313 us with the scales' launch, 2.63 PFLOP/s (matrix pipe busy 62 %; without the loads of
+// codes 282); N 4096, K 12288 174 us.
+//
+// Smaller tiles, four waves of 64 x 128 or 64 x 64 for 128 x 256 and 128 x 128: one wave a SIMD
+// has the registers for two stages' fragments. It reads all of the next stage's between the
+// products of this one, so a slot is free at the barrier where its stage begins, and three or
+// four slots stay under way. Eight waves, each reading as above, took 76 us for SwiGLU of 611
+// rows, N 12288 (these 74) and 34.6 for 1000 rows, N = K = 4096 (these 27.4); of the other
+// way, tiles of 256 x 256, the first takes 86, the second 52.
 //
 // Scales are laid out anew first, by a kernel of their own: the scales of 64 rows and four
 // stages are 1 KB as the instruction's lanes take them, word l of a stage lane l's block
 // of rows l % 16, + 16, + 32, + 48 (the instruction picks the byte). A load brings a stage
 // of them, and three words a stage are all that a wave reads. As rows of bytes their loads
-// cost a line per row and the reads twelve bytes a stage.
+// cost a line per row and the reads twelve bytes a stage: 198 against 194 us for 4096 x 4096
+// x 12288 when it was tried. Where one round of 128 x 128 tiles does it all the launch costs
+// more (2.7 to 4 us), and the scales come by rows (RAW), 16 bytes, four stages', of a row at a
+// time: 784 rows of K 1152, N 4304 17.6 to 14.6 us, 1000 rows above 27.9 to 26.4.
 #include "gemm_tile.h"
 #include "mxfp8.h"
 #include "mxfp8_tile.h"
@@ -36,27 +49,24 @@ struct TileArgs {
   int tiles_m, tiles_n;
 };
 
-// Eight columns of y from n on (of its segment; `left` of them exist), the row's m.
-__device__ __forceinline__ void finish8(const Mx8Args& p, int seg, int64_t m, int n, int col, int left, bool vec,
-                                        bool plain, float (&v)[8]) {
-  if (plain) {
-    const bf16* bias = p.bias[seg];
-    if (bias) {
+// Eight columns of y from col on (`left` of them exist), the row's m. PLAIN: with bias, activation and residual, the
+// last eight values in `res` where all go in 16-byte pieces (`vec`).
+template <bool PLAIN>
+__device__ __forceinline__ void finish8(const Mx8Args& p, int64_t m, int col, int left, bool vec, const float (&bias)[8],
+                                        const bf16x8& res, float (&v)[8]) {
+  if (PLAIN) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left) v[e] += bf2f(bias[n + e]);
-    }
+    for (int e = 0; e < 8; ++e) v[e] += bias[e];
     if (p.act) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = mx8_act(v[e], p.act);
     }
     if (p.res) {
-      const bf16* r = p.res + m * p.ldr + col;
-      if (vec && left >= 8) {
-        const bf16x8 b = *reinterpret_cast<const bf16x8*>(r);
+      if (vec) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += bf2f(b[e]);
+        for (int e = 0; e < 8; ++e) v[e] += bf2f(res[e]);
       } else {
+        const bf16* r = p.res + m * p.ldr + col;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (e < left) v[e] += bf2f(r[e]);
@@ -71,7 +81,7 @@ __device__ __forceinline__ void finish8(const Mx8Args& p, int seg, int64_t m, in
     return;
   }
   bf16* y = p.y + m * p.ldc + col;
-  if (vec && left >= 8) {
+  if (vec) {
     bf16x8 o;
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = f2bf(v[e]);
@@ -100,15 +110,18 @@ __device__ __forceinline__ floatx4 mfma_of(i32x8 a, i32x8 b, floatx4 c, int sa, 
   return c;
 }
 
-template <int BM, int BN, int WM, int WN, int NS, bool SW>
+template <int BM, int BN, int WM, int WN, int NS, bool SW, bool RAW>
 __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t) {
   constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
   constexpr int BN_OUT = SW ? BN / 2 : BN;
   constexpr int GX = BM / 64, GS = (BM + BN) / 64, PS = (GS + NW - 1) / NW;  // groups of 64 rows; loads of scales
   constexpr int PX = BM / 8 / NW, PW = BN / 8 / NW;                          // loads of codes per wave and stage
-  constexpr bool EARLY = NS == 2;  // the weights' slot is released by a barrier of its own
-  constexpr int kX = BM * 128, kW = BN * 128, kS = PS * NW * 256, kLds = NS * (kX + kW) + 4 * kS;
+  constexpr bool EARLY = NW == 8 && NS == 2;  // the weights' slot is released by a barrier of its own
+  constexpr bool PIPE = NW == 4;  // one wave a SIMD: room for two stages' fragments in registers
+  constexpr int kX = BM * 128, kW = BN * 128, kS = RAW ? (BM + BN) * 16 : PS * NW * 256;
+  constexpr int kLds = NS * (kX + kW) + 4 * kS;
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NW % 2 == 0, "whole loads per wave, one swizzle per lane");
+  static_assert(!RAW || (PIPE && GS == NW && NS <= 4), "scales by rows: a wave to 64 rows");
   static_assert(TM % 4 == 0 && TN == 4 && kLds <= 160 * 1024, "wave tiles");
   __shared__ __attribute__((aligned(1024))) char smem[kLds];
 
@@ -149,6 +162,18 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
   // Scales: load s of this wave is a stage of 64 rows, x's and then the weights'.
   const uint8_t* sp[PS];
   int sbytes[PS];
+  const int kb = K / kMx8Block;
+  if constexpr (RAW) {  // by rows: this wave's 64
+    const uint8_t* of = p.xs + (int64_t)(m0 + 64 * wave) * kb;
+    int rows = rows_m - 64 * wave;
+    if (64 * wave >= BM) {
+      const int first = (SW ? 32 : 64) * (wave - BM / 64);
+      of = p.ws[SW ? 0 : seg] + (int64_t)(n0 + first) * kb;
+      rows = rows_n - first;
+    }
+    sp[0] = mx8_pin(of);
+    sbytes[0] = mx8_pin(max(rows, 0) * kb);
+  } else {
 #pragma unroll
   for (int s = 0; s < PS; ++s) {
     const int e = wave + NW * s;
@@ -158,6 +183,7 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
     const int all = of_x ? (p.M + 63) / 64 : SW ? (p.n[0] + 31) / 32 : (p.n[seg] + 63) / 64;
     sp[s] = mx8_pin((of_x ? t.xs : t.ws[seg]) + (int64_t)g * groups_k * 1024);
     sbytes[s] = mx8_pin(e < GS && g < all ? groups_k * 1024 : 0);
+  }
   }
   const uint32_t lbase = lds_addr(smem);
   constexpr int kW0 = NS * kX, kS0 = kW0 + NS * kW;
@@ -175,6 +201,16 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
           lbase + (uint32_t)(kW0 + kt % NS * kW + (wave + NW * i) * 1024));
   };
   auto dma_s = [&](int kt, int s) {
+    if constexpr (RAW) {
+      // 16 of the wave's rows: 16 bytes, the scales of four stages, of the group of stages after kt's
+      const int g = (kt >> 2) + 1, u = kt & 3, row = 16 * u + (lane >> 2), st = 4 * g + (lane & 3);
+      const uint8_t* of = sp[0];
+      int at = row;
+      if (SW && wave >= BM / 64 && u >= 2) of = p.ws[1] + (int64_t)(n0 + 32 * (wave - BM / 64)) * kb, at = row - 32;
+      dma4(make_rsrc(mx8_pin(of), sbytes[0]), st < nk ? (uint32_t)(at * kb + 4 * st) : kOOB,
+           lbase + (uint32_t)(kS0 + (g & 3) * kS + (64 * wave + 16 * u) * 16));
+      return;
+    }
     dma4(make_rsrc(sp[s], sbytes[s]), kt < nk ? (uint32_t)(kt * 256 + lane * 4) : kOOB,
          lbase + (uint32_t)(kS0 + (kt & 3) * kS + (wave + NW * s) * 256));
   };
@@ -215,8 +251,12 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
   };
   auto mf = [&](int i, int j) { acc[i][j] = mfma_of(fw[i], fx[j & 3], acc[i][j], sw, sx[j / 4], i, j & 3); };
 
-  constexpr int kAhead = EARLY ? 2 : NS - 1;  // stages issued before the loop
+  constexpr int kAhead = EARLY ? 2 : PIPE ? NS : NS - 1;  // stages issued before the loop
   constexpr int kAll = PX + PW + PS;
+  if constexpr (RAW) {
+#pragma unroll
+    for (int s = -4; s < 0; ++s) dma_s(s, 0);  // the first four stages'
+  }
 #pragma unroll
   for (int s = 0; s < kAhead; ++s) {
 #pragma unroll
@@ -229,6 +269,78 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
   vm_wait<(kAhead - 1) * kAll>();  // stage 0 has landed
   __syncthreads();
 
+  if constexpr (PIPE) {
+    i32x8 pw[2][TN], px[2][TM];
+    int zw[2][RAW ? TN : 1], zx[2][RAW ? TM : TM / 4];
+    const char* const xrow = smem + (rm + l16) * 128;
+    const char* const wrow = smem + kW0 + (rn + l16) * 128;
+    const int c0 = (q4 ^ (l16 & 7)) << 4, c1 = ((4 + q4) ^ (l16 & 7)) << 4;
+    // Read number n of a stage in slot `at`, to fragments g: the weights', then x's.
+    auto read = [&](int g, int n, int at_x, int at_w) __attribute__((always_inline)) {
+      const bool w = n < 2 * TN;
+      const int f = w ? n / 2 : n / 2 - TN;
+      const char* const from = (w ? wrow + at_w : xrow + at_x) + f * 2048 + (n & 1 ? c1 : c0);
+      const i32x4 v = *reinterpret_cast<const i32x4*>(from);
+      i32x8& to = w ? pw[g][f] : px[g][f];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[4 * (n & 1) + e] = v[e];
+    };
+    auto read_s = [&](int g, int kt) __attribute__((always_inline)) {
+      if constexpr (RAW) {
+        const uint8_t* const z = reinterpret_cast<const uint8_t*>(smem) + kS0 + (kt >> 2 & 3) * kS + (kt & 3) * 4 + l16 * 16 + q4;
+#pragma unroll
+        for (int i = 0; i < TN; ++i) zw[g][i] = z[(BM + rn + 16 * i) * 16];
+#pragma unroll
+        for (int j = 0; j < TM; ++j) zx[g][j] = z[(rm + 16 * j) * 16];
+      } else {
+        const char* const z = smem + kS0 + (kt & 3) * kS + lane * 4;
+        zw[g][0] = *reinterpret_cast<const int*>(z + (GX + rn / 64) * 256);
+#pragma unroll
+        for (int j = 0; j < TM / 4; ++j) zx[g][j] = *reinterpret_cast<const int*>(z + (rm / 64 + j) * 256);
+      }
+    };
+    read_s(0, 0);
+#pragma unroll
+    for (int n = 0; n < 2 * (TN + TM); ++n) read(0, n, 0, 0);
+    int cur = 0;  // slot of the stage at hand
+    auto stage = [&](auto parity, int kt) __attribute__((always_inline)) {
+      constexpr int G = decltype(parity)::value;
+      const int nxt = cur + 1 == NS ? 0 : cur + 1;
+      // Stage kt + 1 has landed, and every wave holds stage kt: its slot is free.
+      vm_wait<(NS - 2) * kAll>();
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      constexpr int kReads = 2 * (TN + TM), kMf = TN * TM, kLoads = PS + PW + PX;
+      int n = 0, d = 0;
+#pragma unroll
+      for (int m = 0; m < kMf; ++m) {
+        acc[m % TN][m / TN] =
+            RAW ? mfma_of(pw[G][m % TN], px[G][m / TN], acc[m % TN][m / TN], zw[G][RAW ? m % TN : 0], zx[G][RAW ? m / TN : 0], 0, 0)
+                : mfma_of(pw[G][m % TN], px[G][m / TN], acc[m % TN][m / TN], zw[G][0], zx[G][RAW ? 0 : m / TN / 4], m % TN, m / TN & 3);
+        if (m == 0) read_s(G ^ 1, kt + 1);
+        for (; n < kReads && n * (kMf - 4) < (m + 1) * kReads; ++n) read(G ^ 1, n, nxt * kX, nxt * kW);
+        for (; d < kLoads && d * (kMf - 2) < m * kLoads; ++d) {
+          const int at = kt + NS;
+          if (d < PS) dma_s(at, d);
+          else if (d < PS + PW) dma16(make_rsrc(SW ? mx8_pin(((wave + NW * (d - PS)) & 4) ? wb : wa) : wa, rows_n * K),
+                                      woff[d - PS] + kofs(at), lbase + (uint32_t)(kW0 + cur * kW + (wave + NW * (d - PS)) * 1024));
+          else dma16(rx, xoff[d - PS - PW] + kofs(at), lbase + (uint32_t)(cur * kX + (wave + NW * (d - PS - PW)) * 1024));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      cur = nxt;
+    };
+    for (int kt = 0; kt < nk; kt += 2) {  // an odd last stage's partner is zeros
+      stage(std::integral_constant<int, 0>{}, kt);
+      stage(std::integral_constant<int, 1>{}, kt + 1);
+    }
+#pragma unroll
+    for (int i = 0; i < TN; ++i)  // (the accumulators stay where they are: without this they are copied around each turn)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) asm volatile("" : "+a"(acc[i][j]));
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+  }
   auto main = [&](auto active_c) {
     constexpr bool A = decltype(active_c)::value;  // a wave without rows loads and waits only
     if constexpr (A) {
@@ -292,20 +404,39 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  if (rm < rows_m) main(std::true_type{});
-  else main(std::false_type{});
+  if constexpr (!PIPE) {
+    if (rm < rows_m) main(std::true_type{});
+    else main(std::false_type{});
+  }
   vm_wait<0>();  // the loads past the last stage (zeros) have landed
 
-  // Epilogue: the accumulators through LDS in fp32, up to RP rows at a time, so that a lane then has eight columns of a
-  // row. 16-byte chunk c of row r lies at c ^ (r & 15).
+  // Epilogue: the accumulators through LDS in fp32, up to RP rows at a time, so that a thread then has eight columns of
+  // a row, the same columns in every RS-th row: its residuals are under way before the accumulators are in LDS (loaded
+  // one row at a time, each row's latency stood in the 6 us after the last product). 16-byte chunk c of row r lies at
+  // c ^ (r & 15).
   constexpr int RP0 = kLds / (BN_OUT * 4), RP = RP0 >= BM ? BM : RP0 >= 128 ? 128 : RP0 >= 64 ? 64 : 32;
-  static_assert(RP0 >= 32 && BN_OUT % 64 == 0, "epilogue");
-  constexpr int C8 = BN_OUT / 8;
+  constexpr int C8 = BN_OUT / 8, RS = NW * 64 / C8;
+  static_assert(RP0 >= 32 && BN_OUT % 64 == 0 && NW * 64 % C8 == 0 && RP % RS == 0, "epilogue");
   float* lds = reinterpret_cast<float*>(smem);
   auto slot = [](int r, int c) { return r * BN_OUT + ((c ^ (r & 15)) << 2); };
-  const bool vec = vec_of(p, col0);
+  const int c8 = tid % C8, r8 = tid / C8, left = rows_n - 8 * c8, n8 = n0 + 8 * c8, col = col0 + n8;
+  const bool vec = vec_of(p, col0) && left >= 8;
+  float bias[8] = {};
+  if (!SW && p.bias[seg]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) bias[e] = bf2f(p.bias[seg][n8 + e]);
+  }
 #pragma unroll
   for (int r0 = 0; r0 < BM; r0 += RP) {
+    bf16x8 res[RP / RS];
+#pragma unroll
+    for (int u = 0; u < RP / RS; ++u) {
+      const int r = r0 + r8 + u * RS;
+      res[u] = bf16x8{};
+      if (!SW && p.res && vec && r < rows_m)
+        res[u] = *reinterpret_cast<const bf16x8*>(p.res + (int64_t)(m0 + r) * p.ldr + col);
+    }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
@@ -325,16 +456,14 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
       }
     }
     __syncthreads();
-    const int items = min(RP, rows_m - r0) * C8;
-    for (int it = tid; it < items; it += NW * 64) {
-      const int r = it / C8, c = it % C8, left = rows_n - 8 * c;
-      if (left <= 0) continue;
-      const floatx4 a = *reinterpret_cast<const floatx4*>(lds + slot(r, 2 * c));
-      const floatx4 b = *reinterpret_cast<const floatx4*>(lds + slot(r, 2 * c + 1));
+#pragma unroll
+    for (int u = 0; u < RP / RS; ++u) {
+      const int r = r8 + u * RS;
+      if (r0 + r >= rows_m || left <= 0) continue;
+      const floatx4 a = *reinterpret_cast<const floatx4*>(lds + slot(r, 2 * c8));
+      const floatx4 b = *reinterpret_cast<const floatx4*>(lds + slot(r, 2 * c8 + 1));
       float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-      const int64_t m = m0 + r0 + r;
-      const int n = n0 + 8 * c;
-      finish8(p, seg, m, n, col0 + n, left, vec, !SW, v);
+      finish8<!SW>(p, m0 + r0 + r, col, left, vec, bias, res[u], v);
     }
   }
 }
@@ -423,44 +552,41 @@ int tiles_of(const Mx8Args& a, int bn) {
   return (int)n;
 }
 
-template <int BM, int BN, int WM, int WN, int NS, bool SW>
+template <int BM, int BN, int WM, int WN, int NS, bool SW, bool RAW = false>
 void launch_tile(TileArgs t, hipStream_t st) {
   t.tiles_m = (int)q3_cdiv(t.a.M, BM);
   t.tiles_n = tiles_of(t.a, SW ? BN / 2 : BN);
-  hipLaunchKernelGGL((mx8_tile_kernel<BM, BN, WM, WN, NS, SW>), dim3((unsigned)(t.tiles_m * t.tiles_n)),
+  hipLaunchKernelGGL((mx8_tile_kernel<BM, BN, WM, WN, NS, SW, RAW>), dim3((unsigned)(t.tiles_m * t.tiles_n)),
                      dim3(WM * WN * 64), 0, st, t);
 }
 
+// Forms: tiles of 256 x 256, 128 x 256, 128 x 128, and of the last with the scales by rows.
 template <bool SW>
 void launch_form(const TileArgs& t, int form, hipStream_t st) {
   if (form == 0) launch_tile<256, 256, 2, 4, 2, SW>(t, st);
-  else if (form == 1) launch_tile<128, 256, 2, 4, 3, SW>(t, st);
-  else launch_tile<128, 128, 2, 2, 2, SW>(t, st);
+  else if (form == 1) launch_tile<128, 256, 1, 4, 3, SW>(t, st);
+  else if (form == 2) launch_tile<128, 128, 2, 2, 4, SW>(t, st);
+  else launch_tile<128, 128, 2, 2, 4, SW, true>(t, st);
 }
 
+// The form whose rounds over the CUs (one block each) cost least; a round's stage takes 1.57, 1.0 and 0.6 us in the
+// forms' full rounds (4096 rows, N 4096 and 24576, epilogues included). Measured with each form forced, in us: SwiGLU of
+// 611 rows, N 12288 86, 77 and 90 (2, 2 and 4 rounds), 2048 rows, N = K = 4096 55, 43 and 48 (1, 1, 2), 3000 rows 56, 72
+// and 69 (1, 2, 3), 1000 rows 52, 38 and 26 (1 each).
 int form_of(const Mx8Args& a, bool swiglu) {
   const int out = swiglu ? 2 : 1;
-  return q3_cdiv(a.M, 256) * tiles_of(a, 256 / out) >= 200 ? 0 : q3_cdiv(a.M, 128) * tiles_of(a, 256 / out) >= 200 ? 1 : 2;
+  auto cost = [&](int bm, int bn, int64_t stage) { return q3_cdiv(q3_cdiv(a.M, bm) * tiles_of(a, bn / out), 256) * stage; };
+  const int64_t c0 = cost(256, 256, 16), c1 = cost(128, 256, 10), c2 = cost(128, 128, 6);
+  if (c0 <= c1 && c0 <= c2) return 0;
+  return c1 <= c2 ? 1 : a.K % 128 == 0 ? 3 : 2;
 }
 
 // Bytes of laid out scales of n rows.
 int64_t laid_bytes(int64_t n, int64_t K) { return q3_cdiv(n, 64) * q3_cdiv(K, 512) * 1024; }
 
-}  // namespace
-
-namespace q3 {
-
-int64_t mx8_tile_workspace(const Mx8Args& a, bool swiglu) {
-  int64_t bytes = laid_bytes(a.M, a.K);
-  if (swiglu) return bytes + laid_bytes(2 * q3_cdiv(a.n[0], 32) * 32, a.K);
-  for (int j = 0; j < a.nseg; ++j) bytes += laid_bytes(a.n[j], a.K);
-  return bytes;
-}
-
-int mx8_tile(const Mx8Args& a, bool swiglu, void* workspace, hipStream_t st) {
-  TileArgs t{};
-  t.a = a;
-
+// The scales of t's operands laid out in the workspace.
+int lay_scales(TileArgs& t, bool swiglu, void* workspace, hipStream_t st) {
+  const Mx8Args& a = t.a;
   LayArgs l{};
   l.kb = a.K / kMx8Block;
   l.groups_k = (int)q3_cdiv(a.K, 512);
@@ -483,7 +609,27 @@ int mx8_tile(const Mx8Args& a, bool swiglu, void* workspace, hipStream_t st) {
   l.waves = (int)waves;
   hipLaunchKernelGGL(mx8_lay_scales_kernel, dim3((unsigned)q3_cdiv(waves, 4)), dim3(256), 0, st, l);
   Q3_LAUNCH_CHECK();
+  return Q3_OK;
+}
+
+}  // namespace
+
+namespace q3 {
+
+int64_t mx8_tile_workspace(const Mx8Args& a, bool swiglu) {
+  if (form_of(a, swiglu) == 3) return 0;
+  int64_t bytes = laid_bytes(a.M, a.K);
+  if (swiglu) return bytes + laid_bytes(2 * q3_cdiv(a.n[0], 32) * 32, a.K);
+  for (int j = 0; j < a.nseg; ++j) bytes += laid_bytes(a.n[j], a.K);
+  return bytes;
+}
+
+int mx8_tile(const Mx8Args& a, bool swiglu, void* workspace, hipStream_t st) {
+  TileArgs t{};
+  t.a = a;
   const int form = form_of(a, swiglu);
+  if (form < 3)
+    if (const int rc = lay_scales(t, swiglu, workspace, st)) return rc;
   if (swiglu) launch_form<true>(t, form, st);
   else launch_form<false>(t, form, st);
   Q3_LAUNCH_CHECK();

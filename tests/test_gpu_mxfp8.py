@@ -326,7 +326,8 @@ def test_segments_of_exact_values(m, ns, k):
     assert torch.equal(y, torch.cat(parts, -1))
 
 
-@pytest.mark.parametrize("m,n,k", [(1030, 2100, 384), (1600, 4400, 256), (3300, 4100, 384), (2600, 6500, 160)])
+@pytest.mark.parametrize("m,n,k", [(1030, 2100, 384), (1600, 4400, 256), (3300, 4100, 384), (2600, 6500, 160),
+                                   (700, 1500, 640), (900, 2300, 1152)])
 def test_tiles_of_every_size(m, n, k):
     """More rows and columns than 512 blocks of 64 by 64 cover: exact sums, one weight, two, and of SwiGLU."""
     x, g, u = ((c, s - 5) for c, s in (exact_pair(r, k, i) for i, r in enumerate((m, n, n))))
@@ -345,6 +346,20 @@ def test_tiles_of_every_size(m, n, k):
     n -= n % 32
     pair = K.matmul_swiglu_mxfp8(xd, (gd[0][:n], gd[1][:n]), (ud[0][:n], ud[1][:n]), quantize=True)
     check_eight_bits(pair, want[:, :n], err[:, :n])
+
+
+@pytest.mark.parametrize("m,n,k", [(700, 2500, 640), (1600, 4400, 128), (3300, 4100, 384)])
+def test_nan_scales_stay_in_their_rows_and_columns_of_tiles(m, n, k):
+    """A row's first block is NaN: its neighbour's scales end right before it."""
+    x, w = exact_pair(m, k, 1), exact_pair(n, k, 2)
+    xs, ws = x[1].clone(), w[1].clone()
+    xs[5::97, 0] = 255
+    ws[7::101, 0] = 255
+    y = torch.isnan(K.matmul_mxfp8(dev((x[0], xs)), dev((w[0], ws)))).cpu()
+    want = torch.zeros(m, n, dtype=torch.bool)
+    want[5::97] = True
+    want[:, 7::101] = True
+    assert torch.equal(y, want)
 
 
 @pytest.mark.parametrize("m", [65, 127, 129, 200])
