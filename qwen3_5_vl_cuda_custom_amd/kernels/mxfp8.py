@@ -43,8 +43,8 @@ def _packed(op: str, codes: torch.Tensor, scales: torch.Tensor, dev: int) -> Pai
     """The pair checked, packed and aligned as the kernels read it."""
     cs, ss = codes.shape, scales.shape
     if (codes.dtype is _F8 and scales.dtype is _U8 and codes.get_device() == dev and scales.get_device() == dev
-            and codes.is_contiguous() and scales.is_contiguous() and cs and cs[:-1] == ss[:-1]
-            and cs[-1] == ss[-1] * MX8_BLOCK and not (codes.data_ptr() % 16 or scales.data_ptr() % 4)):
+            and codes.is_contiguous() and scales.is_contiguous() and len(cs) == 2 and len(ss) == 2 and cs[0] == ss[0]
+            and cs[1] == ss[1] * MX8_BLOCK and not (codes.data_ptr() % 16 or scales.data_ptr() % 4)):
         return codes, scales  # the usual call
     if codes.get_device() != dev or scales.get_device() != dev:
         _off_device(op, codes, scales)
