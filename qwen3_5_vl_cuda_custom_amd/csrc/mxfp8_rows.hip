@@ -47,8 +47,9 @@ __device__ __forceinline__ void finish_block(const Mx8Args& p, const floatx4* su
         for (int e = 0; e < 4; ++e)
           if (e < left) v[e] += bf2f(b[n + e]);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = mx8_act(v[e], p.act);
+      float u[4] = {v[0], v[1], v[2], v[3]};
+      mx8_act(u, p.act);
+      v = floatx4{u[0], u[1], u[2], u[3]};
     }
     if (p.res) {
       const bf16* r = p.res + row * p.ldr + col;

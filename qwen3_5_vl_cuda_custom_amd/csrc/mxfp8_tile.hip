@@ -49,23 +49,21 @@ struct TileArgs {
   int tiles_m, tiles_n, gm;
 };
 
-// Eight columns of y from col on (`left` of them exist), the row's m. PLAIN: with bias, activation and residual, the
-// last eight values in `res` where all go in 16-byte pieces (`vec`).
+// Eight columns of y from col on (`left` of them exist, or less than one), the row's m (`in`: it exists); the lanes ^ 16,
+// ^ 32 and ^ 48 hold the other columns of 32. PLAIN: with bias, activation and residual, the last eight values in `res`
+// where all go in 16-byte pieces (`vec`).
 template <bool PLAIN>
-__device__ __forceinline__ void finish8(const Mx8Args& p, int64_t m, int col, int left, bool vec, const float (&bias)[8],
-                                        const bf16x8& res, float (&v)[8]) {
+__device__ __forceinline__ void finish8(const Mx8Args& p, int64_t m, bool in, int col, int left, bool vec,
+                                        const float (&bias)[8], const bf16x8& res, float (&v)[8]) {
   if (PLAIN) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += bias[e];
-    if (p.act) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = mx8_act(v[e], p.act);
-    }
+    mx8_act(v, p.act);
     if (p.res) {
       if (vec) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += bf2f(res[e]);
-      } else {
+      } else if (in) {
         const bf16* r = p.res + m * p.ldr + col;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -73,13 +71,15 @@ __device__ __forceinline__ void finish8(const Mx8Args& p, int64_t m, int col, in
       }
     }
   }
-  if (p.yc) {  // whole blocks of 32 columns: the four lanes of one are neighbours
+  if (p.yc) {  // whole blocks of 32 columns
     uint32_t byte;
-    const u32x2 c = mx8_quantize8(v, byte);
+    const u32x2 c = mx8_quantize8<16>(v, byte);
+    if (!in || left <= 0) return;
     *reinterpret_cast<u32x2*>(p.yc + m * p.ldc + col) = c;
     if ((col & 31) == 0) p.ys[m * (p.ldc / kMx8Block) + col / kMx8Block] = (uint8_t)byte;
     return;
   }
+  if (!in) return;
   bf16* y = p.y + m * p.ldc + col;
   if (vec) {
     bf16x8 o;
@@ -408,63 +408,69 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
     if (rm < rows_m) main(std::true_type{});
     else main(std::false_type{});
   }
-  vm_wait<0>();  // the loads past the last stage (zeros) have landed
+  vm_wait<0>();  // the loads past the last stage (zeros) have landed: the LDS may go to another block
 
-  // Epilogue: the accumulators through LDS in fp32, up to RP rows at a time, so that a thread then has eight columns of
-  // a row, the same columns in every RS-th row: its residuals are under way before the accumulators are in LDS (loaded
-  // one row at a time, each row's latency stood in the 6 us after the last product). 16-byte chunk c of row r lies at
-  // c ^ (r & 15).
-  constexpr int RP0 = kLds / (BN_OUT * 4), RP = RP0 >= BM ? BM : RP0 >= 128 ? 128 : RP0 >= 64 ? 64 : 32;
-  constexpr int C8 = BN_OUT / 8, RS = NW * 64 / C8;
-  static_assert(RP0 >= 32 && BN_OUT % 64 == 0 && NW * 64 % C8 == 0 && RP % RS == 0, "epilogue");
-  float* lds = reinterpret_cast<float*>(smem);
-  auto slot = [](int r, int c) { return r * BN_OUT + ((c ^ (r & 15)) << 2); };
-  const int c8 = tid % C8, r8 = tid / C8, left = rows_n - 8 * c8, n8 = n0 + 8 * c8, col = col0 + n8;
-  const bool vec = vec_of(p, col0) && left >= 8;
-  float bias[8] = {};
+  // Epilogue: lane (l16, q4) holds columns 4 q4 .. + 3 of row l16 of its products; of two neighbouring products the lane
+  // rows change places (permlane16), and it holds eight: 16-byte pieces, four of them 64 bytes of a row. The residuals of
+  // four rows of products are under way before the first is used. (Through the LDS, fp32 and whole rows: 1 us more of
+  // 8.7 for a 128 x 128 tile with one stage, and 3 to 6 of 175 to 327 us for 4096 rows.)
+  constexpr int OP = (SW ? TN / 2 : TN) / 2, JB = 4;
+  const int c0 = (SW ? rn / 2 : rn) + 16 * (q4 & 1) + 8 * (q4 >> 1);
+  const bool vec = vec_of(p, col0);
+  float bias[OP][8] = {};
   if (!SW && p.bias[seg]) {
+    const bf16* const b = p.bias[seg] + n0 + c0;
+    const bool pieces = (reinterpret_cast<uintptr_t>(p.bias[seg]) & 15) == 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < left) bias[e] = bf2f(p.bias[seg][n8 + e]);
-  }
+    for (int o = 0; o < OP; ++o) {
+      const int left = rows_n - c0 - 32 * o;
+      if (pieces && left >= 8) {
+        const bf16x8 u = *reinterpret_cast<const bf16x8*>(b + 32 * o);
 #pragma unroll
-  for (int r0 = 0; r0 < BM; r0 += RP) {
-    bf16x8 res[RP / RS];
+        for (int e = 0; e < 8; ++e) bias[o][e] = bf2f(u[e]);
+      } else {
 #pragma unroll
-    for (int u = 0; u < RP / RS; ++u) {
-      const int r = r0 + r8 + u * RS;
-      res[u] = bf16x8{};
-      if (!SW && p.res && vec && r < rows_m)
-        res[u] = *reinterpret_cast<const bf16x8*>(p.res + (int64_t)(m0 + r) * p.ldr + col);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      const int r = rm + 16 * j - r0;
-      if (r < 0 || r >= RP) continue;
-#pragma unroll
-      for (int o = 0; o < (SW ? TN / 2 : TN); ++o) {
-        floatx4 v;
-        if constexpr (SW) {
-          const int g = 4 * (o / 2) + o % 2;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = silu_mul(acc[g][j][e], acc[g + 2][j][e]);
-        } else {
-          v = acc[o][j];
-        }
-        *reinterpret_cast<floatx4*>(lds + slot(r + l16, ((SW ? rn / 2 : rn) + 16 * o) / 4 + q4)) = v;
+        for (int e = 0; e < 8; ++e)
+          if (e < left) bias[o][e] = bf2f(b[32 * o + e]);
       }
     }
-    __syncthreads();
+  }
 #pragma unroll
-    for (int u = 0; u < RP / RS; ++u) {
-      const int r = r8 + u * RS;
-      if (r0 + r >= rows_m || left <= 0) continue;
-      const floatx4 a = *reinterpret_cast<const floatx4*>(lds + slot(r, 2 * c8));
-      const floatx4 b = *reinterpret_cast<const floatx4*>(lds + slot(r, 2 * c8 + 1));
-      float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-      finish8<!SW>(p, m0 + r0 + r, col, left, vec, bias, res[u], v);
-    }
+  for (int jb = 0; jb < TM; jb += JB) {
+    bf16x8 res[JB][OP];
+#pragma unroll
+    for (int j = 0; j < JB; ++j)
+#pragma unroll
+      for (int o = 0; o < OP; ++o) {
+        const int r = rm + 16 * (jb + j) + l16, c = c0 + 32 * o;
+        res[j][o] = bf16x8{};
+        if (!SW && p.res && vec && r < rows_m && c + 8 <= rows_n)
+          res[j][o] = *reinterpret_cast<const bf16x8*>(p.res + (int64_t)(m0 + r) * p.ldr + col0 + n0 + c);
+      }
+#pragma unroll
+    for (int j = 0; j < JB; ++j)
+#pragma unroll
+      for (int o = 0; o < OP; ++o) {
+        const int r = rm + 16 * (jb + j) + l16, c = c0 + 32 * o, left = rows_n - c;
+        floatx4 a = acc[2 * o][jb + j], b = acc[2 * o + 1][jb + j];
+        if constexpr (SW) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            a[e] = silu_mul(acc[0][jb + j][e], acc[2][jb + j][e]);
+            b[e] = silu_mul(acc[1][jb + j][e], acc[3][jb + j][e]);
+          }
+        }
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = a[e], y = b[e];
+          const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y),
+                                                          false, false);
+          v[e] = __builtin_bit_cast(float, (uint32_t)s[0]);
+          v[4 + e] = __builtin_bit_cast(float, (uint32_t)s[1]);
+        }
+        finish8<!SW>(p, m0 + r, r < rows_m, col0 + n0 + c, left, vec && left >= 8, bias[o], res[j][o], v);
+      }
   }
 }
 
