@@ -44,10 +44,12 @@ def _packed(op: str, codes: torch.Tensor, scales: torch.Tensor, dev: int) -> Pai
     cs, ss = codes.shape, scales.shape
     if (codes.dtype is _F8 and scales.dtype is _U8 and codes.get_device() == dev and scales.get_device() == dev
             and codes.is_contiguous() and scales.is_contiguous() and len(cs) == 2 and len(ss) == 2 and cs[0] == ss[0]
-            and cs[1] == ss[1] * MX8_BLOCK and not (codes.data_ptr() % 16 or scales.data_ptr() % 4)):
+            and cs[1] == ss[1] * MX8_BLOCK and not (codes.data_ptr() % 16 or scales.data_ptr() % 4 or codes.requires_grad)):
         return codes, scales  # the usual call
     if codes.get_device() != dev or scales.get_device() != dev:
         _off_device(op, codes, scales)
+    if codes.requires_grad:
+        require_no_grad(op, codes)
     if codes.dtype != _F8 or scales.dtype != _U8:
         raise TypeError(f"{op}: codes must be float8_e4m3fn and scales uint8, got {codes.dtype} and {scales.dtype}")
     if not cs or len(cs) != len(ss) or cs[:-1] != ss[:-1] or cs[-1] != ss[-1] * MX8_BLOCK:

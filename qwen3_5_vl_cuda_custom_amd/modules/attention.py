@@ -15,7 +15,7 @@ from ..kernels import (apply_rope, decode_attention, decode_attention_mxfp4, dec
 from .kv_cache import MXFP4KVCache, PagedKVCache, StaticKVCache
 from .linear import CudaLinear
 from .linear_mxfp4 import CudaLinearMXFP4
-from .linear_mxfp8 import CudaLinearMXFP8, norm_to_eight_bits
+from .linear_mxfp8 import QUANTIZED_LINEARS, CudaLinearMXFP8, norm_to_eight_bits
 from .norms import CudaRMSNorm, fused_norm_ok, norm_operands
 from .rotary import MRoPEBinding, TextMRoPE
 
@@ -142,15 +142,8 @@ class CudaFullAttention(nn.Module):
         # q/k/v projections in one GEMM over the three weights (no concatenated
         # copy); q, k, v are column views of its output.
         projs = (self.q_proj, self.k_proj, self.v_proj)
-        four_bit, eight_bit = ([isinstance(p, kind) for p in projs] for kind in (CudaLinearMXFP4, CudaLinearMXFP8))
-        if all(eight_bit):
-            qkv = matmul_segments_mxfp8(norm_to_eight_bits(x, input_norm), [p.pair for p in projs],
-                                        [p.bias for p in projs])
-        elif all(four_bit):
-            nw, eps, x = (None, 0.0, x) if input_norm is None else norm_operands(x, input_norm)
-            qkv = matmul_segments_mxfp4(x, [p.pair for p in projs], [p.bias for p in projs], norm_weight=nw, eps=eps)
-        elif any(four_bit) or any(eight_bit):
-            qkv = self._project_apart(x if input_norm is None else input_norm(x), projs)
+        if any([isinstance(p, QUANTIZED_LINEARS) for p in projs]):
+            qkv = self._project_quantized(x, projs, input_norm)
         else:  # any modules with a weight and a bias
             weights = tuple(p.weight for p in projs)
             biases = tuple(p.bias for p in projs)
@@ -224,15 +217,23 @@ class CudaFullAttention(nn.Module):
                         out=o.transpose(1, 2))
         return self.o_proj(o.view(B, S, Hq * D), residual=residual), (kh, vh)
 
+    def _project_quantized(self, x, projs, input_norm) -> torch.Tensor:
+        if all(isinstance(p, CudaLinearMXFP8) for p in projs):
+            return matmul_segments_mxfp8(norm_to_eight_bits(x, input_norm), [p.pair for p in projs],
+                                         [p.bias for p in projs])
+        if all(isinstance(p, CudaLinearMXFP4) for p in projs):
+            nw, eps, x = (None, 0.0, x) if input_norm is None else norm_operands(x, input_norm)
+            return matmul_segments_mxfp4(x, [p.pair for p in projs], [p.bias for p in projs], norm_weight=nw, eps=eps)
+        return self._project_apart(x if input_norm is None else input_norm(x), projs)
+
     @staticmethod
     def _project_apart(x, projs) -> torch.Tensor:
         """The q/k/v rows side by side where only some projections hold weights in four or eight bits: one product
         each, into its columns."""
-        quantized = (CudaLinearMXFP4, CudaLinearMXFP8)
-        ns = [p.out_features if isinstance(p, quantized) else p.weight.shape[0] for p in projs]
+        ns = [p.out_features if isinstance(p, QUANTIZED_LINEARS) else p.weight.shape[0] for p in projs]
         qkv = torch.empty((*x.shape[:-1], sum(ns)), dtype=x.dtype, device=x.device)
         for p, out in zip(projs, qkv.split(ns, -1)):
-            if isinstance(p, quantized):
+            if isinstance(p, QUANTIZED_LINEARS):
                 p(x, out=out)
             else:
                 matmul(x, p.weight, p.bias, out=out)

@@ -7,6 +7,7 @@ from torch import nn
 from ..kernels import add_rmsnorm_mxfp8, matmul_mxfp8, mxfp8_dequantize, mxfp8_quantize
 from ..kernels.mxfp8 import MX8_BLOCK
 from .linear import CudaLinear
+from .linear_mxfp4 import CudaLinearMXFP4
 from .norms import CudaRMSNorm
 
 
@@ -61,6 +62,9 @@ class CudaLinearMXFP8(nn.Module):
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+QUANTIZED_LINEARS = (CudaLinearMXFP4, CudaLinearMXFP8)
 
 
 def norm_to_eight_bits(x: torch.Tensor, norm: CudaRMSNorm | None) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:

@@ -9,7 +9,7 @@ from ..kernels.backward import needs_grad
 from ..kernels.matmul import line_padded_rows
 from .linear import CudaLinear
 from .linear_mxfp4 import CudaLinearMXFP4
-from .linear_mxfp8 import CudaLinearMXFP8, norm_to_eight_bits
+from .linear_mxfp8 import QUANTIZED_LINEARS, CudaLinearMXFP8, norm_to_eight_bits
 from .norms import CudaRMSNorm, fused_norm_ok, norm_operands
 
 
@@ -40,20 +40,8 @@ class CudaSwiGLUMLP(nn.Module):
                 x = input_norm(x)
             return self.down_proj(swiglu(self.gate_proj(x), self.up_proj(x)), residual=residual)
         no_bias = self.gate_proj.bias is None and self.up_proj.bias is None
-        four_bit, eight_bit = ([isinstance(p, kind) for p in (self.gate_proj, self.up_proj)]
-                               for kind in (CudaLinearMXFP4, CudaLinearMXFP8))
-        if all(eight_bit) and no_bias:
-            act = matmul_swiglu_mxfp8(norm_to_eight_bits(x, input_norm), self.gate_proj.pair, self.up_proj.pair,
-                                      quantize=isinstance(self.down_proj, CudaLinearMXFP8))
-            return self.down_proj(act, residual=residual)
-        if all(four_bit) and no_bias:
-            nw, eps, x = (None, 0.0, x) if input_norm is None else norm_operands(x, input_norm)
-            act = matmul_swiglu_mxfp4(x, self.gate_proj.pair, self.up_proj.pair, norm_weight=nw, eps=eps)
-            return self.down_proj(act, residual=residual)
-        if any(four_bit) or any(eight_bit):  # in one of them, or with a bias: each projection by its own forward
-            if input_norm is not None:
-                x = input_norm(x)
-            return self.down_proj(swiglu(self.gate_proj(x), self.up_proj(x)), residual=residual)
+        if isinstance(self.gate_proj, QUANTIZED_LINEARS) or isinstance(self.up_proj, QUANTIZED_LINEARS):
+            return self._forward_quantized(x, residual, input_norm, no_bias)
         if input_norm is not None and no_bias and fused_norm_ok(x, input_norm):
             act = rmsnorm_matmul_swiglu(x, input_norm.weight, input_norm.eps, self.gate_proj.weight,
                                         self.up_proj.weight)
@@ -63,6 +51,20 @@ class CudaSwiGLUMLP(nn.Module):
         if no_bias:
             act = matmul_swiglu(x, self.gate_proj.weight, self.up_proj.weight)  # gate, up and swiglu in one GEMM
         else:
+            act = swiglu(self.gate_proj(x), self.up_proj(x))
+        return self.down_proj(act, residual=residual)
+
+    def _forward_quantized(self, x, residual, input_norm, no_bias: bool) -> torch.Tensor:
+        projs = (self.gate_proj, self.up_proj)
+        if no_bias and all(isinstance(p, CudaLinearMXFP8) for p in projs):
+            act = matmul_swiglu_mxfp8(norm_to_eight_bits(x, input_norm), self.gate_proj.pair, self.up_proj.pair,
+                                      quantize=isinstance(self.down_proj, CudaLinearMXFP8))
+        elif no_bias and all(isinstance(p, CudaLinearMXFP4) for p in projs):
+            nw, eps, x = (None, 0.0, x) if input_norm is None else norm_operands(x, input_norm)
+            act = matmul_swiglu_mxfp4(x, self.gate_proj.pair, self.up_proj.pair, norm_weight=nw, eps=eps)
+        else:  # of several kinds, or with a bias: each projection by its own forward
+            if input_norm is not None:
+                x = input_norm(x)
             act = swiglu(self.gate_proj(x), self.up_proj(x))
         return self.down_proj(act, residual=residual)
 

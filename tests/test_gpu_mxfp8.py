@@ -435,7 +435,58 @@ def test_layer_half_in_a_row():
     check(y, *reference(cpu[1], d, r=hd.cpu()))
 
 
+# ------------------------------------------------------------------ offsets past 32 bits
+def test_rows_past_two_to_the_31_values():
+    """The norm, the quantisation and the way back over 2.4 thousand million values: 600 times the same rows."""
+    x, w = rnd(1000, 4096, seed=1).to(DEV), torch.ones(4096, dtype=torch.bfloat16, device=DEV)
+    big = x.repeat(600, 1)
+    h, codes, scales = K.add_rmsnorm_mxfp8(big, big, w)
+    h1, codes1, scales1 = K.add_rmsnorm_mxfp8(x, x, w)
+    back, back1 = K.mxfp8_dequantize(codes, scales), K.mxfp8_dequantize(codes1, scales1)
+    codes2, codes3 = K.mxfp8_quantize(big)[0], K.mxfp8_quantize(x)[0]
+    for a, b in ((h, h1), (codes, codes1), (scales, scales1), (back, back1), (codes2, codes3)):
+        a, b = (t.view(torch.uint8) for t in (a, b))
+        assert bool((a.view(600, 1000, -1) == b).all())
+
+
+@pytest.mark.parametrize("m", [2, 40, 700])
+def test_weights_past_two_to_the_31_bytes(m):
+    x, w = dev(exact_pair(m, 4096, 1)), dev(exact_pair(1000, 4096, 2))
+    y = K.matmul_mxfp8(x, tuple(t.view(torch.uint8).repeat(600, 1).view(t.dtype) for t in w))
+    assert bool((y.view(m, 600, 1000) == K.matmul_mxfp8(x, w)[:, None]).all())
+
+
+@pytest.mark.parametrize("k", [128, 96])
+def test_outputs_past_two_to_the_31_values(k):
+    x, w = dev(exact_pair(250, k, 1)), dev(exact_pair(32768, k, 2))
+    big = tuple(t.view(torch.uint8).repeat(280, 1).view(t.dtype) for t in x)
+    want = K.matmul_mxfp8(x, w)
+    assert bool((K.matmul_mxfp8(big, w).view(280, 250, -1) == want).all())
+    r = want.repeat(280, 1)
+    assert bool((K.matmul_mxfp8(big, w, residual=r, out=r).view(280, 250, -1) == K.matmul_mxfp8(x, w, residual=want)).all())
+    codes, scales = K.matmul_mxfp8(big, w, quantize=True)
+    codes1, scales1 = K.matmul_mxfp8(x, w, quantize=True)
+    assert bool((codes.view(torch.uint8).view(280, 250, -1) == codes1.view(torch.uint8)).all())
+    assert bool((scales.view(280, 250, -1) == scales1).all())
+
+
 # ------------------------------------------------------------------ streams, graphs, refusals
+@pytest.mark.parametrize("m", [8, 100, 1500])
+def test_two_streams_at_once(m):
+    """Products of the same weights on two streams, each with workspaces of its own."""
+    w, xs = dev(exact_pair(4352, 1024, 1)), [dev(exact_pair(m, 1024, 2 + i)) for i in range(2)]
+    want = [K.matmul_mxfp8(x, w) for x in xs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(20):
+        for s, x, out in zip(streams, xs, got):
+            with torch.cuda.stream(s):
+                out.append(K.matmul_mxfp8(x, w))
+    torch.cuda.synchronize()
+    for out, y in zip(got, want):
+        assert all(torch.equal(o, y) for o in out)
+
+
 def test_calls_follow_the_current_stream_and_replay_in_a_graph():
     m, n, k = 100, 1024, 4096
     x, r = rnd(m, k, seed=1).to(DEV), rnd(m, k, seed=2).to(DEV)
@@ -492,6 +543,8 @@ def test_refusals():
             bad()
     with torch.enable_grad():
         p = torch.zeros(64, dtype=torch.bfloat16, device=DEV, requires_grad=True)
-        for bad in (lambda: K.matmul_mxfp8(x, w, p), lambda: K.mxfp8_quantize(p), lambda: K.add_rmsnorm_mxfp8(p, None, b)):
+        leaf = x[0].clone().requires_grad_(True)
+        for bad in (lambda: K.matmul_mxfp8(x, w, p), lambda: K.mxfp8_quantize(p), lambda: K.add_rmsnorm_mxfp8(p, None, b),
+                    lambda: K.matmul_mxfp8((leaf, x[1]), w), lambda: K.mxfp8_dequantize(leaf, x[1])):
             with pytest.raises(NotImplementedError):
                 bad()

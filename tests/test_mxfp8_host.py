@@ -111,3 +111,17 @@ def test_workspace_query_takes_any_sizes(L):
     assert q(0, i64(64), 1, 64, 0) == 0 and q(4, None, 1, 64, 0) == 0 and q(4, i64(64), 9, 64, 0) == 0
     assert q(4, i64(-5), 1, 64, 0) == 0 and q(4, i64(64), 1, 48, 0) == 0
     assert all(q(m, i64(n), 1, k, 0) >= 0 for m in (1, 65, 5000) for n in (1, 300, 20000) for k in (32, 4096, 65536))
+
+
+def test_scales_and_workspaces_are_checked(L):
+    def mm(M_=4, N=64, K=256, xs=FAKE, ws=FAKE, work=None, size=0):
+        return L.q3_matmul_mxfp8(FAKE, xs, FAKE, ws, None, None, FAKE, None, None, M_, N, K, 0, N, 0, work, size, None)
+    assert mm(xs=FAKE + 2) == -4 and mm(ws=FAKE + 1) == -4
+    big = dict(M_=4096, N=4096, K=4096)
+    need = L.q3_matmul_mxfp8_workspace_bytes(4096, i64(4096), 1, 4096, 0)
+    assert need == 2 * 4096 * 4096 // 32  # the scales of both
+    assert mm(**big) == -6 and mm(**big, work=FAKE, size=need - 1) == -6 and mm(**big, work=FAKE + 8, size=need) == -4
+    assert mm(**big, size=need) == -6  # a size without memory
+    q = L.q3_matmul_mxfp8_workspace_bytes
+    assert all(q(m, i64(n), 1, k, s) == 0 for m in (1, 64) for n in (1, 200000) for k in (96, 4096) for s in (0, 1))
+    assert q(1000, i64(4096), 1, 4096, 0) == 0 and q(1000, i64(4096), 1, 4128, 0) > 0  # scales by rows: whole words of them
