@@ -338,16 +338,17 @@ void launch_tiles(const Mx8Args& p, unsigned blocks, hipStream_t st) {
 
 namespace q3 {
 
-// Few rows, or rows of which every 64 with up to 64 weight rows (SwiGLU: 32 of each) a block give each CU two blocks at
-// most. What the blocks read is what bounds them, and tiles share more of it, but start slower and find their scales laid
-// out only after another launch. Tiles against this, one block a CU: 100 rows, N 4096, K 4096 29.7 and 12.6 us, K 12288
-// 69.4 and 24.5; two: 128 rows, N 12288, K 4096 32.8 and 27.8, 512 rows, N 4096 32.6 and 31.7; three: SwiGLU of 128 rows,
-// N 12288 36.1 and 42.3; four: 1000 rows, N 4096 34.6 and 63.2.
+// Few rows, or rows of which every 64 with up to 64 weight rows (SwiGLU: 32 of each) a block give each CU one block at
+// most. What the blocks read is what bounds them, and tiles share more of it, but start slower and a tile alone has a
+// CU's share of the loads. One round against tiles, us: 100 rows, N 4096, K 4096 12.6 and 29.7, K 12288 24.5 and 69 (tiles
+// of that time), 256 rows, N 4096, K 4096 over weights past the last cache 16.3 and 28. Two rounds, the same: 512 rows 30.2
+// and 28.3, N = K = 2048, 640 rows 17.4 and 14.1, 128 rows, N 12288 27.3 and 31.1; with weights in the last cache 512 rows
+// 27 and 20.
 bool mx8_rows_takes(const Mx8Args& p, bool swiglu) {
   if (p.M <= 64) return true;
   int64_t blocks = 0;
   for (int j = 0; j < p.nseg; ++j) blocks += q3_cdiv(p.n[j], swiglu ? 32 : 64);
-  return p.K % 128 == 0 && blocks * q3_cdiv(p.M, 64) <= 512;
+  return p.K % 128 == 0 && blocks * q3_cdiv(p.M, 64) <= 256;
 }
 
 int mx8_rows(const Mx8Args& args, bool swiglu, hipStream_t st) {

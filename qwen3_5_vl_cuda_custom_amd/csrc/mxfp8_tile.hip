@@ -34,9 +34,9 @@
 // of rows l % 16, + 16, + 32, + 48 (the instruction picks the byte). A load brings a stage
 // of them, and three words a stage are all that a wave reads. As rows of bytes their loads
 // cost a line per row and the reads twelve bytes a stage: 198 against 194 us for 4096 x 4096
-// x 12288 when it was tried. Where one round of 128 x 128 tiles does it all the launch costs
-// more (2.7 to 4 us), and the scales come by rows (RAW), 16 bytes, four stages', of a row at a
-// time: 784 rows of K 1152, N 4304 17.6 to 14.6 us (12.2 now), the 1000 rows 27.9 to 26.4.
+// x 12288 when it was tried. For small products the launch costs more (2.7 to 4 us), and
+// 128 x 128 tiles take the scales by rows (RAW), 16 bytes, four stages', of a row at a time:
+// 784 rows of K 1152, N 4304 17.6 to 14.6 us (12.2 now), the 1000 rows 27.9 to 26.4.
 #include "gemm_tile.h"
 #include "mxfp8.h"
 #include "mxfp8_tile.h"
@@ -573,7 +573,7 @@ void launch_tile(TileArgs t, hipStream_t st) {
                      dim3(WM * WN * 64), 0, st, t);
 }
 
-// Forms: tiles of 256 x 256, 128 x 256, 128 x 128, and of the last with the scales by rows.
+// Forms: tiles of 256 x 256, 128 x 256, 128 x 128, and of the last size with the scales by rows.
 template <bool SW>
 void launch_form(const TileArgs& t, int form, hipStream_t st) {
   if (form == 0) launch_tile<256, 256, 2, 4, 2, SW>(t, st);
@@ -582,16 +582,24 @@ void launch_form(const TileArgs& t, int form, hipStream_t st) {
   else launch_tile<128, 128, 2, 2, 4, SW, true>(t, st);
 }
 
-// The form whose rounds over the CUs (one block each) cost least; a round's stage takes 1.57, 1.0 and 0.6 us in the
-// forms' full rounds (4096 rows, N 4096 and 24576, epilogues included). Measured with each form forced, in us: SwiGLU of
-// 611 rows, N 12288 86, 77 and 90 (2, 2 and 4 rounds), 2048 rows, N = K = 4096 55, 43 and 48 (1, 1, 2), 3000 rows 56, 72
-// and 69 (1, 2, 3), 1000 rows 52, 38 and 26 (1 each).
+// The form that costs least, by launches + rounds x (first loads and epilogue + stages x a stage), in 10 ns: fitted to one,
+// two and four full rounds (a block on each of the 256 CUs) of K 128 to 12288, within 8 %; a last round of few tiles counts
+// three quarters of a full one, as fewer blocks get their loads sooner. Measured with each form forced, in us, 256 x 256,
+// 128 x 256, 128 x 128 laid out and by rows: 4096 rows, N 4096, K 4096 62, 71, 81, 86; 2048 rows 48, 38, 45, 45; 1024 rows
+// 46, 32, 24.5, 24, K 1152 22, 18, 14, 12, K 12288 111, 67, 55, 56; 4096 rows, N 4304 (a seventeenth tile) 94, 93, 96, 102,
+// K 1152 43, 50, 49, 48. Scales by rows want whole words of them.
 int form_of(const Mx8Args& a, bool swiglu) {
-  const int out = swiglu ? 2 : 1;
-  auto cost = [&](int bm, int bn, int64_t stage) { return q3_cdiv(q3_cdiv(a.M, bm) * tiles_of(a, bn / out), 256) * stage; };
-  const int64_t c0 = cost(256, 256, 16), c1 = cost(128, 256, 10), c2 = cost(128, 128, 6);
-  if (c0 <= c1 && c0 <= c2) return 0;
-  return c1 <= c2 ? 1 : a.K % 128 == 0 ? 3 : 2;
+  const int64_t out = swiglu ? 2 : 1, stages = q3_cdiv(a.K, 128);
+  auto cost = [&](int bm, int bn, int64_t launches, int64_t fixed, int64_t stage) {
+    const int64_t tiles = q3_cdiv(a.M, bm) * tiles_of(a, (int)(bn / out)), rest = tiles % 256;
+    return launches * 1024 + (tiles / 256 * 1024 + (rest ? 768 + rest : 0)) * (fixed + stages * stage);
+  };
+  const int64_t costs[4] = {cost(256, 256, 760, 800, 138), cost(128, 256, 750, 730, 75), cost(128, 128, 430, 540, 43),
+                            cost(128, 128, 230, 540, 49)};
+  int best = 0;
+  for (int j = 1; j < (a.K % 128 == 0 ? 4 : 3); ++j)
+    if (costs[j] < costs[best]) best = j;
+  return best;
 }
 
 // Bytes of laid out scales of n rows.
