@@ -227,7 +227,7 @@ def matmul_mxfp8(x: torch.Tensor | Pair, weight: Pair, bias: torch.Tensor | None
 
     activation: None, "gelu_tanh" or "silu". quantize=True returns the fp32 values in eight bits instead, a pair (N a multiple of
     32). `out`, when given: (..., N) bf16 whose rows have one stride and contiguous elements, written in place (a
-    column slice of a wider buffer).
+    column slice of a wider buffer); it may be the residual itself, and must not overlap it otherwise.
     """
     op = "matmul_mxfp8"
     act = _ACTS.get(activation, -1)
