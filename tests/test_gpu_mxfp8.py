@@ -247,6 +247,15 @@ def test_matmul_many_tiles(m, n, k):
     assert bool(((y.double().cpu() - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("m,n,k", [(5, 24, 131072), (80, 24, 66560), (300, 20, 32800), (129, 6000, 16384)])
+def test_matmul_of_long_rows(m, n, k):
+    """Rows past the lengths whose sums are exact: one value in sixteen is not zero."""
+    x, w = exact_pair(m, k, 1), exact_pair(n, k, 2)
+    x[0].view(torch.uint8)[torch.rand(m, k, generator=torch.Generator().manual_seed(3)) > 1 / 16] = 0
+    want = (M.values(*x).float().to(DEV) @ M.values(*w).float().to(DEV).T).to(torch.bfloat16)
+    assert torch.equal(K.matmul_mxfp8(dev(x), dev(w)), want)
+
+
 def test_matmul_scales_of_every_size():
     """Scales far apart between rows, and between blocks of a row."""
     m, n, k = 70, 50, 256
