@@ -20,7 +20,7 @@
 // loads of codes, 322 with all of them from one place; matrix pipe busy 62 %); N 4096, K 12288
 // 157 us, 2.63 PFLOP/s.
 //
-// Smaller tiles, four waves of 64 x 128 or 64 x 64 for 128 x 256 and 128 x 128: one wave a SIMD
+// Smaller tiles, four waves of 128 x 64 or 64 x 64 for 128 x 256 and 128 x 128: one wave a SIMD
 // has the registers for two stages' fragments. It reads all of the next stage's between the
 // products of this one, so a slot is free at the barrier where its stage begins, and three or
 // four slots stay under way. Waves that read as above took 76 us for SwiGLU of 611 rows, N 12288
@@ -119,11 +119,11 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
   constexpr int BN_OUT = SW ? BN / 2 : BN;
   constexpr int GX = BM / 64, GS = (BM + BN) / 64, PS = (GS + NW - 1) / NW;  // groups of 64 rows; loads of scales
   constexpr int PX = BM / 8 / NW, PW = BN / 8 / NW;                          // loads of codes per wave and stage
-  constexpr bool EARLY = NW == 8 && NS == 2;  // the weights' slot is released by a barrier of its own
   constexpr bool PIPE = NW == 4;  // one wave a SIMD: room for two stages' fragments in registers
   constexpr int kX = BM * 128, kW = BN * 128, kS = RAW ? (BM + BN) * 16 : PS * NW * 256;
   constexpr int kLds = NS * (kX + kW) + 4 * kS;
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NW % 2 == 0, "whole loads per wave, one swizzle per lane");
+  static_assert(PIPE || (NW == 8 && NS == 2), "the two loops");
   static_assert(!RAW || (PIPE && GS == NW && NS <= 4), "scales by rows: a wave to 64 rows");
   static_assert(TM % 4 == 0 && TN == 4 && kLds <= 160 * 1024, "wave tiles");
   __shared__ __attribute__((aligned(1024))) char smem[kLds];
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
     const int r = (wave + NW * i) * 8 + lrow;
     woff[i] = (uint32_t)((SW ? (r >> 6) * 32 + (r & 31) : r) * K);  // SwiGLU: 32 gate rows, the same 32 up rows, ...
   }
-  // Scales: load s of this wave is a stage of 64 rows, x's and then the weights'.
+  // Scales: load s of this wave is a stage of 64 rows, x's and then the weights' (by rows: four stages of 16 rows).
   const uint8_t* sp[PS];
   int sbytes[PS];
   const int kb = K / kMx8Block;
@@ -178,15 +178,15 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
     sbytes[0] = mx8_pin(max(rows, 0) * kb);
   } else {
 #pragma unroll
-  for (int s = 0; s < PS; ++s) {
-    const int e = wave + NW * s;
-    const bool of_x = e < GX;
-    const int g = of_x ? m0 / 64 + e : (SW ? 2 * n0 : n0) / 64 + e - GX;
-    // 64-row groups that exist: of all rows, SwiGLU 32 of each weight to a group
-    const int all = of_x ? (p.M + 63) / 64 : SW ? (p.n[0] + 31) / 32 : (p.n[seg] + 63) / 64;
-    sp[s] = mx8_pin((of_x ? t.xs : t.ws[seg]) + (int64_t)g * groups_k * 1024);
-    sbytes[s] = mx8_pin(e < GS && g < all ? groups_k * 1024 : 0);
-  }
+    for (int s = 0; s < PS; ++s) {
+      const int e = wave + NW * s;
+      const bool of_x = e < GX;
+      const int g = of_x ? m0 / 64 + e : (SW ? 2 * n0 : n0) / 64 + e - GX;
+      // 64-row groups that exist: of all rows, SwiGLU 32 of each weight to a group
+      const int all = of_x ? (p.M + 63) / 64 : SW ? (p.n[0] + 31) / 32 : (p.n[seg] + 63) / 64;
+      sp[s] = mx8_pin((of_x ? t.xs : t.ws[seg]) + (int64_t)g * groups_k * 1024);
+      sbytes[s] = mx8_pin(e < GS && g < all ? groups_k * 1024 : 0);
+    }
   }
   const uint32_t lbase = lds_addr(smem);
   constexpr int kW0 = NS * kX, kS0 = kW0 + NS * kW;
@@ -195,13 +195,14 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
     const int k = kt * 128 + dc * 16;
     return k < K ? (uint32_t)k : kOOB;
   };
-  auto dma_x = [&](int kt, int i) {
-    dma16(rx, xoff[i] + kofs(kt), lbase + (uint32_t)(kt % NS * kX + (wave + NW * i) * 1024));
+  // Load i of stage kt's codes, into a slot.
+  auto dma_x = [&](int kt, int slot, int i) __attribute__((always_inline)) {
+    dma16(rx, xoff[i] + kofs(kt), lbase + (uint32_t)(slot * kX + (wave + NW * i) * 1024));
   };
-  auto dma_w = [&](int kt, int i) {
+  auto dma_w = [&](int kt, int slot, int i) __attribute__((always_inline)) {
     const bool up = SW && ((wave + NW * i) & 4);
     dma16(make_rsrc(SW ? mx8_pin(up ? wb : wa) : wa, rows_n * K), woff[i] + kofs(kt),
-          lbase + (uint32_t)(kW0 + kt % NS * kW + (wave + NW * i) * 1024));
+          lbase + (uint32_t)(kW0 + slot * kW + (wave + NW * i) * 1024));
   };
   auto dma_s = [&](int kt, int s) {
     if constexpr (RAW) {
@@ -217,12 +218,12 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
     dma4(make_rsrc(sp[s], sbytes[s]), kt < nk ? (uint32_t)(kt * 256 + lane * 4) : kOOB,
          lbase + (uint32_t)(kS0 + (kt & 3) * kS + (wave + NW * s) * 256));
   };
-  // d-th load of what is issued in the columns before the stage barrier: scales, weights (and with more slots x).
-  constexpr int ND = PS + PW + (EARLY ? 0 : PX);
-  auto dma = [&](int kt, int d) {
+  constexpr int kAll = PS + PW + PX;
+  // Load d of them.
+  auto dma = [&](int kt, int slot, int d) __attribute__((always_inline)) {
     if (d < PS) dma_s(kt, d);
-    else if (d < PS + PW) dma_w(kt, d - PS);
-    else dma_x(kt, d - PS - PW);
+    else if (d < PS + PW) dma_w(kt, slot, d - PS);
+    else dma_x(kt, slot, d - PS - PW);
   };
 
   floatx4 acc[TN][TM];
@@ -230,46 +231,18 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
   for (int i = 0; i < TN; ++i)
 #pragma unroll
     for (int j = 0; j < TM; ++j) acc[i][j] = floatx4{};
-  i32x8 fw[TN], fx[4];
-  int sw, sx[TM / 4], sw_next, sx_next[TM / 4];  // a stage's words of scales
   const int rn = wn * WTN, rm = wm * WTM;
-  auto frag = [&](const char* slot, int r) {
-    const char* row = slot + r * 128;
-    const i32x4 lo = *reinterpret_cast<const i32x4*>(row + ((q4 ^ swz(r)) << 4));
-    const i32x4 hi = *reinterpret_cast<const i32x4*>(row + (((4 + q4) ^ swz(r)) << 4));
-    return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-  };
-  auto rd_w = [&](int kt, int i) { fw[i] = frag(smem + kW0 + kt % NS * kW, rn + 16 * i + l16); };
-  auto rd_x = [&](int kt, int j) { fx[j & 3] = frag(smem + kt % NS * kX, rm + 16 * j + l16); };
-  auto rd_s = [&](int kt) {
-    const char* s = smem + kS0 + (kt & 3) * kS + lane * 4;
-    sw_next = *reinterpret_cast<const int*>(s + (GX + rn / 64) * 256);
-#pragma unroll
-    for (int g = 0; g < TM / 4; ++g) sx_next[g] = *reinterpret_cast<const int*>(s + (rm / 64 + g) * 256);
-  };
-  auto take_s = [&]() {
-    sw = sw_next;
-#pragma unroll
-    for (int g = 0; g < TM / 4; ++g) sx[g] = sx_next[g];
-  };
-  auto mf = [&](int i, int j) { acc[i][j] = mfma_of(fw[i], fx[j & 3], acc[i][j], sw, sx[j / 4], i, j & 3); };
 
-  constexpr int kAhead = EARLY ? 2 : PIPE ? NS : NS - 1;  // stages issued before the loop
-  constexpr int kAll = PX + PW + PS;
   if constexpr (RAW) {
 #pragma unroll
     for (int s = -4; s < 0; ++s) dma_s(s, 0);  // the first four stages'
   }
 #pragma unroll
-  for (int s = 0; s < kAhead; ++s) {
+  for (int s = 0; s < NS; ++s) {
 #pragma unroll
-    for (int d = 0; d < ND; ++d) dma(s, d);
-    if constexpr (EARLY) {
-#pragma unroll
-      for (int i = 0; i < PX; ++i) dma_x(s, i);
-    }
+    for (int d = 0; d < kAll; ++d) dma(s, s, d);
   }
-  vm_wait<(kAhead - 1) * kAll>();  // stage 0 has landed
+  vm_wait<(NS - 1) * kAll>();  // stage 0 has landed
   __syncthreads();
 
   if constexpr (PIPE) {
@@ -314,7 +287,7 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
       __builtin_amdgcn_s_waitcnt(0xc07f);
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
-      constexpr int kReads = 2 * (TN + TM), kMf = TN * TM, kLoads = PS + PW + PX;
+      constexpr int kReads = 2 * (TN + TM), kMf = TN * TM;
       int n = 0, d = 0;
 #pragma unroll
       for (int m = 0; m < kMf; ++m) {
@@ -323,13 +296,7 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
                 : mfma_of(pw[G][m % TN], px[G][m / TN], acc[m % TN][m / TN], zw[G][0], zx[G][RAW ? 0 : m / TN / 4], m % TN, m / TN & 3);
         if (m == 0) read_s(G ^ 1, kt + 1);
         for (; n < kReads && n * (kMf - 4) < (m + 1) * kReads; ++n) read(G ^ 1, n, nxt * kX, nxt * kW);
-        for (; d < kLoads && d * (kMf - 2) < m * kLoads; ++d) {
-          const int at = kt + NS;
-          if (d < PS) dma_s(at, d);
-          else if (d < PS + PW) dma16(make_rsrc(SW ? mx8_pin(((wave + NW * (d - PS)) & 4) ? wb : wa) : wa, rows_n * K),
-                                      woff[d - PS] + kofs(at), lbase + (uint32_t)(kW0 + cur * kW + (wave + NW * (d - PS)) * 1024));
-          else dma16(rx, xoff[d - PS - PW] + kofs(at), lbase + (uint32_t)(cur * kX + (wave + NW * (d - PS - PW)) * 1024));
-        }
+        for (; d < kAll && d * (kMf - 2) < m * kAll; ++d) dma(kt + NS, cur, d);
         __builtin_amdgcn_sched_barrier(0);
       }
       cur = nxt;
@@ -343,71 +310,90 @@ __global__ __launch_bounds__(WM* WN * 64) void mx8_tile_kernel(const TileArgs t)
 #pragma unroll
       for (int j = 0; j < TM; ++j) asm volatile("" : "+a"(acc[i][j]));
     __builtin_amdgcn_s_waitcnt(0xc07f);
-  }
-  auto main = [&](auto active_c) {
-    constexpr bool A = decltype(active_c)::value;  // a wave without rows loads and waits only
-    if constexpr (A) {
-      rd_s(0);
-      take_s();
+  } else {
+    i32x8 fw[TN], fx[4];
+    int sw, sx[TM / 4], sw_next, sx_next[TM / 4];  // a stage's words of scales
+    auto frag = [&](const char* slot, int r) {
+      const char* row = slot + r * 128;
+      const i32x4 lo = *reinterpret_cast<const i32x4*>(row + ((q4 ^ swz(r)) << 4));
+      const i32x4 hi = *reinterpret_cast<const i32x4*>(row + (((4 + q4) ^ swz(r)) << 4));
+      return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    auto rd_w = [&](int kt, int i) { fw[i] = frag(smem + kW0 + kt % NS * kW, rn + 16 * i + l16); };
+    auto rd_x = [&](int kt, int j) { fx[j & 3] = frag(smem + kt % NS * kX, rm + 16 * j + l16); };
+    auto rd_s = [&](int kt) {
+      const char* s = smem + kS0 + (kt & 3) * kS + lane * 4;
+      sw_next = *reinterpret_cast<const int*>(s + (GX + rn / 64) * 256);
 #pragma unroll
-      for (int i = 0; i < TN; ++i) rd_w(0, i);
+      for (int g = 0; g < TM / 4; ++g) sx_next[g] = *reinterpret_cast<const int*>(s + (rm / 64 + g) * 256);
+    };
+    auto take_s = [&]() {
+      sw = sw_next;
 #pragma unroll
-      for (int j = 0; j < 3; ++j) rd_x(0, j);
-      // Nothing is left under way here, so that the loop's waits are counted from its own loads (lgkmcnt 0).
-      __builtin_amdgcn_s_waitcnt(0xc07f);
-    }
-    for (int kt = 0; kt < nk; ++kt) {
-      const int next = kt + kAhead;  // the stage whose loads go out
-      int d = 0;
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int j = 0; j < TM - 2; ++j) {
-#pragma unroll
-        for (int i = 0; i < TN; ++i) {
-          if constexpr (A) {
-            mf(i, j);
-            if (i == 0 && j + 3 < TM) rd_x(kt, j + 3);
-          }
-          constexpr int slots = TN * (TM - 2) - (EARLY ? TN : 0), gap = slots / ND > 0 ? slots / ND : 1;
-          const int at = j * TN + i - (EARLY ? TN : 0);
-          if (at >= 0 && at % gap == gap - 1 && d < ND) dma(next, d++);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        if (EARLY && j == 0) {  // every wave holds the weights' fragments (read before the last one of x)
-          asm volatile("s_waitcnt lgkmcnt(2)\n\ts_barrier" ::: "memory");
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-#pragma unroll
-      for (; d < ND; ++d) dma(next, d);
-      // Stage kt + 1 has landed (later ones may not have) and every fragment of stage kt is in registers, in every wave.
-      vm_wait<EARLY ? PS + PW : (NS - 2) * kAll>();
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
+      for (int g = 0; g < TM / 4; ++g) sx[g] = sx_next[g];
+    };
+    auto mf = [&](int i, int j) { acc[i][j] = mfma_of(fw[i], fx[j & 3], acc[i][j], sw, sx[j / 4], i, j & 3); };
+    auto main = [&](auto active_c) {
+      constexpr bool A = decltype(active_c)::value;  // a wave without rows loads and waits only
       if constexpr (A) {
-        rd_s(kt + 1);
-        rd_x(kt + 1, 0);
-        rd_x(kt + 1, 1);
+        rd_s(0);
+        take_s();
+#pragma unroll
+        for (int i = 0; i < TN; ++i) rd_w(0, i);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) rd_x(0, j);
+        // Nothing is left under way here, so that the loop's waits are counted from its own loads (lgkmcnt 0).
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+      }
+      for (int kt = 0; kt < nk; ++kt) {
+        const int next = kt + NS;  // the stage whose loads go out
+        int d = 0;                 // scales and weights, after the first column
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < TN; ++i) {
-          mf(i, TM - 2);
-          if (EARLY && i < PX) dma_x(next, i);
-          mf(i, TM - 1);
-          rd_w(kt + 1, i);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        rd_x(kt + 1, 2);
-        take_s();
-      }
-      if constexpr (EARLY) {
+        for (int j = 0; j < TM - 2; ++j) {
 #pragma unroll
-        for (int i = A ? TN : 0; i < PX; ++i) dma_x(next, i);
+          for (int i = 0; i < TN; ++i) {
+            if constexpr (A) {
+              mf(i, j);
+              if (i == 0 && j + 3 < TM) rd_x(kt, j + 3);
+            }
+            constexpr int gap = TN * (TM - 3) / (PS + PW);
+            const int at = (j - 1) * TN + i;
+            if (at >= 0 && at % gap == gap - 1 && d < PS + PW) dma(next, kt % NS, d++);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (j == 0) {  // every wave holds the weights' fragments (read before the last one of x)
+            asm volatile("s_waitcnt lgkmcnt(2)\n\ts_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+#pragma unroll
+        for (; d < PS + PW; ++d) dma(next, kt % NS, d);
+        // Stage kt + 1 has landed (later ones may not have) and every fragment of stage kt is in registers, in every wave.
+        vm_wait<PS + PW>();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (A) {
+          rd_s(kt + 1);
+          rd_x(kt + 1, 0);
+          rd_x(kt + 1, 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < TN; ++i) {
+            mf(i, TM - 2);
+            if (i < PX) dma_x(next, kt % NS, i);
+            mf(i, TM - 1);
+            rd_w(kt + 1, i);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          rd_x(kt + 1, 2);
+          take_s();
+        }
+#pragma unroll
+        for (int i = A ? TN : 0; i < PX; ++i) dma_x(next, kt % NS, i);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-  if constexpr (!PIPE) {
+    };
     if (rm < rows_m) main(std::true_type{});
     else main(std::false_type{});
   }
