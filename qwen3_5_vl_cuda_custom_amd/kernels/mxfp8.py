@@ -190,7 +190,14 @@ def _operand(op: str, x: torch.Tensor | Pair) -> tuple[int, torch.Tensor, torch.
 
 
 def _weight(op: str, weight: Pair, K: int, dev: int) -> Pair:
-    codes, scales = _packed(op, *weight, dev)
+    codes, scales = weight
+    cs, ss = codes.shape, scales.shape
+    if (codes.dtype is _F8 and scales.dtype is _U8 and codes.get_device() == dev and scales.get_device() == dev
+            and codes.is_contiguous() and scales.is_contiguous() and len(cs) == 2 and len(ss) == 2 and cs[0] == ss[0]
+            and cs[1] == K and ss[1] * MX8_BLOCK == K
+            and not (codes.data_ptr() % 16 or scales.data_ptr() % 4 or codes.requires_grad)):
+        return codes, scales  # the usual call, without the calls below
+    codes, scales = _packed(op, codes, scales, dev)
     if codes.dim() != 2 or codes.shape[1] != K:
         raise ValueError(f"{op}: weight codes {tuple(codes.shape)} do not match x (..., {K})")
     return codes, scales
