@@ -39,9 +39,9 @@ class CudaSwiGLUMLP(nn.Module):
             if input_norm is not None:
                 x = input_norm(x)
             return self.down_proj(swiglu(self.gate_proj(x), self.up_proj(x)), residual=residual)
-        no_bias = self.gate_proj.bias is None and self.up_proj.bias is None
         if isinstance(self.gate_proj, QUANTIZED_LINEARS) or isinstance(self.up_proj, QUANTIZED_LINEARS):
-            return self._forward_quantized(x, residual, input_norm, no_bias)
+            return self._forward_quantized(x, residual, input_norm)
+        no_bias = self.gate_proj.bias is None and self.up_proj.bias is None
         if input_norm is not None and no_bias and fused_norm_ok(x, input_norm):
             act = rmsnorm_matmul_swiglu(x, input_norm.weight, input_norm.eps, self.gate_proj.weight,
                                         self.up_proj.weight)
@@ -54,15 +54,15 @@ class CudaSwiGLUMLP(nn.Module):
             act = swiglu(self.gate_proj(x), self.up_proj(x))
         return self.down_proj(act, residual=residual)
 
-    def _forward_quantized(self, x, residual, input_norm, no_bias: bool) -> torch.Tensor:
+    def _forward_quantized(self, x, residual, input_norm) -> torch.Tensor:
         projs = (self.gate_proj, self.up_proj)
-        if no_bias and all(isinstance(p, CudaLinearMXFP8) for p in projs):
+        if all(isinstance(p, CudaLinearMXFP8) and p.bias is None for p in projs):
             act = matmul_swiglu_mxfp8(norm_to_eight_bits(x, input_norm), self.gate_proj.pair, self.up_proj.pair,
                                       quantize=isinstance(self.down_proj, CudaLinearMXFP8))
-        elif no_bias and all(isinstance(p, CudaLinearMXFP4) for p in projs):
+        elif all(isinstance(p, CudaLinearMXFP4) and p.bias is None for p in projs):
             nw, eps, x = (None, 0.0, x) if input_norm is None else norm_operands(x, input_norm)
             act = matmul_swiglu_mxfp4(x, self.gate_proj.pair, self.up_proj.pair, norm_weight=nw, eps=eps)
-        else:  # of several kinds, or with a bias: each projection by its own forward
+        else:  # of several kinds (the other any module), or with a bias: each projection by its own forward
             if input_norm is not None:
                 x = input_norm(x)
             act = swiglu(self.gate_proj(x), self.up_proj(x))

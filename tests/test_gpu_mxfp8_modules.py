@@ -124,6 +124,28 @@ def test_mlp_of_several_kinds_runs_each_by_itself(kinds, bias):
     assert torch.equal(m(x, residual=x, input_norm=norm), want)
 
 
+class _Plain(torch.nn.Module):
+    """A projection that is no linear layer of this package: a weight, and no attribute `bias`."""
+
+    def __init__(self, weight):
+        super().__init__()
+        self.weight = weight
+
+    def forward(self, x):
+        return K.matmul(x, self.weight)
+
+
+@pytest.mark.parametrize("kind", [CudaLinearMXFP4, CudaLinearMXFP8])
+@pytest.mark.parametrize("name", ["gate_proj", "up_proj"])
+def test_mlp_takes_a_module_without_a_bias_beside_a_quantised_projection(kind, name):
+    m, norm, x = _mlp(256, 544, [kind, kind, None]), CudaRMSNorm(256).to(DEV, torch.bfloat16), rnd(9, 256, seed=1)
+    del m._modules[name]
+    setattr(m, name, _Plain(torch.nn.Parameter(rnd(544, 256, seed=4), requires_grad=False)))
+    y = norm(x)
+    want = m.down_proj(K.swiglu(m.gate_proj(y), m.up_proj(y)), residual=x)
+    assert torch.equal(m(x, residual=x, input_norm=norm), want)
+
+
 # ------------------------------------------------------------------ attention
 @pytest.mark.parametrize("cache_kind", [None, StaticKVCache, PagedKVCache, MXFP4KVCache])
 @pytest.mark.parametrize("S", [1, 50])

@@ -125,3 +125,20 @@ def test_scales_and_workspaces_are_checked(L):
     q = L.q3_matmul_mxfp8_workspace_bytes
     assert all(q(m, i64(n), 1, k, s) == 0 for m in (1, 64) for n in (1, 200000) for k in (96, 4096) for s in (0, 1))
     assert q(1000, i64(4096), 1, 4096, 0) == 0 and q(1000, i64(4096), 1, 4128, 0) > 0  # scales by rows: whole words of them
+
+
+@pytest.mark.parametrize("kind", ["CudaLinearMXFP4", "CudaLinearMXFP8"])
+@pytest.mark.parametrize("name", ["gate_proj", "up_proj"])
+def test_mlp_asks_no_bias_of_a_module_beside_a_quantised_projection(kind, name, monkeypatch):
+    """A projection may be any module; the kernels are stubbed, only the way through the MLP is tested."""
+    from qwen3_5_vl_cuda_custom_amd import modules
+    from qwen3_5_vl_cuda_custom_amd.modules import mlp
+    cls = getattr(modules, kind)
+    monkeypatch.setattr(cls, "forward", lambda self, x, residual=None, out=None: x[..., :1].expand(*x.shape[:-1], 64) + 0)
+    monkeypatch.setattr(mlp, "swiglu", lambda g, u: g * u)
+    m = modules.CudaSwiGLUMLP(32, 64).requires_grad_(False)
+    for n in ("gate_proj", "up_proj", "down_proj"):
+        setattr(m, n, torch.nn.Identity() if n == name else cls(32, 64, bias=False))
+    m.down_proj.forward = lambda x, residual=None: x + residual
+    x = torch.full((2, 64), 3.0)
+    assert torch.equal(m(x, residual=x), x * x + x)
