@@ -658,7 +658,8 @@ int q3_flash_attention_cache_mxfp4(const void* q, const void* k_codes, const voi
  * q3_mxfp8_quantize: x (rows, cols) with row stride ldx. cols a multiple of 32 (else Q3_ERR_SHAPE); x 16-byte aligned,
  * ldx whole 16-byte pieces, codes 8-byte aligned.
  * q3_mxfp8_dequantize: n values (a multiple of 32) of packed rows to y, of type dtype, rounded to it (exact in fp32; in
- * bf16 for every value of 2^-133 or more, its smallest). codes 8-byte, y 16-byte aligned. */
+ * bf16 for every value of 2^-133 or more, its smallest). codes 8-byte, y 16-byte aligned.
+ * Both: fewer than 2^36 - 4096 values a call (else Q3_ERR_UNSUPPORTED). */
 int q3_mxfp8_quantize(const void* x, void* codes, void* scales, int64_t rows, int64_t cols, int64_t ldx, int dtype,
                       void* stream);
 int q3_mxfp8_dequantize(const void* codes, const void* scales, void* y, int64_t n, int dtype, void* stream);
@@ -666,7 +667,7 @@ int q3_mxfp8_dequantize(const void* codes, const void* scales, void* y, int64_t 
 /* q3_residual_add, q3_rmsnorm and q3_mxfp8_quantize in one launch: sum = x + residual, rounded to dtype; y = rmsnorm(sum;
  * weight, eps) in fp32, quantised from there (not rounded to dtype in between). x, residual, sum (rows, cols) with row
  * strides ldx, ldr and cols; residual and sum may both be null: the norm of x. sum must not overlap x or residual.
- * cols a multiple of 32 below 2^24; x, residual, weight, sum and their rows 16-byte aligned, codes 8-byte. */
+ * Fewer than 2^31 rows, cols a multiple of 32 below 2^24; x, residual, weight, sum and their rows 16-byte aligned, codes 8-byte. */
 int q3_add_rmsnorm_mxfp8(const void* x, const void* residual, const void* weight, void* sum, void* codes, void* scales,
                          int64_t rows, int64_t cols, int64_t ldx, int64_t ldr, float eps, int dtype, void* stream);
 
@@ -676,6 +677,8 @@ int q3_add_rmsnorm_mxfp8(const void* x, const void* residual, const void* weight
  * row stride ldc, or with y null, y_codes and y_scales: the fp32 values in MXFP8, packed (N a multiple of 32). K a
  * multiple of 32 below 2^23; codes 16-byte aligned (y_codes 8-byte), scales 4-byte. The matrix instruction cuts the products of eight
  * consecutive k 13 bits below the largest of them: a result is within 7 * 2^-13 of the sum of those largest ones.
+ * Products whose launch would have 2^32 threads or more (which takes 2^29 weight rows, or 2^23 tiles of outputs) return
+ * Q3_ERR_UNSUPPORTED.
  * q3_matmul_segments_mxfp8: y (M, sum n_j) = x [w_0; w_1; ...]^T (+ [b_0; b_1; ...]), 1 to 4 weights of n[j] >= 1 rows;
  * w_codes, w_scales and bias are host arrays of device pointers (bias, or any of its entries, may be null).
  * q3_matmul_swiglu_mxfp8: silu(x g^T) * (x u^T), into y or y_codes and y_scales.

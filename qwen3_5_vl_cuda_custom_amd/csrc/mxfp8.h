@@ -96,6 +96,9 @@ __device__ __forceinline__ floatx4 mfma_mx8(i32x8 a, i32x8 b, floatx4 c, int sa,
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
 }
 
+// A launch has less than 2^32 threads along x.
+inline bool mx8_grid_ok(int64_t blocks, int threads) { return blocks * threads < (1ll << 32); }
+
 // Eight values at p (8 bf16 or fp32, 16-byte aligned).
 template <typename T>
 __device__ __forceinline__ void mx8_load8(const T* p, float (&v)[8]) {

@@ -90,7 +90,7 @@ struct NormArgs {
   void* h;                // the sum, packed, where there is an r
   u32x2* codes;           // packed
   uint8_t* scales;
-  int64_t rows, ldx, ldr;
+  int64_t first, ldx, ldr;  // the launch's first row
   int cols8;              // pieces of a row, a multiple of four
   float eps;
 };
@@ -101,7 +101,7 @@ struct NormArgs {
 template <typename T, int P>
 __global__ __launch_bounds__(256) void mx8_norm_kernel(const NormArgs a) {
   __shared__ float sums[4];
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.first + blockIdx.x;
   const int t = threadIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
   const T* r = a.r ? static_cast<const T*>(a.r) + row * a.ldr : nullptr;
@@ -180,9 +180,12 @@ __global__ __launch_bounds__(256) void mx8_norm_kernel(const NormArgs a) {
   }
 }
 
+// Rows of one launch (a block of 256 threads each).
+constexpr int64_t kLaunchRows = (1 << 24) - 1;
+
 template <typename T>
-void launch_norm(const NormArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)a.rows), block(256);
+void launch_norm(const NormArgs& a, int64_t rows, hipStream_t st) {
+  const dim3 grid((unsigned)rows), block(256);
   const int p = (a.cols8 + 255) / 256;
   if (p <= 1) hipLaunchKernelGGL((mx8_norm_kernel<T, 1>), grid, block, 0, st, a);
   else if (p <= 2) hipLaunchKernelGGL((mx8_norm_kernel<T, 2>), grid, block, 0, st, a);
@@ -203,7 +206,7 @@ int q3_mxfp8_quantize(const void* x, void* codes, void* scales, int64_t rows, in
   Q3_REQUIRE(q3_aligned(x, 16) && ldx * size % 16 == 0 && q3_aligned(codes, 8), Q3_ERR_ALIGN);
   if (rows == 0 || cols == 0) return Q3_OK;
   const int64_t pieces = rows * (cols / 8), blocks = q3_cdiv(pieces, 256 * kPieces);
-  Q3_REQUIRE(blocks < (1ll << 31), Q3_ERR_UNSUPPORTED);
+  Q3_REQUIRE(mx8_grid_ok(blocks, 256), Q3_ERR_UNSUPPORTED);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)blocks), block(256);
   u32x2* c = static_cast<u32x2*>(codes);
@@ -230,7 +233,7 @@ int q3_mxfp8_dequantize(const void* codes, const void* scales, void* y, int64_t 
   Q3_REQUIRE(q3_aligned(codes, 8) && q3_aligned(y, 16), Q3_ERR_ALIGN);
   if (n == 0) return Q3_OK;
   const int64_t pieces = n / 8, blocks = q3_cdiv(pieces, 256 * kPieces);
-  Q3_REQUIRE(blocks < (1ll << 31), Q3_ERR_UNSUPPORTED);
+  Q3_REQUIRE(mx8_grid_ok(blocks, 256), Q3_ERR_UNSUPPORTED);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)blocks), block(256);
   const u32x2* c = static_cast<const u32x2*>(codes);
@@ -259,13 +262,16 @@ int q3_add_rmsnorm_mxfp8(const void* x, const void* residual, const void* weight
   a.x = x, a.r = residual, a.w = weight, a.h = sum;
   a.codes = static_cast<u32x2*>(codes);
   a.scales = static_cast<uint8_t*>(scales);
-  a.rows = rows, a.ldx = ldx, a.ldr = ldr;
+  a.ldx = ldx, a.ldr = ldr;
   a.cols8 = (int)(cols / 8);
   a.eps = eps;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == Q3_BF16) launch_norm<bf16>(a, st);
-  else launch_norm<float>(a, st);
-  Q3_LAUNCH_CHECK();
+  for (a.first = 0; a.first < rows; a.first += kLaunchRows) {
+    const int64_t n = std::min(kLaunchRows, rows - a.first);
+    if (dtype == Q3_BF16) launch_norm<bf16>(a, n, st);
+    else launch_norm<float>(a, n, st);
+    Q3_LAUNCH_CHECK();
+  }
   return Q3_OK;
 }
 

@@ -376,6 +376,7 @@ int mx8_rows(const Mx8Args& args, bool swiglu, hipStream_t st) {
     int r = unit;
     while (r < most && blocks(r) * parts > 256 * rounds) r += unit;
     p.r = r;
+    Q3_REQUIRE(mx8_grid_ok(blocks(r) * parts, 64 * kWaves), Q3_ERR_UNSUPPORTED);
     const unsigned n = (unsigned)(blocks(r) * parts);
     if (swiglu) {
       if (p.M <= 8) launch_ring<8, true>(p, n, st);
@@ -393,6 +394,7 @@ int mx8_rows(const Mx8Args& args, bool swiglu, hipStream_t st) {
   }
   // 32 weight rows a block where the output's blocks of 32 ask for it, or where that still gives every CU two blocks.
   const bool wide = p.yc || blocks(32) >= 512;
+  Q3_REQUIRE(mx8_grid_ok(blocks(wide ? 32 : 16), 64 * kWaves), Q3_ERR_UNSUPPORTED);
   const unsigned n = (unsigned)blocks(wide ? 32 : 16);
   if (swiglu) {
     if (wide) launch_tiles<2, true>(p, n, st);

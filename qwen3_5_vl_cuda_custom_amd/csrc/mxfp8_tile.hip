@@ -541,16 +541,16 @@ __global__ __launch_bounds__(256) void mx8_lay_scales_kernel(const LayArgs a) {
   }
 }
 
-int tiles_of(const Mx8Args& a, int bn) {
+int64_t tiles_of(const Mx8Args& a, int bn) {
   int64_t n = 0;
   for (int j = 0; j < a.nseg; ++j) n += q3_cdiv(a.n[j], bn);
-  return (int)n;
+  return n;
 }
 
 template <int BM, int BN, int WM, int WN, int NS, bool SW, bool RAW = false>
 void launch_tile(TileArgs t, hipStream_t st) {
   t.tiles_m = (int)q3_cdiv(t.a.M, BM);
-  t.tiles_n = tiles_of(t.a, SW ? BN / 2 : BN);
+  t.tiles_n = (int)tiles_of(t.a, SW ? BN / 2 : BN);
   // The tiles along m in even groups of at most 1024 rows: a remainder of one tile read the weights once more for itself
   // (SwiGLU of 611 rows, N 12288: 4 + 1 tiles 77 us, 5 71.5). Groups of 768 to 2048 rows: within 2 %.
   constexpr int kGroup = 1024 / BM;
@@ -560,6 +560,8 @@ void launch_tile(TileArgs t, hipStream_t st) {
 }
 
 // Forms: tiles of 256 x 256, 128 x 256, 128 x 128, and of the last size with the scales by rows.
+constexpr int kFormBM[4] = {256, 128, 128, 128}, kFormBN[4] = {256, 256, 128, 128}, kFormThreads[4] = {512, 256, 256, 256};
+
 template <bool SW>
 void launch_form(const TileArgs& t, int form, hipStream_t st) {
   if (form == 0) launch_tile<256, 256, 2, 4, 2, SW>(t, st);
@@ -577,7 +579,8 @@ void launch_form(const TileArgs& t, int form, hipStream_t st) {
 int form_of(const Mx8Args& a, bool swiglu) {
   const int64_t out = swiglu ? 2 : 1, stages = q3_cdiv(a.K, 128);
   auto cost = [&](int bm, int bn, int64_t launches, int64_t fixed, int64_t stage) {
-    const int64_t tiles = q3_cdiv(a.M, bm) * tiles_of(a, (int)(bn / out)), rest = tiles % 256;
+    // (past 2^32 tiles, more than a launch takes, any count will do)
+    const int64_t tiles = std::min<int64_t>(q3_cdiv(a.M, bm) * tiles_of(a, (int)(bn / out)), 1ll << 32), rest = tiles % 256;
     return launches * 1024 + (tiles / 256 * 1024 + (rest ? 768 + rest : 0)) * (fixed + stages * stage);
   };
   const int64_t costs[4] = {cost(256, 256, 760, 800, 138), cost(128, 256, 750, 730, 75), cost(128, 128, 430, 540, 43),
@@ -612,7 +615,7 @@ int lay_scales(TileArgs& t, bool swiglu, void* workspace, hipStream_t st) {
     waves += groups * l.nb;
     out += groups * l.groups_k * 1024;
   }
-  Q3_REQUIRE(waves < (1ll << 31) - 4, Q3_ERR_UNSUPPORTED);
+  Q3_REQUIRE(mx8_grid_ok(q3_cdiv(waves, 4), 256), Q3_ERR_UNSUPPORTED);
   l.waves = (int)waves;
   hipLaunchKernelGGL(mx8_lay_scales_kernel, dim3((unsigned)q3_cdiv(waves, 4)), dim3(256), 0, st, l);
   Q3_LAUNCH_CHECK();
@@ -635,6 +638,8 @@ int mx8_tile(const Mx8Args& a, bool swiglu, void* workspace, hipStream_t st) {
   TileArgs t{};
   t.a = a;
   const int form = form_of(a, swiglu);
+  Q3_REQUIRE(mx8_grid_ok(q3_cdiv(a.M, kFormBM[form]) * tiles_of(a, kFormBN[form] / (swiglu ? 2 : 1)), kFormThreads[form]),
+             Q3_ERR_UNSUPPORTED);
   if (form < 3)
     if (const int rc = lay_scales(t, swiglu, workspace, st)) return rc;
   if (swiglu) launch_form<true>(t, form, st);

@@ -460,6 +460,19 @@ def test_rows_past_two_to_the_31_values():
         assert bool((a.view(600, 1000, -1) == b).all())
 
 
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_of_more_rows_than_a_launch_has_blocks(residual):
+    """2^24 rows of a block of 256 threads each would be 2^32 threads."""
+    x, w = rnd(1021, 32, seed=1).to(DEV), rnd(32, seed=2).to(DEV)
+    rows = (1 << 24) + 5
+    of = torch.arange(rows, device=DEV) % 1021
+    big = x[of]
+    h, codes, scales = K.add_rmsnorm_mxfp8(big, big if residual else None, w)
+    h1, codes1, scales1 = K.add_rmsnorm_mxfp8(x, x if residual else None, w)
+    assert torch.equal(h, h1[of]) and torch.equal(scales, scales1[of])
+    assert torch.equal(codes.view(torch.uint8), codes1.view(torch.uint8)[of])
+
+
 @pytest.mark.parametrize("m", [2, 40, 700])
 def test_weights_past_two_to_the_31_bytes(m):
     x, w = dev(exact_pair(m, 4096, 1)), dev(exact_pair(1000, 4096, 2))

@@ -142,3 +142,24 @@ def test_mlp_asks_no_bias_of_a_module_beside_a_quantised_projection(kind, name, 
     m.down_proj.forward = lambda x, residual=None: x + residual
     x = torch.full((2, 64), 3.0)
     assert torch.equal(m(x, residual=x), x * x + x)
+
+
+def test_launches_of_2_to_the_32_threads_are_refused(L):
+    """A launch has less than 2^32 threads along x: what would need more says so before any device work."""
+    q, d = L.q3_mxfp8_quantize, L.q3_mxfp8_dequantize
+    assert q(FAKE, FAKE, FAKE, 1 << 31, 32, 32, 1, None) == -5 and q(FAKE, FAKE, FAKE, 1 << 20, 1 << 16, 1 << 16, 0, None) == -5
+    assert d(FAKE, FAKE, FAKE, 1 << 36, 1, None) == -5
+
+    def mm(M_, N, K, work=FAKE, size=1 << 62):
+        return L.q3_matmul_mxfp8(FAKE, FAKE, FAKE, FAKE, None, None, FAKE, None, None, M_, N, K, 0, N, 0, work, size, None)
+    assert mm(1, 1 << 29, 32) == -5  # weight rows by 32, loads into registers
+    assert mm(1, (1 << 31) - 300, 128) == -5  # by 96, through the ring
+    assert mm((1 << 31) - 300, 600, 32) == -5  # tiles of any size
+
+    def seg(M_, n, K):
+        ns = i64(*n)
+        return L.q3_matmul_segments_mxfp8(FAKE, FAKE, ptrs(*[FAKE] * len(n)), ptrs(*[FAKE] * len(n)), None, ns, len(n), FAKE,
+                                          M_, K, sum(n), FAKE, 1 << 62, None)
+    assert seg(1 << 29, (1, 1, 1, 1), 32) == -5
+    sw = L.q3_matmul_swiglu_mxfp8
+    assert sw(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None, None, 33, 1 << 29, 128, 1 << 29, None, 0, None) == -5
