@@ -685,6 +685,10 @@ int q3_add_rmsnorm_mxfp8(const void* x, const void* residual, const void* weight
  * Workspace: q3_matmul_mxfp8_workspace_bytes (n: the rows of each weight, one for SwiGLU); 16-byte aligned, needs no
  * clearing, calls that may run at the same time must not share it. */
 int64_t q3_matmul_mxfp8_workspace_bytes(int64_t M, const int64_t* n, int64_t nseg, int64_t K, int swiglu);
+/* The kernel that takes such a product: whole weight rows into registers (0) or through a ring in LDS (1), tiles of
+ * 256 x 256 (2), 128 x 256 (3), 128 x 128 (4), and 128 x 128 with the scales by rows (5); Q3_ERR_SHAPE for sizes that no
+ * call takes. The arguments are those of the workspace's query. */
+int q3_matmul_mxfp8_form(int64_t M, const int64_t* n, int64_t nseg, int64_t K, int swiglu);
 int q3_matmul_mxfp8(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales,
                     const void* bias, const void* residual, void* y, void* y_codes, void* y_scales, int64_t M,
                     int64_t N, int64_t K, int64_t ldr, int64_t ldc, int act, void* workspace, int64_t workspace_bytes,

@@ -133,6 +133,7 @@ _SIGS: dict[str, tuple] = {
     "q3_mxfp8_dequantize": (c_int, [_V, _V, _V, _I, c_int, _V]),
     "q3_add_rmsnorm_mxfp8": (c_int, [_V, _V, _V, _V, _V, _V, _I, _I, _I, _I, c_float, c_int, _V]),
     "q3_matmul_mxfp8_workspace_bytes": (c_int64, [_I, _V, _I, _I, c_int]),
+    "q3_matmul_mxfp8_form": (c_int, [_I, _V, _I, _I, c_int]),
     "q3_matmul_mxfp8": (c_int, [_V, _V, _V, _V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _I, c_int, _V, _I, _V]),
     "q3_matmul_segments_mxfp8": (c_int, [_V, _V, _V, _V, _V, _V, _I, _V, _I, _I, _I, _V, _I, _V]),
     "q3_matmul_swiglu_mxfp8": (c_int, [_V, _V, _V, _V, _V, _V, _V, _V, _V, _I, _I, _I, _I, _V, _I, _V]),

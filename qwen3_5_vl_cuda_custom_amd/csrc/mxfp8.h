@@ -166,6 +166,8 @@ __device__ __forceinline__ void mx8_act(float (&v)[N], int act) {
 
 // Whether mx8_rows takes the product: it needs no workspace.
 bool mx8_rows_takes(const Mx8Args& a, bool swiglu);
+// Whether it goes through the ring (else fragments and scales straight into registers).
+inline bool mx8_rows_ring(const Mx8Args& a) { return a.K % 128 == 0; }
 int mx8_rows(const Mx8Args& a, bool swiglu, hipStream_t st);
 
 }  // namespace q3

@@ -59,24 +59,36 @@ int launch(const Call& c, bool swiglu, void* workspace, int64_t workspace_bytes,
   return mx8_rows_takes(c.a, swiglu) ? mx8_rows(c.a, swiglu, st) : mx8_tile(c.a, swiglu, workspace, st);
 }
 
+// The sizes of a call that there may be, as its form goes by them.
+bool sizes(Mx8Args& a, int64_t M, const int64_t* n, int64_t nseg, int64_t K) {
+  if (!n || nseg < 1 || nseg > kMx8Segments || M <= 0 || K < kMx8Block || K % kMx8Block) return false;
+  int64_t N = 0;
+  for (int j = 0; j < nseg; ++j) {
+    if (n[j] < 1 || n[j] >= (1ll << 31) - 256) return false;
+    a.n[j] = (int)n[j];
+    N += n[j];
+  }
+  if (N >= (1ll << 31) - 256 || M >= (1ll << 31) - 256 || K >= (1 << 23)) return false;
+  a.nseg = (int)nseg;
+  a.M = (int)M;
+  a.K = (int)K;
+  return true;
+}
+
 }  // namespace
 
 extern "C" {
 
 int64_t q3_matmul_mxfp8_workspace_bytes(int64_t M, const int64_t* n, int64_t nseg, int64_t K, int swiglu) {
-  if (!n || nseg < 1 || nseg > kMx8Segments || M <= 0 || K < kMx8Block || K % kMx8Block) return 0;
   Mx8Args a{};
-  int64_t N = 0;
-  for (int j = 0; j < nseg; ++j) {
-    if (n[j] < 1 || n[j] >= (1ll << 31) - 256) return 0;
-    a.n[j] = (int)n[j];
-    N += n[j];
-  }
-  if (N >= (1ll << 31) - 256 || M >= (1ll << 31) - 256 || K >= (1 << 23)) return 0;
-  a.nseg = (int)nseg;
-  a.M = (int)M;
-  a.K = (int)K;
-  return workspace_of(a, swiglu != 0);
+  return sizes(a, M, n, nseg, K) ? workspace_of(a, swiglu != 0) : 0;
+}
+
+int q3_matmul_mxfp8_form(int64_t M, const int64_t* n, int64_t nseg, int64_t K, int swiglu) {
+  Mx8Args a{};
+  if (!sizes(a, M, n, nseg, K)) return Q3_ERR_SHAPE;
+  if (mx8_rows_takes(a, swiglu != 0)) return mx8_rows_ring(a) ? 1 : 0;
+  return 2 + mx8_tile_form(a, swiglu != 0);
 }
 
 int q3_matmul_mxfp8(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales,

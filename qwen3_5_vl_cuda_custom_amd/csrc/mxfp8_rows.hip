@@ -348,7 +348,7 @@ bool mx8_rows_takes(const Mx8Args& p, bool swiglu) {
   if (p.M <= 64) return true;
   int64_t blocks = 0;
   for (int j = 0; j < p.nseg; ++j) blocks += q3_cdiv(p.n[j], swiglu ? 32 : 64);
-  return p.K % 128 == 0 && blocks * q3_cdiv(p.M, 64) <= 256;
+  return mx8_rows_ring(p) && blocks * q3_cdiv(p.M, 64) <= 256;
 }
 
 int mx8_rows(const Mx8Args& args, bool swiglu, hipStream_t st) {
@@ -364,7 +364,7 @@ int mx8_rows(const Mx8Args& args, bool swiglu, hipStream_t st) {
     for (int j = 0; j < p.nseg; ++j) n += q3_cdiv(p.n[j], rows);
     return n;
   };
-  if (p.K % 128 == 0) {
+  if (mx8_rows_ring(p)) {
     // The fewest rows a block (whole 8-byte pieces of y, or whole blocks of 32 in eight bits) that give every CU one block,
     // or an equal number of them where even the largest block does not cover N. One row of K 4096, us by rows a block:
     // N 12288 13.2 (48), 24576 24.9, 25.6, 26.3 and 23.1 (16, 32, 64, 96), 49152 45.1, 44.8, 46.1 and 43.1; 32 rows, N

@@ -626,6 +626,8 @@ int lay_scales(TileArgs& t, bool swiglu, void* workspace, hipStream_t st) {
 
 namespace q3 {
 
+int mx8_tile_form(const Mx8Args& a, bool swiglu) { return form_of(a, swiglu); }
+
 int64_t mx8_tile_workspace(const Mx8Args& a, bool swiglu) {
   if (form_of(a, swiglu) == 3) return 0;
   int64_t bytes = laid_bytes(a.M, a.K);
