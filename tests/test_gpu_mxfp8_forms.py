@@ -121,3 +121,55 @@ def test_swiglu(f, m, n, k):
     n -= n % 32
     pair = K.matmul_swiglu_mxfp8(xd, head(gd, n), head(ud, n), quantize=True)
     check_eight_bits(pair, want[:, :n].cpu(), err[:, :n].cpu())
+
+
+def with_nan(pair, *places):
+    """The pair with NaN for the scales (rows, block) of `places`, and which rows have one."""
+    scales = pair[1].clone()
+    rows = torch.zeros(len(scales), dtype=torch.bool)
+    for at, block in places:
+        scales[at, block] = 255
+        rows[at] = True
+    return (pair[0], scales), rows.to(DEV)
+
+
+def nan_exactly(y, rows, columns, want):
+    """y is NaN in those rows and columns, and the correctly rounded `want` elsewhere."""
+    bad = rows[:, None] | columns[None]
+    assert torch.equal(torch.isnan(y), bad)
+    assert torch.equal(y[~bad], want[~bad].to(torch.bfloat16))
+
+
+def nan_x(m, k):
+    return with_nan(exact_pair(m, k, 1), (slice(min(5, m - 1), None, 97), 0), (-1, -1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f,m,n,k", PLAIN)
+def test_nan_scales_of_products_stay_where_they_are(f, m, n, k):
+    """NaN in a row's first block, behind its neighbour's end, and in a matrix's last one; of two weights side by side in
+    the rows that meet."""
+    (x, rows), w = nan_x(m, k), exact_pair(n, k, 2)
+    a = values(exact_pair(m, k, 1)) @ values(w).T
+    v, columns = with_nan(w, (slice(7, None, 101), 0), (-1, -1))
+    nan_exactly(K.matmul_mxfp8(dev(x), dev(v)), rows, columns, a)
+    c = cut(n)
+    v, columns = with_nan(w, (c - 1, -1), (c, 0), (-1, -1))
+    vd = dev(v)
+    y = K.matmul_segments_mxfp8(dev(x), [head(vd, c), (vd[0][c:], vd[1][c:])])
+    nan_exactly(y, rows, columns, a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f,m,n,k", SWIGLU)
+def test_nan_scales_of_swiglu_stay_where_they_are(f, m, n, k):
+    """Gate's and up's in different rows; where neither has one the result is that of the weights without any."""
+    (x, rows), g, u = nan_x(m, k), exact_pair(n, k, 2), exact_pair(n, k, 3)
+    gv, gc = with_nan(g, (slice(7, None, 101), 0), (31, -1))
+    uv, uc = with_nan(u, (slice(11, None, 103), -1), (32, 0), (-1, -1))
+    want = K.matmul_swiglu_mxfp8(dev(exact_pair(m, k, 1)), dev(g), dev(u))
+    nan_exactly(K.matmul_swiglu_mxfp8(dev(x), dev(gv), dev(uv)), rows, gc | uc, want)
+    n -= n % 32
+    codes, scales = K.matmul_swiglu_mxfp8(dev(x), head(dev(gv), n), head(dev(uv), n), quantize=True)
+    blocks = rows[:, None] | (gc | uc)[:n].view(-1, 32).any(-1)[None]
+    assert torch.equal(scales == 255, blocks)
