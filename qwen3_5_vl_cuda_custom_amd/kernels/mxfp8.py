@@ -20,7 +20,7 @@ from .. import _lib
 from ._common import require_device, require_no_grad
 
 MX8_BLOCK = 32
-_FEW_ROWS = 64  # up to which the products need no workspace (csrc/mxfp8_matmul.hip)
+_FEW_ROWS = 64  # up to which the products need no workspace (mx8_rows_takes, csrc/mxfp8_rows.hip)
 _U8, _F8, _BF16 = torch.uint8, torch.float8_e4m3fn, torch.bfloat16
 _i64s = [Struct(f"{n}q").pack for n in range(5)]  # C arrays of up to four numbers or addresses
 _ACTS = {None: 0, "gelu_tanh": 1, "silu": 2}
@@ -40,7 +40,8 @@ def _off_device(op: str, *tensors: torch.Tensor | None) -> None:
 
 
 def _packed(op: str, codes: torch.Tensor, scales: torch.Tensor, dev: int) -> Pair:
-    """The pair checked, packed and aligned as the kernels read it."""
+    """The pair checked, packed and aligned as the kernels read it. (_weight asks the first condition too, in place: a
+    change to one is a change to both.)"""
     cs, ss = codes.shape, scales.shape
     if (codes.dtype is _F8 and scales.dtype is _U8 and codes.get_device() == dev and scales.get_device() == dev
             and codes.is_contiguous() and scales.is_contiguous() and len(cs) == 2 and len(ss) == 2 and cs[0] == ss[0]
@@ -196,7 +197,7 @@ def _weight(op: str, weight: Pair, K: int, dev: int) -> Pair:
             and codes.is_contiguous() and scales.is_contiguous() and len(cs) == 2 and len(ss) == 2 and cs[0] == ss[0]
             and cs[1] == K and ss[1] * MX8_BLOCK == K
             and not (codes.data_ptr() % 16 or scales.data_ptr() % 4 or codes.requires_grad)):
-        return codes, scales  # the usual call, without the calls below
+        return codes, scales  # the usual call: _packed's condition and the shape of x, without the calls below
     codes, scales = _packed(op, codes, scales, dev)
     if codes.dim() != 2 or codes.shape[1] != K:
         raise ValueError(f"{op}: weight codes {tuple(codes.shape)} do not match x (..., {K})")

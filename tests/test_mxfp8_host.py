@@ -163,3 +163,14 @@ def test_launches_of_2_to_the_32_threads_are_refused(L):
     assert seg(1 << 29, (1, 1, 1, 1), 32) == -5
     sw = L.q3_matmul_swiglu_mxfp8
     assert sw(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None, None, 33, 1 << 29, 128, 1 << 29, None, 0, None) == -5
+
+
+def test_products_of_few_rows_need_no_workspace(L):
+    """Up to _FEW_ROWS rows the calls do not ask for its size."""
+    from qwen3_5_vl_cuda_custom_amd.kernels.mxfp8 import _FEW_ROWS
+    q = L.q3_matmul_mxfp8_workspace_bytes
+    for m in (1, 16, _FEW_ROWS):
+        for k in (32, 96, 128, 4096, 65536, (1 << 23) - 32):
+            for ns in ((1,), (300,), (151936,), ((1 << 31) - 300,), (4096, 1024, 1024), (5, 300, 1, 77)):
+                assert q(m, i64(*ns), len(ns), k, 0) == 0
+                assert len(ns) > 1 or q(m, i64(*ns), 1, k, 1) == 0
