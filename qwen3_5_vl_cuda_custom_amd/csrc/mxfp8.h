@@ -166,7 +166,10 @@ __device__ __forceinline__ void mx8_act(float (&v)[N], int act) {
 
 // Whether mx8_rows takes the product: it needs no workspace.
 bool mx8_rows_takes(const Mx8Args& a, bool swiglu);
-// Whether it goes through the ring (else fragments and scales straight into registers).
+// Whether it goes through the ring (else fragments and scales straight into registers): the ring brings a row's scales in
+// words, so every row of them has to start at one. The same holds for the ring past 64 rows and the tiles with the scales
+// by rows. N 4096, weights past the last cache, K 4096 and K 4128, us: 1 row 6.5 and 8.8, 32 rows 8.0 and 12.3, 100 rows
+// 10.9 and 40.1 (tiles), 1000 rows 27.0 and 40.1; K 1024 and 1056: 3.6 and 3.7, 4.5 and 4.3, 6.2 and 16.5, 10.8 and 18.1.
 inline bool mx8_rows_ring(const Mx8Args& a) { return a.K % 128 == 0; }
 int mx8_rows(const Mx8Args& a, bool swiglu, hipStream_t st);
 

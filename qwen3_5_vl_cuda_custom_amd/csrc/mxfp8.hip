@@ -4,10 +4,12 @@
 // All are bound by memory: eight values (a 16-byte load of bf16, 8 bytes of
 // codes) per lane and piece, so the four lanes of a block exchange their largest
 // magnitude with two lane shuffles and nothing but a row's sum goes through LDS.
-// The norm with its sum of 16384 x 4096 bf16 takes 76 us (471 MB, 6.2 TB/s, where a
-// copy of 1 GiB reaches 5.1: part of it stays in the last cache), one row 2.7, 777 rows
-// of 2048 fp32 values 3.8; back to bf16 16384 x 4096 32 us (203 MB), 1000 x 4096 bf16
-// to eight bits 3.3.
+// The norm with its sum of 16384 x 4096 bf16 takes 84 us over inputs past the last cache
+// (472 MB, 5.6 TB/s), 77 where part of them stays in it, one row 2.8, 777 rows of 2048
+// fp32 values 3.8; rows of more than 8192 values, whose kernel reads them twice (the
+// second time from the caches in part), 4096 x 12288 86 us (354 MB, 4.1 TB/s). Back to
+// bf16 16384 x 4096 31 us (203 MB); 1000 x 4096 bf16 to eight bits 4.3 (3.1 out of the
+// last cache), as columns of wider rows 4.5; 16384 rows 32.8 and 34.8.
 #include "mxfp8.h"
 
 namespace {

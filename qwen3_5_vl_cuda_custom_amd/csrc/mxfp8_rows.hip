@@ -369,6 +369,9 @@ int mx8_rows(const Mx8Args& args, bool swiglu, hipStream_t st) {
     // or an equal number of them where even the largest block does not cover N. One row of K 4096, us by rows a block:
     // N 12288 13.2 (48), 24576 24.9, 25.6, 26.3 and 23.1 (16, 32, 64, 96), 49152 45.1, 44.8, 46.1 and 43.1; 32 rows, N
     // 49152 77.9, 57.5, 49.6 and 49.2. (N 151936 would be 8 % faster in blocks of 32, two on a CU: 121 against 131.)
+    // Measured for bf16 outputs; whole blocks of 32 fill the CUs less evenly. SwiGLU of K 4096 in bf16 and in eight bits,
+    // us: one row, N 9728 18.1 (244 blocks of 40) and 20.9 (152 of 64), N 12288 21.1 (256 of 48) and 22.9 (192 of 64), N
+    // 22016 34.8 (501 of 44) and 40.5 (344 of 64); 32 rows 20.6 and 24.6 (304 of 32), 23.0 and 27.0 (384 of 32), 38.5 and 40.8.
     const int unit = p.yc ? 32 : 4;
     int most = 16 * (p.M <= 8 ? (swiglu ? 4 : 6) : p.M <= 32 ? (swiglu ? 3 : 6) : swiglu ? 2 : 4);
     most = most / unit * unit;

@@ -16,27 +16,25 @@
 // fill the LDS; a stage's weight slot is free once every wave has the fragments, after the
 // first column: a second barrier there lets the weights after next, which come from further
 // away than x, set out most of a stage earlier. Gate and up of 4096 rows, N 12288, K 4096:
-// 317 us and 5 for the scales, 2.60 PFLOP/s (of an earlier form's 336 it took 282 without the
-// loads of codes, 322 with all of them from one place; matrix pipe busy 62 %); N 4096, K 12288
-// 157 us, 2.63 PFLOP/s.
+// 316 us and 5 for the scales, 2.61 PFLOP/s; N 4096, K 12288 154 us, 2.68 PFLOP/s. What is
+// left is the clock, the loads of codes beside the products, and the barriers.
 //
 // Smaller tiles, four waves of 128 x 64 or 64 x 64 for 128 x 256 and 128 x 128: one wave a SIMD
 // has the registers for two stages' fragments. It reads all of the next stage's between the
 // products of this one, so a slot is free at the barrier where its stage begins, and three or
-// four slots stay under way. Waves that read as above took 76 us for SwiGLU of 611 rows, N 12288
-// (128 x 256, eight waves; these 74 then, 54 without the loads of codes) and 34.6 for 1000 rows,
-// N = K = 4096 (128 x 128, these 28.8 then); tiles of 256 x 256 take 86 and 52. What is left of
-// 67 and 24 us: 64 and 32 stages of 0.6 and 0.3 us of products, the waits for codes between
-// them, and 7.5 us with one stage alone (launch, first loads, epilogue).
+// four slots stay under way. Waves that read as above, eight to a tile of 128 x 256, took 3 %
+// longer for SwiGLU of 611 rows, N 12288, and for 128 x 128 and 1000 rows, N = K = 4096, 20 %;
+// tiles of 256 x 256 take 86 and 52 us there, these 64 to 67 and 24 to 26: 64 and 32 stages of
+// 0.6 and 0.3 us of products, the waits for codes between them, and 7.6 us of a tile with one
+// stage alone (launch, first loads, epilogue).
 //
 // Scales are laid out anew first, by a kernel of their own: the scales of 64 rows and four
 // stages are 1 KB as the instruction's lanes take them, word l of a stage lane l's block
 // of rows l % 16, + 16, + 32, + 48 (the instruction picks the byte). A load brings a stage
 // of them, and three words a stage are all that a wave reads. As rows of bytes their loads
-// cost a line per row and the reads twelve bytes a stage: 198 against 194 us for 4096 x 4096
-// x 12288 when it was tried. For small products the launch costs more (2.7 to 4 us), and
-// 128 x 128 tiles take the scales by rows (RAW), 16 bytes, four stages', of a row at a time:
-// 784 rows of K 1152, N 4304 17.6 to 14.6 us (12.2 now), the 1000 rows 27.9 to 26.4.
+// cost a line per row and the reads twelve bytes a stage: 2 % more for 4096 x 4096 x 12288.
+// For small products the launch costs more (2.7 to 4 us), and 128 x 128 tiles take the
+// scales by rows (RAW), 16 bytes, four stages', of a row at a time (both ways: form_of).
 #include "gemm_tile.h"
 #include "mxfp8.h"
 #include "mxfp8_tile.h"
